@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define SMOL_LM_ABI_VERSION 6
+#define SMOL_LM_ABI_VERSION 7
 
 enum { SMOL_LM_BF16 = 0, SMOL_LM_F32 = 1 };
 /* token mixers */
@@ -293,7 +293,8 @@ typedef struct SmolLmStep {
 typedef struct SmolLm SmolLm;
 
 int smol_lm_abi_version(void);
-size_t smol_lm_struct_bytes(int which);          /* sizeof of SmolLmLayer (0), SmolLmConfig (1), SmolLmGlobals (2), SmolLmStep (3): a binding checks its mirror */
+size_t smol_lm_struct_bytes(int which);          /* sizeof of SmolLmLayer (0), SmolLmConfig (1), SmolLmGlobals (2), SmolLmStep (3), SmolLmCache8 (4), SmolLmCache8Batch (5),
+                                                    SmolLmCache8Append (6), SmolLmCache8Attend (7): a binding checks its mirror */
 const char* smol_lm_last_error(void);
 
 /* layers / run_layer are HOST arrays, copied.  run_layer[n] = index of the layer that run n executes. */
@@ -316,6 +317,68 @@ int smol_lm_sample(SmolLm* m, const float* d_logits, int32_t rows, int32_t n, fl
 
 /* Stand-alone operations of the engine, for tests and benchmarks: y fp32 [M, N] = a [M, K] . w [N, K]^T in the engine's element type. */
 int smol_lm_linear(SmolLm* m, const void* d_a, const void* d_w, float* d_y, int32_t M, int32_t N, int32_t K, void* stream);
+
+/* --- A key/value cache in 8 bits, on its own (no engine needed).  A position holds, per key/value head, a row of e4m3 codes for the key and one
+ *     for the value; 16 positions that follow one another share a scale per head, keys and values each their own: a power of two, negative
+ *     where the block holds a NaN.  Value = code * |scale|. --- */
+typedef struct SmolLmCache8 {
+    void *k, *v;                 /* e4m3 [n_pages][kv_heads][page_size][dim, vdim rounded up to 16], 16-byte aligned; zeros behind dim / vdim */
+    float *k_scale, *v_scale;    /* [n_pages][kv_heads][page_size / 16] */
+    size_t k_page, v_page;       /* bytes from a page's codes to the next page's (0: as above, nothing between) */
+    size_t k_scale_page, v_scale_page;   /* floats from a page's scales to the next page's (0: likewise) */
+    int32_t n_pages, page_size;  /* page_size: a multiple of 16 */
+    int32_t kv_heads, dim, vdim; /* dim, vdim <= 256 */
+    int32_t* err;                /* device word, set where a block table names a page outside the cache (1) or the arrays of a batch do not fit
+                                    what it says of itself (2) */
+} SmolLmCache8;
+
+/* Rows seq_start[s] .. seq_start[s + 1] - 1 are the positions seq_pos0[s], + 1, ... of sequence s; rows outside every sequence are left alone.
+ * max_new: most rows of a sequence; max_len: most positions of a sequence, these rows included (attention only: sizes its grid; longer ones are
+ * attended to as a whole all the same). */
+typedef struct SmolLmCache8Batch {
+    int32_t n_tokens, n_seqs, max_pages, max_new, max_len;
+    const int32_t *seq_start, *seq_pos0, *block_table;      /* device: [n_seqs + 1], [n_seqs], [n_seqs][max_pages] */
+    const int32_t* kv_len;       /* attention, device [n_seqs]: keys at and behind kv_len[s] are hidden, whatever the rows' positions (NULL: none) */
+} SmolLmCache8Batch;
+
+/* Appends the rows' keys and values, and writes the queries where they are wanted.  Keys and queries are rotated on their leading rot_dims
+ * coordinates (rot_half 1: coordinate i with i + rot_dims / 2, 0: 2i with 2i + 1) by position * freq[i], the angle in 64 bits; rot_mult multiplies cosine
+ * and sine.  Magnitudes above 2^100 are clamped, a NaN stays one.  A block's scale is the smallest power of two with |value| <= 448 scale for the
+ * new rows; where an earlier call began the block it never shrinks, and the codes already there follow it when it grows.  No page may be
+ * written by two sequences of one batch.  Strides in elements. */
+typedef struct SmolLmCache8Append {
+    int32_t dtype;               /* SMOL_LM_BF16 / SMOL_LM_F32: of keys, values and queries */
+    const void *k, *v;           /* [n_tokens][kv_heads][dim], [n_tokens][kv_heads][vdim] */
+    size_t k_row, k_head, v_row, v_head;
+    int32_t heads;
+    const void* q;               /* [n_tokens][heads][dim] (NULL: none) */
+    void* q_out;                 /* [n_tokens][heads][dim], no part of q (NULL where q is) */
+    size_t q_row, q_head, q_out_row, q_out_head;
+    int32_t rot_dims, rot_half;
+    const float* freq;           /* device [rot_dims / 2] */
+    float rot_mult;
+} SmolLmCache8Append;
+
+/* Softmax attention of the rows over the cache.  A row at position i sees the keys j <= i with window == 0 or i - j < window or j < first;
+ * s = scale q.k, bent to softcap tanh(s / softcap) where softcap > 0, less dist_r1 ln(1 + dist_r2 (i - j)), less dist_slope (i - j); the sink logit
+ * joins the denominator.  A row that sees no key gives zeros.  The result times out_scale, and times sigmoid(gate). */
+typedef struct SmolLmCache8Attend {
+    int32_t dtype;               /* of queries and results */
+    int32_t heads;               /* a multiple of kv_heads */
+    const void* q;               /* [n_tokens][heads][dim] */
+    void* out;                   /* [n_tokens][heads][vdim] */
+    size_t q_row, q_head, out_row, out_head;
+    float scale, softcap, out_scale;
+    int32_t window, first;
+    const float *sink, *dist_slope, *dist_r1, *dist_r2;     /* device [heads], each NULL: none */
+    const float* gate;           /* device, row t at gate + t * gate_row: [heads * vdim] (NULL: none) */
+    size_t gate_row;
+} SmolLmCache8Attend;
+
+int smol_lm_cache8_append(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Append* a, void* stream);
+/* bytes of workspace the call below needs on the current device (often 0) */
+int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, size_t* bytes);
+int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, void* workspace, size_t workspace_bytes, void* stream);
 
 int64_t smol_lm_launch_count(const SmolLm* m);
 int32_t* smol_lm_error_word(SmolLm* m);           /* device word, nonzero after a step that addressed outside its pools */

@@ -11,7 +11,7 @@ import os
 from . import build as _build
 from ._errors import SMOL_OK, SmolError
 
-SMOL_LM_ABI_VERSION = 6
+SMOL_LM_ABI_VERSION = 7
 SMOL_LM_BF16, SMOL_LM_F32 = 0, 1
 
 
@@ -62,6 +62,30 @@ class SmolLmStep(C.Structure):
                                   "logits", "trace")]
 
 
+class SmolLmCache8(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, C.c_size_t) for n in ("k_page", "v_page", "k_scale_page", "v_scale_page")] + [
+        (n, C.c_int32) for n in ("n_pages", "page_size", "kv_heads", "dim", "vdim")] + [("err", C.c_void_p)]
+
+
+class SmolLmCache8Batch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_tokens", "n_seqs", "max_pages", "max_new", "max_len")] + [
+        (n, C.c_void_p) for n in ("seq_start", "seq_pos0", "block_table", "kv_len")]
+
+
+class SmolLmCache8Append(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_size_t) for n in ("k_row", "k_head", "v_row", "v_head")] + [
+        ("heads", C.c_int32), ("q", C.c_void_p), ("q_out", C.c_void_p)] + [(n, C.c_size_t) for n in ("q_row", "q_head", "q_out_row", "q_out_head")] + [
+        ("rot_dims", C.c_int32), ("rot_half", C.c_int32), ("freq", C.c_void_p), ("rot_mult", C.c_float)]
+
+
+class SmolLmCache8Attend(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("q", C.c_void_p), ("out", C.c_void_p)] + [
+        (n, C.c_size_t) for n in ("q_row", "q_head", "out_row", "out_head")] + [(n, C.c_float) for n in ("scale", "softcap", "out_scale")] + [
+        ("window", C.c_int32), ("first", C.c_int32)] + [(n, C.c_void_p) for n in ("sink", "dist_slope", "dist_r1", "dist_r2", "gate")] + [
+        ("gate_row", C.c_size_t)]
+
+
 PROTOTYPES = {
     "smol_lm_abi_version": (C.c_int, []),
     "smol_lm_struct_bytes": (C.c_size_t, [C.c_int]),
@@ -76,6 +100,11 @@ PROTOTYPES = {
     "smol_lm_sample": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_float, C.c_int32, C.c_float, C.c_float, C.c_uint64,
                                  C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "smol_lm_linear": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_void_p]),
+    "smol_lm_cache8_append": (C.c_int, [C.POINTER(SmolLmCache8), C.POINTER(SmolLmCache8Batch), C.POINTER(SmolLmCache8Append), C.c_void_p]),
+    "smol_lm_cache8_workspace_bytes": (C.c_int, [C.POINTER(SmolLmCache8), C.POINTER(SmolLmCache8Batch), C.POINTER(SmolLmCache8Attend),
+                                                 C.POINTER(C.c_size_t)]),
+    "smol_lm_cache8_attend": (C.c_int, [C.POINTER(SmolLmCache8), C.POINTER(SmolLmCache8Batch), C.POINTER(SmolLmCache8Attend), C.c_void_p,
+                                        C.c_size_t, C.c_void_p]),
     "smol_lm_launch_count": (C.c_int64, [C.c_void_p]),
     "smol_lm_error_word": (C.c_void_p, [C.c_void_p]),
 }
@@ -100,7 +129,7 @@ def load() -> C.CDLL:
         fn.argtypes = args
     if lib.smol_lm_abi_version() != SMOL_LM_ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {lib.smol_lm_abi_version()} != {SMOL_LM_ABI_VERSION}")
-    for which, mirror in enumerate((SmolLmLayer, SmolLmConfig, SmolLmGlobals, SmolLmStep)):
+    for which, mirror in enumerate((SmolLmLayer, SmolLmConfig, SmolLmGlobals, SmolLmStep, SmolLmCache8, SmolLmCache8Batch, SmolLmCache8Append, SmolLmCache8Attend)):
         if lib.smol_lm_struct_bytes(which) != C.sizeof(mirror):
             raise RuntimeError(f"{path}: {mirror.__name__} is {lib.smol_lm_struct_bytes(which)} bytes in the library, {C.sizeof(mirror)} in the binding")
     _lib = lib

@@ -1,0 +1,220 @@
+// The 8-bit key/value cache: launches and the C entries of include/smoltts_b200_lm.h.
+#include <algorithm>
+#include <atomic>
+#include <utility>
+
+#include "../../include/smoltts_b200_lm.h"
+#include "cache8.cuh"
+#include "cache8_append.cuh"
+#include "cache8_rows.cuh"
+#include "lm_report.h"
+
+#define SMOL_OK 0
+#define SMOL_ERR_INVALID (-1)
+#define SMOL_ERR_CUDA (-3)
+#define SMOL_ERR_UNSUPPORTED (-4)
+#define SMOL_ERR_CAPACITY (-5)
+
+namespace smol {
+namespace c8 {
+
+using lm::report;
+
+// Every kernel here begins with the wait for the kernel in front of it, so all of them may be set up early.
+template <class... P, class... X>
+static cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, X&&... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<X>(args))...);
+}
+
+// Shared memory above 48 KB is asked for once per kernel and device.
+template <class K>
+static cudaError_t more_smem(K kernel, int bytes, std::atomic<uint64_t>& asked) {
+    if (bytes <= 48 * 1024) return cudaSuccess;
+    int dev = 0;
+    if (cudaError_t e = cudaGetDevice(&dev)) return e;
+    if (dev < 64 && (asked.load() >> dev & 1)) return cudaSuccess;
+    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    if (dev < 64) asked.fetch_or(1ull << dev);
+    return cudaSuccess;
+}
+
+template <class T>
+static cudaError_t append_as(const AppendArgs& A, int n_sms, cudaStream_t st) {
+    const int blocks = (A.b.max_new + 2 * kBlock - 2) / kBlock, units = 2 * A.c.G + A.H, warps = kAppendThreads / 32;
+    // a block of threads per 16 positions while that fills the SMs a few times; its heads are shared out over several where it does not
+    const int most = (units + warps - 1) / warps, z = std::min<long long>(most, std::max<long long>(1, (4ll * n_sms + (long long)blocks * A.b.S - 1) / ((long long)blocks * A.b.S)));
+    const dim3 grid(blocks, A.b.S, z);
+    if (std::max(A.c.ldk, A.c.ldv) <= 128) return launch(append_kernel<T, 1>, grid, kAppendThreads, 0, st, A);
+    return launch(append_kernel<T, 2>, grid, kAppendThreads, 0, st, A);
+}
+cudaError_t append(const AppendArgs& A, bool f32, int n_sms, cudaStream_t st) { return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st); }
+
+int splits_for(const AttendArgs& A, bool f32, int n_sms) {
+    const int Gq = A.H / A.c.G;
+    const long long base = (long long)A.b.S * A.c.G * ((A.b.max_new * (long long)Gq + kRowTile - 1) / kRowTile);
+    long long keys = A.b.max_len;
+    if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
+    const long long blocks = (keys + kBlock - 1) / kBlock;
+    const long long want = std::min((4ll * n_sms + base - 1) / base, (blocks + 4 * kRowWarps - 1) / (4 * kRowWarps));
+    return (int)std::max(1ll, std::min(want, 128ll));
+}
+
+template <class T, int D, bool BENT>
+static cudaError_t rows_as(const AttendArgs& A, cudaStream_t st) {
+    static std::atomic<uint64_t> asked{0};
+    constexpr int bytes = row_smem(D, D, sizeof(T) == 4 ? 2 : 1);
+    if (cudaError_t e = more_smem(attend_rows_kernel<T, D, D, BENT>, bytes, asked)) return e;
+    const int tiles = (A.b.max_new * (A.H / A.c.G) + kRowTile - 1) / kRowTile;
+    return launch(attend_rows_kernel<T, D, D, BENT>, dim3(tiles * A.n_splits, A.c.G, A.b.S), kRowThreads, bytes, st, A);
+}
+template <class T, int D>
+static cudaError_t rows_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? rows_as<T, D, false>(A, st) : rows_as<T, D, true>(A, st); }
+template <class T>
+static cudaError_t attend_rows(const AttendArgs& A, int* launches, cudaStream_t st) {
+    const int d = std::max(A.c.d, A.c.dv);
+    if (cudaError_t e = d <= 64 ? rows_of<T, 64>(A, st) : d <= 128 ? rows_of<T, 128>(A, st) : rows_of<T, 256>(A, st)) return e;
+    *launches += 1;
+    if (A.n_splits == 1) return cudaSuccess;
+    *launches += 1;
+    return launch(attend_join_kernel<T>, (int)(((long long)A.b.T * A.H + 3) / 4), 128, 0, st, A);
+}
+
+bool tiles_serve(const AttendArgs& A, bool f32) { return false; }
+cudaError_t attend(const AttendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st) {
+    return f32 ? attend_rows<float>(A, launches, st) : attend_rows<bf16>(A, launches, st);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+
+static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+static int n_sms_of_device(int* n) {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev < 64 && known[dev].load() > 0) { *n = known[dev].load(); return SMOL_OK; }
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return report(SMOL_ERR_CUDA, "8-bit cache", cudaGetErrorString(e));
+    if (dev < 64) known[dev].store(*n);
+    return SMOL_OK;
+}
+
+static int cache_of(const SmolLmCache8* s, Cache& c, const char* me) {
+    if (!s->k || !s->v || !s->k_scale || !s->v_scale || !s->err) return report(SMOL_ERR_INVALID, me, "null pointer in the cache");
+    if (s->n_pages < 1 || s->page_size < kBlock || s->page_size % kBlock) return report(SMOL_ERR_INVALID, me, "page_size must be a multiple of 16, with at least one page");
+    if (s->kv_heads < 1 || s->dim < 1 || s->vdim < 1) return report(SMOL_ERR_INVALID, me, "kv_heads, dim and vdim must be positive");
+    if (s->dim > kMaxDim || s->vdim > kMaxDim) return report(SMOL_ERR_UNSUPPORTED, me, "head sizes above 256");
+    if (s->kv_heads > 65535) return report(SMOL_ERR_UNSUPPORTED, me, "more than 65535 key/value heads");
+    c.ldk = (s->dim + 15) / 16 * 16;
+    c.ldv = (s->vdim + 15) / 16 * 16;
+    const size_t scales = (size_t)s->kv_heads * (s->page_size / kBlock);
+    c.k_page = s->k_page ? s->k_page : (size_t)s->kv_heads * s->page_size * c.ldk;
+    c.v_page = s->v_page ? s->v_page : (size_t)s->kv_heads * s->page_size * c.ldv;
+    c.ks_page = s->k_scale_page ? s->k_scale_page : scales;
+    c.vs_page = s->v_scale_page ? s->v_scale_page : scales;
+    if (!aligned(s->k, 16) || !aligned(s->v, 16) || c.k_page % 16 || c.v_page % 16 || !aligned(s->k_scale, 4) || !aligned(s->v_scale, 4))
+        return report(SMOL_ERR_INVALID, me, "codes must lie on 16-byte boundaries, page by page");
+    c.k = static_cast<uint8_t*>(s->k); c.v = static_cast<uint8_t*>(s->v); c.ks = s->k_scale; c.vs = s->v_scale;
+    c.n_pages = s->n_pages; c.page = s->page_size; c.G = s->kv_heads; c.d = s->dim; c.dv = s->vdim; c.err = s->err;
+    return SMOL_OK;
+}
+static int batch_of(const SmolLmCache8Batch* s, Batch& b, const char* me) {
+    if (!s->seq_start || !s->seq_pos0 || !s->block_table) return report(SMOL_ERR_INVALID, me, "null array");
+    if (s->n_seqs < 1 || s->n_tokens < 1 || s->max_pages < 1 || s->max_new < 1 || s->max_len < 1) return report(SMOL_ERR_INVALID, me, "n_seqs, n_tokens, max_pages, max_new and max_len must be positive");
+    if (s->n_seqs > 65535) return report(SMOL_ERR_CAPACITY, me, "more than 65535 sequences");
+    if (s->max_new > (1 << 24)) return report(SMOL_ERR_CAPACITY, me, "max_new above 2^24");
+    b.start = s->seq_start; b.pos0 = s->seq_pos0; b.table = s->block_table; b.kv_len = s->kv_len;
+    b.S = s->n_seqs; b.T = s->n_tokens; b.max_pages = s->max_pages; b.max_new = std::min(s->max_new, s->n_tokens); b.max_len = s->max_len;
+    return SMOL_OK;
+}
+// whether rows of n elements are whole, aligned groups of four
+static bool whole_fours(const void* p, size_t row, size_t head, int n, bool f32) { return n % 4 == 0 && row % 4 == 0 && head % 4 == 0 && aligned(p, f32 ? 16 : 8); }
+
+static int attend_of(const SmolLmCache8* c, const SmolLmCache8Batch* b, const SmolLmCache8Attend* a, AttendArgs& A, bool pointers) {
+    const char* me = "smol_lm_cache8_attend";
+    if (!c || !b || !a) return report(SMOL_ERR_INVALID, me, "null argument");
+    if (int rc = cache_of(c, A.c, me)) return rc;
+    if (int rc = batch_of(b, A.b, me)) return rc;
+    if (a->dtype != SMOL_LM_BF16 && a->dtype != SMOL_LM_F32) return report(SMOL_ERR_INVALID, me, "dtype must be 0 (bf16) or 1 (f32)");
+    if (a->heads < 1 || a->heads % A.c.G) return report(SMOL_ERR_INVALID, me, "heads must be a multiple of kv_heads");
+    if ((long long)A.b.max_new * (a->heads / A.c.G) > (1ll << 30) || (long long)A.b.T * a->heads > (1ll << 31) - 64)
+        return report(SMOL_ERR_CAPACITY, me, "more query rows than 32 bits count");
+    if (a->window < 0 || a->first < 0 || !(a->softcap >= 0.0f)) return report(SMOL_ERR_INVALID, me, "window, first and softcap must not be negative");
+    if (!a->dist_r1 != !a->dist_r2) return report(SMOL_ERR_INVALID, me, "dist_r1 and dist_r2 come together");
+    if (pointers && (!a->q || !a->out)) return report(SMOL_ERR_INVALID, me, "null queries or results");
+    const bool f32 = a->dtype == SMOL_LM_F32;
+    A.q = a->q; A.out = a->out; A.q_row = a->q_row; A.q_head = a->q_head; A.o_row = a->out_row; A.o_head = a->out_head;
+    A.H = a->heads; A.window = a->window; A.first = a->first; A.scale = a->scale; A.softcap = a->softcap;
+    A.sink = a->sink; A.slope = a->dist_slope; A.r1 = a->dist_r1; A.r2 = a->dist_r2; A.gate = a->gate; A.gate_row = a->gate_row; A.out_scale = a->out_scale;
+    A.part = nullptr; A.n_splits = 1;
+    A.q_vec = whole_fours(a->q, a->q_row, a->q_head, A.c.d, f32);
+    A.o_vec = whole_fours(a->out, a->out_row, a->out_head, A.c.dv, f32);
+    return SMOL_OK;
+}
+
+}  // namespace c8
+}  // namespace smol
+
+using namespace smol::c8;
+using smol::lm::report;
+
+extern "C" int smol_lm_cache8_append(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Append* a, void* stream) {
+    const char* me = "smol_lm_cache8_append";
+    if (!cache || !batch || !a) return report(SMOL_ERR_INVALID, me, "null argument");
+    AppendArgs A{};
+    if (int rc = cache_of(cache, A.c, me)) return rc;
+    if (int rc = batch_of(batch, A.b, me)) return rc;
+    if (a->dtype != SMOL_LM_BF16 && a->dtype != SMOL_LM_F32) return report(SMOL_ERR_INVALID, me, "dtype must be 0 (bf16) or 1 (f32)");
+    if (!a->k || !a->v || !a->q != !a->q_out || (a->q && a->heads < 1)) return report(SMOL_ERR_INVALID, me, "null keys or values, or queries without heads or a place to go");
+    if (a->rot_dims < 0 || a->rot_dims % 2 || a->rot_dims > A.c.d || (a->rot_dims > 0 && !a->freq)) return report(SMOL_ERR_INVALID, me, "rot_dims must be even and at most dim, with frequencies");
+    const bool f32 = a->dtype == SMOL_LM_F32;
+    A.k = a->k; A.v = a->v; A.q = a->q; A.q_out = a->q_out;
+    A.k_row = a->k_row; A.k_head = a->k_head; A.v_row = a->v_row; A.v_head = a->v_head;
+    A.q_row = a->q_row; A.q_head = a->q_head; A.o_row = a->q_out_row; A.o_head = a->q_out_head;
+    A.H = a->q ? a->heads : 0; A.freq = a->freq; A.pairs = a->rot_dims / 2; A.half = a->rot_half; A.mult = a->rot_mult;
+    A.k_vec = whole_fours(a->k, a->k_row, a->k_head, A.c.d, f32);
+    A.v_vec = whole_fours(a->v, a->v_row, a->v_head, A.c.dv, f32);
+    A.q_vec = A.H == 0 || (whole_fours(a->q, a->q_row, a->q_head, A.c.d, f32) && whole_fours(a->q_out, a->q_out_row, a->q_out_head, A.c.d, f32));
+    int n_sms = 0;
+    if (int rc = n_sms_of_device(&n_sms)) return rc;
+    const cudaError_t e = append(A, f32, n_sms, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SMOL_OK : report(SMOL_ERR_CUDA, me, cudaGetErrorString(e));
+}
+
+extern "C" int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, size_t* bytes) {
+    if (!bytes) return report(SMOL_ERR_INVALID, "smol_lm_cache8_workspace_bytes", "null argument");
+    AttendArgs A{};
+    if (int rc = attend_of(cache, batch, a, A, false)) return rc;
+    int n_sms = 0;
+    if (int rc = n_sms_of_device(&n_sms)) return rc;
+    const bool f32 = a->dtype == SMOL_LM_F32;
+    const int splits = tiles_serve(A, f32) ? 1 : splits_for(A, f32, n_sms);
+    *bytes = splits == 1 ? 0 : (size_t)A.b.T * A.H * splits * (A.c.dv + 2) * sizeof(float);
+    return SMOL_OK;
+}
+
+extern "C" int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, void* workspace, size_t workspace_bytes, void* stream) {
+    AttendArgs A{};
+    if (int rc = attend_of(cache, batch, a, A, true)) return rc;
+    int n_sms = 0, launches = 0;
+    if (int rc = n_sms_of_device(&n_sms)) return rc;
+    const bool f32 = a->dtype == SMOL_LM_F32;
+    if (!tiles_serve(A, f32)) {
+        A.n_splits = splits_for(A, f32, n_sms);
+        if (A.n_splits > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < (size_t)A.b.T * A.H * A.n_splits * (A.c.dv + 2) * sizeof(float)))
+            return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
+        A.part = static_cast<float*>(workspace);
+    }
+    const cudaError_t e = attend(A, f32, n_sms, &launches, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? SMOL_OK : report(SMOL_ERR_CUDA, "smol_lm_cache8_attend", cudaGetErrorString(e));
+}

@@ -1,0 +1,527 @@
+// Attention over the 8-bit key/value cache for few query rows per sequence (decoding, short portions), and for every size and type the tiles
+// of cache8_tiles.cuh do not serve.  Included by cache8.cu.
+//
+// One block per (16 query rows of a sequence and key/value head, key/value head, sequence, share of the keys): the rows are the step's tokens
+// times the query heads that share the key/value head, so that a cached row is read once for all of them.  Its four warps take the share's
+// blocks of 16 positions in turn, each with a running softmax of its own, and are joined at the end.
+//
+// Keys and values go from global memory through a ring in shared memory into mma.sync fragments without changing hands: every lane copies
+// (cp.async) exactly the 16 bytes that it multiplies later, so that no barrier stands between a copy and its use.  That is possible because the
+// order of a product's terms is free -- lane c of four takes bytes 16 c .. + 15 of a key row, which is four steps of four coordinates, and the
+// query fragments are laid out to match; for the values a lane holds the same DV / 8 columns of four positions, and the column index of the
+// product's eight columns is the lane's group.  Codes become f16 by moving bits (cache8.cuh); queries are scaled to below 2^15 per row and
+// enter as one f16 part (bf16 queries: exact) or two (float32), weights likewise, as 2^8 exp2(s - m) times the block's value scale over the
+// largest one so far.  Scores, maxima, denominators and results are fp32.
+//
+// What bounds it: the bytes of the cache, as long as enough of them are under way.
+#pragma once
+
+#include "cache8.cuh"
+
+namespace smol {
+namespace c8 {
+
+constexpr int kRowWarps = 4, kRowTile = 16, kRowThreads = kRowWarps * 32;
+
+__host__ __device__ constexpr int row_stage_bytes(int DK, int DV) { return kBlock * (DK + DV); }
+__host__ __device__ constexpr int row_stages(int DK, int DV) { return DK + DV <= 256 ? 4 : 3; }
+__host__ __device__ constexpr bool q_in_smem(int DK, int PARTS) { return DK * PARTS > 128; }
+__host__ __device__ constexpr int row_q_bytes(int DK, int PARTS) { return q_in_smem(DK, PARTS) ? DK / 16 * PARTS * 512 : 0; }
+__host__ __device__ constexpr int row_join_bytes(int DV) { return kRowWarps * kRowTile * (DV + 4) * 4; }
+__host__ __device__ constexpr int row_smem(int DK, int DV, int PARTS) {
+    const int ring = kRowWarps * row_stages(DK, DV) * row_stage_bytes(DK, DV) + row_q_bytes(DK, PARTS), join = row_join_bytes(DV);
+    return ring > join ? ring : join;
+}
+
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool in) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t to, const void* from, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(in ? 8 : 0) : "memory");
+}
+template <int N> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// The blocks of 16 positions that rows at positions first_pos .. last_pos see: `lead` of them from the sequence's start (the first tokens, in
+// front of the window), then those from `from` up to the last visible key.
+struct Seen {
+    int lead, from, count, end;      // end: one behind the last visible key
+};
+__device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
+    Seen x;
+    x.end = max(min(kv_len, last_pos + 1), 0);
+    const int blocks = (x.end + kBlock - 1) / kBlock;
+    x.from = A.window > 0 ? min(max(first_pos - A.window + 1, 0) / kBlock, blocks) : 0;
+    x.lead = A.window > 0 ? min((A.first + kBlock - 1) / kBlock, x.from) : 0;
+    x.count = x.lead + blocks - x.from;
+    return x;
+}
+__device__ __forceinline__ bool sees(const AttendArgs& A, int pos, int j, int end) {
+    return j <= pos && j < end && (A.window == 0 || pos - j < A.window || j < A.first);
+}
+
+// What follows the scaled product, in units of log2: soft cap and distance penalties.  EXACT: the library's functions (float32).
+template <bool EXACT>
+__device__ __forceinline__ float bent_score(const AttendArgs& A, float s, int dist, float r1, float r2, float slope) {
+    if (A.softcap > 0.0f) {
+        if (EXACT) s = A.softcap * tanhf(s / A.softcap);
+        else s = A.softcap * (1.0f - __fdividef(2.0f, exp2_fast(2.0f * kLog2e * s / A.softcap) + 1.0f));
+    }
+    const float d = (float)max(dist, 0);
+    if (A.r1) s -= EXACT ? r1 * log1pf(r2 * d) : r1 * 0.69314718f * log2_fast(fmaf(r2, d, 1.0f));
+    return (s - slope * d) * kLog2e;
+}
+
+template <class T> struct Elem;
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float get(const float* p) { return *p; }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
+template <> struct Elem<bf16> {
+    static __device__ __forceinline__ float get(const bf16* p) { return __bfloat162float(*p); }
+    static __device__ __forceinline__ void put(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
+};
+
+__device__ __forceinline__ float finished(const AttendArgs& A, int t, int h, int c, float v) {
+    v *= A.out_scale;
+    if (A.gate) v /= 1.0f + expf(-A.gate[(size_t)t * A.gate_row + (size_t)h * A.c.dv + c]);
+    return v;
+}
+
+// Blocks of scale sign < 0 hold NaN codes, which the products took for 480: a row that sees one of them becomes NaN, all of it where a key holds
+// one, the value's column otherwise (mark(row, column)).  Rare, and slow.
+template <class Mark>
+__device__ void mark_nans(const AttendArgs& A, int s, int g, int t0, int row0, int rows, int pos0, int Gq, int kv_len, Mark mark) {
+    for (int r = 0; r < rows; ++r) {
+        const int pos = pos0 + (row0 + r) / Gq, end = min(kv_len, pos + 1);
+        for (int b = 0; b * kBlock < end; ++b) {
+            const int pg = b * kBlock / A.c.page;
+            const int page = pg < A.b.max_pages ? A.b.table[(size_t)s * A.b.max_pages + pg] : -1;
+            if (page < 0 || page >= A.c.n_pages) continue;
+            const int in_page = b * kBlock - pg * A.c.page, at = g * (A.c.page / kBlock) + in_page / kBlock;
+            const bool kbad = A.c.ks[(size_t)page * A.c.ks_page + at] < 0.0f, vbad = A.c.vs[(size_t)page * A.c.vs_page + at] < 0.0f;
+            if (!kbad && !vbad) continue;
+            for (int i = 0; i < kBlock; ++i) {
+                if (!sees(A, pos, b * kBlock + i, kv_len)) continue;
+                const size_t row = (size_t)g * A.c.page + in_page + i;
+                const uint8_t *k = A.c.k + (size_t)page * A.c.k_page + row * A.c.ldk, *v = A.c.v + (size_t)page * A.c.v_page + row * A.c.ldv;
+                if (kbad)
+                    for (int c = threadIdx.x; c < A.c.d; c += blockDim.x)
+                        if ((k[c] & 0x7f) == 0x7f)
+                            for (int o = 0; o < A.c.dv; ++o) mark(r, o);
+                if (vbad)
+                    for (int c = threadIdx.x; c < A.c.dv; c += blockDim.x)
+                        if ((v[c] & 0x7f) == 0x7f) mark(r, c);
+            }
+        }
+    }
+}
+
+// T: type of queries and results; PARTS: f16 parts of a query and of a weight; DK, DV: head sizes padded; BENT: soft cap or distance penalties
+template <class T, int DK, int DV, bool BENT>
+__global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs A) {
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
+    constexpr bool QS = q_in_smem(DK, PARTS);
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float s_max[kRowWarps][kRowTile], s_sum[kRowWarps][kRowTile], s_weight[kRowWarps][kRowTile], s_top[kRowTile], s_total[kRowTile];
+    __shared__ int s_bad;
+    dep_wait();
+    dep_go();
+    const int s = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / A.n_splits, split = blockIdx.x % A.n_splits;
+    const int t0 = A.b.start[s], n_all = A.b.start[s + 1] - t0, n = min(n_all, A.b.max_new), pos0 = A.b.pos0[s];
+    const int Gq = A.H / A.c.G, row0 = tile * kRowTile, rows = min(n * Gq - row0, kRowTile);
+    if (rows <= 0 || t0 < 0 || t0 + n_all > A.b.T) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
+    const int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq;
+    const Seen seen = seen_blocks(A, first_pos, last_pos, kv_len);
+    const int share = (seen.count + A.n_splits - 1) / A.n_splits, b_lo = min(split * share, seen.count), b_hi = min(b_lo + share, seen.count);
+    const int mine = b_hi - b_lo > warp ? (b_hi - b_lo - warp + kRowWarps - 1) / kRowWarps : 0;      // blocks of this warp: b_lo + warp, + 4, ...
+    if (threadIdx.x == 0) s_bad = 0;
+
+    // where the warp's blocks are: lane i knows block number i of 32 (`now`), and of the 32 that follow
+    struct Place { int page, in_page; float ks, vs; };
+    auto block_of = [&](int i) { const int x = b_lo + warp + i * kRowWarps; return x < seen.lead ? x : seen.from + x - seen.lead; };
+    auto look_up = [&](int i0) {
+        Place p;
+        p.page = -1; p.in_page = 0; p.ks = 0.0f; p.vs = 0.0f;
+        if (i0 + lane < mine) {
+            const int j = block_of(i0 + lane) * kBlock, pg = j / A.c.page;
+            p.page = pg < A.b.max_pages ? A.b.table[(size_t)s * A.b.max_pages + pg] : -1;
+            p.in_page = j - pg * A.c.page;
+            if (p.page < 0 || p.page >= A.c.n_pages) {
+                p.page = -1;
+                atomicExch(A.c.err, 1);
+            } else {
+                const int at = g * (A.c.page / kBlock) + p.in_page / kBlock;
+                p.ks = A.c.ks[(size_t)p.page * A.c.ks_page + at];
+                p.vs = A.c.vs[(size_t)p.page * A.c.vs_page + at];
+            }
+        }
+        return p;
+    };
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (NS * SB) + lane * 16;
+    // a block's copies: pieces KP per key row (two rows a lane), then the lane's columns of four value rows
+    auto copy_block = [&](int i, const Place& p) {
+        const int page = __shfl_sync(0xffffffffu, p.page, i & 31), in_page = __shfl_sync(0xffffffffu, p.in_page, i & 31);
+        const bool live = i < mine && page >= 0;
+        const uint32_t to = ring + (i % NS) * SB;
+        const uint8_t* k = A.c.k + (size_t)max(page, 0) * A.c.k_page + ((size_t)g * A.c.page + in_page) * A.c.ldk;
+        const uint8_t* v = A.c.v + (size_t)max(page, 0) * A.c.v_page + ((size_t)g * A.c.page + in_page) * A.c.ldv;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < KP; ++y) {
+                const int at = (c + 4 * y) * 16;
+                const bool in = live && at < A.c.ldk;
+                copy16(to + (x * KP + y) * 512, in ? k + (size_t)(r + 8 * x) * A.c.ldk + at : A.c.k, in);
+            }
+        // positions 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint8_t* row = v + (size_t)(2 * c + (x & 1) + 8 * (x >> 1)) * A.c.ldv;
+            if (VB == 8) {
+                const bool in = live && r * 8 < A.c.ldv;
+                copy8(to - lane * 8 + kBlock * DK + x * 256, in ? row + r * 8 : A.c.v, in);
+            } else {
+#pragma unroll
+                for (int y = 0; y < VB / 16; ++y) {
+                    const int at = r * VB + 16 * y;
+                    const bool in = live && at < A.c.ldv;
+                    copy16(to + kBlock * DK + (x * (VB / 16) + y) * 512, in ? row + at : A.c.v, in);
+                }
+            }
+        }
+        copies_end();
+    };
+    Place now = look_up(0), next = look_up(32);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) copy_block(i, now);
+
+    // ---- queries: fragments of rows r and r + 8, scaled so that the largest magnitude lies in [2^14, 2^15) ----
+    float rowmul[2];
+    uint32_t qa[QS ? 1 : KS][QS ? 1 : PARTS][4];
+    uint4* qs = reinterpret_cast<uint4*>(smem + kRowWarps * NS * SB);
+    {
+        const T* q[2];
+        float up[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int row = min(row0 + r + 8 * x, n * Gq - 1);
+            q[x] = static_cast<const T*>(A.q) + (size_t)(t0 + row / Gq) * A.q_row + (size_t)(g * Gq + row % Gq) * A.q_head;
+            uint32_t top = 0;
+            for (int k = c; k < A.c.d; k += 4) top = max(top, __float_as_uint(fabsf(Elem<T>::get(q[x] + k))));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // (2^(14 - e) for a largest magnitude of m 2^e: within fp32 for e from -110 to 127; smaller rows are scaled by 2^124)
+            const int e = max((int)(top >> 23) - 127, -110);
+            up[x] = pow2(14 - e);
+            rowmul[x] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 14) * (A.scale * kCodeUnit * (BENT ? 1.0f : kLog2e));
+        }
+        auto fragment = [&](int k, uint32_t (&part)[PARTS][4]) {
+            // step k: word k % 4 of the lane's piece c + 4 (k / 4); its bytes 1 and 3, then 0 and 2
+            const int at = ((k / 4) * 4 + c) * 16 + (k % 4) * 4;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = at + e < A.c.d ? Elem<T>::get(q[x] + at + e) * up[x] : 0.0f;
+                const uint32_t odd = pack_f16(v[1], v[3]), even = pack_f16(v[0], v[2]);
+                part[0][x] = odd;
+                part[0][2 + x] = even;
+                if (PARTS == 2) {
+                    const float2 o = unpack_f16(odd), z = unpack_f16(even);
+                    part[PARTS - 1][x] = pack_f16(v[1] - o.x, v[3] - o.y);
+                    part[PARTS - 1][2 + x] = pack_f16(v[0] - z.x, v[2] - z.y);
+                }
+            }
+        };
+        if constexpr (QS) {
+            for (int k = warp; k < KS; k += kRowWarps) {
+                uint32_t part[PARTS][4];
+                fragment(k, part);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) qs[(k * PARTS + p) * 32 + lane] = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < KS; ++k) fragment(k, qa[k]);
+        }
+    }
+    __syncthreads();
+
+    float r1[2], r2[2], slope[2];
+    int pos[2];
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int row = min(row0 + r + 8 * x, n * Gq - 1), h = g * Gq + row % Gq;
+        pos[x] = pos0 + row / Gq;
+        r1[x] = BENT && A.r1 ? A.r1[h] : 0.0f;
+        r2[x] = BENT && A.r1 ? A.r2[h] : 0.0f;
+        slope[x] = BENT && A.slope ? A.slope[h] : 0.0f;
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, unit = 0.0f;      // unit: the largest value scale so far, what o is in units of
+    float o[VB][4];
+#pragma unroll
+    for (int t = 0; t < VB; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[t][e] = 0.0f;
+    bool bad = false;
+
+    for (int i = 0; i < mine; ++i) {
+        if (i > 0 && (i & 31) == 0) {
+            now = next;
+            next = look_up(i + 32);
+        }
+        {
+            const int ahead = i + NS - 1;
+            copy_block(ahead, (ahead & ~31) == (i & ~31) ? now : next);
+        }
+        const int page = __shfl_sync(0xffffffffu, now.page, i & 31);
+        const float ks = __shfl_sync(0xffffffffu, now.ks, i & 31), vs = __shfl_sync(0xffffffffu, now.vs, i & 31);
+        copies_left<NS - 1>();
+        if (page < 0) continue;
+        bad |= ks < 0.0f || vs < 0.0f;
+        const unsigned char* st = smem + warp * (NS * SB) + (i % NS) * SB;
+        // ---- scores of 16 rows and 16 positions ----
+        float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+        for (int y = 0; y < KP; ++y) {
+            uint4 w[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) w[x] = *reinterpret_cast<const uint4*>(st + (x * KP + y) * 512 + lane * 16);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                uint32_t a[PARTS][4];
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    if constexpr (QS) {
+                        const uint4 u = qs[((y * 4 + z) * PARTS + p) * 32 + lane];
+                        a[p][0] = u.x; a[p][1] = u.y; a[p][2] = u.z; a[p][3] = u.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) a[p][e] = qa[y * 4 + z][p][e];
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint32_t word = z == 0 ? w[x].x : z == 1 ? w[x].y : z == 2 ? w[x].z : w[x].w;
+                    const uint32_t b0 = odd_codes(word), b1 = even_codes(word);
+#pragma unroll
+                    for (int p = 0; p < PARTS; ++p) mma_f16_16816(sc[x], a[p][0], a[p][1], a[p][2], a[p][3], b0, b1);
+                }
+            }
+        }
+        // ---- running softmax, in units of log2; a lane has positions 2c, 2c + 1, 2c + 8, 2c + 9 of rows r and r + 8 ----
+        const int j0 = block_of(i) * kBlock + 2 * c;
+        const float km = fabsf(ks);
+        const bool whole = j0 - 2 * c + kBlock <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 - 2 * c > last_pos - A.window || j0 - 2 * c + kBlock <= A.first);
+        float p[2][4], top[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const float mul = rowmul[x] * km;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = j0 + (e & 1) + 8 * (e >> 1);
+                float v = sc[e >> 1][2 * x + (e & 1)] * mul;
+                if (BENT) v = bent_score<PARTS == 2>(A, v, pos[x] - j, r1[x], r2[x], slope[x]);
+                p[x][e] = whole || sees(A, pos[x], j, seen.end) ? v : -INFINITY;
+            }
+            top[x] = fmaxf(fmaxf(p[x][0], p[x][1]), fmaxf(p[x][2], p[x][3]));
+            top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
+            top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
+        }
+        const float v_unit = fmaxf(fabsf(vs), 7.5231638e-37f);      // 2^-120: below every scale
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]) || v_unit > unit) {
+            const float grown = fmaxf(unit, v_unit), down = unit / grown;      // powers of two
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float mn = fmaxf(m[x], top[x]), corr = mn == -INFINITY ? 1.0f : exp2_fast(m[x] - mn);
+                m[x] = mn;
+                l[x] *= corr;
+#pragma unroll
+                for (int t = 0; t < VB; ++t) {
+                    o[t][2 * x] *= corr * down;
+                    o[t][2 * x + 1] *= corr * down;
+                }
+            }
+            unit = grown;
+        }
+        const float vmul = kCodeUnit * (v_unit / unit);
+        uint32_t pa[PARTS][4];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const float base = m[x] == -INFINITY ? 0.0f : m[x];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[x][e] = exp2_fast(p[x][e] - base);
+            l[x] += (p[x][0] + p[x][1]) + (p[x][2] + p[x][3]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float a = p[x][2 * y] * vmul, b = p[x][2 * y + 1] * vmul;
+                pa[0][x + 2 * y] = pack_f16(a, b);
+                if (PARTS == 2) {
+                    const float2 h = unpack_f16(pa[0][x + 2 * y]);
+                    pa[PARTS - 1][x + 2 * y] = pack_f16(a - h.x, b - h.y);
+                }
+            }
+        }
+        // ---- weights x values: column of the product = lane group r', VB columns of it a lane ----
+#pragma unroll
+        for (int y = 0; y < VB / 4; y += VB == 8 ? 2 : 4) {
+            uint32_t w[4][4];      // words of the four positions' rows
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (VB == 8) {
+                    const uint2 u = *reinterpret_cast<const uint2*>(st + kBlock * DK + x * 256 + lane * 8);
+                    w[x][0] = u.x; w[x][1] = u.y; w[x][2] = 0; w[x][3] = 0;
+                } else {
+                    const uint4 u = *reinterpret_cast<const uint4*>(st + kBlock * DK + (x * (VB / 16) + y / 4) * 512 + lane * 16);
+                    w[x][0] = u.x; w[x][1] = u.y; w[x][2] = u.z; w[x][3] = u.w;
+                }
+            }
+#pragma unroll
+            for (int z = 0; z < (VB == 8 ? 2 : 4); ++z) {
+                // columns 4 z .. + 3 of positions 2c and 2c + 1, and of 2c + 8 and 2c + 9: (second, first | second, first), (fourth, third | ...)
+                const uint32_t a01 = __byte_perm(w[0][z], w[1][z], 0x4501), a23 = __byte_perm(w[0][z], w[1][z], 0x6723);
+                const uint32_t b01 = __byte_perm(w[2][z], w[3][z], 0x4501), b23 = __byte_perm(w[2][z], w[3][z], 0x6723);
+                const int t = (y + z) * 4;
+#pragma unroll
+                for (int pp = 0; pp < PARTS; ++pp) {
+                    mma_f16_16816(o[t], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], odd_codes(a01), odd_codes(b01));
+                    mma_f16_16816(o[t + 1], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], even_codes(a01), even_codes(b01));
+                    mma_f16_16816(o[t + 2], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], odd_codes(a23), odd_codes(b23));
+                    mma_f16_16816(o[t + 3], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], even_codes(a23), even_codes(b23));
+                }
+            }
+        }
+    }
+    copies_left<0>();
+    // ---- the warps' results are joined ----
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
+        l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
+        if (c == 0) {
+            s_max[warp][r + 8 * x] = m[x];
+            s_sum[warp][r + 8 * x] = l[x];
+        }
+    }
+    if (bad && lane == 0) s_bad = 1;
+    __syncthreads();      // everybody's copies are used up: the ring becomes the results' place
+    constexpr int LD = DV + 4;
+    float* join = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            float* to = join + (warp * kRowTile + r + 8 * x) * LD + (2 * c + e) * VB;
+#pragma unroll
+            for (int t = 0; t < VB; t += 4)
+                *reinterpret_cast<float4*>(to + t) = make_float4(o[t][2 * x + e] * unit, o[t + 1][2 * x + e] * unit, o[t + 2][2 * x + e] * unit, o[t + 3][2 * x + e] * unit);
+        }
+    if (threadIdx.x < kRowTile) {
+        const int row = threadIdx.x;
+        const float M = fmaxf(fmaxf(s_max[0][row], s_max[1][row]), fmaxf(s_max[2][row], s_max[3][row]));
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
+            // a row of NaN scores has no maximum: its sums say so
+            const float f = s_max[w][row] == -INFINITY ? (s_sum[w][row] == 0.0f ? 0.0f : s_sum[w][row]) : exp2_fast(s_max[w][row] - M);
+            s_weight[w][row] = f;
+            total = fmaf(s_sum[w][row], f, total);
+        }
+        s_top[row] = M;
+        s_total[row] = total;
+    }
+    __syncthreads();
+    auto joined = [&](int row, int col) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) v = fmaf(join[(w * kRowTile + row) * LD + col], s_weight[w][row], v);
+        return v;
+    };
+    if (s_bad) {
+        mark_nans(A, s, g, t0, row0, rows, pos0, Gq, min(kv_len, seen.end), [&](int row, int col) { join[row * LD + col] = __int_as_float(0x7fffffff); });      // (times whatever weight: NaN)
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < rows * A.c.dv; i += kRowThreads) {
+        const int row = i / A.c.dv, col = i - row * A.c.dv, tok = t0 + (row0 + row) / Gq, h = g * Gq + (row0 + row) % Gq;
+        const float v = joined(row, col);
+        if (A.n_splits > 1) {
+            float* to = A.part + (((size_t)tok * A.H + h) * A.n_splits + split) * (A.c.dv + 2);
+            if (col == 0) { to[0] = s_top[row]; to[1] = s_total[row]; }
+            to[2 + col] = v;
+        } else {
+            const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, s_top[row]);
+            const float f = s_top[row] == -INFINITY ? 1.0f : exp2_fast(s_top[row] - M), total = fmaf(s_total[row], f, M == -INFINITY ? 0.0f : exp2_fast(sink - M));
+            // nothing visible: no weights, and the result is zero
+            const float out = total == 0.0f ? v : v * f / total;
+            Elem<T>::put(static_cast<T*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, out));
+        }
+    }
+}
+
+// A warp per (token, head): joins the shares of the keys, and the sink.
+template <class T>
+__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs A) {
+    dep_wait();
+    dep_go();
+    const int unit = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t = unit / A.H, h = unit % A.H;
+    if (t >= A.b.T) return;
+    // rows in front of the first sequence, behind the last or behind max_new of their own are nobody's
+    int lo = 0, hi = A.b.S;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (A.b.start[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const int t0 = A.b.start[lo];
+    if (t < t0 || t >= A.b.start[lo + 1] || t0 < 0 || A.b.start[lo + 1] > A.b.T) return;
+    if (t - t0 >= A.b.max_new) return;
+    const float* p = A.part + (size_t)unit * A.n_splits * (A.c.dv + 2);
+    const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY;
+    float M = sink;
+    for (int z = lane; z < A.n_splits; z += 32) M = fmaxf(M, p[(size_t)z * (A.c.dv + 2)]);
+    M = warp_max(M);
+    float total = 0.0f, acc[kMaxDim / 32];
+#pragma unroll
+    for (int e = 0; e < kMaxDim / 32; ++e) acc[e] = 0.0f;
+    for (int z0 = 0; z0 < A.n_splits; z0 += 32) {
+        float f = 0.0f;
+        if (z0 + lane < A.n_splits) {
+            const float* q = p + (size_t)(z0 + lane) * (A.c.dv + 2);
+            // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
+            f = q[0] == -INFINITY ? (q[1] == 0.0f ? 1.0f : q[1]) : exp2_fast(q[0] - M);
+            total = fmaf(q[1], f, total);
+        }
+        const int cnt = min(32, A.n_splits - z0);
+#pragma unroll 4
+        for (int z = 0; z < cnt; ++z) {
+            const float fz = __shfl_sync(0xffffffffu, f, z);
+            const float* q = p + (size_t)(z0 + z) * (A.c.dv + 2) + 2;
+#pragma unroll
+            for (int e = 0; e < kMaxDim / 32; ++e)
+                if (lane + 32 * e < A.c.dv) acc[e] = fmaf(q[lane + 32 * e], fz, acc[e]);
+        }
+    }
+    total = warp_sum(total) + (M == -INFINITY ? 0.0f : exp2_fast(sink - M));
+#pragma unroll
+    for (int e = 0; e < kMaxDim / 32; ++e) {
+        const int col = lane + 32 * e;
+        if (col < A.c.dv)
+            Elem<T>::put(static_cast<T*>(A.out) + (size_t)t * A.o_row + (size_t)h * A.o_head + col, finished(A, t, h, col, total == 0.0f ? acc[e] : acc[e] / total));
+    }
+}
+
+}  // namespace c8
+}  // namespace smol

@@ -17,6 +17,7 @@
 #include "../../include/smoltts_b200_lm.h"
 #include "common.cuh"
 #include "f32_tile.cuh"
+#include "lm_report.h"
 #include "sampler.cuh"
 #include "tmap_host.h"
 #include "umma.cuh"
@@ -2236,6 +2237,13 @@ static int fail(int code, const std::string& msg) {
     g_err = msg;
     return code;
 }
+int smol::lm::report(int code, const char* who, const char* what) noexcept {
+    try {
+        g_err.assign(who).append(": ").append(what);
+    } catch (...) {      // out of memory: the code alone
+    }
+    return code;
+}
 #define CU(expr)                                                                                  \
     do {                                                                                          \
         cudaError_t e_ = (expr);                                                                  \
@@ -2371,7 +2379,9 @@ static void push_frequencies(std::vector<float>& table, const SmolLmLayer& L, bo
 
 extern "C" int smol_lm_abi_version(void) { return SMOL_LM_ABI_VERSION; }
 extern "C" size_t smol_lm_struct_bytes(int which) {
-    return which == 0 ? sizeof(SmolLmLayer) : which == 1 ? sizeof(SmolLmConfig) : which == 2 ? sizeof(SmolLmGlobals) : which == 3 ? sizeof(SmolLmStep) : 0;
+    const size_t bytes[] = {sizeof(SmolLmLayer), sizeof(SmolLmConfig), sizeof(SmolLmGlobals), sizeof(SmolLmStep),
+                            sizeof(SmolLmCache8), sizeof(SmolLmCache8Batch), sizeof(SmolLmCache8Append), sizeof(SmolLmCache8Attend)};
+    return which >= 0 && which < 8 ? bytes[which] : 0;
 }
 extern "C" const char* smol_lm_last_error(void) { return g_err.c_str(); }
 
