@@ -1,13 +1,16 @@
 // The 8-bit key/value cache: launches and the C entries of include/smoltts_b200_lm.h.
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 #include <utility>
 
 #include "../../include/smoltts_b200_lm.h"
 #include "cache8.cuh"
 #include "cache8_append.cuh"
+#include "cache8_few.cuh"
 #include "cache8_rows.cuh"
 #include "lm_report.h"
+#include "tmap_host.h"
 
 #define SMOL_OK 0
 #define SMOL_ERR_INVALID (-1)
@@ -36,10 +39,10 @@ static cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t sm
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<X>(args))...);
 }
 
-// Shared memory above 48 KB is asked for once per kernel and device.
+// Shared memory above 48 KB, a few of which are static, is asked for once per kernel and device.
 template <class K>
 static cudaError_t more_smem(K kernel, int bytes, std::atomic<uint64_t>& asked) {
-    if (bytes <= 48 * 1024) return cudaSuccess;
+    if (bytes <= 40 * 1024) return cudaSuccess;
     int dev = 0;
     if (cudaError_t e = cudaGetDevice(&dev)) return e;
     if (dev < 64 && (asked.load() >> dev & 1)) return cudaSuccess;
@@ -59,43 +62,73 @@ static cudaError_t append_as(const AppendArgs& A, int n_sms, cudaStream_t st) {
 }
 cudaError_t append(const AppendArgs& A, bool f32, int n_sms, cudaStream_t st) { return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st); }
 
+// query rows of a block of threads
+static int row_tile(const AttendArgs& A, bool f32) { return f32 ? kRowTile : A.b.max_new * (A.H / A.c.G) <= 8 ? 8 : 16; }
+static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new * (long long)(A.H / A.c.G) + row_tile(A, f32) - 1) / row_tile(A, f32)); }
+
 int splits_for(const AttendArgs& A, bool f32, int n_sms) {
-    const int Gq = A.H / A.c.G;
-    const long long base = (long long)A.b.S * A.c.G * ((A.b.max_new * (long long)Gq + kRowTile - 1) / kRowTile);
+    const long long base = (long long)A.b.S * A.c.G * row_tiles(A, f32);
     long long keys = A.b.max_len;
     if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
-    const long long blocks = (keys + kBlock - 1) / kBlock;
-    const long long want = std::min((4ll * n_sms + base - 1) / base, (blocks + 4 * kRowWarps - 1) / (4 * kRowWarps));
-    return (int)std::max(1ll, std::min(want, 128ll));
+    static const int f_waves = getenv("C8W") ? atoi(getenv("C8W")) : 2, f_min = getenv("C8M") ? atoi(getenv("C8M")) : 256;
+    const long long want = std::min(((long long)f_waves * n_sms + base - 1) / base, (keys + f_min - 1) / f_min);
+    return (int)std::max(1ll, std::min(want, (long long)kMaxSplits));
 }
 
-template <class T, int D, bool BENT>
+// Rows of a head's codes, page by page: boxes of 128 bytes by `box` positions; bytes behind the row read as zeros.
+static bool codes_map(CUtensorMap* map, const uint8_t* base, int ld, size_t page_bytes, const Cache& c, int box) {
+    TensorMapEncodeTiledFn encode = tensor_map_encoder();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)ld, (cuuint64_t)c.G * c.page, (cuuint64_t)c.n_pages}, strides[2] = {(cuuint64_t)ld, (cuuint64_t)page_bytes};
+    const cuuint32_t boxes[3] = {128u, (cuuint32_t)box, 1u}, ones[3] = {1u, 1u, 1u};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// positions that lie together and begin at a multiple of themselves: the largest power of two that divides the page, at most a step's
+static int box_of(const Cache& c) { return std::min(c.page & -c.page, kFewStep); }
+
+template <int D, int NR, bool BENT>
+static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
+    static std::atomic<uint64_t> asked{0};
+    constexpr int bytes = few_smem(D, NR);
+    if (cudaError_t e = more_smem(attend_few_kernel<D, NR, BENT>, bytes, asked)) return e;
+    CUtensorMap kmap, vmap;
+    const int box = box_of(A.c);
+    if (!codes_map(&kmap, A.c.k, A.c.ldk, A.c.k_page, A.c, box) || !codes_map(&vmap, A.c.v, A.c.ldv, A.c.v_page, A.c, box)) return cudaErrorInvalidValue;
+    return launch(attend_few_kernel<D, NR, BENT>, dim3(row_tiles(A, false) * A.n_splits, A.c.G, A.b.S), kFewThreads, bytes, st, A, kmap, vmap, box);
+}
+template <int D, int NR>
+static cudaError_t few_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? few_as<D, NR, false>(A, st) : few_as<D, NR, true>(A, st); }
+template <int D>
+static cudaError_t few_rows(const AttendArgs& A, cudaStream_t st) { return row_tile(A, false) == 8 ? few_of<D, 8>(A, st) : few_of<D, 16>(A, st); }
+static cudaError_t attend_few(const AttendArgs& A, cudaStream_t st) { return std::max(A.c.d, A.c.dv) <= 128 ? few_rows<128>(A, st) : few_rows<256>(A, st); }
+
+template <int D, bool BENT>
 static cudaError_t rows_as(const AttendArgs& A, cudaStream_t st) {
     static std::atomic<uint64_t> asked{0};
-    constexpr int bytes = row_smem(D, D, sizeof(T) == 4 ? 2 : 1);
-    if (cudaError_t e = more_smem(attend_rows_kernel<T, D, D, BENT>, bytes, asked)) return e;
-    const int tiles = (A.b.max_new * (A.H / A.c.G) + kRowTile - 1) / kRowTile;
-    return launch(attend_rows_kernel<T, D, D, BENT>, dim3(tiles * A.n_splits, A.c.G, A.b.S), kRowThreads, bytes, st, A);
+    constexpr int bytes = row_smem(D, D, 2);
+    if (cudaError_t e = more_smem(attend_rows_kernel<float, D, D, BENT>, bytes, asked)) return e;
+    return launch(attend_rows_kernel<float, D, D, BENT>, dim3(row_tiles(A, true) * A.n_splits, A.c.G, A.b.S), kRowThreads, bytes, st, A);
 }
-template <class T, int D>
-static cudaError_t rows_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? rows_as<T, D, false>(A, st) : rows_as<T, D, true>(A, st); }
-template <class T>
-static cudaError_t attend_rows(const AttendArgs& A, int* launches, cudaStream_t st) {
+template <int D>
+static cudaError_t rows_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? rows_as<D, false>(A, st) : rows_as<D, true>(A, st); }
+static cudaError_t attend_rows(const AttendArgs& A, cudaStream_t st) {
     const int d = std::max(A.c.d, A.c.dv);
-    if (cudaError_t e = d <= 64 ? rows_of<T, 64>(A, st) : d <= 128 ? rows_of<T, 128>(A, st) : rows_of<T, 256>(A, st)) return e;
-    *launches += 1;
-    if (A.n_splits == 1) return cudaSuccess;
-    *launches += 1;
-    return launch(attend_join_kernel<T>, (int)(((long long)A.b.T * A.H + 3) / 4), 128, 0, st, A);
+    return d <= 64 ? rows_of<64>(A, st) : d <= 128 ? rows_of<128>(A, st) : rows_of<256>(A, st);
 }
 
 bool tiles_serve(const AttendArgs& A, bool f32) { return false; }
 cudaError_t attend(const AttendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st) {
-    return f32 ? attend_rows<float>(A, launches, st) : attend_rows<bf16>(A, launches, st);
+    if (cudaError_t e = f32 ? attend_rows(A, st) : attend_few(A, st)) return e;
+    *launches += 1;
+    if (A.n_splits == 1) return cudaSuccess;
+    *launches += 1;
+    return f32 ? launch(attend_join_kernel<float>, A.b.T * A.H, kJoinWarps * 32, 0, st, A) : launch(attend_join_kernel<bf16>, A.b.T * A.H, kJoinWarps * 32, 0, st, A);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 
+static size_t part_bytes(const AttendArgs& A, int splits) { return (part_floats(A, splits) + 2ull * A.b.T * A.H * splits) * sizeof(float); }
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 static int n_sms_of_device(int* n) {
@@ -199,7 +232,7 @@ extern "C" int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const S
     if (int rc = n_sms_of_device(&n_sms)) return rc;
     const bool f32 = a->dtype == SMOL_LM_F32;
     const int splits = tiles_serve(A, f32) ? 1 : splits_for(A, f32, n_sms);
-    *bytes = splits == 1 ? 0 : (size_t)A.b.T * A.H * splits * (A.c.dv + 2) * sizeof(float);
+    *bytes = splits == 1 ? 0 : part_bytes(A, splits);
     return SMOL_OK;
 }
 
@@ -211,7 +244,7 @@ extern "C" int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCach
     const bool f32 = a->dtype == SMOL_LM_F32;
     if (!tiles_serve(A, f32)) {
         A.n_splits = splits_for(A, f32, n_sms);
-        if (A.n_splits > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < (size_t)A.b.T * A.H * A.n_splits * (A.c.dv + 2) * sizeof(float)))
+        if (A.n_splits > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < part_bytes(A, A.n_splits)))
             return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
         A.part = static_cast<float*>(workspace);
     }

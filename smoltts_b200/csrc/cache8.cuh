@@ -64,10 +64,14 @@ struct AttendArgs {
     const float* gate;               // [T] rows of gate_row floats: the result is multiplied by sigmoid(gate[t][h * dv + c]) (nullptr: not)
     size_t gate_row;
     float out_scale;
-    float* part;                     // [T * H][n_splits][dv + 2]: maximum, denominator, unnormalised result
+    float* part;                     // shares of the keys: unnormalised results [T * H][n_splits][dv rounded up to 4], then (maximum, denominator) [T * H][n_splits]
     int n_splits;
     int q_vec, o_vec;
 };
+
+constexpr int kMaxSplits = 128;
+__host__ __device__ inline size_t part_floats(const AttendArgs& A, int splits) { return (size_t)A.b.T * A.H * splits * ((A.c.dv + 3) / 4 * 4); }
+__device__ __forceinline__ float2* part_stats(const AttendArgs& A) { return reinterpret_cast<float2*>(A.part + part_floats(A, A.n_splits)); }
 
 // what a score goes through in either attention kernel is the plain scaled product
 inline bool plain_scores(const AttendArgs& A) { return A.softcap == 0.0f && !A.slope && !A.r1; }

@@ -98,10 +98,17 @@ __device__ __forceinline__ float finished(const AttendArgs& A, int t, int h, int
     return v;
 }
 
+// An unnormalised result over its denominator, the sink's part included; nothing visible: no weights, and the result is zero.
+__device__ __forceinline__ float with_sink(const AttendArgs& A, int h, float top, float total, float v) {
+    const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, top);
+    const float f = top == -INFINITY ? 1.0f : exp2_fast(top - M), all = fmaf(total, f, M == -INFINITY ? 0.0f : exp2_fast(sink - M));
+    return all == 0.0f ? v : v * f / all;
+}
+
 // Blocks of scale sign < 0 hold NaN codes, which the products took for 480: a row that sees one of them becomes NaN, all of it where a key holds
 // one, the value's column otherwise (mark(row, column)).  Rare, and slow.
 template <class Mark>
-__device__ void mark_nans(const AttendArgs& A, int s, int g, int t0, int row0, int rows, int pos0, int Gq, int kv_len, Mark mark) {
+__device__ void mark_nans(const AttendArgs& A, int s, int g, int row0, int rows, int pos0, int Gq, int kv_len, Mark mark) {
     for (int r = 0; r < rows; ++r) {
         const int pos = pos0 + (row0 + r) / Gq, end = min(kv_len, pos + 1);
         for (int b = 0; b * kBlock < end; ++b) {
@@ -127,14 +134,61 @@ __device__ void mark_nans(const AttendArgs& A, int s, int g, int t0, int row0, i
     }
 }
 
+// What the rows of a block of threads are: rows row0 .. row0 + rows - 1 of sequence s (token by token, the heads of key/value head g within one).
+struct Rows {
+    int s, g, t0, row0, rows, pos0, Gq, kv_len, end;
+};
+template <int ROWS>
+struct Join {
+    float max[kRowWarps][ROWS], sum[kRowWarps][ROWS], weight[kRowWarps][ROWS], top[ROWS], total[ROWS];
+    int bad;
+};
+__host__ __device__ constexpr int join_ld(int DV) { return DV + 4; }
+
+// The four warps' maxima, sums and unnormalised results join[(warp * ROWS + row) * LD + column], joined and finished, or written as this share's part.
+template <class T, int ROWS, int LD>
+__device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, float* join, const Rows& W, int split) {
+    if (threadIdx.x < ROWS) {
+        const int row = threadIdx.x;
+        const float M = fmaxf(fmaxf(J.max[0][row], J.max[1][row]), fmaxf(J.max[2][row], J.max[3][row]));
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
+            // a row of NaN scores has no maximum: its sums say so
+            const float f = J.max[w][row] == -INFINITY ? (J.sum[w][row] == 0.0f ? 0.0f : J.sum[w][row]) : exp2_fast(J.max[w][row] - M);
+            J.weight[w][row] = f;
+            total = fmaf(J.sum[w][row], f, total);
+        }
+        J.top[row] = M;
+        J.total[row] = total;
+    }
+    __syncthreads();
+    if (J.bad) {
+        mark_nans(A, W.s, W.g, W.row0, W.rows, W.pos0, W.Gq, min(W.kv_len, W.end), [&](int row, int col) { join[row * LD + col] = __int_as_float(0x7fffffff); });      // (times whatever weight: NaN)
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < W.rows * A.c.dv; i += kRowThreads) {
+        const int row = i / A.c.dv, col = i - row * A.c.dv, tok = W.t0 + (W.row0 + row) / W.Gq, h = W.g * W.Gq + (W.row0 + row) % W.Gq;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) v = fmaf(join[(w * ROWS + row) * LD + col], J.weight[w][row], v);
+        if (A.n_splits > 1) {
+            const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
+            if (col == 0) part_stats(A)[at] = make_float2(J.top[row], J.total[row]);
+            A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = v;
+        } else {
+            Elem<T>::put(static_cast<T*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, J.top[row], J.total[row], v)));
+        }
+    }
+}
+
 // T: type of queries and results; PARTS: f16 parts of a query and of a weight; DK, DV: head sizes padded; BENT: soft cap or distance penalties
 template <class T, int DK, int DV, bool BENT>
 __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs A) {
     constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
     constexpr bool QS = q_in_smem(DK, PARTS);
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ float s_max[kRowWarps][kRowTile], s_sum[kRowWarps][kRowTile], s_weight[kRowWarps][kRowTile], s_top[kRowTile], s_total[kRowTile];
-    __shared__ int s_bad;
+    __shared__ Join<kRowTile> J;
     dep_wait();
     dep_go();
     const int s = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / A.n_splits, split = blockIdx.x % A.n_splits;
@@ -147,7 +201,8 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     const Seen seen = seen_blocks(A, first_pos, last_pos, kv_len);
     const int share = (seen.count + A.n_splits - 1) / A.n_splits, b_lo = min(split * share, seen.count), b_hi = min(b_lo + share, seen.count);
     const int mine = b_hi - b_lo > warp ? (b_hi - b_lo - warp + kRowWarps - 1) / kRowWarps : 0;      // blocks of this warp: b_lo + warp, + 4, ...
-    if (threadIdx.x == 0) s_bad = 0;
+    const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
+    if (threadIdx.x == 0) J.bad = 0;
 
     // where the warp's blocks are: lane i knows block number i of 32 (`now`), and of the 32 that follow
     struct Place { int page, in_page; float ks, vs; };
@@ -412,13 +467,13 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
         l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
         if (c == 0) {
-            s_max[warp][r + 8 * x] = m[x];
-            s_sum[warp][r + 8 * x] = l[x];
+            J.max[warp][r + 8 * x] = m[x];
+            J.sum[warp][r + 8 * x] = l[x];
         }
     }
-    if (bad && lane == 0) s_bad = 1;
+    if (bad && lane == 0) J.bad = 1;
     __syncthreads();      // everybody's copies are used up: the ring becomes the results' place
-    constexpr int LD = DV + 4;
+    constexpr int LD = join_ld(DV);
     float* join = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -429,55 +484,18 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int t = 0; t < VB; t += 4)
                 *reinterpret_cast<float4*>(to + t) = make_float4(o[t][2 * x + e] * unit, o[t + 1][2 * x + e] * unit, o[t + 2][2 * x + e] * unit, o[t + 3][2 * x + e] * unit);
         }
-    if (threadIdx.x < kRowTile) {
-        const int row = threadIdx.x;
-        const float M = fmaxf(fmaxf(s_max[0][row], s_max[1][row]), fmaxf(s_max[2][row], s_max[3][row]));
-        float total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) {
-            // a row of NaN scores has no maximum: its sums say so
-            const float f = s_max[w][row] == -INFINITY ? (s_sum[w][row] == 0.0f ? 0.0f : s_sum[w][row]) : exp2_fast(s_max[w][row] - M);
-            s_weight[w][row] = f;
-            total = fmaf(s_sum[w][row], f, total);
-        }
-        s_top[row] = M;
-        s_total[row] = total;
-    }
-    __syncthreads();
-    auto joined = [&](int row, int col) {
-        float v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kRowWarps; ++w) v = fmaf(join[(w * kRowTile + row) * LD + col], s_weight[w][row], v);
-        return v;
-    };
-    if (s_bad) {
-        mark_nans(A, s, g, t0, row0, rows, pos0, Gq, min(kv_len, seen.end), [&](int row, int col) { join[row * LD + col] = __int_as_float(0x7fffffff); });      // (times whatever weight: NaN)
-        __syncthreads();
-    }
-    for (int i = threadIdx.x; i < rows * A.c.dv; i += kRowThreads) {
-        const int row = i / A.c.dv, col = i - row * A.c.dv, tok = t0 + (row0 + row) / Gq, h = g * Gq + (row0 + row) % Gq;
-        const float v = joined(row, col);
-        if (A.n_splits > 1) {
-            float* to = A.part + (((size_t)tok * A.H + h) * A.n_splits + split) * (A.c.dv + 2);
-            if (col == 0) { to[0] = s_top[row]; to[1] = s_total[row]; }
-            to[2 + col] = v;
-        } else {
-            const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, s_top[row]);
-            const float f = s_top[row] == -INFINITY ? 1.0f : exp2_fast(s_top[row] - M), total = fmaf(s_total[row], f, M == -INFINITY ? 0.0f : exp2_fast(sink - M));
-            // nothing visible: no weights, and the result is zero
-            const float out = total == 0.0f ? v : v * f / total;
-            Elem<T>::put(static_cast<T*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, out));
-        }
-    }
+    join_rows<T, kRowTile, LD>(A, J, join, W, split);
 }
 
-// A warp per (token, head): joins the shares of the keys, and the sink.
+// A block of threads per (token, head): joins the shares of the keys, and the sink.  Latency is all there is to it, so everything a warp needs is
+// on its way at once: the shares' maxima first, then eight shares' results at a time, dealt out to the eight warps.
+constexpr int kJoinWarps = 8;
 template <class T>
-__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs A) {
+__global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const AttendArgs A) {
+    __shared__ float4 s_acc[kJoinWarps][kMaxDim / 4];
+    const int unit = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, t = unit / A.H, h = unit % A.H;
     dep_wait();
     dep_go();
-    const int unit = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, t = unit / A.H, h = unit % A.H;
-    if (t >= A.b.T) return;
     // rows in front of the first sequence, behind the last or behind max_new of their own are nobody's
     int lo = 0, hi = A.b.S;
     while (hi - lo > 1) {
@@ -485,41 +503,59 @@ __global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs A) {
         if (A.b.start[mid] <= t) lo = mid;
         else hi = mid;
     }
-    const int t0 = A.b.start[lo];
-    if (t < t0 || t >= A.b.start[lo + 1] || t0 < 0 || A.b.start[lo + 1] > A.b.T) return;
-    if (t - t0 >= A.b.max_new) return;
-    const float* p = A.part + (size_t)unit * A.n_splits * (A.c.dv + 2);
+    const int t0 = A.b.start[lo], t1 = A.b.start[lo + 1];
+    if (t < t0 || t >= t1 || t0 < 0 || t1 > A.b.T || t - t0 >= A.b.max_new) return;
+    const int pieces = (A.c.dv + 3) / 4;
+    const float2* stat = part_stats(A) + (size_t)unit * A.n_splits;
+    const float4* part = reinterpret_cast<const float4*>(A.part) + (size_t)unit * A.n_splits * pieces;
     const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY;
+    float2 st[kMaxSplits / 32];
     float M = sink;
-    for (int z = lane; z < A.n_splits; z += 32) M = fmaxf(M, p[(size_t)z * (A.c.dv + 2)]);
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 32; ++x) {
+        st[x] = lane + 32 * x < A.n_splits ? stat[lane + 32 * x] : make_float2(-INFINITY, 0.0f);
+        M = fmaxf(M, st[x].x);
+    }
     M = warp_max(M);
-    float total = 0.0f, acc[kMaxDim / 32];
+    float total = 0.0f;
 #pragma unroll
-    for (int e = 0; e < kMaxDim / 32; ++e) acc[e] = 0.0f;
-    for (int z0 = 0; z0 < A.n_splits; z0 += 32) {
-        float f = 0.0f;
-        if (z0 + lane < A.n_splits) {
-            const float* q = p + (size_t)(z0 + lane) * (A.c.dv + 2);
-            // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
-            f = q[0] == -INFINITY ? (q[1] == 0.0f ? 1.0f : q[1]) : exp2_fast(q[0] - M);
-            total = fmaf(q[1], f, total);
-        }
-        const int cnt = min(32, A.n_splits - z0);
-#pragma unroll 4
-        for (int z = 0; z < cnt; ++z) {
-            const float fz = __shfl_sync(0xffffffffu, f, z);
-            const float* q = p + (size_t)(z0 + z) * (A.c.dv + 2) + 2;
+    for (int x = 0; x < kMaxSplits / 32; ++x) {
+        // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
+        const float f = st[x].x == -INFINITY ? (st[x].y == 0.0f ? 0.0f : st[x].y) : exp2_fast(st[x].x - M);
+        total = fmaf(st[x].y, f, total);
+        st[x].x = f;
+    }
+    float4 acc[kMaxDim / 128];
 #pragma unroll
-            for (int e = 0; e < kMaxDim / 32; ++e)
-                if (lane + 32 * e < A.c.dv) acc[e] = fmaf(q[lane + 32 * e], fz, acc[e]);
+    for (int e = 0; e < kMaxDim / 128; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 32; ++x) {
+        if (32 * x >= A.n_splits) break;
+#pragma unroll
+        for (int i = 0; i < 32 / kJoinWarps; ++i) {
+            const int z = 32 * x + i * kJoinWarps + warp;
+            const float f = __shfl_sync(0xffffffffu, st[x].x, z & 31);
+#pragma unroll
+            for (int e = 0; e < kMaxDim / 128; ++e)
+                if (z < A.n_splits && lane + 32 * e < pieces) {
+                    const float4 v = part[(size_t)z * pieces + lane + 32 * e];
+                    acc[e].x = fmaf(v.x, f, acc[e].x);
+                    acc[e].y = fmaf(v.y, f, acc[e].y);
+                    acc[e].z = fmaf(v.z, f, acc[e].z);
+                    acc[e].w = fmaf(v.w, f, acc[e].w);
+                }
         }
     }
-    total = warp_sum(total) + (M == -INFINITY ? 0.0f : exp2_fast(sink - M));
 #pragma unroll
-    for (int e = 0; e < kMaxDim / 32; ++e) {
-        const int col = lane + 32 * e;
-        if (col < A.c.dv)
-            Elem<T>::put(static_cast<T*>(A.out) + (size_t)t * A.o_row + (size_t)h * A.o_head + col, finished(A, t, h, col, total == 0.0f ? acc[e] : acc[e] / total));
+    for (int e = 0; e < kMaxDim / 128; ++e) s_acc[warp][lane + 32 * e] = acc[e];
+    __syncthreads();
+    total = warp_sum(total) + (M == -INFINITY ? 0.0f : exp2_fast(sink - M));
+    const float* flat = reinterpret_cast<const float*>(s_acc);
+    for (int col = threadIdx.x; col < A.c.dv; col += kJoinWarps * 32) {
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) v += flat[w * kMaxDim + col];
+        Elem<T>::put(static_cast<T*>(A.out) + (size_t)t * A.o_row + (size_t)h * A.o_head + col, finished(A, t, h, col, total == 0.0f ? v : v / total));
     }
 }
 

@@ -99,9 +99,14 @@ def attention(q, k, v, pos, scale, window=0, first=0, softcap=0.0, sink=None, sl
 
 def tolerance(dtype, want, spread, size, bent=0.0):
     """How far a result may be off, element by element.  Rounding of the result: half a step.  A weight's relative error times the sum of
-    weight * |value|: 2^-11 (one f16 part) or 2^-22 (two) from its rounding and 2^-22 from the exponential; its score's absolute error -- a
+    weight * |value|: its rounding, and 2^-22 from the exponential; its score's absolute error -- a
     product of d <= 256 terms is at most 32 tensor-core sums, each cut off below 2^-23 of what is summed, `size` at most (2^-18 size), the
     parts of the query 2^-22 size, roundings of the scaled score and of its difference to the maximum 2^-22 size, and what the soft cap and the
-    penalties add, a few 2^-21 of their own size `bent`; the weighted sum itself, at most 32 cut-off sums in a warp's share (2^-18)."""
-    part = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
+    penalties add, a few 2^-21 of their own size `bent`; the weighted sum itself, at most 32 cut-off sums in a warp's share (2^-18).
+
+    A weight's rounding for float32: two f16 parts, 2^-22.  For bfloat16: two e4m3 parts.  Let the weight be x in [1, 2) of its binade.  e4m3 has three
+    bits behind the point, steps of 2^-3, so the first part leaves a remainder of at most 2^-4.  The second part takes that remainder in a binade of
+    at most [2^-5, 2^-4), whose steps are 2^-8, and is off by half of one: 2^-9 absolute, at most 2^-9 of x.  (A remainder of exactly 2^-4 is a
+    power of two and exact.)  The f16 number taken apart is itself off by 2^-11."""
+    part = 2.0 ** -9 + 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
     return HALF_STEP[dtype] * want.abs() + (part + 2.0 ** -17 * (1.0 + size) + 2.0 ** -19 * bent) * spread + 1e-30
