@@ -9,8 +9,8 @@
 //
 // e4m3 on both sides (kind::f8f6f4).  A query, scaled by a power of two to a largest magnitude in [128, 256), is the sum of two e4m3 parts, the second 16
 // times finer: four bits each and the sign of the remainder hold bf16's eight bits, down to 2^-13 of the row's largest coordinate, and 2^-23 of
-// it below.  A weight exp2(s - m), times its block's value scale over the largest so far, is taken apart the same way, on 256: a relative
-// error of at most 2^-9, as a weight in bf16 would have, or 2^-23 of the row's largest weight.  Parts are columns of their own.
+// it below.  A weight exp2(s - m), times its block's value scale over the largest so far, is taken apart the same way, on 64: a relative
+// error of at most 2^-9, as a weight in bf16 would have, or 2^-20 of the reference's (m: see kSlack).  Parts are columns of their own.
 //
 // Roles: a warp that looks pages up and issues the copies (tensor maps, 128-byte swizzle, boxes of up to 128 positions that lie together), a thread
 // that issues the products, four warps for the softmax.  A NaN code is a NaN to the product even under a weight of 0: in steps with positions that
@@ -73,6 +73,18 @@ __device__ uint32_t nan_columns(const AttendArgs& A, const Rows& W, int col) {
     return rows;
 }
 
+constexpr float kWeightUnit = 64.0f, kSlack = 2.75f;      // 64 * 2^2.75 < 448, the largest code
+// whether x holds for any thread of the four softmax warps
+__device__ __forceinline__ bool any_of_four(bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(any) : "r"((uint32_t)x) : "memory");
+    return any != 0;
+}
 __device__ __forceinline__ float warp_top(float v) {
     asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
     return v;
@@ -329,9 +341,13 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const AttendArg
                     }
                 }
             }
-            // ---- the rows' maxima over the step, and the largest value scale ----
+            // ---- The reference of a row's weights is the maximum when it was last set: a weight may be 2^kSlack, and only a step that has a larger one (or a
+            // larger value scale) sets references anew, which takes the four warps' maxima and waits for the product before. ----
             const float v_unit = page < 0 ? 0.0f : fmaxf(fabsf(sc.y), 7.5231638e-37f);      // 2^-120: below every scale
-            {
+            bool beyond = v_unit > unit;
+#pragma unroll
+            for (int r = 0; r < NR; ++r) beyond |= S[r] > m[r] + kSlack;
+            if (any_of_four(beyond)) {
                 float mine = warp_top(v_unit);
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
@@ -339,23 +355,16 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const AttendArg
                     mine = lane == r ? top : mine;
                 }
                 if (lane <= NR) s_top[b][warp][lane] = mine;
-            }
-            sync4();
-            float mx[NR], grown = unit;
-            bool grows = false;
+                sync4();
+                float grown = unit;
 #pragma unroll
-            for (int r = 0; r < NR; ++r) {
-                mx[r] = fmaxf(fmaxf(s_top[b][0][r], s_top[b][1][r]), fmaxf(s_top[b][2][r], s_top[b][3][r]));
-                grows |= mx[r] > m[r];
-            }
-#pragma unroll
-            for (int w = 0; w < 4; ++w) grown = fmaxf(grown, s_top[b][w][NR]);
-            if (grows || grown > unit) {      // the same in all four warps
+                for (int w = 0; w < 4; ++w) grown = fmaxf(grown, s_top[b][w][NR]);
                 const float down = grown > 0.0f ? unit / grown : 1.0f;      // powers of two
                 float corr[NR];
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    const float mn = fmaxf(m[r], mx[r]), f = mn == -INFINITY ? 1.0f : exp2_fast(m[r] - mn);
+                    const float mn = fmaxf(m[r], fmaxf(fmaxf(s_top[b][0][r], s_top[b][1][r]), fmaxf(s_top[b][2][r], s_top[b][3][r])));
+                    const float f = mn == -INFINITY ? 1.0f : exp2_fast(m[r] - mn);
                     m[r] = mn;
                     l[r] *= f;
                     corr[r] = f * down;
@@ -384,7 +393,7 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const AttendArg
             }
             // ---- weights: hi at row r, lo at row NR + r, this position's byte ----
             if (i >= 2) wait_bar(&bars.o_full[b], ((i - 2) >> 1) & 1, stop, A.c.err);
-            const float vmul = 256.0f * (v_unit / fmaxf(unit, 7.5231638e-37f));
+            const float vmul = kWeightUnit * (v_unit / fmaxf(unit, 7.5231638e-37f));
             unsigned char* P = Ps + b * (N * 128);
 #pragma unroll
             for (int r = 0; r < NR; r += 2) {
@@ -416,7 +425,7 @@ __global__ void __launch_bounds__(kFewThreads) attend_few_kernel(const AttendArg
         wait_bar(&bars.o_full[(steps - 1) & 1], ((steps - 1) >> 1) & 1, stop, A.c.err);
         sync4();
         umma::fence_after_sync();
-        const float out_unit = unit * (1.0f / 256.0f);
+        const float out_unit = unit * (1.0f / kWeightUnit);
 #pragma unroll
         for (int x = 0; x < HALVES; ++x) {
             __syncwarp();
