@@ -1,7 +1,6 @@
 // The 8-bit key/value cache: launches and the C entries of include/smoltts_b200_lm.h.
 #include <algorithm>
 #include <atomic>
-#include <cstdlib>
 #include <utility>
 
 #include "../../include/smoltts_b200_lm.h"
@@ -25,18 +24,25 @@ using lm::report;
 
 // Every kernel here begins with the wait for the kernel in front of it, so all of them may be set up early.
 template <class... P, class... X>
-static cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, X&&... args) {
+static cudaError_t launch_cluster(int cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, X&&... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
+    cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<X>(args))...);
+}
+template <class... P, class... X>
+static cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, X&&... args) {
+    return launch_cluster(1, kernel, grid, block, smem, st, std::forward<X>(args)...);
 }
 
 // Shared memory above 48 KB, a few of which are static, is asked for once per kernel and device.
@@ -63,15 +69,21 @@ static cudaError_t append_as(const AppendArgs& A, int n_sms, cudaStream_t st) {
 cudaError_t append(const AppendArgs& A, bool f32, int n_sms, cudaStream_t st) { return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st); }
 
 // query rows of a block of threads
-static int row_tile(const AttendArgs& A, bool f32) { return f32 ? kRowTile : A.b.max_new * (A.H / A.c.G) <= 8 ? 8 : 16; }
+static int row_tile(const AttendArgs& A, bool f32) {
+    const long long rows = A.b.max_new * (long long)(A.H / A.c.G);
+    return f32 ? kRowTile : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+}
 static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new * (long long)(A.H / A.c.G) + row_tile(A, f32) - 1) / row_tile(A, f32)); }
 
 int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     const long long base = (long long)A.b.S * A.c.G * row_tiles(A, f32);
     long long keys = A.b.max_len;
     if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
-    static const int f_waves = getenv("C8W") ? atoi(getenv("C8W")) : 2, f_min = getenv("C8M") ? atoi(getenv("C8M")) : 256;
-    const long long want = std::min(((long long)f_waves * n_sms + base - 1) / base, (keys + f_min - 1) / f_min);
+    // as many shares as the SMs hold blocks at once, none of less than 256 keys (a share of 128 is one step: 15.1 us against 15.7 for a token of 12 heads
+    // at 2048 positions, appended and attended to, but twice the blocks; of 512 17.7).  More blocks than are held at once wait for whole others: 64
+    // sequences at up to 8192 positions, 512 blocks, 145 us in one share, 181 in two; one at 131072 33 us in 111 shares, 42 in 128 and more.
+    const int held = f32 ? 4 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
+    const long long want = std::min((long long)held * n_sms / base, (keys + 255) / 256);
     return (int)std::max(1ll, std::min(want, (long long)kMaxSplits));
 }
 
@@ -85,22 +97,25 @@ static bool codes_map(CUtensorMap* map, const uint8_t* base, int ld, size_t page
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 // positions that lie together and begin at a multiple of themselves: the largest power of two that divides the page, at most a step's
-static int box_of(const Cache& c) { return std::min(c.page & -c.page, kFewStep); }
+static int box_of(const Cache& c) { return std::min(c.page & -c.page, kStep); }
 
-template <int D, int NR, bool BENT>
+static bool joins_in_cluster(int splits, bool f32) { return !f32 && splits > 1 && splits <= kMostCluster; }
+
+template <int D, int RA, bool BENT>
 static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
     static std::atomic<uint64_t> asked{0};
-    constexpr int bytes = few_smem(D, NR);
-    if (cudaError_t e = more_smem(attend_few_kernel<D, NR, BENT>, bytes, asked)) return e;
+    constexpr int bytes = few_smem(D, RA);
+    if (cudaError_t e = more_smem(attend_few_kernel<D, RA, BENT>, bytes, asked)) return e;
     CUtensorMap kmap, vmap;
     const int box = box_of(A.c);
     if (!codes_map(&kmap, A.c.k, A.c.ldk, A.c.k_page, A.c, box) || !codes_map(&vmap, A.c.v, A.c.ldv, A.c.v_page, A.c, box)) return cudaErrorInvalidValue;
-    return launch(attend_few_kernel<D, NR, BENT>, dim3(row_tiles(A, false) * A.n_splits, A.c.G, A.b.S), kFewThreads, bytes, st, A, kmap, vmap, box);
+    return launch_cluster(joins_in_cluster(A.n_splits, false) ? A.n_splits : 1, attend_few_kernel<D, RA, BENT>, dim3(row_tiles(A, false) * A.n_splits, A.c.G, A.b.S), kFewThreads, bytes, st, A, kmap,
+                          vmap, box);
 }
-template <int D, int NR>
-static cudaError_t few_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? few_as<D, NR, false>(A, st) : few_as<D, NR, true>(A, st); }
+template <int D, int RA>
+static cudaError_t few_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? few_as<D, RA, false>(A, st) : few_as<D, RA, true>(A, st); }
 template <int D>
-static cudaError_t few_rows(const AttendArgs& A, cudaStream_t st) { return row_tile(A, false) == 8 ? few_of<D, 8>(A, st) : few_of<D, 16>(A, st); }
+static cudaError_t few_rows(const AttendArgs& A, cudaStream_t st) { return row_tile(A, false) == 4 ? few_of<D, 4>(A, st) : row_tile(A, false) == 8 ? few_of<D, 8>(A, st) : few_of<D, 16>(A, st); }
 static cudaError_t attend_few(const AttendArgs& A, cudaStream_t st) { return std::max(A.c.d, A.c.dv) <= 128 ? few_rows<128>(A, st) : few_rows<256>(A, st); }
 
 template <int D, bool BENT>
@@ -121,7 +136,7 @@ bool tiles_serve(const AttendArgs& A, bool f32) { return false; }
 cudaError_t attend(const AttendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st) {
     if (cudaError_t e = f32 ? attend_rows(A, st) : attend_few(A, st)) return e;
     *launches += 1;
-    if (A.n_splits == 1) return cudaSuccess;
+    if (A.n_splits == 1 || joins_in_cluster(A.n_splits, f32)) return cudaSuccess;
     *launches += 1;
     return f32 ? launch(attend_join_kernel<float>, A.b.T * A.H, kJoinWarps * 32, 0, st, A) : launch(attend_join_kernel<bf16>, A.b.T * A.H, kJoinWarps * 32, 0, st, A);
 }
@@ -232,7 +247,7 @@ extern "C" int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const S
     if (int rc = n_sms_of_device(&n_sms)) return rc;
     const bool f32 = a->dtype == SMOL_LM_F32;
     const int splits = tiles_serve(A, f32) ? 1 : splits_for(A, f32, n_sms);
-    *bytes = splits == 1 ? 0 : part_bytes(A, splits);
+    *bytes = splits == 1 || joins_in_cluster(splits, f32) ? 0 : part_bytes(A, splits);
     return SMOL_OK;
 }
 
@@ -244,7 +259,7 @@ extern "C" int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCach
     const bool f32 = a->dtype == SMOL_LM_F32;
     if (!tiles_serve(A, f32)) {
         A.n_splits = splits_for(A, f32, n_sms);
-        if (A.n_splits > 1 && (!workspace || !aligned(workspace, 16) || workspace_bytes < part_bytes(A, A.n_splits)))
+        if (A.n_splits > 1 && !joins_in_cluster(A.n_splits, f32) && (!workspace || !aligned(workspace, 16) || workspace_bytes < part_bytes(A, A.n_splits)))
             return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
         A.part = static_cast<float*>(workspace);
     }

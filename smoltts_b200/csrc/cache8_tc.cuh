@@ -3,7 +3,7 @@
 
 #include <cuda.h>
 
-#include "cache8.cuh"
+#include "cache8_rows.cuh"
 #include "umma.cuh"
 
 namespace smol {
@@ -78,6 +78,8 @@ __device__ __forceinline__ void load_box(uint32_t dst, const void* map, int x, i
                  ::"r"(dst), "l"(map), "r"(umma::s2u(bar)), "r"(x), "r"(y), "r"(z) : "memory");
 }
 
+constexpr float kLeastScale = 7.5231638e-37f;      // 2^-120: below every scale
+
 // NaN codes of four cleared
 __device__ __forceinline__ uint32_t without_nans(uint32_t w) {
     const uint32_t nan = (((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7;
@@ -91,6 +93,100 @@ __device__ __forceinline__ void two_parts(__half2 x, uint32_t& hi, uint32_t& lo)
     // the remainder times 16: exact (eight bits at most)
     const __half2_raw rest = __hmul2(__hsub2(x, back), __float2half2_rn(16.0f));
     lo = __nv_cvt_halfraw2_to_fp8x2(rest, __NV_SATFINITE, __NV_E4M3);
+}
+
+__device__ __forceinline__ float warp_top(float v) {
+    asm volatile("redux.sync.max.f32 %0, %0, 0xffffffff;" : "+f"(v));
+    return v;
+}
+
+// ---- steps of 128 positions ----
+constexpr int kStep = 128, kStepBlocks = kStep / kBlock;
+
+// The steps that rows first_pos .. last_pos see: `lead` of them from the sequence's start (the first tokens, in front of the window), then those from
+// `from` up to the last visible key.
+__device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
+    Seen x;
+    x.end = max(min(kv_len, last_pos + 1), 0);
+    const int steps = (x.end + kStep - 1) / kStep;
+    x.from = A.window > 0 ? min(max(first_pos - A.window + 1, 0) / kStep, steps) : 0;
+    x.lead = A.window > 0 ? min((A.first + kStep - 1) / kStep, x.from) : 0;
+    x.count = x.lead + steps - x.from;
+    return x;
+}
+// first position of step i of a share that begins at number lo
+__device__ __forceinline__ int step_place(const Seen& seen, int lo, int i) { return (lo + i < seen.lead ? lo + i : seen.from + lo + i - seen.lead) * kStep; }
+
+// What the copying warp leaves beside a stage: the scales of the step's blocks (0: nothing there; the values' sign says whether a block holds a NaN).
+struct StepScales {
+    float k[kStepBlocks], v[kStepBlocks];
+};
+
+// The copying warp: keys and values of every step into a ring of NS stages (keys: HALVES tiles of 128 positions by 128 bytes, then the values'), 128-byte
+// swizzle, in boxes of `box` positions that lie together.  Lane x < 8 looks up block x of a step; entries are loaded two steps ahead and scales one,
+// so that nothing waits for them here.
+template <int HALVES, int NS>
+__device__ __forceinline__ void copy_steps(const AttendArgs& A, const CUtensorMap* kmap, const CUtensorMap* vmap, int box, const Rows& W, const Seen& seen, int lo, int steps, int first_pos,
+                                           unsigned char* ring, StepScales* scales, uint64_t* full, uint64_t* empty, volatile int* stop) {
+    constexpr int SB = kStep * 256 * HALVES;
+    const int lane = threadIdx.x & 31, per = box / kBlock;
+    struct Entry { int page, in_page, seen; };      // in_page < 0: nobody sees the block's box; seen: the block itself
+    auto near = [&](int j, int n) { return j < seen.end && (A.window == 0 || j + n > first_pos - A.window + 1 || j < A.first); };
+    auto entry = [&](int i) {
+        Entry e{-1, -1, 0};
+        if (i < steps && lane < kStepBlocks) {
+            const int j = step_place(seen, lo, i) + lane * kBlock, pg = j / A.c.page;
+            if (near(j / box * box, box)) {
+                e.in_page = j - pg * A.c.page;
+                e.seen = near(j, kBlock);      // (the scales of places that nobody has written yet must not count)
+                if (pg < A.b.max_pages) e.page = A.b.table[(size_t)W.s * A.b.max_pages + pg];
+            }
+        }
+        return e;
+    };
+    auto scales_at = [&](const Entry& e) {
+        if (!e.seen || e.page < 0 || e.page >= A.c.n_pages) return make_float2(0.0f, 0.0f);
+        const int at = W.g * (A.c.page / kBlock) + e.in_page / kBlock;
+        // (a scale that nobody has written counts as the least there is; 0 stands for no page)
+        const float k = A.c.ks[(size_t)e.page * A.c.ks_page + at], v = A.c.vs[(size_t)e.page * A.c.vs_page + at];
+        return make_float2(fmaxf(fabsf(k), kLeastScale), copysignf(fmaxf(fabsf(v), kLeastScale), v));
+    };
+    Entry now = entry(0), next = entry(1);
+    float2 sc = scales_at(now);
+    int issued = 0;
+    for (int i = 0; i < steps; ++i) {
+        const Entry after = entry(i + 2);
+        const float2 sc1 = scales_at(next);
+        const int st = i % NS;
+        bool ok = true;
+        if (i >= NS) ok = wait_bar(&empty[st], (i / NS - 1) & 1, stop, A.c.err);
+        if (!__all_sync(0xffffffffu, ok)) break;
+        const bool held = now.in_page >= 0 && now.page >= 0 && now.page < A.c.n_pages;
+        if (now.in_page >= 0 && !held) atomicExch(A.c.err, 1);
+        const bool mine = held && lane % per == 0;      // a box's first block issues it
+        const int live = __popc(__ballot_sync(0xffffffffu, mine));
+        if (lane < kStepBlocks) {
+            scales[st].k[lane] = sc.x;
+            scales[st].v[lane] = sc.y;
+        }
+        __syncwarp();
+        if (lane == 0) umma::bar_expect_tx(&full[st], (uint32_t)(live * box * 256 * HALVES));
+        __syncwarp();
+        if (mine) {
+            const uint32_t to = umma::s2u(ring + st * SB) + lane * kBlock * 128;
+#pragma unroll
+            for (int x = 0; x < HALVES; ++x) load_box(to + x * (kStep * 128), kmap, 128 * x, W.g * A.c.page + now.in_page, now.page, &full[st]);
+#pragma unroll
+            for (int x = 0; x < HALVES; ++x) load_box(to + (HALVES + x) * (kStep * 128), vmap, 128 * x, W.g * A.c.page + now.in_page, now.page, &full[st]);
+        }
+        issued = i + 1;
+        now = next;
+        next = after;
+        sc = sc1;
+    }
+    // nothing may land in shared memory that is another's by then
+    if (*stop)
+        for (int i = max(issued - NS, 0); i < issued; ++i) drain_bar(&full[i % NS], (i / NS) & 1);
 }
 
 }  // namespace c8

@@ -11,7 +11,8 @@ its softmax attention layers from such a cache with ``kv_bits=8``.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Tuple
+import struct
+from typing import Dict, Optional, Tuple
 
 import torch
 
@@ -20,6 +21,12 @@ from ._errors import SMOL_ERR_CAPACITY, SMOL_OK, SmolError
 
 BLOCK = 16          # positions that share a scale
 _DTYPES = {torch.bfloat16: _capi_lm.SMOL_LM_BF16, torch.float32: _capi_lm.SMOL_LM_F32}
+# The arguments' structs of include/smoltts_b200_lm.h as native layouts: packing one takes a microsecond, filling a ctypes structure several.
+_BATCH = struct.Struct("@5i4P")
+_APPEND = struct.Struct("@i2P4Ni2P4N2iPf0P")
+_ATTEND = struct.Struct("@2i2P4N3f2i5PN0P")
+for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCache8Append), (_ATTEND, _capi_lm.SmolLmCache8Attend)):
+    assert _s.size == C.sizeof(_m)
 
 
 def _padded(n: int) -> int:
@@ -46,12 +53,19 @@ class KVCache8:
                 raise ValueError(f"scales must be float32 {(n, g, page // BLOCK)}")
         if not k.is_cuda or any(t.device != k.device or not t.is_contiguous() for t in (k, v, k_scale, v_scale)):
             raise ValueError("codes and scales must be contiguous tensors of one CUDA device")
-        self.lib = _capi_lm.load()
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.n_pages, self.kv_heads, self.page_size, self.device = n, g, page, k.device
+        self.n_pages, self.kv_heads, self.page_size = n, g, page
+        self.device, self._index = k.device, k.device.index
         self._err = torch.zeros(1, dtype=torch.int32, device=self.device)
-        self._c = _capi_lm.SmolLmCache8(k=k.data_ptr(), v=v.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(), n_pages=n, page_size=page,
-                                        kv_heads=g, dim=self.dim, vdim=self.vdim, err=self._err.data_ptr())
+        self._c = bytes(_capi_lm.SmolLmCache8(k=k.data_ptr(), v=v.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(), n_pages=n, page_size=page,
+                                              kv_heads=g, dim=self.dim, vdim=self.vdim, err=self._err.data_ptr()))
+        lib = _capi_lm.load()
+        # (functions of this module's own: their arguments are packed structs)
+        self._append, self._attend, self._workspace = lib["smol_lm_cache8_append"], lib["smol_lm_cache8_attend"], lib["smol_lm_cache8_workspace_bytes"]
+        self._append.argtypes = [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p]
+        self._attend.argtypes = [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p]
+        self._workspace.argtypes = [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p]
+        self._need: Dict[tuple, int] = {}      # bytes of workspace by what they depend on
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, kv_heads: int, dim: int, vdim: Optional[int] = None, device=None) -> "KVCache8":
@@ -65,46 +79,46 @@ class KVCache8:
         return cls(codes[0], codes[1], scales[0], scales[1], dim=dim, vdim=vdim)
 
     # ------------------------------------------------------------------ arguments
-    def _rows(self, x: torch.Tensor, heads: Optional[int], width: int, what: str) -> Tuple[int, int]:
+    def _rows(self, x: torch.Tensor, tokens: Optional[int], heads: Optional[int], width: int, dtype: Optional[torch.dtype], what: str) -> Tuple[int, int]:
         """Checks a ``[tokens, heads, width]`` tensor and returns its strides; rows may be slices of something wider."""
-        if x.dim() != 3 or x.shape[2] != width or (heads is not None and x.shape[1] != heads):
-            raise ValueError(f"{what} must be [tokens, {heads if heads is not None else 'heads'}, {width}], got {tuple(x.shape)}")
-        if x.dtype not in _DTYPES or x.device != self.device:
-            raise ValueError(f"{what} must be bfloat16 or float32 on {self.device}, got {x.dtype} on {x.device}")
+        shape = x.shape
+        if len(shape) != 3 or shape[2] != width or (heads is not None and shape[1] != heads) or (tokens is not None and shape[0] != tokens):
+            raise ValueError(f"{what} must be [{'tokens' if tokens is None else tokens}, {'heads' if heads is None else heads}, {width}], got {tuple(shape)}")
+        if x.dtype not in _DTYPES or (dtype is not None and x.dtype != dtype) or x.device != self.device:
+            raise ValueError(f"{what} must be {'bfloat16 or float32' if dtype is None else dtype} on {self.device}, got {x.dtype} on {x.device}")
         row, head, one = x.stride()
-        if (one != 1 and width > 1) or row < 0 or head < 0:
+        if one != 1 and width > 1:
             raise ValueError(f"{what}: the last dimension must be contiguous")
         return row, head
 
     def _ints(self, x: torch.Tensor, shape: tuple, what: str) -> int:
-        if x.dtype != torch.int32 or x.device != self.device or tuple(x.shape) != shape or not x.is_contiguous():
+        if x.dtype != torch.int32 or x.shape != shape or x.device != self.device or not x.is_contiguous():
             raise ValueError(f"{what} must be contiguous int32 {shape} on {self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
         return x.data_ptr()
 
-    def _floats(self, x: Optional[torch.Tensor], n: int, what: str) -> Optional[int]:
+    def _floats(self, x: Optional[torch.Tensor], n: int, what: str) -> int:
         if x is None:
-            return None
-        if x.dtype != torch.float32 or x.device != self.device or tuple(x.shape) != (n,) or not x.is_contiguous():
+            return 0
+        if x.dtype != torch.float32 or x.shape != (n,) or x.device != self.device or not x.is_contiguous():
             raise ValueError(f"{what} must be contiguous float32 [{n}] on {self.device}")
         return x.data_ptr()
 
-    def _batch(self, tokens: int, seq_start, seq_pos0, block_table, max_new: int, max_len: int, kv_len=None) -> "_capi_lm.SmolLmCache8Batch":
-        if block_table.dim() != 2 or block_table.shape[0] < 1 or block_table.shape[1] < 1:
+    def _batch(self, tokens: int, seq_start, seq_pos0, block_table, max_new: int, max_len: int, kv_len=None) -> bytes:
+        if block_table.dim() != 2:
             raise ValueError("block_table must be [sequences, pages]")
         n, pages = block_table.shape
-        if tokens < 1 or max_new < 1 or max_len < 1:
-            raise ValueError("a batch needs at least one row, max_new and max_len at least 1")
-        return _capi_lm.SmolLmCache8Batch(tokens, n, pages, max_new, max_len, self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"),
-                                          self._ints(block_table, (n, pages), "block_table"), None if kv_len is None else self._ints(kv_len, (n,), "kv_len"))
+        if tokens < 1 or n < 1 or pages < 1 or max_new < 1 or max_len < 1:
+            raise ValueError("a batch needs at least one row, sequence and page, max_new and max_len at least 1")
+        return _BATCH.pack(tokens, n, pages, max_new, max_len, self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"),
+                           self._ints(block_table, (n, pages), "block_table"), 0 if kv_len is None else self._ints(kv_len, (n,), "kv_len"))
 
     def _call(self, call, *args) -> None:
         """On the cache's device and its current stream."""
-        index = self.device.index
-        if index == torch.cuda.current_device():
-            rc = call(*args, torch.cuda.current_stream().cuda_stream)
+        if self._index == torch._C._cuda_getDevice():      # (a few tenths of a microsecond; torch.cuda's own two functions take four)
+            rc = call(self._c, *args, torch._C._cuda_getCurrentRawStream(self._index))
         else:
-            with torch.cuda.device(index):
-                rc = call(*args, torch.cuda.current_stream().cuda_stream)
+            with torch.cuda.device(self._index):
+                rc = call(self._c, *args, torch._C._cuda_getCurrentRawStream(self._index))
         if rc != SMOL_OK:
             _capi_lm.check(rc)
 
@@ -122,33 +136,35 @@ class KVCache8:
         A block's 16 positions share the smallest power of two with |value| <= 448 * scale; where an earlier call began the block the
         scale never shrinks, and the older codes follow it when it grows.  Magnitudes above 2^100 are clamped; a NaN stays a NaN.  Two
         sequences of a batch must not write the same page.  The rows of a sequence have to follow what it already holds."""
-        k_row, k_head = self._rows(k, self.kv_heads, self.dim, "k")
-        v_row, v_head = self._rows(v, self.kv_heads, self.vdim, "v")
-        tokens = k.shape[0]
-        if v.shape[0] != tokens or v.dtype != k.dtype:
-            raise ValueError("k and v must have the same rows and type")
+        tokens, dtype = k.shape[0], k.dtype
+        k_row, k_head = self._rows(k, None, self.kv_heads, self.dim, None, "k")
+        v_row, v_head = self._rows(v, tokens, self.kv_heads, self.vdim, dtype, "v")
         batch = self._batch(tokens, seq_start, seq_pos0, block_table, max_new, max_new)
-        a = _capi_lm.SmolLmCache8Append(dtype=_DTYPES[k.dtype], k=k.data_ptr(), v=v.data_ptr(), k_row=k_row, k_head=k_head, v_row=v_row, v_head=v_head,
-                                        rot_half=1 if rot_half else 0, rot_mult=rot_mult)
+        pairs = freq_ptr = heads = q_ptr = q_row = q_head = out_ptr = out_row = out_head = 0
         if freq is not None:
             if freq.dim() != 1 or 2 * freq.shape[0] > self.dim:
                 raise ValueError(f"freq must be [pairs] with at most {self.dim // 2} pairs")
-            a.rot_dims, a.freq = 2 * freq.shape[0], self._floats(freq, freq.shape[0], "freq")
+            pairs = freq.shape[0]
+            freq_ptr = self._floats(freq, pairs, "freq") if pairs else 0
         if q is not None:
-            a.q_row, a.q_head = self._rows(q, None, self.dim, "q")
-            if q.shape[0] != tokens or q.dtype != k.dtype or q.shape[1] < 1:
-                raise ValueError("q must have k's rows and type")
+            q_row, q_head = self._rows(q, tokens, None, self.dim, dtype, "q")
+            heads = q.shape[1]
+            if heads < 1:
+                raise ValueError("q without heads")
             if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            elif q_out.dtype != q.dtype or q_out.shape[0] != tokens:
-                raise ValueError("q_out must have q's rows and type")
-            elif q_out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
-                raise ValueError("q_out must not share q's memory: a row is read while others are written")
-            a.heads, a.q, a.q_out = q.shape[1], q.data_ptr(), q_out.data_ptr()
-            a.q_out_row, a.q_out_head = self._rows(q_out, q.shape[1], self.dim, "q_out")
+                q_out = q.new_empty((tokens, heads, self.dim))
+                out_row, out_head = heads * self.dim, self.dim
+            else:
+                out_row, out_head = self._rows(q_out, tokens, heads, self.dim, dtype, "q_out")
+                if q_out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+                    raise ValueError("q_out must not share q's memory: a row is read while others are written")
+                if (out_row < self.dim and tokens > 1) or (out_head < self.dim and heads > 1):
+                    raise ValueError("q_out: rows must not overlap")
+            q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        self._call(self.lib.smol_lm_cache8_append, self._c, batch, a)
+        self._call(self._append, batch, _APPEND.pack(_DTYPES[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, heads, q_ptr, out_ptr, q_row, q_head,
+                                                     out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, rot_mult))
         return q_out
 
     def attend(self, q: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, max_new: int, max_len: int,
@@ -165,36 +181,37 @@ class KVCache8:
         ``max_new``: most rows a sequence brings; ``max_len``: most positions a sequence holds, the rows included (host numbers;
         the grid is chosen by them -- a longer sequence is attended to as a whole all the same, rows beyond ``max_new`` are left alone).
         Returns ``[tokens, heads, vdim]`` of q's type, in ``out`` if given; rows outside every sequence are left as they were."""
-        q_row, q_head = self._rows(q, None, self.dim, "q")
-        tokens, heads = q.shape[0], q.shape[1]
+        q_row, q_head = self._rows(q, None, None, self.dim, None, "q")
+        tokens, heads, dtype = q.shape[0], q.shape[1], q.dtype
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key/value heads")
         if window < 0 or first < 0 or not softcap >= 0.0:
             raise ValueError("window, first and softcap must not be negative")
         batch = self._batch(tokens, seq_start, seq_pos0, block_table, max_new, max_len, kv_len)
         if out is None:
-            out = torch.empty((tokens, heads, self.vdim), dtype=q.dtype, device=q.device)
-        elif out.dtype != q.dtype or out.shape[0] != tokens:
-            raise ValueError("out must have q's rows and type")
-        out_row, out_head = self._rows(out, heads, self.vdim, "out")
-        if (out_row < self.vdim and tokens > 1) or (out_head < self.vdim and heads > 1):
-            raise ValueError("out: rows must not overlap")
-        a = _capi_lm.SmolLmCache8Attend(_DTYPES[q.dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head,
-                                        self.dim ** -0.5 if scale is None else scale, softcap, 1.0, window, first, self._floats(sink, heads, "sink"),
-                                        self._floats(slope, heads, "slope"))
-        if penalty is not None:
-            a.dist_r1, a.dist_r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
-        need = C.c_size_t()
-        if self.device.index == torch.cuda.current_device():
-            rc = self.lib.smol_lm_cache8_workspace_bytes(self._c, batch, a, need)
+            out = q.new_empty((tokens, heads, self.vdim))
+            out_row, out_head = heads * self.vdim, self.vdim
         else:
-            with torch.cuda.device(self.device):
-                rc = self.lib.smol_lm_cache8_workspace_bytes(self._c, batch, a, need)
-        if rc != SMOL_OK:
-            _capi_lm.check(rc)
+            out_row, out_head = self._rows(out, tokens, heads, self.vdim, dtype, "out")
+            if (out_row < self.vdim and tokens > 1) or (out_head < self.vdim and heads > 1):
+                raise ValueError("out: rows must not overlap")
+        r1 = r2 = 0
+        if penalty is not None:
+            r1, r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
+        a = _ATTEND.pack(_DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else scale, softcap, 1.0,
+                         window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0)
+        key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first)
+        need = self._need.get(key)
+        if need is None:
+            size = C.c_size_t()
+            with torch.cuda.device(self._index):
+                _capi_lm.check(self._workspace(self._c, batch, a, C.byref(size)))
+            if len(self._need) >= 4096:
+                self._need.clear()
+            need = self._need[key] = size.value
         # of the call's own: from torch's allocator for this stream, or for the graph that is being captured
-        work = torch.empty(need.value, dtype=torch.uint8, device=self.device) if need.value else None
-        self._call(self.lib.smol_lm_cache8_attend, self._c, batch, a, work.data_ptr() if work is not None else None, need.value)
+        work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+        self._call(self._attend, batch, a, work.data_ptr() if need else None, need)
         return out
 
     # ------------------------------------------------------------------ looking in
