@@ -7,6 +7,7 @@
 #include "cache8.cuh"
 #include "cache8_append.cuh"
 #include "cache8_few.cuh"
+#include "cache8_tiles.cuh"
 #include "cache8_rows.cuh"
 #include "lm_report.h"
 #include "tmap_host.h"
@@ -68,10 +69,13 @@ static cudaError_t append_as(const AppendArgs& A, int n_sms, cudaStream_t st) {
 }
 cudaError_t append(const AppendArgs& A, bool f32, int n_sms, cudaStream_t st) { return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st); }
 
+constexpr int kFewMost = 32;      // query rows of a sequence and key/value head up to which the kernel for few rows takes them
+bool tiles_serve(const AttendArgs& A, bool f32) { return !f32 && A.b.max_new * (long long)(A.H / A.c.G) > kFewMost; }
+
 // query rows of a block of threads
 static int row_tile(const AttendArgs& A, bool f32) {
     const long long rows = A.b.max_new * (long long)(A.H / A.c.G);
-    return f32 ? kRowTile : rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
+    return f32 ? kRowTile : rows <= 4 ? 4 : rows <= 8 ? 8 : tiles_serve(A, f32) ? kTileRows : 16;
 }
 static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new * (long long)(A.H / A.c.G) + row_tile(A, f32) - 1) / row_tile(A, f32)); }
 
@@ -82,7 +86,7 @@ int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     // as many shares as the SMs hold blocks at once, none of less than 256 keys (a share of 128 is one step: 15.1 us against 15.7 for a token of 12 heads
     // at 2048 positions, appended and attended to, but twice the blocks; of 512 17.7).  More blocks than are held at once wait for whole others: 64
     // sequences at up to 8192 positions, 512 blocks, 145 us in one share, 181 in two; one at 131072 33 us in 111 shares, 42 in 128 and more.
-    const int held = f32 ? 4 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
+    const int held = f32 ? 2 : tiles_serve(A, f32) ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
     const long long want = std::min((long long)held * n_sms / base, (keys + 255) / 256);
     return (int)std::max(1ll, std::min(want, (long long)kMaxSplits));
 }
@@ -99,7 +103,7 @@ static bool codes_map(CUtensorMap* map, const uint8_t* base, int ld, size_t page
 // positions that lie together and begin at a multiple of themselves: the largest power of two that divides the page, at most a step's
 static int box_of(const Cache& c) { return std::min(c.page & -c.page, kStep); }
 
-static bool joins_in_cluster(int splits, bool f32) { return !f32 && splits > 1 && splits <= kMostCluster; }
+static bool joins_in_cluster(const AttendArgs& A, int splits, bool f32) { return !f32 && !tiles_serve(A, f32) && splits > 1 && splits <= kMostCluster; }
 
 template <int D, int RA, bool BENT>
 static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
@@ -109,7 +113,7 @@ static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
     CUtensorMap kmap, vmap;
     const int box = box_of(A.c);
     if (!codes_map(&kmap, A.c.k, A.c.ldk, A.c.k_page, A.c, box) || !codes_map(&vmap, A.c.v, A.c.ldv, A.c.v_page, A.c, box)) return cudaErrorInvalidValue;
-    return launch_cluster(joins_in_cluster(A.n_splits, false) ? A.n_splits : 1, attend_few_kernel<D, RA, BENT>, dim3(row_tiles(A, false) * A.n_splits, A.c.G, A.b.S), kFewThreads, bytes, st, A, kmap,
+    return launch_cluster(joins_in_cluster(A, A.n_splits, false) ? A.n_splits : 1, attend_few_kernel<D, RA, BENT>, dim3(row_tiles(A, false) * A.n_splits, A.c.G, A.b.S), kFewThreads, bytes, st, A, kmap,
                           vmap, box);
 }
 template <int D, int RA>
@@ -132,11 +136,25 @@ static cudaError_t attend_rows(const AttendArgs& A, cudaStream_t st) {
     return d <= 64 ? rows_of<64>(A, st) : d <= 128 ? rows_of<128>(A, st) : rows_of<256>(A, st);
 }
 
-bool tiles_serve(const AttendArgs& A, bool f32) { return false; }
+template <int DK, bool BENT>
+static cudaError_t tiles_as(const AttendArgs& A, cudaStream_t st) {
+    static std::atomic<uint64_t> asked{0};
+    constexpr int bytes = tile_smem(DK);
+    if (cudaError_t e = more_smem(attend_tiles_kernel<DK, BENT>, bytes, asked)) return e;
+    CUtensorMap kmap, vmap;
+    const int box = box_of(A.c);
+    if (!codes_map(&kmap, A.c.k, A.c.ldk, A.c.k_page, A.c, box) || !codes_map(&vmap, A.c.v, A.c.ldv, A.c.v_page, A.c, box)) return cudaErrorInvalidValue;
+    return launch(attend_tiles_kernel<DK, BENT>, dim3(row_tiles(A, false) * ((A.c.dv + 127) / 128) * A.n_splits, A.c.G, A.b.S), kTileThreads, bytes, st, A, kmap, vmap, box);
+}
+static cudaError_t attend_tiles(const AttendArgs& A, cudaStream_t st) {
+    if (A.c.d <= 128) return plain_scores(A) ? tiles_as<128, false>(A, st) : tiles_as<128, true>(A, st);
+    return plain_scores(A) ? tiles_as<256, false>(A, st) : tiles_as<256, true>(A, st);
+}
+
 cudaError_t attend(const AttendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st) {
-    if (cudaError_t e = f32 ? attend_rows(A, st) : attend_few(A, st)) return e;
+    if (cudaError_t e = f32 ? attend_rows(A, st) : tiles_serve(A, f32) ? attend_tiles(A, st) : attend_few(A, st)) return e;
     *launches += 1;
-    if (A.n_splits == 1 || joins_in_cluster(A.n_splits, f32)) return cudaSuccess;
+    if (A.n_splits == 1 || joins_in_cluster(A, A.n_splits, f32)) return cudaSuccess;
     *launches += 1;
     return f32 ? launch(attend_join_kernel<float>, A.b.T * A.H, kJoinWarps * 32, 0, st, A) : launch(attend_join_kernel<bf16>, A.b.T * A.H, kJoinWarps * 32, 0, st, A);
 }
@@ -246,8 +264,8 @@ extern "C" int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const S
     int n_sms = 0;
     if (int rc = n_sms_of_device(&n_sms)) return rc;
     const bool f32 = a->dtype == SMOL_LM_F32;
-    const int splits = tiles_serve(A, f32) ? 1 : splits_for(A, f32, n_sms);
-    *bytes = splits == 1 || joins_in_cluster(splits, f32) ? 0 : part_bytes(A, splits);
+    const int splits = splits_for(A, f32, n_sms);
+    *bytes = splits == 1 || joins_in_cluster(A, splits, f32) ? 0 : part_bytes(A, splits);
     return SMOL_OK;
 }
 
@@ -257,12 +275,10 @@ extern "C" int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCach
     int n_sms = 0, launches = 0;
     if (int rc = n_sms_of_device(&n_sms)) return rc;
     const bool f32 = a->dtype == SMOL_LM_F32;
-    if (!tiles_serve(A, f32)) {
-        A.n_splits = splits_for(A, f32, n_sms);
-        if (A.n_splits > 1 && !joins_in_cluster(A.n_splits, f32) && (!workspace || !aligned(workspace, 16) || workspace_bytes < part_bytes(A, A.n_splits)))
-            return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
-        A.part = static_cast<float*>(workspace);
-    }
+    A.n_splits = splits_for(A, f32, n_sms);
+    if (A.n_splits > 1 && !joins_in_cluster(A, A.n_splits, f32) && (!workspace || !aligned(workspace, 16) || workspace_bytes < part_bytes(A, A.n_splits)))
+        return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
+    A.part = static_cast<float*>(workspace);
     const cudaError_t e = attend(A, f32, n_sms, &launches, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SMOL_OK : report(SMOL_ERR_CUDA, "smol_lm_cache8_attend", cudaGetErrorString(e));
 }

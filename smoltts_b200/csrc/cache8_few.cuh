@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     volatile int* stop = &bars.stop;
 
     if (warp == kFewCopies) {
-        copy_steps<HALVES, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop);
+        copy_steps<HALVES, HALVES, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, 0);
     } else if (warp == kFewProducts) {
         if (lane == 0 && steps > 0) {
             // ---- products: whichever can be made next, so that neither the keys' waits for the weights nor the values' (and the stage they free) for the

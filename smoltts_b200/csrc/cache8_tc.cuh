@@ -122,13 +122,13 @@ struct StepScales {
     float k[kStepBlocks], v[kStepBlocks];
 };
 
-// The copying warp: keys and values of every step into a ring of NS stages (keys: HALVES tiles of 128 positions by 128 bytes, then the values'), 128-byte
-// swizzle, in boxes of `box` positions that lie together.  Lane x < 8 looks up block x of a step; entries are loaded two steps ahead and scales one,
+// The copying warp: keys and values of every step into a ring of NS stages (keys: KH tiles of 128 positions by 128 bytes, then VH of the values from
+// column v_col on), 128-byte swizzle, in boxes of `box` positions that lie together.  Lane x < 8 looks up block x of a step; entries are loaded two steps ahead and scales one,
 // so that nothing waits for them here.
-template <int HALVES, int NS>
+template <int KH, int VH, int NS>
 __device__ __forceinline__ void copy_steps(const AttendArgs& A, const CUtensorMap* kmap, const CUtensorMap* vmap, int box, const Rows& W, const Seen& seen, int lo, int steps, int first_pos,
-                                           unsigned char* ring, StepScales* scales, uint64_t* full, uint64_t* empty, volatile int* stop) {
-    constexpr int SB = kStep * 256 * HALVES;
+                                           unsigned char* ring, StepScales* scales, uint64_t* full, uint64_t* empty, volatile int* stop, int v_col) {
+    constexpr int SB = kStep * 128 * (KH + VH);
     const int lane = threadIdx.x & 31, per = box / kBlock;
     struct Entry { int page, in_page, seen; };      // in_page < 0: nobody sees the block's box; seen: the block itself
     auto near = [&](int j, int n) { return j < seen.end && (A.window == 0 || j + n > first_pos - A.window + 1 || j < A.first); };
@@ -170,14 +170,14 @@ __device__ __forceinline__ void copy_steps(const AttendArgs& A, const CUtensorMa
             scales[st].v[lane] = sc.y;
         }
         __syncwarp();
-        if (lane == 0) umma::bar_expect_tx(&full[st], (uint32_t)(live * box * 256 * HALVES));
+        if (lane == 0) umma::bar_expect_tx(&full[st], (uint32_t)(live * box * 128 * (KH + VH)));
         __syncwarp();
         if (mine) {
             const uint32_t to = umma::s2u(ring + st * SB) + lane * kBlock * 128;
 #pragma unroll
-            for (int x = 0; x < HALVES; ++x) load_box(to + x * (kStep * 128), kmap, 128 * x, W.g * A.c.page + now.in_page, now.page, &full[st]);
+            for (int x = 0; x < KH; ++x) load_box(to + x * (kStep * 128), kmap, 128 * x, W.g * A.c.page + now.in_page, now.page, &full[st]);
 #pragma unroll
-            for (int x = 0; x < HALVES; ++x) load_box(to + (HALVES + x) * (kStep * 128), vmap, 128 * x, W.g * A.c.page + now.in_page, now.page, &full[st]);
+            for (int x = 0; x < VH; ++x) load_box(to + (KH + x) * (kStep * 128), vmap, v_col + 128 * x, W.g * A.c.page + now.in_page, now.page, &full[st]);
         }
         issued = i + 1;
         now = next;

@@ -1,0 +1,394 @@
+// Attention over the 8-bit key/value cache for many bf16 query rows per sequence (prompts), on tcgen05.  Included by cache8.cu.
+//
+// One block of threads per (128 query rows of a sequence and key/value head, 128 columns of the values, key/value head, sequence, share of the keys).
+// The rows are the step's tokens times the query heads that share the key/value head: what is staged once serves all of them, and a short
+// portion fills a tile.  128 positions a step.  As for few rows (cache8_few.cuh) the codes go to the tensor cores as they are, and queries and
+// weights are the sum of two e4m3 parts; here both parts have one unit and one accumulator, so that a product is eight instructions for 128 terms,
+// as many cycles as bf16 operands would take.  That leaves a query's coordinates exact down to 2^-10 of the row's largest and 2^-18 of it
+// below, and a weight's error at 2^-9, or 2^-18 of the row's largest in the step.
+//
+// Roles: a warp that copies, a thread that issues the products, sixteen warps for the softmax: four threads per row, 32 columns of the scores and of
+// the result each.  Scores are double-buffered in tensor memory, so that the next step's are multiplied while this step's are worked on; a step's product
+// with the values is read back while the next one's is made, and joins the fp32 running results in registers.  Value codes that are NaN are
+// cleaned away in steps that some row does not see as a whole, as for few rows.
+#pragma once
+
+#include "cache8_tc.cuh"
+
+namespace smol {
+namespace c8 {
+
+constexpr int kTileRows = 128, kTileParts = 4, kTileCols = kStep / kTileParts, kTileSoft = 4 * kTileParts, kTileThreads = (kTileSoft + 2) * 32;
+__host__ __device__ constexpr int tile_stages(int DK) { return DK <= 128 ? 3 : 2; }
+__host__ __device__ constexpr int tile_weights(int DK) { return DK <= 128 ? 2 : 1; }      // buffers of weights
+__host__ __device__ constexpr int tile_stage_bytes(int DK) { return kStep * (DK + 128); }
+__host__ __device__ constexpr int tile_smem(int DK) { return 1024 + 2 * kTileRows * DK + tile_stages(DK) * tile_stage_bytes(DK) + tile_weights(DK) * 2 * kTileRows * 128; }
+
+struct TileBars {
+    uint64_t full[3], empty[3];      // stages
+    uint64_t s_full[2], s_empty[2];  // scores in tensor memory
+    uint64_t p_full[2], o_full[2];   // weights in shared memory; their product in tensor memory
+    uint64_t q_full, drained;
+    uint32_t tmem;
+    int stop;
+};
+
+// Two f16 numbers of magnitude at most 256 as e4m3 parts of one unit: hi + lo
+__device__ __forceinline__ void two_equal_parts(__half2 x, uint32_t& hi, uint32_t& lo) {
+    hi = __nv_cvt_halfraw2_to_fp8x2((__half2_raw)x, __NV_SATFINITE, __NV_E4M3);
+    const __half2_raw rest = __hsub2(x, __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi, __NV_E4M3)));
+    lo = __nv_cvt_halfraw2_to_fp8x2(rest, __NV_SATFINITE, __NV_E4M3);
+}
+
+// Columns col .. col + 31 (a bit each) of the values in which a row at `pos` sees a NaN.  Rare, and slow.
+__device__ __noinline__ uint32_t nan_bits(const AttendArgs& A, const Rows& W, int pos, int col) {
+    uint32_t bits = 0;
+    for (int b = 0; b * kBlock < min(W.end, pos + 1); ++b) {
+        const int pg = b * kBlock / A.c.page;
+        const int page = pg < A.b.max_pages ? A.b.table[(size_t)W.s * A.b.max_pages + pg] : -1;
+        if (page < 0 || page >= A.c.n_pages) continue;
+        const int in_page = b * kBlock - pg * A.c.page;
+        if (A.c.vs[(size_t)page * A.c.vs_page + W.g * (A.c.page / kBlock) + in_page / kBlock] >= 0.0f) continue;
+        for (int i = 0; i < kBlock; ++i) {
+            if (!sees(A, pos, b * kBlock + i, W.end)) continue;
+            const uint8_t* v = A.c.v + (size_t)page * A.c.v_page + ((size_t)W.g * A.c.page + in_page + i) * A.c.ldv + col;
+            for (int c = 0; c < 32 && col + c < A.c.dv; ++c)
+                if ((v[c] & 0x7f) == 0x7f) bits |= 1u << c;
+        }
+    }
+    return bits;
+}
+
+// DK: key size padded
+template <int DK, bool BENT>
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
+    constexpr int NS = tile_stages(DK), SB = tile_stage_bytes(DK), KH = DK / 128, PB = tile_weights(DK);
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TileBars bars;
+    __shared__ StepScales s_scales[NS];
+    __shared__ float s_max[2][kTileParts][kTileRows], s_rowmul[kTileRows];
+    __shared__ int s_bad;
+    unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    unsigned char *KV = base, *Qs = KV + NS * SB, *Ps = Qs + 2 * kTileRows * DK;      // Qs, Ps: first parts, then second parts
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < NS; ++i) { umma::bar_init(&bars.full[i], 1); umma::bar_init(&bars.empty[i], 1); }
+        for (int i = 0; i < 2; ++i) {
+            umma::bar_init(&bars.s_full[i], 1);
+            umma::bar_init(&bars.s_empty[i], kTileSoft);
+            umma::bar_init(&bars.p_full[i], kTileSoft);
+            umma::bar_init(&bars.o_full[i], 1);
+        }
+        umma::bar_init(&bars.q_full, kTileSoft);
+        umma::bar_init(&bars.drained, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&kmap), "l"(&vmap) : "memory");
+        bars.stop = 0;
+        s_bad = 0;
+    }
+    if (warp == kTileSoft + 1) tmem_take<512>(&bars.tmem);
+    dep_wait();
+    const int Gq = A.H / A.c.G, v_halves = (A.c.dv + 127) / 128, tiles = gridDim.x / (A.n_splits * v_halves);
+    const int split = blockIdx.x % A.n_splits, v_col = blockIdx.x / A.n_splits % v_halves * 128, tile = tiles - 1 - blockIdx.x / (A.n_splits * v_halves);      // the tiles with the most keys first
+    const int s = blockIdx.z, g = blockIdx.y;
+    const int t0 = A.b.start[s], n_all = A.b.start[s + 1] - t0, n = min(n_all, A.b.max_new), pos0 = A.b.pos0[s];
+    const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
+    const int row0 = tile * kTileRows, rows = min(n * Gq - row0, kTileRows);
+    const bool any = rows > 0 && t0 >= 0 && t0 + n_all <= A.b.T;
+    const int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq;
+    const Seen seen = seen_steps(A, first_pos, last_pos, kv_len);
+    const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
+    const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = min(split * share, seen.count);
+    const int steps = any ? min(lo + share, seen.count) - lo : 0;
+    umma::fence_before_sync();
+    __syncthreads();
+    umma::fence_after_sync();
+    dep_go();      // behind the allocation: a kernel set up early that wants tensor memory too must not get it first
+    const uint32_t tmem = bars.tmem, tm_o = tmem + 2 * kStep;      // scores of even and odd steps, then products likewise
+    volatile int* stop = &bars.stop;
+
+    if (warp == kTileSoft) {
+        copy_steps<KH, 1, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, v_col);
+    } else if (warp == kTileSoft + 1) {
+        if (lane == 0 && steps > 0) {
+            // ---- products: whichever can be made next ----
+            const uint32_t q0 = umma::s2u(Qs), id_s = desc_e4m3(128, kStep, false, false), id_o = desc_e4m3(128, 128, false, true);
+            const int ksteps = (A.c.d + 31) / 32;
+            int scores = 0, values = 0;      // steps whose product has been issued
+            bool ok = wait_bar(&bars.q_full, 0, stop, A.c.err);
+            long long begin = clock64();
+            while (ok && values < steps) {
+                if (scores < steps && passed(&bars.full[scores % NS], (scores / NS) & 1) && (scores < 2 || passed(&bars.s_empty[scores & 1], ((scores >> 1) - 1) & 1))) {
+                    const int b = scores & 1, st = scores % NS;
+                    umma::fence_after_sync();
+                    const uint32_t k0 = umma::s2u(KV + st * SB);
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+                        for (int k = 0; k < ksteps; ++k)
+                            mma_e4m3(tmem + b * kStep, umma::smem_desc_sw128(q0 + (part * KH + (k >> 2)) * (kTileRows * 128) + (k & 3) * 32), umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32),
+                                     id_s, part > 0 || k > 0 ? 1u : 0u);
+                    umma::commit(&bars.s_full[b]);
+                    ++scores;
+                    begin = clock64();
+                } else if (values < scores && passed(&bars.p_full[values & 1], (values >> 1) & 1)) {
+                    const int b = values & 1, st = values % NS;
+                    umma::fence_after_sync();
+                    const uint32_t v = umma::s2u(KV + st * SB) + KH * (kStep * 128), p = umma::s2u(Ps + (PB == 2 ? b : 0) * (2 * kTileRows * 128));
+#pragma unroll
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int k = 0; k < kStep / 32; ++k)
+                            mma_e4m3(tm_o + b * 128, umma::smem_desc_sw128(p + part * (kTileRows * 128) + k * 32), umma::smem_desc_sw128(v + k * 32 * 128), id_o, part > 0 || k > 0 ? 1u : 0u);
+                    umma::commit(&bars.empty[st]);
+                    umma::commit(&bars.o_full[b]);
+                    ++values;
+                    begin = clock64();
+                } else if (*stop || clock64() - begin > kWaitCycles) {
+                    if (!*stop) atomicExch(A.c.err, 3);
+                    *stop = 1;
+                    ok = false;
+                }
+            }
+            umma::commit(&bars.drained);      // nothing of the block's is in flight once this is through
+            drain_bar(&bars.drained, 0);
+        }
+    } else if (steps > 0) {
+        // ---- queries into shared memory, a warp per row ----
+#pragma unroll 2
+        for (int r = warp; r < kTileRows; r += kTileSoft) {
+            const int row = min(row0 + r, n * Gq - 1), h = g * Gq + row % Gq;
+            const bf16* q = static_cast<const bf16*>(A.q) + (size_t)(t0 + row / Gq) * A.q_row + (size_t)h * A.q_head;
+            float v[KH][4];
+            uint32_t top = 0;
+#pragma unroll
+            for (int x = 0; x < KH; ++x) {
+                const int at = x * 128 + lane * 4;
+                if (A.q_vec) {
+                    const uint2 u = at < A.c.d ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0u, 0u);
+                    v[x][0] = bf_lo(u.x); v[x][1] = bf_hi(u.x); v[x][2] = bf_lo(u.y); v[x][3] = bf_hi(u.y);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[x][e] = at + e < A.c.d ? __bfloat162float(q[at + e]) : 0.0f;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[x][e])));
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            const int e = max((int)(top >> 23) - 127, -110);      // (below: rows of less than 2^-110 keep a factor that fp32 holds)
+            const float up = pow2(7 - e);
+#pragma unroll
+            for (int x = 0; x < KH; ++x) {
+                uint32_t hi[2], part[2];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) two_equal_parts(__floats2half2_rn(v[x][2 * y] * up, v[x][2 * y + 1] * up), hi[y], part[y]);
+                *reinterpret_cast<uint32_t*>(Qs + x * (kTileRows * 128) + sw128_byte(r, lane * 4)) = hi[0] | (hi[1] << 16);
+                *reinterpret_cast<uint32_t*>(Qs + (KH + x) * (kTileRows * 128) + sw128_byte(r, lane * 4)) = part[0] | (part[1] << 16);
+            }
+            // (a row that is not finite: every score of it is a NaN)
+            if (lane == 0) s_rowmul[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 7) * (A.scale * (BENT ? 1.0f : kLog2e));
+        }
+        umma::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) arrive(&bars.q_full);
+        asm volatile("bar.sync 5, %0;" ::"n"(kTileSoft * 32) : "memory");
+
+        // ---- softmax: warps q, q + 4, q + 8, q + 12 share rows 32 q .. + 31; part p has columns 32 p .. + 31 of the scores and of the result ----
+        const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane, my_row = min(row0 + row, n * Gq - 1), pos = pos0 + my_row / Gq, h = g * Gq + my_row % Gq;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+        const float rowmul = s_rowmul[row], r1 = BENT && A.r1 ? A.r1[h] : 0.0f, r2 = BENT && A.r1 ? A.r2[h] : 0.0f, slope = BENT && A.slope ? A.slope[h] : 0.0f;
+        auto row_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(quad + 1), "n"(kTileParts * 32) : "memory"); };
+        float m = -INFINITY, l = 0.0f, m_step = -INFINITY, l_step = 0.0f, unit = 0.0f, o[kTileCols];
+#pragma unroll
+        for (int c = 0; c < kTileCols; ++c) o[c] = 0.0f;
+        auto join_product = [&](int i) {
+            const int b = i & 1;
+            wait_bar(&bars.o_full[b], (i >> 1) & 1, stop, A.c.err);
+            __syncwarp();
+            umma::fence_after_sync();
+            const float mn = fmaxf(m, m_step), keep = m == mn ? 1.0f : exp2_fast(m - mn);
+            float add = m_step == -INFINITY ? 0.0f : exp2_fast(m_step - mn);
+            m = mn;
+            l = fmaf(l_step, add, l * keep);
+            add *= unit;
+#pragma unroll
+            for (int x = 0; x < kTileCols / 16; ++x) {
+                uint32_t v[2][8];
+                umma::tmem_ld8_issue(tm_o + b * 128 + part * kTileCols + 16 * x + lanes, v[0]);
+                umma::tmem_ld8_issue(tm_o + b * 128 + part * kTileCols + 16 * x + 8 + lanes, v[1]);
+                umma::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[16 * x + e] = fmaf(__uint_as_float(v[e / 8][e % 8]), add, o[16 * x + e] * keep);
+            }
+            umma::fence_before_sync();
+        };
+        for (int i = 0; i < steps; ++i) {
+            const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), jc = j0 + part * kTileCols;
+            // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
+            wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
+            float ks[2], vs[2], v_top = 0.0f;
+            bool nans = false, holes = false;      // in the whole step
+#pragma unroll
+            for (int x = 0; x < kStepBlocks; ++x) {
+                const float v = s_scales[st].v[x];
+                v_top = fmaxf(v_top, fabsf(v));
+                nans |= v < 0.0f;
+                holes |= v == 0.0f;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                ks[x] = s_scales[st].k[2 * part + x];
+                vs[x] = fabsf(s_scales[st].v[2 * part + x]);
+            }
+            wait_bar(&bars.s_full[b], (i >> 1) & 1, stop, A.c.err);
+            __syncwarp();
+            umma::fence_after_sync();
+            float S[kTileCols];
+            {
+                uint32_t v[kTileCols / 8][8];
+#pragma unroll
+                for (int x = 0; x < kTileCols / 8; ++x) umma::tmem_ld8_issue(tmem + b * kStep + part * kTileCols + 8 * x + lanes, v[x]);
+                umma::tmem_ld_wait();
+#pragma unroll
+                for (int e = 0; e < kTileCols; ++e) S[e] = __uint_as_float(v[e / 8][e % 8]);
+            }
+            umma::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) arrive(&bars.s_empty[b]);
+            const bool whole = !holes && j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
+            // scores in units of log2: S times mul
+            const bool direct = !BENT && whole && A.scale > 0.0f;
+            float mul[2] = {rowmul * ks[0], rowmul * ks[1]};
+            if (!direct) {
+#pragma unroll
+                for (int e = 0; e < kTileCols; ++e) {
+                    S[e] *= mul[e / kBlock];
+                    if (BENT) S[e] = bent_score<false>(A, S[e], pos - (jc + e), r1, r2, slope);
+                }
+                mul[0] = mul[1] = 1.0f;
+            }
+            if (!whole) {
+                const int far = A.window > 0 ? A.window : 0x7fffffff, last = min(pos + 1, seen.end) - jc, lead = A.first - jc, dist = pos - jc;
+#pragma unroll
+                for (int e = 0; e < kTileCols; ++e)
+                    if (e >= last || ks[e / kBlock] == 0.0f || (dist - e >= far && e >= lead)) S[e] = -INFINITY;
+            }
+            if (!whole || nans) {
+                // the step's value codes without NaNs, 32 bytes a thread
+                if (nans) s_bad = 1;
+#pragma unroll 1
+                for (int x = threadIdx.x; x < kStep * 8; x += kTileSoft * 32) {
+                    uint4& at = reinterpret_cast<uint4*>(KV + st * SB + KH * (kStep * 128))[x];
+                    const uint4 w = at, z = make_uint4(without_nans(w.x), without_nans(w.y), without_nans(w.z), without_nans(w.w));
+                    if (w.x != z.x || w.y != z.y || w.z != z.z || w.w != z.w) at = z;
+                }
+            }
+            // ---- the row's maximum over the step ----
+            float top = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float t[4] = {S[16 * x], S[16 * x + 1], S[16 * x + 2], S[16 * x + 3]};
+#pragma unroll
+                for (int e = 4; e < 16; ++e) t[e % 4] = fmaxf(t[e % 4], S[16 * x + e]);
+                top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * mul[x]);
+            }
+            s_max[b][part][row] = top;
+            row_barrier();
+            top = fmaxf(fmaxf(s_max[b][0][row], s_max[b][1][row]), fmaxf(s_max[b][2][row], s_max[b][3][row]));
+            if (PB == 1 && i > 0) join_product(i - 1);      // (its weights lie where this step's go)
+            // ---- weights, times 256 and the block's share of the largest value scale ----
+            const float under = (top == -INFINITY ? 0.0f : top) - 8.0f;
+            unsigned char* P = Ps + (PB == 2 ? b : 0) * (2 * kTileRows * 128) + row * 128;
+            float sum = 0.0f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const __half2 ratio = __float2half2_rn(vs[x] / fmaxf(v_top, kLeastScale));      // a power of two (0 below 2^-24)
+                float sums[2] = {0.0f, 0.0f};
+                uint32_t hi[4], rest[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    uint32_t a[2], c[2];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        const float p0 = exp2_fast(fmaf(S[16 * x + 4 * y + 2 * z], mul[x], -under)), p1 = exp2_fast(fmaf(S[16 * x + 4 * y + 2 * z + 1], mul[x], -under));
+                        sums[z] += p0 + p1;
+                        two_equal_parts(__hmul2(__floats2half2_rn(p0, p1), ratio), a[z], c[z]);
+                    }
+                    hi[y] = a[0] | (a[1] << 16);
+                    rest[y] = c[0] | (c[1] << 16);
+                }
+                sum += sums[0] + sums[1];
+                unsigned char* to = P + (((2 * part + x) ^ (row & 7)) << 4);
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                *reinterpret_cast<uint4*>(to + kTileRows * 128) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+            }
+            umma::fence_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive(&bars.p_full[b]);
+            if (PB == 2 && i > 0) join_product(i - 1);
+            m_step = top;
+            l_step = sum * (1.0f / 256.0f);
+            unit = v_top * (1.0f / 256.0f);
+        }
+        join_product(steps - 1);
+        // ---- the row's denominator, then 32 columns a thread ----
+        row_barrier();
+        s_max[0][part][row] = l;
+        row_barrier();
+        const float total = (s_max[0][0][row] + s_max[0][1][row]) + (s_max[0][2][row] + s_max[0][3][row]);
+        const int col = v_col + part * kTileCols;
+        if (row < rows && col < A.c.dv && !*stop) {
+            const int tok = t0 + my_row / Gq;
+            const uint32_t bits = s_bad ? nan_bits(A, W, pos, col) : 0u;
+#pragma unroll
+            for (int c = 0; c < kTileCols; ++c)
+                if (bits >> c & 1) o[c] = __int_as_float(0x7fffffff);
+            if (A.n_splits > 1) {
+                const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
+                if (col == 0) part_stats(A)[at] = make_float2(m, total);
+                float* to = A.part + at * ((A.c.dv + 3) / 4 * 4) + col;
+#pragma unroll
+                for (int c = 0; c < kTileCols; ++c)
+                    if (col + c < A.c.dv) to[c] = o[c];
+            } else {
+                bf16* to = static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col;
+                // one division a row
+                const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, m);
+                const float f = m == -INFINITY ? 1.0f : exp2_fast(m - M), all = fmaf(total, f, M == -INFINITY ? 0.0f : exp2_fast(sink - M)), r = all == 0.0f ? 1.0f : f / all;
+                if (A.o_vec && !A.gate) {
+#pragma unroll
+                    for (int c = 0; c < kTileCols; c += 4)
+                        if (col + c < A.c.dv) {
+                            float v[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = o[c + e] * r * A.out_scale;
+                            *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+                        }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kTileCols; ++c)
+                        if (col + c < A.c.dv) to[c] = __float2bfloat16_rn(finished(A, tok, h, col + c, o[c] * r));
+                }
+            }
+        }
+    } else if (any) {
+        // no key in this share
+        for (int i = threadIdx.x; i < rows * 128; i += kTileSoft * 32) {
+            const int row = i / 128, col = v_col + i % 128, tok = t0 + (row0 + row) / Gq, h = g * Gq + (row0 + row) % Gq;
+            if (col >= A.c.dv) continue;
+            if (A.n_splits > 1) {
+                const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
+                if (col == 0) part_stats(A)[at] = make_float2(-INFINITY, 0.0f);
+                A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = 0.0f;
+            } else {
+                static_cast<bf16*>(A.out)[(size_t)tok * A.o_row + (size_t)h * A.o_head + col] = __float2bfloat16_rn(0.0f);
+            }
+        }
+    }
+    __syncwarp();
+    umma::fence_before_sync();
+    __syncthreads();
+    if (warp == kTileSoft + 1) tmem_give<512>(tmem);
+}
+
+}  // namespace c8
+}  // namespace smol
