@@ -49,7 +49,7 @@ struct AppendArgs {
     const float* freq;
     int pairs, half;
     float mult;
-    int k_vec, v_vec, q_vec;         // rows are whole, aligned groups of four elements
+    int k_vec, v_vec, q_vec;         // rows are whole groups of eight elements, on 16-byte boundaries
 };
 
 struct AttendArgs {
