@@ -239,6 +239,8 @@ typedef struct SmolLmLayer {
      *     m <- max(f + m, i), S <- exp(f + m_old - m) S + exp(i - m) k v^T, n likewise with k alone, q times score_scale,
      *     o = S^T q / (max(|n.q|, exp(-m)) + den_eps); RMS division per head, times out_norm [heads*vdim], times sigmoid(gate) --- */
     float gate_cap, den_eps;
+    /* --- softmax attention over a cache in 8 bits (SmolLmConfig.kv_bits 8) with a window: the sequence's first positions that stay visible --- */
+    int32_t first_visible;
 } SmolLmLayer;
 
 typedef struct SmolLmConfig {
@@ -261,6 +263,8 @@ typedef struct SmolLmConfig {
     const int32_t* run_flags; /* HOST array [n_runs] of SMOL_LM_RUN_* bits, copied by create (NULL: none set) */
     float residual_mult;      /* parallel block */
     float logit_softcap;      /* logits <- logit_softcap * tanh(logits / logit_softcap) after logit_scale (0: none) */
+    int32_t kv_bits;          /* cached keys and values: 0 or 16 = the engine's element type; 8 = e4m3 codes with a power-of-two scale per 16 positions and
+                                 head (SmolLmCache8): softmax attention of one map with heads of at most 256 only, page_size a multiple of 16 */
 } SmolLmConfig;
 
 typedef struct SmolLmGlobals {

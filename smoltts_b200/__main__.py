@@ -19,13 +19,22 @@ def _dtype(name: str):
     return {"bfloat16": torch.bfloat16, "float32": torch.float32}[name]
 
 
+def _cache(a) -> dict:
+    return {"kv_bits": 8, "first_tokens": a.first_tokens} if a.kv_bits == 8 else {}
+
+
+def _cache_arguments(p) -> None:
+    p.add_argument("--kv-bits", type=int, choices=[8, 16], default=16, help="8: cached keys and values as e4m3 codes with block scales")
+    p.add_argument("--first-tokens", type=int, default=0, help="with --kv-bits 8: first positions that windowed layers go on seeing")
+
+
 def cmd_generate(a) -> int:
     from .registry import load_model
     from .serving import TokenBatcher
 
     prompts = [[int(t) for t in p.split(",")] for p in a.prompt]
     longest = max(len(p) for p in prompts) + a.max_new_tokens
-    model = load_model(a.model, dtype=_dtype(a.dtype), max_tokens=a.max_tokens or 4 * (longest + 64), max_seqs=a.max_seqs)
+    model = load_model(a.model, dtype=_dtype(a.dtype), max_tokens=a.max_tokens or 4 * (longest + 64), max_seqs=a.max_seqs, **_cache(a))
     batcher = TokenBatcher(model, temp=a.temp, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed, eos_id=a.eos)
     for p, out in zip(prompts, batcher.generate(prompts, a.max_new_tokens)):
         print(json.dumps({"prompt": p, "tokens": out}))
@@ -41,7 +50,7 @@ def cmd_trace(a) -> int:
     from .serving import TokenBatcher
 
     try:
-        model = load_model(a.model, dtype=_dtype(a.dtype), max_tokens=a.max_tokens, max_seqs=a.max_seqs)
+        model = load_model(a.model, dtype=_dtype(a.dtype), max_tokens=a.max_tokens, max_seqs=a.max_seqs, **_cache(a))
     except TypeError:
         print("this design's engine does not take explicit-token steps", file=sys.stderr)
         return 4
@@ -83,6 +92,7 @@ def main(argv=None) -> int:
     g.add_argument("--eos", type=int, default=None)
     g.add_argument("--max-tokens", type=int, default=0, help="positions of the key/value pool (default: fits the prompts)")
     g.add_argument("--max-seqs", type=int, default=4)
+    _cache_arguments(g)
     g.set_defaults(fn=cmd_generate)
     t = sub.add_parser("trace", help="replay a step schedule and write logits")
     t.add_argument("--model", required=True)
@@ -90,12 +100,15 @@ def main(argv=None) -> int:
     t.add_argument("--out", required=True)
     t.add_argument("--max-tokens", type=int, required=True, help="positions live requests hold at any time (rounded up to pages)")
     t.add_argument("--max-seqs", type=int, default=4)
+    _cache_arguments(t)
     t.set_defaults(fn=cmd_trace)
     c = sub.add_parser("convert", help="trainer checkpoint -> exported checkpoint")
     c.add_argument("rest", nargs=argparse.REMAINDER)
     b = sub.add_parser("build", help="compile the CUDA libraries")
     b.add_argument("--only", choices=["core", "lm"], default=None)
     a = ap.parse_args(argv)
+    if getattr(a, "first_tokens", 0) and a.kv_bits != 8:
+        ap.error("--first-tokens needs --kv-bits 8")
     if a.cmd == "convert":
         from . import convert
 

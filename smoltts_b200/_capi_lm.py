@@ -41,7 +41,7 @@ SmolLmLayer._fields_ = [(n, C.c_int32) for n in ("mixer", "heads", "kv_heads", "
     (n, C.c_int32) for n in ("ff_plain", "group_rank_top", "shared_ff")] + [(n, C.c_void_p) for n in ("w_shared_in", "w_shared_out")] + [
     ("q_temp_coef", C.c_float), ("q_temp_every", C.c_float), ("rot_half", C.c_int32), ("router_bias", C.c_void_p), ("shared_gate", C.c_int32), ("n_maps", C.c_int32),
     ("diff_lambda", C.c_float), ("diff_scale", C.c_float), ("kv_from", C.c_int32)] + [
-    (n, C.c_float) for n in ("rot_mult", "rot_yarn", "rot_fast", "rot_slow", "gate_cap", "den_eps")]
+    (n, C.c_float) for n in ("rot_mult", "rot_yarn", "rot_fast", "rot_slow", "gate_cap", "den_eps")] + [("first_visible", C.c_int32)]
 
 
 class SmolLmConfig(C.Structure):
@@ -49,7 +49,7 @@ class SmolLmConfig(C.Structure):
                                          "max_step_seqs", "max_want", "max_context", "use_graph")] + [
         ("embed_scale", C.c_float), ("norm_eps", C.c_float), ("block", C.c_int32), ("residual_alpha", C.c_float), ("logit_scale", C.c_float),
         ("norm_plain", C.c_int32), ("norm_kind", C.c_int32), ("run_flags", C.POINTER(C.c_int32)),
-        ("residual_mult", C.c_float), ("logit_softcap", C.c_float)]
+        ("residual_mult", C.c_float), ("logit_softcap", C.c_float), ("kv_bits", C.c_int32)]
 
 
 class SmolLmGlobals(C.Structure):

@@ -72,7 +72,10 @@ static cudaError_t append_as(const AppendArgs& A, int n_sms, cudaStream_t st) {
     const int ld = std::max(A.c.ldk, A.c.ldv);
     return ld <= 64 ? append_of<T, 2>(A, grid, st) : ld <= 128 ? append_of<T, 4>(A, grid, st) : append_of<T, 8>(A, grid, st);
 }
-cudaError_t append(const AppendArgs& A, bool f32, int n_sms, cudaStream_t st) { return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st); }
+cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st) {
+    *launches += 1;
+    return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st);
+}
 
 constexpr int kFewMost = 32;      // query rows of a sequence and key/value head up to which the kernel for few rows takes them
 bool tiles_serve(const AttendArgs& A, bool f32) { return !f32 && A.b.max_new * (long long)(A.H / A.c.G) > kFewMost; }
@@ -84,7 +87,8 @@ static int row_tile(const AttendArgs& A, bool f32) {
 }
 static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new * (long long)(A.H / A.c.G) + row_tile(A, f32) - 1) / row_tile(A, f32)); }
 
-int splits_for(const AttendArgs& A, bool f32, int n_sms) {
+// shares of the keys: one block of threads each
+static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     const long long base = (long long)A.b.S * A.c.G * row_tiles(A, f32);
     long long keys = A.b.max_len;
     if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
@@ -156,17 +160,40 @@ static cudaError_t attend_tiles(const AttendArgs& A, cudaStream_t st) {
     return plain_scores(A) ? tiles_as<256, false>(A, st) : tiles_as<256, true>(A, st);
 }
 
-cudaError_t attend(const AttendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st) {
+// A batch whose sequences may bring anything from one row to many: those of few rows go to the kernel for few rows, which shares their keys out.  With short
+// contexts (a tile walks 2048 positions in 35 us) or one sequence that is not worth a launch.
+static bool mixed(const AttendArgs& A, bool f32) { return tiles_serve(A, f32) && A.b.S > 1 && A.b.max_len > 2048 && A.H / A.c.G <= kFewMost && A.rows_most > kFewMost; }
+
+size_t attend_bytes(const AttendArgs& A, bool f32, int n_sms) {
+    const int splits = splits_for(A, f32, n_sms);
+    return splits == 1 || joins_in_cluster(A, splits, f32) ? 0 : (part_floats(A, splits) + 2ull * A.b.T * A.H * splits) * sizeof(float);
+}
+// There are shares only while blocks (of at most 128 rows) times shares are no more than the SMs hold, 3 each of at most 16 rows or 1 of 128.
+size_t attend_bytes_most(int dv) { return (size_t)256 * kTileRows * ((dv + 3) / 4 * 4 + 2) * sizeof(float); }
+
+cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* launches, cudaStream_t st) {
+    AttendArgs few = A;
+    const bool two = mixed(A, f32);
+    if (two) A.rows_over = kFewMost;
+    A.n_splits = splits_for(A, f32, n_sms);
+    A.part = static_cast<float*>(workspace);
     if (cudaError_t e = f32 ? attend_rows(A, st) : tiles_serve(A, f32) ? attend_tiles(A, st) : attend_few(A, st)) return e;
     *launches += 1;
-    if (A.n_splits == 1 || joins_in_cluster(A, A.n_splits, f32)) return cudaSuccess;
+    if (A.n_splits > 1 && !joins_in_cluster(A, A.n_splits, f32)) {
+        *launches += 1;
+        if (cudaError_t e = f32 ? launch(attend_join_kernel<float>, A.b.T * A.H, kJoinWarps * 32, 0, st, A) : launch(attend_join_kernel<bf16>, A.b.T * A.H, kJoinWarps * 32, 0, st, A)) return e;
+    }
+    if (!two) return cudaSuccess;
+    few.rows_most = kFewMost;
+    few.b.max_new = kFewMost / (A.H / A.c.G);
+    few.n_splits = std::min(splits_for(few, f32, n_sms), kMostCluster);      // (joined without the workspace, which the tiles' shares may be in)
+    few.part = nullptr;
     *launches += 1;
-    return f32 ? launch(attend_join_kernel<float>, A.b.T * A.H, kJoinWarps * 32, 0, st, A) : launch(attend_join_kernel<bf16>, A.b.T * A.H, kJoinWarps * 32, 0, st, A);
+    return attend_few(few, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 
-static size_t part_bytes(const AttendArgs& A, int splits) { return (part_floats(A, splits) + 2ull * A.b.T * A.H * splits) * sizeof(float); }
 static bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 static int n_sms_of_device(int* n) {
@@ -178,6 +205,19 @@ static int n_sms_of_device(int* n) {
     if (e != cudaSuccess) return report(SMOL_ERR_CUDA, "8-bit cache", cudaGetErrorString(e));
     if (dev < 64) known[dev].store(*n);
     return SMOL_OK;
+}
+
+// whether rows of n elements are whole groups of eight on 16-byte boundaries, or of four as one load
+static bool whole_eights(const void* p, size_t row, size_t head, int n, bool f32) { return n % 8 == 0 && (row | head) * (f32 ? 4 : 2) % 16 == 0 && aligned(p, 16); }
+static bool whole_fours(const void* p, size_t row, size_t head, int n, bool f32) { return n % 4 == 0 && row % 4 == 0 && head % 4 == 0 && aligned(p, f32 ? 16 : 8); }
+void note_alignment(AppendArgs& A, bool f32) {
+    A.k_vec = whole_eights(A.k, A.k_row, A.k_head, A.c.d, f32);
+    A.v_vec = whole_eights(A.v, A.v_row, A.v_head, A.c.dv, f32);
+    A.q_vec = A.H == 0 || (whole_eights(A.q, A.q_row, A.q_head, A.c.d, f32) && whole_eights(A.q_out, A.o_row, A.o_head, A.c.d, f32));
+}
+void note_alignment(AttendArgs& A, bool f32) {
+    A.q_vec = whole_fours(A.q, A.q_row, A.q_head, A.c.d, f32);
+    A.o_vec = whole_fours(A.out, A.o_row, A.o_head, A.c.dv, f32);
 }
 
 static int cache_of(const SmolLmCache8* s, Cache& c, const char* me) {
@@ -208,10 +248,6 @@ static int batch_of(const SmolLmCache8Batch* s, Batch& b, const char* me) {
     b.S = s->n_seqs; b.T = s->n_tokens; b.max_pages = s->max_pages; b.max_new = std::min(s->max_new, s->n_tokens); b.max_len = s->max_len;
     return SMOL_OK;
 }
-// whether rows of n elements are whole groups of eight on 16-byte boundaries, or of four as one load
-static bool whole_eights(const void* p, size_t row, size_t head, int n, bool f32) { return n % 8 == 0 && (row | head) * (f32 ? 4 : 2) % 16 == 0 && aligned(p, 16); }
-static bool whole_fours(const void* p, size_t row, size_t head, int n, bool f32) { return n % 4 == 0 && row % 4 == 0 && head % 4 == 0 && aligned(p, f32 ? 16 : 8); }
-
 static int attend_of(const SmolLmCache8* c, const SmolLmCache8Batch* b, const SmolLmCache8Attend* a, AttendArgs& A, bool pointers) {
     const char* me = "smol_lm_cache8_attend";
     if (!c || !b || !a) return report(SMOL_ERR_INVALID, me, "null argument");
@@ -229,8 +265,8 @@ static int attend_of(const SmolLmCache8* c, const SmolLmCache8Batch* b, const Sm
     A.H = a->heads; A.window = a->window; A.first = a->first; A.scale = a->scale; A.softcap = a->softcap;
     A.sink = a->sink; A.slope = a->dist_slope; A.r1 = a->dist_r1; A.r2 = a->dist_r2; A.gate = a->gate; A.gate_row = a->gate_row; A.out_scale = a->out_scale;
     A.part = nullptr; A.n_splits = 1;
-    A.q_vec = whole_fours(a->q, a->q_row, a->q_head, A.c.d, f32);
-    A.o_vec = whole_fours(a->out, a->out_row, a->out_head, A.c.dv, f32);
+    A.rows_over = 0; A.rows_most = 0x7fffffff;
+    note_alignment(A, f32);
     return SMOL_OK;
 }
 
@@ -254,12 +290,10 @@ extern "C" int smol_lm_cache8_append(const SmolLmCache8* cache, const SmolLmCach
     A.k_row = a->k_row; A.k_head = a->k_head; A.v_row = a->v_row; A.v_head = a->v_head;
     A.q_row = a->q_row; A.q_head = a->q_head; A.o_row = a->q_out_row; A.o_head = a->q_out_head;
     A.H = a->q ? a->heads : 0; A.freq = a->freq; A.pairs = a->rot_dims / 2; A.half = a->rot_half; A.mult = a->rot_mult;
-    A.k_vec = whole_eights(a->k, a->k_row, a->k_head, A.c.d, f32);
-    A.v_vec = whole_eights(a->v, a->v_row, a->v_head, A.c.dv, f32);
-    A.q_vec = A.H == 0 || (whole_eights(a->q, a->q_row, a->q_head, A.c.d, f32) && whole_eights(a->q_out, a->q_out_row, a->q_out_head, A.c.d, f32));
-    int n_sms = 0;
+    note_alignment(A, f32);
+    int n_sms = 0, launches = 0;
     if (int rc = n_sms_of_device(&n_sms)) return rc;
-    const cudaError_t e = append(A, f32, n_sms, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = append(A, f32, n_sms, &launches, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SMOL_OK : report(SMOL_ERR_CUDA, me, cudaGetErrorString(e));
 }
 
@@ -269,9 +303,7 @@ extern "C" int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const S
     if (int rc = attend_of(cache, batch, a, A, false)) return rc;
     int n_sms = 0;
     if (int rc = n_sms_of_device(&n_sms)) return rc;
-    const bool f32 = a->dtype == SMOL_LM_F32;
-    const int splits = splits_for(A, f32, n_sms);
-    *bytes = splits == 1 || joins_in_cluster(A, splits, f32) ? 0 : part_bytes(A, splits);
+    *bytes = attend_bytes(A, a->dtype == SMOL_LM_F32, n_sms);
     return SMOL_OK;
 }
 
@@ -281,10 +313,8 @@ extern "C" int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCach
     int n_sms = 0, launches = 0;
     if (int rc = n_sms_of_device(&n_sms)) return rc;
     const bool f32 = a->dtype == SMOL_LM_F32;
-    A.n_splits = splits_for(A, f32, n_sms);
-    if (A.n_splits > 1 && !joins_in_cluster(A, A.n_splits, f32) && (!workspace || !aligned(workspace, 16) || workspace_bytes < part_bytes(A, A.n_splits)))
-        return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
-    A.part = static_cast<float*>(workspace);
-    const cudaError_t e = attend(A, f32, n_sms, &launches, static_cast<cudaStream_t>(stream));
+    const size_t need = attend_bytes(A, f32, n_sms);
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need)) return report(SMOL_ERR_CAPACITY, "smol_lm_cache8_attend", "workspace too small or not on a 16-byte boundary");
+    const cudaError_t e = attend(A, f32, n_sms, workspace, &launches, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? SMOL_OK : report(SMOL_ERR_CUDA, "smol_lm_cache8_attend", cudaGetErrorString(e));
 }

@@ -67,6 +67,7 @@ struct AttendArgs {
     float* part;                     // shares of the keys: unnormalised results [T * H][n_splits][dv rounded up to 4], then (maximum, denominator) [T * H][n_splits]
     int n_splits;
     int q_vec, o_vec;
+    int rows_over, rows_most;        // only sequences of more than rows_over and at most rows_most query rows per key/value head
 };
 
 constexpr int kMaxSplits = 128;
@@ -105,12 +106,15 @@ __device__ __forceinline__ float log2_fast(float x) {
     return y;
 }
 
-// Launches on `st`; 0 or a CUDA error.
-cudaError_t append(const AppendArgs& A, bool f32, int n_sms, cudaStream_t st);
-// splits of the keys the kernel for few rows takes (1: no partial results)
-int splits_for(const AttendArgs& A, bool f32, int n_sms);
-bool tiles_serve(const AttendArgs& A, bool f32);
-cudaError_t attend(const AttendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st);
+// Launches on `st`; 0 or a CUDA error.  `launches` counts them.
+cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st);
+// Bytes of workspace attend needs for these sizes, and the most it needs for results of dv columns on any device of up to 256 SMs.
+size_t attend_bytes(const AttendArgs& A, bool f32, int n_sms);
+size_t attend_bytes_most(int dv);
+cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* launches, cudaStream_t st);
+// What a caller that fills the structs itself leaves to be worked out: whether rows are whole, aligned pieces.
+void note_alignment(AppendArgs& A, bool f32);
+void note_alignment(AttendArgs& A, bool f32);
 
 constexpr float kLog2e = 1.4426950408889634f;
 

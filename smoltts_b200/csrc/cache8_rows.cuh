@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
         else hi = mid;
     }
     const int t0 = A.b.start[lo], t1 = A.b.start[lo + 1];
-    if (t < t0 || t >= t1 || t0 < 0 || t1 > A.b.T || t - t0 >= A.b.max_new) return;
+    if (t < t0 || t >= t1 || t0 < 0 || t1 > A.b.T || t - t0 >= A.b.max_new || (long long)(t1 - t0) * (A.H / A.c.G) <= A.rows_over) return;
     const int pieces = (A.c.dv + 3) / 4;
     const float2* stat = part_stats(A) + (size_t)unit * A.n_splits;
     const float4* part = reinterpret_cast<const float4*>(A.part) + (size_t)unit * A.n_splits * pieces;

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "../../include/smoltts_b200_lm.h"
+#include "cache8.cuh"
 #include "common.cuh"
 #include "f32_tile.cuh"
 #include "lm_report.h"
@@ -852,7 +853,15 @@ struct AttnArgs {
     int rot_pairs = 0, rot_half = 0;             // rotated pairs of q and k (whole-projection norms only): i with i + rot_pairs, or 2i with 2i + 1
     float rot_mult = 1.0f;                       // multiplies cosine and sine
     const float* freq = nullptr;                 // [rot_pairs]
+    int by_row = 0;                              // keys and values go to `pool` as rows of the step, [head][page_size = n_tokens][d / dv], and not into pages
 };
+
+// where the preparation puts token t, which stands at `pos`: page (below 0: nowhere) and position in it
+__device__ __forceinline__ void attn_place(const AttnArgs& A, int t, int pos, int& page, int& in_pg) {
+    const int pg = pos / A.page_size;
+    in_pg = A.by_row ? t : pos - pg * A.page_size;
+    page = A.by_row ? 0 : pg < A.max_pages ? A.block_table[(size_t)A.tok_seq[t] * A.max_pages + pg] : -1;
+}
 
 // what a query at `pos` is multiplied by: 1 + coef * ln(floor((pos + 1) / every) + 1)
 __device__ __forceinline__ float attn_temperature(const AttnArgs& A, int pos) {
@@ -886,8 +895,8 @@ __global__ void attn_prep_kernel(const AttnArgs A, T* __restrict__ qbuf, T* __re
     const int HQ = A.H * A.maps, GK = A.G * A.maps, slots = HQ + (A.own_kv ? GK + A.G : 0);
     if (unit >= A.n_tokens * slots) { dep_wait(); return; }
     const int t = unit / slots, s = unit % slots, pos = A.tok_pos[t];
-    const int pg = pos / A.page_size, in_pg = pos % A.page_size;
-    const int page = s >= HQ && pg < A.max_pages ? A.block_table[(size_t)A.tok_seq[t] * A.max_pages + pg] : -1;
+    int page = -1, in_pg = 0;
+    if (s >= HQ) attn_place(A, t, pos, page, in_pg);
     dep_wait();
     dep_go();
     const float* row = A.proj + (size_t)t * A.n_in;
@@ -934,8 +943,8 @@ __global__ void __launch_bounds__(128) attn_prep_vec_kernel(const AttnArgs A, T*
     const int HQ = A.H * A.maps, GK = A.G * A.maps, slots = HQ + (A.own_kv ? GK + A.G : 0);
     const bool live = unit < A.n_tokens * slots;
     const int t = live ? unit / slots : 0, s = unit - t * slots, pos = A.tok_pos[t];
-    const int pg = pos / A.page_size, in_pg = pos - pg * A.page_size;
-    const int page = s >= HQ && pg < A.max_pages ? A.block_table[(size_t)A.tok_seq[t] * A.max_pages + pg] : -1;
+    int page = -1, in_pg = 0;
+    if (s >= HQ) attn_place(A, t, pos, page, in_pg);
     const bool key = s >= HQ && s < HQ + GK, in = live && c < (s < HQ + GK ? A.d : A.dv);
     const int at = (s < HQ + GK ? s * A.d : (HQ + GK) * A.d + (s - HQ - GK) * A.dv) + c;
     const float* norm = s < HQ ? A.q_norm : key ? A.k_norm : nullptr;
@@ -976,8 +985,8 @@ __global__ void __launch_bounds__(256) attn_prep_whole_kernel(const AttnArgs A, 
     const int t = blockIdx.x, nq = A.H * A.d, nk = A.G * A.d, nv = A.G * A.dv;
     const float* row = A.proj + (size_t)t * A.n_in;
     const int pos = A.tok_pos[t];
-    const int pg = pos / A.page_size, in_pg = pos % A.page_size;
-    const int page = pg < A.max_pages ? A.block_table[(size_t)A.tok_seq[t] * A.max_pages + pg] : -1;
+    int page, in_pg;
+    attn_place(A, t, pos, page, in_pg);
     // sum of squares of row[lo .. lo + n) + bias
     auto sum_sq = [&](int lo, int n) {
         float ss = 0.0f;
@@ -2257,6 +2266,7 @@ struct RunInfo {
     size_t freq_off = 0;           // latent attention: float offset of the run's rotation frequencies in the table
     size_t conv_off = 0;           // state-space, gated delta: float offset of the convolution's last inputs inside a slot
     size_t unit_off = 0, m_off = 0;   // mLSTM: float offsets of the key sums and the running maxima inside a slot
+    size_t k8 = 0, v8 = 0, ks8 = 0, vs8 = 0;   // 8-bit cache: byte offsets of codes and scales inside a page
     int flags = 0;                 // SMOL_LM_RUN_*
 };
 
@@ -2273,6 +2283,9 @@ struct SmolLm {
     int max_pair_heads = 0;
     SmolLmGlobals g{};
     size_t page_elems = 0, slot_floats = 0, esize = 2;
+    size_t page8_bytes = 0;               // 8-bit cache: bytes of a page (0: cached in the element type)
+    size_t o_stage = 0, o_part8 = 0;      // 8-bit cache: a step's keys and values before they are appended, shares of the keys
+    int max_stage = 0;
     int max_in = 0, max_mix = 0, max_ff = 0, max_hd = 0, max_q = 0;
     bool any_restart = false, any_own_proj = false, any_merge = false;
     // workspace carving (byte offsets)
@@ -2427,6 +2440,8 @@ extern "C" int smol_lm_create(const SmolLmConfig* cfg, const SmolLmLayer* layers
     if (cfg->vocab < 1 || cfg->width < 1 || cfg->n_layers < 1 || cfg->n_runs < 1 || cfg->page_size < 1 || cfg->max_step_tokens < 1 ||
         cfg->max_step_seqs < 1 || cfg->max_want < 1 || cfg->max_context < 1)
         return fail(SMOL_ERR_INVALID, "smol_lm_create: sizes must be positive");
+    if (cfg->kv_bits != 0 && cfg->kv_bits != 8 && cfg->kv_bits != 16) return fail(SMOL_ERR_INVALID, "smol_lm_create: kv_bits must be 0, 8 or 16");
+    if (cfg->kv_bits == 8 && cfg->page_size % smol::c8::kBlock) return fail(SMOL_ERR_INVALID, "smol_lm_create: an 8-bit cache needs a page_size that is a multiple of 16");
     SmolLm* m = new SmolLm();
     m->cfg = *cfg;
     m->cfg.run_flags = nullptr;      // the caller's array is read below and not kept
@@ -2442,6 +2457,8 @@ extern "C" int smol_lm_create(const SmolLmConfig* cfg, const SmolLmLayer* layers
     // places one mixer's cache or state in the pools and widens the workspace for it; returns 0 or an error code
     auto place = [&](const SmolLmLayer& L, RunInfo& r) -> int {
         if (L.heads < 1 || (L.dim < 1 && L.mixer != SMOL_LM_MIX_STATE_SPACE)) return fail(SMOL_ERR_INVALID, "a layer needs heads >= 1 and dim >= 1");
+        if (cfg->kv_bits == 8 && (L.mixer == SMOL_LM_MIX_LATENT_ATTENTION || L.mixer == SMOL_LM_MIX_SIGMOID_ATTENTION))
+            return fail(SMOL_ERR_UNSUPPORTED, "8-bit cache: softmax attention over keys and values only");
         if (L.in_bias && !pairable(L)) return fail(SMOL_ERR_UNSUPPORTED, "in_bias: softmax attention and the state-space recurrence only");
         if (L.mixer == SMOL_LM_MIX_SINK_ATTENTION) {
             if (L.kv_heads < 1 || L.heads % L.kv_heads != 0 || L.vdim < 1) return fail(SMOL_ERR_INVALID, "attention: heads must be a multiple of kv_heads");
@@ -2454,6 +2471,8 @@ extern "C" int smol_lm_create(const SmolLmConfig* cfg, const SmolLmLayer* layers
             if (L.rot_dims > 0 && (!L.norm_whole || L.rot_dims > 2 * kMaxRotPairs)) return fail(SMOL_ERR_UNSUPPORTED, "attention: rotation needs norm_whole and at most 512 coordinates");
             const size_t split_smem = ((size_t)std::min(L.heads / L.kv_heads * maps, 8) * (L.dim + 32) * 4 + 15) / 16 * 16 +
                                       (size_t)32 * (maps * (L.dim + 16 / m->esize + 1) + L.vdim + 16 / m->esize + 1) * m->esize;
+            if (L.first_visible < 0 || (L.first_visible > 0 && cfg->kv_bits != 8)) return fail(SMOL_ERR_UNSUPPORTED, "attention: first_visible needs the 8-bit cache");
+            if (cfg->kv_bits == 8 && (maps != 1 || L.dim > 256 || L.vdim > 256)) return fail(SMOL_ERR_UNSUPPORTED, "8-bit cache: one map, key and value sizes of at most 256");
             if (split_smem > (size_t)kAttnSplitSmemMax) return fail(SMOL_ERR_UNSUPPORTED, "attention: key and value sizes need more shared memory than an SM has");
             if (L.kv_from > 0) {
                 // another layer's cache, as its latest run leaves it
@@ -2466,6 +2485,15 @@ extern "C" int smol_lm_create(const SmolLmConfig* cfg, const SmolLmLayer* layers
                     return fail(SMOL_ERR_INVALID, "attention: kv_from must name an attention layer with own keys and values and the same sizes");
                 r.k_off = lender->k_off;
                 r.v_off = lender->v_off;
+                r.k8 = lender->k8; r.v8 = lender->v8; r.ks8 = lender->ks8; r.vs8 = lender->vs8;
+            } else if (cfg->kv_bits == 8) {
+                const size_t rows = (size_t)L.kv_heads * cfg->page_size, scales = rows / smol::c8::kBlock * sizeof(float);
+                r.k8 = m->page8_bytes;
+                r.v8 = r.k8 + rows * ((L.dim + 15) / 16 * 16);
+                r.ks8 = r.v8 + rows * ((L.vdim + 15) / 16 * 16);
+                r.vs8 = r.ks8 + scales;
+                m->page8_bytes = (r.vs8 + scales + 15) / 16 * 16;
+                m->max_stage = std::max(m->max_stage, L.kv_heads * (L.dim + L.vdim));
             } else {
                 r.k_off = m->page_elems;
                 r.v_off = r.k_off + (size_t)L.kv_heads * maps * cfg->page_size * L.dim;
@@ -2692,6 +2720,10 @@ extern "C" int smol_lm_create(const SmolLmConfig* cfg, const SmolLmLayer* layers
     m->split_len = std::max(64, ((ctx + 255) / 256 + 63) / 64 * 64);
     m->max_splits = ((ctx + m->split_len - 1) / m->split_len + 3) / 4 * 4;
     m->o_part = carve((size_t)cfg->max_step_seqs * kShortSeq * m->max_heads * m->max_splits * (m->max_vdim + 2) * 4);
+    if (m->page8_bytes > 0) {
+        m->o_stage = carve(T * (size_t)m->max_stage * E);
+        m->o_part8 = carve(smol::c8::attend_bytes_most(m->max_vdim));
+    }
     if (cfg->block == SMOL_LM_BLOCK_POSTNORM) m->o_hist = carve((size_t)(cfg->n_runs + 1) * T * D * 4);
     if (m->max_cq > 0) {
         m->o_cq = carve(T * (size_t)m->max_cq * E);
@@ -2748,7 +2780,7 @@ extern "C" int smol_lm_create(const SmolLmConfig* cfg, const SmolLmLayer* layers
 }
 
 extern "C" void smol_lm_destroy(SmolLm* m) { delete m; }
-extern "C" size_t smol_lm_page_bytes(const SmolLm* m) { return m ? std::max<size_t>(m->page_elems, 8) * m->esize : 0; }
+extern "C" size_t smol_lm_page_bytes(const SmolLm* m) { return !m ? 0 : m->page8_bytes > 0 ? m->page8_bytes : std::max<size_t>(m->page_elems, 8) * m->esize; }
 extern "C" size_t smol_lm_slot_bytes(const SmolLm* m) { return m ? std::max<size_t>(m->slot_floats, 4) * 4 : 0; }
 extern "C" size_t smol_lm_workspace_bytes(const SmolLm* m) { return m ? m->total : 0; }
 extern "C" int64_t smol_lm_launch_count(const SmolLm* m) { return m ? m->launches : 0; }
@@ -3681,6 +3713,44 @@ static int step_impl(SmolLm* m, const SmolLmStep* s, cudaStream_t st) {
         const T* mix_in = mix;          // what the output projection reads
         cudaStream_t ms = st;           // the stream the current mixer runs on
         // Softmax attention over keys and values in the paged pool.  pj / bias: this mixer's rows of the fused projection.
+        // The step's keys and values into the 8-bit cache, and attention over it; P: what the preparation was given.
+        auto attend_coded = [&](const SmolLmLayer& M, const RunInfo& Ri, const AttnArgs& P, T* mix_at) -> int {
+            namespace c8 = smol::c8;
+            char* pages = static_cast<char*>(m->pages);
+            c8::Cache C;
+            C.k = reinterpret_cast<uint8_t*>(pages + Ri.k8); C.v = reinterpret_cast<uint8_t*>(pages + Ri.v8);
+            C.ks = reinterpret_cast<float*>(pages + Ri.ks8); C.vs = reinterpret_cast<float*>(pages + Ri.vs8);
+            C.k_page = C.v_page = m->page8_bytes; C.ks_page = C.vs_page = m->page8_bytes / sizeof(float);
+            C.n_pages = m->n_pages; C.page = c.page_size; C.G = M.kv_heads; C.d = M.dim; C.dv = M.vdim;
+            C.ldk = (M.dim + 15) / 16 * 16; C.ldv = (M.vdim + 15) / 16 * 16; C.err = err;
+            c8::Batch B;
+            B.start = s->seq_start; B.pos0 = s->seq_pos0; B.table = s->block_table; B.kv_len = nullptr;
+            B.S = s->n_seqs; B.T = Tn; B.max_pages = s->max_pages; B.max_new = std::min(max_n, Tn);
+            B.max_len = 1 + (s->max_pos > 0 ? std::min(s->max_pos, c.max_context - 1) : c.max_context - 1);
+            int launches = 0;
+            if (M.kv_from == 0) {
+                c8::AppendArgs W{};
+                W.c = C; W.b = B;
+                W.k = reinterpret_cast<const T*>(m->ws + m->o_stage); W.v = reinterpret_cast<const T*>(m->ws + m->o_stage) + P.v_off;
+                W.k_row = M.dim; W.k_head = (size_t)Tn * M.dim; W.v_row = M.vdim; W.v_head = (size_t)Tn * M.vdim;
+                W.mult = 1.0f;
+                c8::note_alignment(W, kIsF32);
+                CU(c8::append(W, kIsF32, m->n_sms, &launches, ms));
+            }
+            c8::AttendArgs R{};
+            R.c = C; R.b = B;
+            R.q = qbuf; R.q_row = (size_t)M.heads * M.dim; R.q_head = M.dim;
+            R.out = mix_at; R.o_row = P.out_ld; R.o_head = M.vdim;
+            R.H = M.heads; R.window = M.window; R.first = M.first_visible; R.scale = M.score_scale; R.softcap = M.softcap;
+            R.sink = M.sink; R.slope = M.dist_slope; R.r1 = M.dist_r1; R.r2 = M.dist_r2;
+            R.gate = P.has_gate ? P.proj + P.gate_off : nullptr; R.gate_row = P.n_in; R.out_scale = P.out_scale;
+            R.rows_over = 0; R.rows_most = 0x7fffffff;
+            c8::note_alignment(R, kIsF32);
+            if (c8::attend_bytes(R, kIsF32, m->n_sms) > c8::attend_bytes_most(m->max_vdim)) return fail(SMOL_ERR_CAPACITY, "8-bit cache: the workspace is smaller than the step's shares of the keys");
+            CU(c8::attend(R, kIsF32, m->n_sms, m->ws + m->o_part8, &launches, ms));
+            m->launches += launches;
+            return SMOL_OK;
+        };
         auto attention = [&](const SmolLmLayer& M, const RunInfo& Ri, const float* pj, const float* bias, T* mix_at) -> int {
             AttnArgs A;
             A.proj = pj; A.n_in = n_in; A.bias = bias;
@@ -3698,22 +3768,30 @@ static int step_impl(SmolLm* m, const SmolLmStep* s, cudaStream_t st) {
             A.out_ld = out_ld_now; A.out_scale = M.mix_scale;
             A.temp_coef = M.q_temp_coef; A.temp_every = M.q_temp_every;
             A.maps = maps_of(M); A.diff_lambda = M.diff_lambda; A.diff_scale = M.diff_scale; A.own_kv = M.kv_from == 0;
+            // 8-bit cache: the preparation leaves keys and values as rows of the step, which the append then rounds into the pages
+            const bool coded = m->page8_bytes > 0;
+            T* const rows = coded ? reinterpret_cast<T*>(m->ws + m->o_stage) : pool;
+            if (coded) {
+                A.by_row = 1; A.page_size = Tn; A.page_elems = 0;
+                A.k_off = 0; A.v_off = (size_t)M.kv_heads * Tn * M.dim;
+            }
             if (M.norm_whole) {
                 const int threads = Tn > 64 ? 128 : 256;      // few tokens: more loads in flight per token
                 A.rot_pairs = M.rot_dims / 2; A.rot_half = M.rot_half; A.rot_mult = M.rot_mult != 0.0f ? M.rot_mult : 1.0f;
                 A.freq = reinterpret_cast<const float*>(m->ws + m->o_freq) + Ri.freq_off;
-                if (A.rot_pairs > 0) pdl_launch(attn_prep_whole_kernel<T, true>, Tn, threads, 0, ms, A, qbuf, pool);
-                else pdl_launch(attn_prep_whole_kernel<T, false>, Tn, threads, 0, ms, A, qbuf, pool);
+                if (A.rot_pairs > 0) pdl_launch(attn_prep_whole_kernel<T, true>, Tn, threads, 0, ms, A, qbuf, rows);
+                else pdl_launch(attn_prep_whole_kernel<T, false>, Tn, threads, 0, ms, A, qbuf, rows);
             } else {
                 const int units = Tn * (M.heads * A.maps + (A.own_kv ? M.kv_heads * (A.maps + 1) : 0));
                 // whole 16-byte pieces of every row read, 4-element pieces of every row written
-                const bool vec = M.dim % 4 == 0 && M.vdim % 4 == 0 && n_in % 4 == 0 && Ri.k_off % 4 == 0 && Ri.v_off % 4 == 0 && m->page_elems % 4 == 0 &&
-                                 addresses_of(pj, bias, M.q_norm, M.k_norm, qbuf, pool) % 16 == 0;
-                if (vec && std::max(M.dim, M.vdim) <= 64) pdl_launch(attn_prep_vec_kernel<T, 16>, (units + 7) / 8, 128, 0, ms, A, qbuf, pool);
-                else if (vec && std::max(M.dim, M.vdim) <= 128) pdl_launch(attn_prep_vec_kernel<T, 32>, (units + 3) / 4, 128, 0, ms, A, qbuf, pool);
-                else pdl_launch(attn_prep_kernel<T>, (units + 3) / 4, 128, 0, ms, A, qbuf, pool);
+                const bool vec = M.dim % 4 == 0 && M.vdim % 4 == 0 && n_in % 4 == 0 && A.k_off % 4 == 0 && A.v_off % 4 == 0 && A.page_elems % 4 == 0 &&
+                                 addresses_of(pj, bias, M.q_norm, M.k_norm, qbuf, rows) % 16 == 0;
+                if (vec && std::max(M.dim, M.vdim) <= 64) pdl_launch(attn_prep_vec_kernel<T, 16>, (units + 7) / 8, 128, 0, ms, A, qbuf, rows);
+                else if (vec && std::max(M.dim, M.vdim) <= 128) pdl_launch(attn_prep_vec_kernel<T, 32>, (units + 3) / 4, 128, 0, ms, A, qbuf, rows);
+                else pdl_launch(attn_prep_kernel<T>, (units + 3) / 4, 128, 0, ms, A, qbuf, rows);
             }
             m->launches += 1;
+            if (coded) return attend_coded(M, Ri, A, mix_at);
             const bool flash = sizeof(T) == 2 && std::max(M.dim, M.vdim) <= 128;
             if (A.maps == 2) {
                 if (M.vdim <= 256) launch_attention<T, 8, 2>(m, s, A, flash, qbuf, pool, mix_at, ms);

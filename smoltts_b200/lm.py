@@ -87,11 +87,22 @@ class HybridLM:
 
     def __init__(self, config, dtype: torch.dtype = torch.bfloat16, device: Optional[torch.device] = None,
                  max_tokens: int = 8192, max_seqs: int = 4, page_size: int = 64, max_step_tokens: int = 2048,
-                 max_want: Optional[int] = None, use_graph: bool = True):
+                 max_want: Optional[int] = None, use_graph: bool = True, kv_bits: int = 16, first_tokens: int = 0):
+        """``kv_bits=8`` keeps the keys and values of softmax attention layers as e4m3 codes with a power-of-two scale per 16
+        positions and head (``kv_cache.KVCache8``): half the bytes of a bf16 pool.  ``first_tokens``: positions at the start of a sequence that windowed
+        layers go on seeing (8-bit cache only).  Designs whose attention caches something else are refused by ``load_state_dict``."""
         if not torch.cuda.is_available():
             raise RuntimeError("smoltts_b200 needs a CUDA device: there is no CPU fallback")
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError("dtype must be torch.bfloat16 or torch.float32")
+        if kv_bits not in (8, 16):
+            raise ValueError("kv_bits must be 8 or 16")
+        if kv_bits == 8 and page_size % 16:
+            raise ValueError("an 8-bit cache needs a page_size that is a multiple of 16")
+        if first_tokens < 0 or (first_tokens and kv_bits != 8):
+            raise ValueError("first_tokens needs kv_bits=8 and must not be negative")
+        self.kv_bits = kv_bits
+        self.first_tokens = first_tokens
         self.lib = _capi_lm.load()
         self.config = config
         self.dtype = dtype
@@ -158,12 +169,16 @@ class HybridLM:
         for c in layers:
             c.mix_scale = 1.0
         desc = self._describe(sd, layers, mat, vec)
+        for c in layers:
+            for mixer in (c, c.side[0] if c.side else None):
+                if mixer is not None and mixer.mixer == MIXER_KINDS["attention"] and mixer.window > 0:
+                    mixer.first_visible = self.first_tokens
         ccfg = _capi_lm.SmolLmConfig(
             dtype=_capi_lm.SMOL_LM_F32 if dt == torch.float32 else _capi_lm.SMOL_LM_BF16, vocab=cfg.vocab, width=cfg.width,
             n_layers=len(cfg.layers), n_runs=len(self.runs), page_size=self.page_size, max_step_tokens=self.max_step_tokens,
             max_step_seqs=self.max_seqs, max_want=self.max_want,
             max_context=self.page_pool.n * self.page_size, use_graph=int(self.use_graph), embed_scale=1.0, norm_eps=cfg.norm_eps,
-            block=BLOCK_SANDWICH, residual_alpha=1.0, logit_scale=1.0)
+            block=BLOCK_SANDWICH, residual_alpha=1.0, logit_scale=1.0, kv_bits=self.kv_bits)
         for k, v in desc["config"].items():
             setattr(ccfg, k, v)
         runs = (C.c_int32 * len(self.runs))(*self.runs)

@@ -52,3 +52,37 @@ def test_null_structs():
     assert lib.smol_lm_cache8_append(None, ctypes.byref(batch), ctypes.byref(app), None) == -1
     assert lib.smol_lm_cache8_attend(ctypes.byref(cache), None, ctypes.byref(att), None, 0, None) == -1
     assert lib.smol_lm_cache8_workspace_bytes(ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(att), None) == -1
+
+
+def lm_config(**over):
+    c = dict(dtype=0, vocab=64, width=32, n_layers=1, n_runs=1, page_size=32, max_step_tokens=64, max_step_seqs=2, max_want=8, max_context=256, use_graph=1, embed_scale=1.0,
+             norm_eps=1e-5, kv_bits=8)
+    c.update(over)
+    layers = (cl.SmolLmLayer * 1)()
+    layers[0].mixer, layers[0].heads, layers[0].kv_heads, layers[0].dim, layers[0].vdim = 0, 4, 2, 24, 64
+    return cl.SmolLmConfig(**c), layers
+
+
+def test_engine_pages_of_codes():
+    """A page: 2 heads x 32 positions x (24 rounded up to 32, 64) codes, and as many scales as 16-position blocks for keys and values."""
+    lib, h, runs = cl.load(), ctypes.c_void_p(), (ctypes.c_int32 * 1)(0)
+
+    def create(layers, cfg):
+        return lib.smol_lm_create(ctypes.byref(cfg), layers, runs, ctypes.byref(h))
+
+    cfg, layers = lm_config()
+    assert create(layers, cfg) == 0
+    assert lib.smol_lm_page_bytes(h) == 2 * 32 * (32 + 64) + 2 * 2 * 2 * 4
+    lib.smol_lm_destroy(h)
+    layers[0].window, layers[0].first_visible = 10, 4
+    assert create(layers, cfg) == 0
+    lib.smol_lm_destroy(h)
+    assert create(layers, lm_config(kv_bits=16)[0]) == -4 and create(layers, lm_config(kv_bits=4)[0]) == -1 and create(layers, lm_config(page_size=40)[0]) == -1
+    layers[0].first_visible = -1
+    assert create(layers, cfg) == -4
+    layers[0].first_visible, layers[0].n_maps = 0, 2
+    assert create(layers, cfg) == -4
+    layers[0].n_maps, layers[0].dim = 0, 257
+    assert create(layers, cfg) == -4
+    layers[0].dim, layers[0].mixer, layers[0].rot_dim, layers[0].q_rank, layers[0].kv_rank = 24, 2, 0, 8, 8
+    assert create(layers, cfg) == -4

@@ -324,6 +324,24 @@ def test_attention_of_many_rows(dtype, H, G, d, dv, page, counts, pos0):
     check_attention(c, table, q, counts, pos0, out)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H,G", [(8, 2), (40, 1)])
+def test_portions_and_single_tokens_in_one_batch(dtype, H, G):
+    """Long contexts: sequences of few rows beside one of many, which may go to different kernels; the shares of either are joined."""
+    d, counts, pos0 = 64, [1, 150, 0, 3, 9, 1], [5000, 100, 7, 2500, 3000, 0]
+    lens = [p + n for p, n in zip(pos0, counts)]
+    c, table = cache_of(lens, 64, G, d, d, seed=1)
+    fill(c, table, lens, seed=1)
+    q = randn(sum(counts) + 2, H, d, seed=4).to(dtype)
+    for o in (dict(), dict(window=700, first=5)):
+        out = torch.full((sum(counts) + 2, H, d), 7.0, device="cuda", dtype=dtype)
+        c.attend(q, ints(starts(counts)), ints(pos0), table, max_new=150, max_len=max(lens), out=out, **o)
+        check_attention(c, table, q, counts, pos0, out, **o)
+        assert (out[sum(counts):] == 7).all()
+    one = c.attend(q[:1], ints([0, 1]), ints([5000]), table[:1], max_new=1, max_len=5001, window=700, first=5)      # a row does not depend on its company
+    assert (one.double() - out[:1].double()).abs().max() <= 4 * HALF_STEP[dtype] * out[:1].abs().max() if dtype == torch.bfloat16 else torch.allclose(one, out[:1], rtol=1e-4, atol=1e-5)
+
+
 def test_strides_and_rows_of_nobody():
     """Queries and results as slices of something wider; rows in front, behind and of sequences without rows stay as they were."""
     H, G, d = 4, 2, 64
