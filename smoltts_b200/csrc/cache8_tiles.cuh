@@ -8,7 +8,8 @@
 // below, and a weight's error at 2^-9, or 2^-18 of the row's largest in the step.
 //
 // Roles: a warp that copies, a thread that issues the products, sixteen warps for the softmax: four threads per row, 32 columns of the scores and of
-// the result each.  Scores are double-buffered in tensor memory, so that the next step's are multiplied while this step's are worked on; a step's product
+// the result each.  Scores are double-buffered in tensor memory, so that the next step's are multiplied while this step's are worked on, and weights
+// take their place there (as the product's first operand: through shared memory the fence between the two proxies cost 600 cycles a step); a step's product
 // with the values is read back while the next one's is made, and joins the fp32 running results in registers.  Value codes that are NaN are
 // cleaned away in steps that some row does not see as a whole, as for few rows.
 #pragma once
@@ -20,24 +21,49 @@ namespace c8 {
 
 constexpr int kTileRows = 128, kTileParts = 4, kTileCols = kStep / kTileParts, kTileSoft = 4 * kTileParts, kTileThreads = (kTileSoft + 2) * 32;
 __host__ __device__ constexpr int tile_stages(int DK) { return DK <= 128 ? 3 : 2; }
-__host__ __device__ constexpr int tile_weights(int DK) { return DK <= 128 ? 2 : 1; }      // buffers of weights
 __host__ __device__ constexpr int tile_stage_bytes(int DK) { return kStep * (DK + 128); }
-__host__ __device__ constexpr int tile_smem(int DK) { return 1024 + 2 * kTileRows * DK + tile_stages(DK) * tile_stage_bytes(DK) + tile_weights(DK) * 2 * kTileRows * 128; }
+__host__ __device__ constexpr int tile_smem(int DK) { return 1024 + 2 * kTileRows * DK + tile_stages(DK) * tile_stage_bytes(DK); }
 
 struct TileBars {
     uint64_t full[3], empty[3];      // stages
-    uint64_t s_full[2], s_empty[2];  // scores in tensor memory
-    uint64_t p_full[2], o_full[2];   // weights in shared memory; their product in tensor memory
+    uint64_t s_full[2], p_full[2];   // scores in tensor memory, weights in their place
+    uint64_t o_full[2];              // the weights' product in tensor memory
     uint64_t q_full, drained;
     uint32_t tmem;
     int stop;
 };
 
-// Two f16 numbers of magnitude at most 256 as e4m3 parts of one unit: hi + lo
-__device__ __forceinline__ void two_equal_parts(__half2 x, uint32_t& hi, uint32_t& lo) {
-    hi = __nv_cvt_halfraw2_to_fp8x2((__half2_raw)x, __NV_SATFINITE, __NV_E4M3);
-    const __half2_raw rest = __hsub2(x, __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi, __NV_E4M3)));
-    lo = __nv_cvt_halfraw2_to_fp8x2(rest, __NV_SATFINITE, __NV_E4M3);
+// Four f16 numbers of magnitude at most 256 as e4m3 parts of one unit, hi + lo, codes in order
+__device__ __forceinline__ void four_equal_parts(uint32_t x, uint32_t y, uint32_t& hi, uint32_t& lo) {
+    asm("{\n\t.reg .b16 a, b, c, d;\n\t.reg .b32 f, g;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 a, %2;\n\tcvt.rn.satfinite.e4m3x2.f16x2 b, %3;\n\t"
+        "mov.b32 %0, {a, b};\n\t"
+        "cvt.rn.f16x2.e4m3x2 f, a;\n\tcvt.rn.f16x2.e4m3x2 g, b;\n\t"
+        "sub.rn.f16x2 f, %2, f;\n\tsub.rn.f16x2 g, %3, g;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f16x2 c, f;\n\tcvt.rn.satfinite.e4m3x2.f16x2 d, g;\n\t"
+        "mov.b32 %1, {c, d};\n\t}"
+        : "=&r"(hi), "=&r"(lo) : "r"(x), "r"(y));
+}
+// two fp32 numbers in one instruction
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ void of_two(uint64_t d, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(d)); }
+__device__ __forceinline__ uint64_t fma_two(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_two(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t half_two(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // Columns col .. col + 31 (a bit each) of the values in which a row at `pos` sees a NaN.  Rare, and slow.
@@ -59,23 +85,24 @@ __device__ __noinline__ uint32_t nan_bits(const AttendArgs& A, const Rows& W, in
     return bits;
 }
 
+constexpr float kFarAbove = 64.0f;      // in units of log2
+
 // DK: key size padded
 template <int DK, bool BENT>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
-    constexpr int NS = tile_stages(DK), SB = tile_stage_bytes(DK), KH = DK / 128, PB = tile_weights(DK);
+    constexpr int NS = tile_stages(DK), SB = tile_stage_bytes(DK), KH = DK / 128;
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
     __shared__ StepScales s_scales[NS];
     __shared__ float s_max[2][kTileParts][kTileRows], s_rowmul[kTileRows];
     __shared__ int s_bad;
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *KV = base, *Qs = KV + NS * SB, *Ps = Qs + 2 * kTileRows * DK;      // Qs, Ps: first parts, then second parts
+    unsigned char *KV = base, *Qs = KV + NS * SB;      // Qs: first parts, then second parts
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < NS; ++i) { umma::bar_init(&bars.full[i], 1); umma::bar_init(&bars.empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
             umma::bar_init(&bars.s_full[i], 1);
-            umma::bar_init(&bars.s_empty[i], kTileSoft);
             umma::bar_init(&bars.p_full[i], kTileSoft);
             umma::bar_init(&bars.o_full[i], 1);
         }
@@ -110,82 +137,88 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
     if (warp == kTileSoft) {
         copy_steps<KH, 1, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, v_col);
     } else if (warp == kTileSoft + 1) {
-        if (lane == 0 && steps > 0) {
-            // ---- products: whichever can be made next ----
+        if (steps > 0) {
+            const uint32_t on = elected();
+            // ---- products ----
             const uint32_t q0 = umma::s2u(Qs), id_s = desc_e4m3(128, kStep, false, false), id_o = desc_e4m3(128, 128, false, true);
             const int ksteps = (A.c.d + 31) / 32;
-            int scores = 0, values = 0;      // steps whose product has been issued
-            bool ok = wait_bar(&bars.q_full, 0, stop, A.c.err);
-            long long begin = clock64();
-            while (ok && values < steps) {
-                if (scores < steps && passed(&bars.full[scores % NS], (scores / NS) & 1) && (scores < 2 || passed(&bars.s_empty[scores & 1], ((scores >> 1) - 1) & 1))) {
-                    const int b = scores & 1, st = scores % NS;
-                    umma::fence_after_sync();
-                    const uint32_t k0 = umma::s2u(KV + st * SB);
+            auto scores = [&](int i) {
+                const int b = i & 1, st = i % NS;
+                if (!warp_wait(&bars.full[st], (i / NS) & 1, stop, A.c.err)) return false;
+                umma::fence_after_sync();
+                const uint32_t k0 = umma::s2u(KV + st * SB);
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
-                        for (int k = 0; k < ksteps; ++k)
-                            mma_e4m3(tmem + b * kStep, umma::smem_desc_sw128(q0 + (part * KH + (k >> 2)) * (kTileRows * 128) + (k & 3) * 32), umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32),
-                                     id_s, part > 0 || k > 0 ? 1u : 0u);
-                    umma::commit(&bars.s_full[b]);
-                    ++scores;
-                    begin = clock64();
-                } else if (values < scores && passed(&bars.p_full[values & 1], (values >> 1) & 1)) {
-                    const int b = values & 1, st = values % NS;
-                    umma::fence_after_sync();
-                    const uint32_t v = umma::s2u(KV + st * SB) + KH * (kStep * 128), p = umma::s2u(Ps + (PB == 2 ? b : 0) * (2 * kTileRows * 128));
+                for (int part = 0; part < 2; ++part)
+                    for (int k = 0; k < ksteps; ++k)
+                        mma_e4m3(on, tmem + b * kStep, umma::smem_desc_sw128(q0 + (part * KH + (k >> 2)) * (kTileRows * 128) + (k & 3) * 32), umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32),
+                                 id_s, part > 0 || k > 0 ? 1u : 0u);
+                commit_on(on, &bars.s_full[b]);
+                return true;
+            };
+            // A step's scores are multiplied behind the values of the step before last, whose weights lie where they go (products are made in the order of
+            // their issue); they are wanted a whole step later.
+            bool ok = warp_wait(&bars.q_full, 0, stop, A.c.err) && scores(0) && (steps < 2 || scores(1));
+            for (int i = 0; ok && i < steps; ++i) {
+                const int b = i & 1, st = i % NS;
+                ok = warp_wait(&bars.p_full[b], (i >> 1) & 1, stop, A.c.err);
+                if (!ok) break;
+                umma::fence_after_sync();
+                const uint32_t v = umma::s2u(KV + st * SB) + KH * (kStep * 128);
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
+                for (int part = 0; part < 2; ++part)
 #pragma unroll
-                        for (int k = 0; k < kStep / 32; ++k)
-                            mma_e4m3(tm_o + b * 128, umma::smem_desc_sw128(p + part * (kTileRows * 128) + k * 32), umma::smem_desc_sw128(v + k * 32 * 128), id_o, part > 0 || k > 0 ? 1u : 0u);
-                    umma::commit(&bars.empty[st]);
-                    umma::commit(&bars.o_full[b]);
-                    ++values;
-                    begin = clock64();
-                } else if (*stop || clock64() - begin > kWaitCycles) {
-                    if (!*stop) atomicExch(A.c.err, 3);
-                    *stop = 1;
-                    ok = false;
-                }
+                    for (int k = 0; k < kStep / 32; ++k)
+                        mma_e4m3_weights(on, tm_o + b * 128, tmem + b * kStep + part * (kStep / 4) + k * 8, umma::smem_desc_sw128(v + k * 32 * 128), id_o, part > 0 || k > 0 ? 1u : 0u);
+                commit_on(on, &bars.empty[st]);
+                commit_on(on, &bars.o_full[b]);
+                ok = i + 2 >= steps || scores(i + 2);
             }
-            umma::commit(&bars.drained);      // nothing of the block's is in flight once this is through
+            commit_on(on, &bars.drained);      // nothing of the block's is in flight once this is through
             drain_bar(&bars.drained, 0);
         }
     } else if (steps > 0) {
         // ---- queries into shared memory, a warp per row ----
-#pragma unroll 2
-        for (int r = warp; r < kTileRows; r += kTileSoft) {
-            const int row = min(row0 + r, n * Gq - 1), h = g * Gq + row % Gq;
-            const bf16* q = static_cast<const bf16*>(A.q) + (size_t)(t0 + row / Gq) * A.q_row + (size_t)h * A.q_head;
-            float v[KH][4];
-            uint32_t top = 0;
+        constexpr int AT_ONCE = 8 / KH;      // rows whose loads are on their way together
+#pragma unroll 1
+        for (int r0 = warp; r0 < kTileRows; r0 += kTileSoft * AT_ONCE) {
+            float v[AT_ONCE][KH][4];
 #pragma unroll
-            for (int x = 0; x < KH; ++x) {
-                const int at = x * 128 + lane * 4;
-                if (A.q_vec) {
-                    const uint2 u = at < A.c.d ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0u, 0u);
-                    v[x][0] = bf_lo(u.x); v[x][1] = bf_hi(u.x); v[x][2] = bf_lo(u.y); v[x][3] = bf_hi(u.y);
-                } else {
+            for (int y = 0; y < AT_ONCE; ++y) {
+                const int row = min(row0 + r0 + y * kTileSoft, n * Gq - 1), tok = row / Gq;
+                const bf16* q = static_cast<const bf16*>(A.q) + (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) v[x][e] = at + e < A.c.d ? __bfloat162float(q[at + e]) : 0.0f;
+                for (int x = 0; x < KH; ++x) {
+                    const int at = x * 128 + lane * 4;
+                    if (A.q_vec) {
+                        const uint2 u = at < A.c.d ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0u, 0u);
+                        v[y][x][0] = bf_lo(u.x); v[y][x][1] = bf_hi(u.x); v[y][x][2] = bf_lo(u.y); v[y][x][3] = bf_hi(u.y);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[y][x][e] = at + e < A.c.d ? __bfloat162float(q[at + e]) : 0.0f;
+                    }
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[x][e])));
             }
-            top = __reduce_max_sync(0xffffffffu, top);
-            const int e = max((int)(top >> 23) - 127, -110);      // (below: rows of less than 2^-110 keep a factor that fp32 holds)
-            const float up = pow2(7 - e);
 #pragma unroll
-            for (int x = 0; x < KH; ++x) {
-                uint32_t hi[2], part[2];
+            for (int y = 0; y < AT_ONCE; ++y) {
+                const int r = r0 + y * kTileSoft;
+                uint32_t top = 0;
 #pragma unroll
-                for (int y = 0; y < 2; ++y) two_equal_parts(__floats2half2_rn(v[x][2 * y] * up, v[x][2 * y + 1] * up), hi[y], part[y]);
-                *reinterpret_cast<uint32_t*>(Qs + x * (kTileRows * 128) + sw128_byte(r, lane * 4)) = hi[0] | (hi[1] << 16);
-                *reinterpret_cast<uint32_t*>(Qs + (KH + x) * (kTileRows * 128) + sw128_byte(r, lane * 4)) = part[0] | (part[1] << 16);
+                for (int x = 0; x < KH; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[y][x][e])));
+                top = __reduce_max_sync(0xffffffffu, top);
+                const int e = max((int)(top >> 23) - 127, -110);      // (below: rows of less than 2^-110 keep a factor that fp32 holds)
+                const float up = pow2(7 - e);
+#pragma unroll
+                for (int x = 0; x < KH; ++x) {
+                    uint32_t hi, rest;
+                    four_equal_parts(half_two(v[y][x][0] * up, v[y][x][1] * up), half_two(v[y][x][2] * up, v[y][x][3] * up), hi, rest);
+                    *reinterpret_cast<uint32_t*>(Qs + x * (kTileRows * 128) + sw128_byte(r, lane * 4)) = hi;
+                    *reinterpret_cast<uint32_t*>(Qs + (KH + x) * (kTileRows * 128) + sw128_byte(r, lane * 4)) = rest;
+                }
+                // (a row that is not finite: every score of it is a NaN)
+                if (lane == 0) s_rowmul[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 7) * (A.scale * (BENT ? 1.0f : kLog2e));
             }
-            // (a row that is not finite: every score of it is a NaN)
-            if (lane == 0) s_rowmul[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 7) * (A.scale * (BENT ? 1.0f : kLog2e));
         }
         umma::fence_async_smem();
         __syncwarp();
@@ -205,19 +238,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             wait_bar(&bars.o_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
             umma::fence_after_sync();
-            const float mn = fmaxf(m, m_step), keep = m == mn ? 1.0f : exp2_fast(m - mn);
-            float add = m_step == -INFINITY ? 0.0f : exp2_fast(m_step - mn);
-            m = mn;
-            l = fmaf(l_step, add, l * keep);
+            // m is what results and denominator are relative to: the first step's maximum, and a later one's only where fp32 would come near its end
+            if (__any_sync(0xffffffffu, m_step > m + kFarAbove)) {
+                const float mn = m_step > m + kFarAbove ? m_step : m, keep = m == mn ? 1.0f : exp2_fast(m - mn);
+                m = mn;
+                l *= keep;
+#pragma unroll
+                for (int c = 0; c < kTileCols; ++c) o[c] *= keep;
+            }
+            float add = m_step == -INFINITY ? 0.0f : exp2_fast(m_step - m);
+            l = fmaf(l_step, add, l);
             add *= unit;
 #pragma unroll
-            for (int x = 0; x < kTileCols / 16; ++x) {
-                uint32_t v[2][8];
-                umma::tmem_ld8_issue(tm_o + b * 128 + part * kTileCols + 16 * x + lanes, v[0]);
-                umma::tmem_ld8_issue(tm_o + b * 128 + part * kTileCols + 16 * x + 8 + lanes, v[1]);
+            for (int x = 0; x < kTileCols / 32; ++x) {
+                uint32_t v[4][8];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) umma::tmem_ld8_issue(tm_o + b * 128 + part * kTileCols + 32 * x + 8 * y + lanes, v[y]);
                 umma::tmem_ld_wait();
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[16 * x + e] = fmaf(__uint_as_float(v[e / 8][e % 8]), add, o[16 * x + e] * keep);
+                for (int e = 0; e < 32; e += 2) {
+                    float &o0 = o[32 * x + e], &o1 = o[32 * x + e + 1];
+                    of_two(fma_two(two(__uint_as_float(v[e / 8][e % 8]), __uint_as_float(v[e / 8][e % 8 + 1])), two(add, add), two(o0, o1)), o0, o1);
+                }
             }
             umma::fence_before_sync();
         };
@@ -225,7 +267,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), jc = j0 + part * kTileCols;
             // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
             wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
-            float ks[2], vs[2], v_top = 0.0f;
+            float ks[kTileCols / kBlock], vs[kTileCols / kBlock], v_top = 0.0f;
             bool nans = false, holes = false;      // in the whole step
 #pragma unroll
             for (int x = 0; x < kStepBlocks; ++x) {
@@ -235,9 +277,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                 holes |= v == 0.0f;
             }
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                ks[x] = s_scales[st].k[2 * part + x];
-                vs[x] = fabsf(s_scales[st].v[2 * part + x]);
+            for (int x = 0; x < kTileCols / kBlock; ++x) {
+                ks[x] = s_scales[st].k[part * (kTileCols / kBlock) + x];
+                vs[x] = fabsf(s_scales[st].v[part * (kTileCols / kBlock) + x]);
             }
             wait_bar(&bars.s_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
@@ -251,20 +293,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
 #pragma unroll
                 for (int e = 0; e < kTileCols; ++e) S[e] = __uint_as_float(v[e / 8][e % 8]);
             }
-            umma::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) arrive(&bars.s_empty[b]);
             const bool whole = !holes && j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             // scores in units of log2: S times mul
             const bool direct = !BENT && whole && A.scale > 0.0f;
-            float mul[2] = {rowmul * ks[0], rowmul * ks[1]};
+            float mul[kTileCols / kBlock];
+#pragma unroll
+            for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = rowmul * ks[x];
             if (!direct) {
 #pragma unroll
                 for (int e = 0; e < kTileCols; ++e) {
                     S[e] *= mul[e / kBlock];
                     if (BENT) S[e] = bent_score<false>(A, S[e], pos - (jc + e), r1, r2, slope);
                 }
-                mul[0] = mul[1] = 1.0f;
+#pragma unroll
+                for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = 1.0f;
             }
             if (!whole) {
                 const int far = A.window > 0 ? A.window : 0x7fffffff, last = min(pos + 1, seen.end) - jc, lead = A.first - jc, dist = pos - jc;
@@ -285,7 +327,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             // ---- the row's maximum over the step ----
             float top = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
+            for (int x = 0; x < kTileCols / kBlock; ++x) {
                 float t[4] = {S[16 * x], S[16 * x + 1], S[16 * x + 2], S[16 * x + 3]};
 #pragma unroll
                 for (int e = 4; e < 16; ++e) t[e % 4] = fmaxf(t[e % 4], S[16 * x + e]);
@@ -293,40 +335,53 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             }
             s_max[b][part][row] = top;
             row_barrier();
-            top = fmaxf(fmaxf(s_max[b][0][row], s_max[b][1][row]), fmaxf(s_max[b][2][row], s_max[b][3][row]));
-            if (PB == 1 && i > 0) join_product(i - 1);      // (its weights lie where this step's go)
+#pragma unroll
+            for (int x = 0; x < kTileParts; ++x) top = fmaxf(top, s_max[b][x][row]);
             // ---- weights, times 256 and the block's share of the largest value scale ----
             const float under = (top == -INFINITY ? 0.0f : top) - 8.0f;
-            unsigned char* P = Ps + (PB == 2 ? b : 0) * (2 * kTileRows * 128) + row * 128;
-            float sum = 0.0f;
+            // (behind the barrier all of the row's scores are in registers: weights go where they were, first parts into the first 32 columns, second parts into the next)
+            const uint32_t P = tmem + b * kStep + part * (kTileCols / 4) + lanes;
+            const uint64_t under2 = two(-under, -under);
+            uint64_t sum = two(0.0f, 0.0f);
+            uint32_t hi[8], rest[8];
+            static_assert(kTileCols == 32, "eight columns of weights a thread");
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const __half2 ratio = __float2half2_rn(vs[x] / fmaxf(v_top, kLeastScale));      // a power of two (0 below 2^-24)
-                float sums[2] = {0.0f, 0.0f};
-                uint32_t hi[4], rest[4];
+            for (int x = 0; x < kTileCols / kBlock; ++x) {
+                const uint64_t mul2 = two(mul[x], mul[x]);
+                uint32_t w[8];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    uint32_t a[2], c[2];
-#pragma unroll
-                    for (int z = 0; z < 2; ++z) {
-                        const float p0 = exp2_fast(fmaf(S[16 * x + 4 * y + 2 * z], mul[x], -under)), p1 = exp2_fast(fmaf(S[16 * x + 4 * y + 2 * z + 1], mul[x], -under));
-                        sums[z] += p0 + p1;
-                        two_equal_parts(__hmul2(__floats2half2_rn(p0, p1), ratio), a[z], c[z]);
-                    }
-                    hi[y] = a[0] | (a[1] << 16);
-                    rest[y] = c[0] | (c[1] << 16);
+                for (int y = 0; y < 8; ++y) {
+                    float p0, p1;
+                    of_two(fma_two(two(S[16 * x + 2 * y], S[16 * x + 2 * y + 1]), mul2, under2), p0, p1);
+                    p0 = exp2_fast(p0);
+                    p1 = exp2_fast(p1);
+                    sum = add_two(sum, two(p0, p1));
+                    w[y] = half_two(p0, p1);
                 }
-                sum += sums[0] + sums[1];
-                unsigned char* to = P + (((2 * part + x) ^ (row & 7)) << 4);
-                *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                *reinterpret_cast<uint4*>(to + kTileRows * 128) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+                if (vs[x] != v_top) {
+                    const __half2 ratio = __float2half2_rn(vs[x] / fmaxf(v_top, kLeastScale));      // a power of two (0 below 2^-24)
+#pragma unroll
+                    for (int y = 0; y < 8; ++y) {
+                        const __half2 t = __hmul2(*reinterpret_cast<const __half2*>(&w[y]), ratio);
+                        w[y] = *reinterpret_cast<const uint32_t*>(&t);
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) four_equal_parts(w[2 * y], w[2 * y + 1], hi[4 * x + y], rest[4 * x + y]);
             }
-            umma::fence_async_smem();
+            tmem_st8(P, hi);
+            tmem_st8(P + kStep / 4, rest);
+            tmem_st_wait();
+            // (value codes that were cleaned)
+            if (!whole || nans) umma::fence_async_smem();
+            umma::fence_before_sync();
             __syncwarp();
             if (lane == 0) arrive(&bars.p_full[b]);
-            if (PB == 2 && i > 0) join_product(i - 1);
+            if (i > 0) join_product(i - 1);
             m_step = top;
-            l_step = sum * (1.0f / 256.0f);
+            float sum0, sum1;
+            of_two(sum, sum0, sum1);
+            l_step = (sum0 + sum1) * (1.0f / 256.0f);
             unit = v_top * (1.0f / 256.0f);
         }
         join_product(steps - 1);
@@ -334,14 +389,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
         row_barrier();
         s_max[0][part][row] = l;
         row_barrier();
-        const float total = (s_max[0][0][row] + s_max[0][1][row]) + (s_max[0][2][row] + s_max[0][3][row]);
+        float total = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kTileParts; ++x) total += s_max[0][x][row];
         const int col = v_col + part * kTileCols;
         if (row < rows && col < A.c.dv && !*stop) {
             const int tok = t0 + my_row / Gq;
-            const uint32_t bits = s_bad ? nan_bits(A, W, pos, col) : 0u;
+            if (s_bad) {
 #pragma unroll
-            for (int c = 0; c < kTileCols; ++c)
-                if (bits >> c & 1) o[c] = __int_as_float(0x7fffffff);
+                for (int x = 0; x < kTileCols / 32; ++x) {
+                    const uint32_t bits = nan_bits(A, W, pos, col + 32 * x);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (bits >> c & 1) o[32 * x + c] = __int_as_float(0x7fffffff);
+                }
+            }
             if (A.n_splits > 1) {
                 const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
                 if (col == 0) part_stats(A)[at] = make_float2(m, total);
