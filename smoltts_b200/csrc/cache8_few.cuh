@@ -148,7 +148,6 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         copy_steps<HALVES, HALVES, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, 0);
     } else if (warp == kFewProducts) {
         if (steps > 0) {
-            const uint32_t on = elected();
             // ---- products: whichever can be made next, so that neither the keys' waits for the weights nor the values' (and the stage they free) for the
             // next step's keys ----
             const uint32_t q0 = umma::s2u(Qs), id_s = desc_e4m3(128, N, false, false), id_o = desc_e4m3(128, N, true, false);
@@ -160,24 +159,32 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                 const bool keys = scores < steps && has_passed(&bars.full[scores % NS], (scores / NS) & 1) && (scores < 2 || has_passed(&bars.s_empty[scores & 1], ((scores >> 1) - 1) & 1));
                 if (__all_sync(0xffffffffu, keys)) {
                     const int b = scores & 1, st = scores % NS;
-                    umma::fence_after_sync();
-                    const uint32_t k0 = umma::s2u(KV + st * SB);
-                    for (int k = 0; k < ksteps; ++k)
-                        mma_e4m3(on, tmem + b * N, umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32), umma::smem_desc_sw128(q0 + (k >> 2) * (N * 128) + (k & 3) * 32), id_s, k > 0 ? 1u : 0u);
-                    commit_on(on, &bars.s_full[b]);
+                    __syncwarp();
+                    if (elected()) {
+                        umma::fence_after_sync();
+                        const uint32_t k0 = umma::s2u(KV + st * SB);
+                        for (int k = 0; k < ksteps; ++k)
+                            mma_e4m3(tmem + b * N, umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32), umma::smem_desc_sw128(q0 + (k >> 2) * (N * 128) + (k & 3) * 32), id_s, k > 0 ? 1u : 0u);
+                        umma::commit(&bars.s_full[b]);
+                    }
+                    __syncwarp();
                     ++scores;
                     begin = clock64();
                 } else if (__all_sync(0xffffffffu, values < scores && has_passed(&bars.p_full[values & 1], (values >> 1) & 1))) {
                     const int b = values & 1, st = values % NS;
-                    umma::fence_after_sync();
-                    const uint32_t v = umma::s2u(KV + st * SB) + HALVES * (kStep * 128), p = umma::s2u(Ps + b * (N * 128));
+                    __syncwarp();
+                    if (elected()) {
+                        umma::fence_after_sync();
+                        const uint32_t v = umma::s2u(KV + st * SB) + HALVES * (kStep * 128), p = umma::s2u(Ps + b * (N * 128));
 #pragma unroll
-                    for (int x = 0; x < HALVES; ++x)
+                        for (int x = 0; x < HALVES; ++x)
 #pragma unroll
-                        for (int k = 0; k < kStep / 32; ++k)
-                            mma_e4m3(on, tm_o + (b * HALVES + x) * N, umma::smem_desc_sw128(v + x * (kStep * 128) + k * 32 * 128), umma::smem_desc_sw128(p + k * 32), id_o, k > 0 ? 1u : 0u);
-                    commit_on(on, &bars.empty[st]);
-                    commit_on(on, &bars.o_full[b]);
+                            for (int k = 0; k < kStep / 32; ++k)
+                                mma_e4m3(tm_o + (b * HALVES + x) * N, umma::smem_desc_sw128(v + x * (kStep * 128) + k * 32 * 128), umma::smem_desc_sw128(p + k * 32), id_o, k > 0 ? 1u : 0u);
+                        umma::commit(&bars.empty[st]);
+                        umma::commit(&bars.o_full[b]);
+                    }
+                    __syncwarp();
                     ++values;
                     begin = clock64();
                 } else if (__any_sync(0xffffffffu, *stop || clock64() - begin > kWaitCycles)) {
@@ -186,7 +193,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                     ok = false;
                 }
             }
-            commit_on(on, &bars.drained);      // nothing of the block's is in flight once this is through
+            if (elected()) umma::commit(&bars.drained);      // nothing of the block's is in flight once this is through
             drain_bar(&bars.drained, 0);
         }
     } else if (steps > 0) {

@@ -47,7 +47,9 @@ __device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity, volatil
 }
 // by a whole warp: true if it is for every lane
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* stop, int32_t* err) {
-    return __all_sync(0xffffffffu, wait_bar(bar, parity, stop, err));
+    const bool ok = __all_sync(0xffffffffu, wait_bar(bar, parity, stop, err));
+    __syncwarp();
+    return ok;
 }
 // the same for what is still in flight when a block ends
 __device__ __noinline__ void drain_bar(uint64_t* bar, uint32_t parity) {
@@ -77,33 +79,27 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ constexpr uint32_t desc_e4m3(int m, int n, bool a_mn, bool b_mn) {
     return (1u << 4) | (a_mn ? 1u << 15 : 0u) | (b_mn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// One lane of a converged warp.  The whole warp walks through the issuing code and each instruction carries the lane's predicate: issued from a branch that
-// only one thread takes, a tcgen05.mma costs 198 cycles whatever its size, this way 59 to 71 (of up to 128 columns) and 128 (of 256).
-__device__ __forceinline__ uint32_t elected() {
+// One lane of the warp.  The products' warp waits as a whole and issues inside `if (elected())`: issued by a thread that a branch on its index picked, a tcgen05.mma
+// costs 198 cycles whatever its size, this way 75 (16 columns) to 115 (128).
+__device__ __forceinline__ bool elected() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
-    return p;
+    return p != 0;
 }
-__device__ __forceinline__ void mma_e4m3(uint32_t on, uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
-        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // the same with A in tensor memory, four codes a column
-__device__ __forceinline__ void mma_e4m3_weights(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void mma_e4m3_weights(uint32_t d_tmem, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}\n"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate), "r"(on) : "memory");
-}
-__device__ __forceinline__ void commit_on(uint32_t on, uint64_t* bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n"
-        ::"r"(umma::s2u(bar)), "r"(on) : "memory");
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], %2, %3, p;\n\t}\n"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 // byte of byte x of row r in a tile of 128-byte rows with the 128-byte swizzle
 __device__ __forceinline__ int sw128_byte(int r, int x) { return r * 128 + (((x >> 4) ^ (r & 7)) << 4) + (x & 15); }

@@ -138,21 +138,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
         copy_steps<KH, 1, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, v_col);
     } else if (warp == kTileSoft + 1) {
         if (steps > 0) {
-            const uint32_t on = elected();
             // ---- products ----
             const uint32_t q0 = umma::s2u(Qs), id_s = desc_e4m3(128, kStep, false, false), id_o = desc_e4m3(128, 128, false, true);
             const int ksteps = (A.c.d + 31) / 32;
             auto scores = [&](int i) {
                 const int b = i & 1, st = i % NS;
                 if (!warp_wait(&bars.full[st], (i / NS) & 1, stop, A.c.err)) return false;
-                umma::fence_after_sync();
-                const uint32_t k0 = umma::s2u(KV + st * SB);
+                if (elected()) {
+                    umma::fence_after_sync();
+                    const uint32_t k0 = umma::s2u(KV + st * SB);
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
-                    for (int k = 0; k < ksteps; ++k)
-                        mma_e4m3(on, tmem + b * kStep, umma::smem_desc_sw128(q0 + (part * KH + (k >> 2)) * (kTileRows * 128) + (k & 3) * 32), umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32),
-                                 id_s, part > 0 || k > 0 ? 1u : 0u);
-                commit_on(on, &bars.s_full[b]);
+                    for (int part = 0; part < 2; ++part)
+                        for (int k = 0; k < ksteps; ++k)
+                            mma_e4m3(tmem + b * kStep, umma::smem_desc_sw128(q0 + (part * KH + (k >> 2)) * (kTileRows * 128) + (k & 3) * 32), umma::smem_desc_sw128(k0 + (k >> 2) * (kStep * 128) + (k & 3) * 32),
+                                     id_s, part > 0 || k > 0 ? 1u : 0u);
+                    umma::commit(&bars.s_full[b]);
+                }
+                __syncwarp();
                 return true;
             };
             // A step's scores are multiplied behind the values of the step before last, whose weights lie where they go (products are made in the order of
@@ -162,18 +164,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                 const int b = i & 1, st = i % NS;
                 ok = warp_wait(&bars.p_full[b], (i >> 1) & 1, stop, A.c.err);
                 if (!ok) break;
-                umma::fence_after_sync();
-                const uint32_t v = umma::s2u(KV + st * SB) + KH * (kStep * 128);
+                if (elected()) {
+                    umma::fence_after_sync();
+                    const uint32_t v = umma::s2u(KV + st * SB) + KH * (kStep * 128);
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+                    for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int k = 0; k < kStep / 32; ++k)
-                        mma_e4m3_weights(on, tm_o + b * 128, tmem + b * kStep + part * (kStep / 4) + k * 8, umma::smem_desc_sw128(v + k * 32 * 128), id_o, part > 0 || k > 0 ? 1u : 0u);
-                commit_on(on, &bars.empty[st]);
-                commit_on(on, &bars.o_full[b]);
+                        for (int k = 0; k < kStep / 32; ++k)
+                            mma_e4m3_weights(tm_o + b * 128, tmem + b * kStep + part * (kStep / 4) + k * 8, umma::smem_desc_sw128(v + k * 32 * 128), id_o, part > 0 || k > 0 ? 1u : 0u);
+                    umma::commit(&bars.empty[st]);
+                    umma::commit(&bars.o_full[b]);
+                }
+                __syncwarp();
                 ok = i + 2 >= steps || scores(i + 2);
             }
-            commit_on(on, &bars.drained);      // nothing of the block's is in flight once this is through
+            if (elected()) umma::commit(&bars.drained);      // nothing of the block's is in flight once this is through
             drain_bar(&bars.drained, 0);
         }
     } else if (steps > 0) {
