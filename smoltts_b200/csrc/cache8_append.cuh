@@ -2,7 +2,7 @@
 //
 // One block of threads per (16 positions, sequence, share of the heads).  The cosines and sines of the block's positions are made once, in
 // shared memory, for all heads: the angle pos * freq and its remainder in units of half turns in 64 bits (in 32 the angle of position 100000
-// is off by 0.004), the rest by sincospif.  A warp takes a head's 16 rows into registers, all loads at once: a lane has sixteen coordinates of a row
+// is off by 0.004), the rest by sincospif at the nearest float and a first-order step from there.  A warp takes a head's 16 rows into registers, all loads at once: a lane has sixteen coordinates of a row
 // that are rotated with one another (eight and the eight they go with, or eight pairs of neighbours), so that nothing is read twice and
 // cosines serve both; the largest magnitude, and with it the scale, is known before anything is rounded.
 //
@@ -149,10 +149,12 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     for (int i = threadIdx.x; i < (hi - lo) * A.pairs; i += kAppendThreads) {
         const int r = lo + i / A.pairs, j = i % A.pairs;
         const double half_turns = (double)(p0 + r) * (double)A.freq[j] * 0.3183098861837906715;      // the angle over pi
+        const double at = half_turns - 2.0 * rint(0.5 * half_turns);
+        const float near = (float)at, rest = (float)((at - (double)near) * 3.141592653589793);      // (a rounding of the angle of up to 2^-25 pi is twice that of the cosine)
         float sn, cs;
-        sincospif((float)(half_turns - 2.0 * rint(0.5 * half_turns)), &sn, &cs);
-        turn[0][r][j] = cs * A.mult;
-        turn[1][r][j] = sn * A.mult;
+        sincospif(near, &sn, &cs);
+        turn[0][r][j] = fmaf(-sn, rest, cs) * A.mult;
+        turn[1][r][j] = fmaf(cs, rest, sn) * A.mult;
     }
     if (A.pairs > 0) __syncthreads();
     const bool held = page >= 0 && page < A.c.n_pages;
