@@ -62,7 +62,7 @@ __device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, 
     x.end = max(min(kv_len, last_pos + 1), 0);
     const int blocks = (x.end + kBlock - 1) / kBlock;
     x.from = A.window > 0 ? min(max(first_pos - A.window + 1, 0) / kBlock, blocks) : 0;
-    x.lead = A.window > 0 ? min((A.first + kBlock - 1) / kBlock, x.from) : 0;
+    x.lead = A.window > 0 ? min(A.first / kBlock + (A.first % kBlock > 0), x.from) : 0;
     x.count = x.lead + blocks - x.from;
     return x;
 }

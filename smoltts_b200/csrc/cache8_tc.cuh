@@ -141,7 +141,7 @@ __device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, i
     x.end = max(min(kv_len, last_pos + 1), 0);
     const int steps = (x.end + kStep - 1) / kStep;
     x.from = A.window > 0 ? min(max(first_pos - A.window + 1, 0) / kStep, steps) : 0;
-    x.lead = A.window > 0 ? min((A.first + kStep - 1) / kStep, x.from) : 0;
+    x.lead = A.window > 0 ? min(A.first / kStep + (A.first % kStep > 0), x.from) : 0;
     x.count = x.lead + steps - x.from;
     return x;
 }

@@ -359,6 +359,19 @@ def test_strides_and_rows_of_nobody():
             assert (out[:2] == 7).all() and (out[2 + 2 * n:] == 7).all() and (out[..., d:] == 7).all()
 
 
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_windows_and_first_positions_of_any_size(n, dtype):
+    """The largest numbers that the arguments hold: everything is visible."""
+    H, G, d, L, most = 4, 2, 64, 700, 2 ** 31 - 1
+    c, table = cache_of([L], 64, G, d, d)
+    fill(c, table, [L])
+    q = randn(n, H, d, seed=3).to(dtype)
+    for window, first in ((16, most), (16, most - 100), (most, 0), (most, most), (most - 5, 3)):
+        options = dict(window=window, first=first)
+        check_attention(c, table, q, [n], [L - n], c.attend(q, ints([0, n]), ints([L - n]), table, max_new=n, max_len=L, **options), **options)
+
+
 def test_host_numbers_that_are_too_small():
     """A longer sequence than max_len is attended to as a whole; rows beyond max_new are left as they were."""
     H, G, d = 4, 2, 64
