@@ -333,7 +333,7 @@ typedef struct SmolLmCache8 {
     int32_t n_pages, page_size;  /* page_size: a multiple of 16 */
     int32_t kv_heads, dim, vdim; /* dim, vdim <= 256 */
     int32_t* err;                /* device word, set where a block table names a page outside the cache (1) or the arrays of a batch do not fit
-                                    what it says of itself (2) */
+                                    what it says of itself (2); 3: a wait inside a kernel ran out, results are missing */
 } SmolLmCache8;
 
 /* Rows seq_start[s] .. seq_start[s + 1] - 1 are the positions seq_pos0[s], + 1, ... of sequence s; rows outside every sequence are left alone.
@@ -349,7 +349,7 @@ typedef struct SmolLmCache8Batch {
  * coordinates (rot_half 1: coordinate i with i + rot_dims / 2, 0: 2i with 2i + 1) by position * freq[i], the angle in 64 bits; rot_mult multiplies cosine
  * and sine.  Magnitudes above 2^100 are clamped, a NaN stays one.  A block's scale is the smallest power of two with |value| <= 448 scale for the
  * new rows; where an earlier call began the block it never shrinks, and the codes already there follow it when it grows.  No page may be
- * written by two sequences of one batch.  Strides in elements. */
+ * written twice in one batch.  Strides in elements. */
 typedef struct SmolLmCache8Append {
     int32_t dtype;               /* SMOL_LM_BF16 / SMOL_LM_F32: of keys, values and queries */
     const void *k, *v;           /* [n_tokens][kv_heads][dim], [n_tokens][kv_heads][vdim] */
@@ -370,7 +370,7 @@ typedef struct SmolLmCache8Attend {
     int32_t dtype;               /* of queries and results */
     int32_t heads;               /* a multiple of kv_heads */
     const void* q;               /* [n_tokens][heads][dim] */
-    void* out;                   /* [n_tokens][heads][vdim] */
+    void* out;                   /* [n_tokens][heads][vdim], no part of q */
     size_t q_row, q_head, out_row, out_head;
     float scale, softcap, out_scale;
     int32_t window, first;

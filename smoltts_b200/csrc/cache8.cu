@@ -257,7 +257,7 @@ static int attend_of(const SmolLmCache8* c, const SmolLmCache8Batch* b, const Sm
     if (a->heads < 1 || a->heads % A.c.G) return report(SMOL_ERR_INVALID, me, "heads must be a multiple of kv_heads");
     if ((long long)A.b.max_new * (a->heads / A.c.G) > (1ll << 30) || (long long)A.b.T * a->heads > (1ll << 31) - 64)
         return report(SMOL_ERR_CAPACITY, me, "more query rows than 32 bits count");
-    if (a->window < 0 || a->first < 0 || !(a->softcap >= 0.0f)) return report(SMOL_ERR_INVALID, me, "window, first and softcap must not be negative");
+    if (a->window < 0 || a->first < 0 || !(a->softcap >= 0.0f) || a->softcap > 3.4e38f) return report(SMOL_ERR_INVALID, me, "window, first and softcap must not be negative, and softcap finite");
     if (!a->dist_r1 != !a->dist_r2) return report(SMOL_ERR_INVALID, me, "dist_r1 and dist_r2 come together");
     if (pointers && (!a->q || !a->out)) return report(SMOL_ERR_INVALID, me, "null queries or results");
     const bool f32 = a->dtype == SMOL_LM_F32;

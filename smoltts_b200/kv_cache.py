@@ -5,19 +5,20 @@ attends to them.
 Half the bytes of a bf16 cache: twice the positions in the same pool, and half the traffic of decoding.  Pages are the
 indices of a ``pool.PagePool``; a batch is ragged, as in an engine step: sequence ``s`` brings the rows ``seq_start[s] ..
 seq_start[s + 1] - 1``, which are its positions ``seq_pos0[s], seq_pos0[s] + 1, ...``.  Everything runs on the current stream
-of the cache's device and nothing synchronises, so that calls can be captured into a CUDA graph.  ``lm.HybridLM`` serves
+of the cache's device and nothing synchronises, so that calls can be captured into a CUDA graph; results carry no gradient.  ``lm.HybridLM`` serves
 its softmax attention layers from such a cache with ``kv_bits=8``.
 """
 from __future__ import annotations
 
 import ctypes as C
+import math
 import struct
 from typing import Dict, Optional, Tuple
 
 import torch
 
 from . import _capi_lm
-from ._errors import SMOL_ERR_CAPACITY, SMOL_OK, SmolError
+from ._errors import SMOL_ERR_CAPACITY, SMOL_ERR_CUDA, SMOL_OK, SmolError
 
 BLOCK = 16          # positions that share a scale
 _DTYPES = {torch.bfloat16: _capi_lm.SMOL_LM_BF16, torch.float32: _capi_lm.SMOL_LM_F32}
@@ -31,6 +32,25 @@ for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCa
 
 def _padded(n: int) -> int:
     return (n + 15) // 16 * 16
+
+
+def _extent(x: torch.Tensor) -> Tuple[int, int]:
+    """First byte and the one behind the last that a tensor reaches."""
+    at = x.data_ptr()
+    return at, at + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
+
+
+def _check_written(out: torch.Tensor, what: str, **read: torch.Tensor) -> None:
+    """A result must not overlap itself, nor what is read while it is written."""
+    (tokens, heads, width), (row, head, _) = out.shape, out.stride()
+    if not ((heads == 1 or head >= width) and (tokens == 1 or row >= (heads - 1) * head + width) or
+            (tokens == 1 or row >= width) and (heads == 1 or head >= (tokens - 1) * row + width)):
+        raise ValueError(f"{what}: rows must not overlap")
+    lo, hi = _extent(out)
+    for name, x in read.items():
+        a, b = _extent(x)
+        if a < hi and lo < b:
+            raise ValueError(f"{what} must not reach into {name}'s memory: it is read while {what} is written")
 
 
 class KVCache8:
@@ -135,7 +155,7 @@ class KVCache8:
 
         A block's 16 positions share the smallest power of two with |value| <= 448 * scale; where an earlier call began the block the
         scale never shrinks, and the older codes follow it when it grows.  Magnitudes above 2^100 are clamped; a NaN stays a NaN.  Two
-        sequences of a batch must not write the same page.  The rows of a sequence have to follow what it already holds."""
+        sequences of a batch must not write the same page, nor one write a page twice.  The rows of a sequence have to follow what it already holds."""
         tokens, dtype = k.shape[0], k.dtype
         k_row, k_head = self._rows(k, None, self.kv_heads, self.dim, None, "k")
         v_row, v_head = self._rows(v, tokens, self.kv_heads, self.vdim, dtype, "v")
@@ -156,10 +176,7 @@ class KVCache8:
                 out_row, out_head = heads * self.dim, self.dim
             else:
                 out_row, out_head = self._rows(q_out, tokens, heads, self.dim, dtype, "q_out")
-                if q_out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
-                    raise ValueError("q_out must not share q's memory: a row is read while others are written")
-                if (out_row < self.dim and tokens > 1) or (out_head < self.dim and heads > 1):
-                    raise ValueError("q_out: rows must not overlap")
+                _check_written(q_out, "q_out", q=q, k=k, v=v)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
@@ -180,21 +197,21 @@ class KVCache8:
 
         ``max_new``: most rows a sequence brings; ``max_len``: most positions a sequence holds, the rows included (host numbers;
         the grid is chosen by them -- a longer sequence is attended to as a whole all the same, rows beyond ``max_new`` are left alone).
-        Returns ``[tokens, heads, vdim]`` of q's type, in ``out`` if given; rows outside every sequence are left as they were."""
+        Returns ``[tokens, heads, vdim]`` of q's type, in ``out`` if given (which must not reach into q's memory); rows outside every sequence are left as
+        they were, which in a new tensor is anything."""
         q_row, q_head = self._rows(q, None, None, self.dim, None, "q")
         tokens, heads, dtype = q.shape[0], q.shape[1], q.dtype
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} query heads over {self.kv_heads} key/value heads")
-        if window < 0 or first < 0 or not softcap >= 0.0:
-            raise ValueError("window, first and softcap must not be negative")
+        if window < 0 or first < 0 or not 0.0 <= softcap < math.inf:
+            raise ValueError("window, first and softcap must not be negative, and softcap finite")
         batch = self._batch(tokens, seq_start, seq_pos0, block_table, max_new, max_len, kv_len)
         if out is None:
             out = q.new_empty((tokens, heads, self.vdim))
             out_row, out_head = heads * self.vdim, self.vdim
         else:
             out_row, out_head = self._rows(out, tokens, heads, self.vdim, dtype, "out")
-            if (out_row < self.vdim and tokens > 1) or (out_head < self.vdim and heads > 1):
-                raise ValueError("out: rows must not overlap")
+            _check_written(out, "out", q=q)
         r1 = r2 = 0
         if penalty is not None:
             r1, r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
@@ -226,5 +243,7 @@ class KVCache8:
     def check_device_errors(self) -> None:
         """Raises if a call met a page outside the cache or arrays that contradict one another (reads a device word; synchronises)."""
         word = int(self._err.item())
+        if word == 3:
+            raise SmolError(SMOL_ERR_CUDA, "device-side error word 3: a wait inside a kernel ran out, results of that call are missing")
         if word:
             raise SmolError(SMOL_ERR_CAPACITY, f"device-side error word {word}: " + ("a block table names a page outside the cache" if word == 1 else "a batch's arrays do not fit its sizes"))

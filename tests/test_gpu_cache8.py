@@ -542,3 +542,44 @@ def test_refusals():
     wide = KVCache8.allocate(4, 16, 1, 272)
     refused(wide.append, randn(1, 1, 272), randn(1, 1, 272), start, pos0, ints([[0]]), max_new=1)
     refused(wide.attend, randn(1, 1, 272), start, pos0, ints([[0]]), max_new=1, max_len=1)
+
+
+@pytest.mark.parametrize("n", [2, 40])
+def test_results_that_overlap_what_is_read_or_themselves_are_refused(n):
+    H, G, d = 4, 2, 64
+    c, table = cache_of([64], 32, G, d, d)
+    fill(c, table, [64])
+    batch, room = (ints([0, n]), ints([64 - n]), table), torch.zeros(4 * n * H * d, device="cuda", dtype=torch.bfloat16)
+    cut = lambda at, *stride: room.as_strided((n, H, d), stride or (H * d, d, 1), at)  # noqa: E731
+    q, k, v = cut(0), randn(n, G, d, seed=4).to(torch.bfloat16), randn(n, G, d, seed=5).to(torch.bfloat16)
+    q.copy_(randn(n, H, d, seed=3))
+    far = n * H * d
+    for out in (q, cut(d), cut(far - 1), cut(far, d, d, 1), cut(far, H * d, d - 1, 1), cut(far, (H - 1) * d, d, 1), cut(far, d, (n - 1) * d, 1)):
+        with pytest.raises(ValueError):
+            c.attend(q, *batch, max_new=n, max_len=64, out=out)
+        with pytest.raises(ValueError):
+            c.append(k, v, *batch, max_new=n, q=q, q_out=out)
+    with pytest.raises(ValueError):
+        c.append(k, v, *batch, max_new=n, q=randn(n, G, d).to(torch.bfloat16), q_out=k)
+    # what lies apart in the same memory, and heads in front of rows, are served
+    for out in (cut(far), cut(far, d, n * d, 1), cut(far, H * d + 24, d + 8, 1)):
+        if n == 2 or out.stride(0) != H * d + 24:
+            check_attention(c, table, q, [n], [64 - n], c.attend(q, *batch, max_new=n, max_len=64, out=out).contiguous())
+            want = c.append(k, v, *batch, max_new=n, q=q)
+            assert torch.equal(c.append(k, v, *batch, max_new=n, q=q, q_out=out), want)
+
+
+def test_softcap_must_be_finite():
+    c, table = cache_of([64], 32, 2, 64, 64)
+    with pytest.raises(ValueError):
+        c.attend(randn(1, 4, 64), ints([0, 1]), ints([63]), table, max_new=1, max_len=64, softcap=math.inf)
+
+
+def test_device_words_are_told_apart():
+    from smoltts_b200._errors import SmolError
+
+    c, _ = cache_of([64], 32, 2, 64, 64)
+    for word, text in ((1, "page outside"), (2, "do not fit"), (3, "ran out")):
+        c._err.fill_(word)
+        with pytest.raises(SmolError, match=text):
+            c.check_device_errors()
