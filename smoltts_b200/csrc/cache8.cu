@@ -77,8 +77,16 @@ cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cuda
     return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st);
 }
 
-constexpr int kFewMost = 32;      // query rows of a sequence and key/value head up to which the kernel for few rows takes them
-bool tiles_serve(const AttendArgs& A, bool f32) { return !f32 && A.b.max_new * (long long)(A.H / A.c.G) > kFewMost; }
+// Query rows of a sequence and key/value head up to which the kernel for few rows takes them: it reads the keys once per 16 rows and shares them out finely, the
+// tiles pay for 128 rows whatever they hold.  Both measured, few rows / tiles, 8 heads of 128: 16 sequences at 4096 positions with 16 rows 51 / 69 us,
+// 24 rows 82 / 69, 32 rows 81 / 69; 64 at 2048 92 / 160, 187 / 162, 180 / 162; one at 32768 27 / 42, 44 / 44, 45 / 45.  Where all of it is too little
+// to fill the GPU the keys' shares are what counts: one at 2048 with 32 rows 15.9 / 18.1, with 64 17.0 / 22.3, with 96 32 / 25.
+constexpr int kFewMost = 16, kFewMostSmall = 64;
+constexpr long long kSmall = 1 << 16;      // sequences times heads times positions (16384: the last of these; 262144: the one at 32768)
+bool tiles_serve(const AttendArgs& A, bool f32) {
+    const long long rows = A.b.max_new * (long long)(A.H / A.c.G), most = (long long)A.b.S * A.c.G * A.b.max_len <= kSmall ? kFewMostSmall : kFewMost;
+    return !f32 && rows > most;
+}
 
 // query rows of a block of threads
 static int row_tile(const AttendArgs& A, bool f32) {
@@ -161,8 +169,11 @@ static cudaError_t attend_tiles(const AttendArgs& A, cudaStream_t st) {
 }
 
 // A batch whose sequences may bring anything from one row to many: those of few rows go to the kernel for few rows, which shares their keys out.  With short
-// contexts (a tile walks 2048 positions in 35 us) or one sequence that is not worth a launch.
-static bool mixed(const AttendArgs& A, bool f32) { return tiles_serve(A, f32) && A.b.S > 1 && A.b.max_len > 2048 && A.H / A.c.G <= kFewMost && A.rows_most > kFewMost; }
+// contexts (a tile walks 2048 positions in 35 us), one sequence, or as many rows as if all brought max_new, that is not worth a launch (8 us of 77 where it finds
+// nothing to do: 16 sequences of 6 rows at 4096 positions).
+static bool mixed(const AttendArgs& A, bool f32) {
+    return tiles_serve(A, f32) && A.b.S > 1 && A.b.T < (long long)A.b.S * A.b.max_new && A.b.max_len > 2048 && A.H / A.c.G <= kFewMost && A.rows_most > kFewMost;
+}
 
 size_t attend_bytes(const AttendArgs& A, bool f32, int n_sms) {
     const int splits = splits_for(A, f32, n_sms);
