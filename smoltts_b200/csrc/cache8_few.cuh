@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                 if (BENT) {
                     s_r1[r] = A.r1 ? A.r1[h] : 0.0f;
                     s_r2[r] = A.r1 ? A.r2[h] : 0.0f;
-                    s_slope[r] = A.slope ? A.slope[h] : 0.0f;
+                    s_slope[r] = A.slope ? A.slope[h] * kLog2e : 0.0f;
                 }
             }
         }
@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         // ---- softmax: a position per thread; a column of the result per thread and half ----
         const int me = threadIdx.x;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const Bend bend(A);
         float m[RA], l[RA], o[HALVES][RA];              // running maximum, this thread's part of the denominator, results in full
         float m_step[RA], l_step[RA], unit = 0.0f;      // of the step before, whose product is not yet joined; what it is in units of
 #pragma unroll
@@ -315,7 +316,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             arrive(&bars.s_empty[b]);
             if (BENT) {
 #pragma unroll
-                for (int r = 0; r < RA; ++r) S[r] = bent_score<false>(A, S[r], s_pos[r] - j, s_r1[r], s_r2[r], s_slope[r]);
+                for (int r = 0; r < RA; ++r) S[r] = bend(A, S[r], (float)(s_pos[r] - j), s_r1[r], s_r2[r], s_slope[r]);
             }
             const bool whole = j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             bool hidden = ks == 0.0f;      // from some row

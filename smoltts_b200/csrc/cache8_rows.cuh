@@ -70,17 +70,25 @@ __device__ __forceinline__ bool sees(const AttendArgs& A, int pos, int j, int en
     return j <= pos && j < end && (A.window == 0 || pos - j < A.window || j < A.first);
 }
 
-// What follows the scaled product, in units of log2: soft cap and distance penalties.  EXACT: the library's functions (float32).
-template <bool EXACT>
+// What follows the scaled product, in units of log2: soft cap and distance penalties, with the library's functions (float32).
 __device__ __forceinline__ float bent_score(const AttendArgs& A, float s, int dist, float r1, float r2, float slope) {
-    if (A.softcap > 0.0f) {
-        if (EXACT) s = A.softcap * tanhf(s / A.softcap);
-        else s = A.softcap * (1.0f - __fdividef(2.0f, exp2_fast(2.0f * kLog2e * s / A.softcap) + 1.0f));
-    }
+    if (A.softcap > 0.0f) s = A.softcap * tanhf(s / A.softcap);
     const float d = (float)max(dist, 0);
-    if (A.r1) s -= EXACT ? r1 * log1pf(r2 * d) : r1 * 0.69314718f * log2_fast(fmaf(r2, d, 1.0f));
+    if (A.r1) s -= r1 * log1pf(r2 * d);
     return (s - slope * d) * kLog2e;
 }
+// The same with the hardware's (bf16): cap tanh(s / cap) log2 e = c - 2 c / (2^(s in) + 1) with c = cap log2 e and in = 2 log2 e / cap, and r ln(x) log2 e = r log2(x);
+// slope comes in units of log2.  (Of a distance below zero, that is hidden anyway, a NaN is made.)
+struct Bend {
+    float in, c;
+    __device__ __forceinline__ explicit Bend(const AttendArgs& A) : in(A.softcap > 0.0f ? fminf(2.0f * kLog2e / A.softcap, 3e38f) : 0.0f), c(A.softcap * kLog2e) {}
+    __device__ __forceinline__ float operator()(const AttendArgs& A, float s, float dist, float r1, float r2, float slope) const {
+        if (c > 0.0f) s = fmaf(-2.0f * c, __fdividef(1.0f, exp2_fast(s * in) + 1.0f), c);
+        else s *= kLog2e;
+        if (A.r1) s = fmaf(-r1, log2_fast(fmaf(r2, dist, 1.0f)), s);
+        return fmaf(-slope, dist, s);
+    }
+};
 
 template <class T> struct Elem;
 template <> struct Elem<float> {
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int e = 0; e < 4; ++e) {
                 const int j = j0 + (e & 1) + 8 * (e >> 1);
                 float v = sc[e >> 1][2 * x + (e & 1)] * mul;
-                if (BENT) v = bent_score<PARTS == 2>(A, v, pos[x] - j, r1[x], r2[x], slope[x]);
+                if (BENT) v = bent_score(A, v, pos[x] - j, r1[x], r2[x], slope[x]);
                 p[x][e] = whole || sees(A, pos[x], j, seen.end) ? v : -INFINITY;
             }
             top[x] = fmaxf(fmaxf(p[x][0], p[x][1]), fmaxf(p[x][2], p[x][3]));

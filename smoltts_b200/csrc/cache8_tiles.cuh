@@ -233,7 +233,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
         // ---- softmax: warps q, q + 4, q + 8, q + 12 share rows 32 q .. + 31; part p has columns 32 p .. + 31 of the scores and of the result ----
         const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane, my_row = min(row0 + row, n * Gq - 1), pos = pos0 + my_row / Gq, h = g * Gq + my_row % Gq;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
-        const float rowmul = s_rowmul[row], r1 = BENT && A.r1 ? A.r1[h] : 0.0f, r2 = BENT && A.r1 ? A.r2[h] : 0.0f, slope = BENT && A.slope ? A.slope[h] : 0.0f;
+        const float rowmul = s_rowmul[row], r1 = BENT && A.r1 ? A.r1[h] : 0.0f, r2 = BENT && A.r1 ? A.r2[h] : 0.0f, slope = BENT && A.slope ? A.slope[h] * kLog2e : 0.0f;
+        const Bend bend(A);
         auto row_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(quad + 1), "n"(kTileParts * 32) : "memory"); };
         float m = -INFINITY, l = 0.0f, m_step = -INFINITY, l_step = 0.0f, unit = 0.0f, o[kTileCols];
 #pragma unroll
@@ -305,10 +306,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
 #pragma unroll
             for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = rowmul * ks[x];
             if (!direct) {
+                const float d0 = (float)(pos - jc);
 #pragma unroll
                 for (int e = 0; e < kTileCols; ++e) {
                     S[e] *= mul[e / kBlock];
-                    if (BENT) S[e] = bent_score<false>(A, S[e], pos - (jc + e), r1, r2, slope);
+                    if (BENT) S[e] = bend(A, S[e], d0 - (float)e, r1, r2, slope);
                 }
 #pragma unroll
                 for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = 1.0f;
