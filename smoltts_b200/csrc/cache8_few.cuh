@@ -198,21 +198,19 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         }
     } else if (steps > 0) {
         // ---- queries into shared memory: row r's first parts at row r, its second parts at row NR + r ----
-        for (int r = warp; r < RA; r += 4) {
-            const int row = min(row0 + r, n * Gq - 1), h = g * Gq + row % Gq;
-            const bf16* q = static_cast<const bf16*>(A.q) + (size_t)(t0 + row / Gq) * A.q_row + (size_t)h * A.q_head;
+        uint2 u[RA / 4][HALVES];
+        load_queries<RA / 4, HALVES>(u, A, [&](int y) {
+            const int row = min(row0 + warp + 4 * y, n * Gq - 1), tok = row / Gq;
+            return static_cast<const bf16*>(A.q) + (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
+        });
+#pragma unroll
+        for (int i = 0; i < RA / 4; ++i) {
+            const int r = warp + 4 * i, row = min(row0 + r, n * Gq - 1), h = g * Gq + row % Gq;
             float v[HALVES][4];
             uint32_t top = 0;
 #pragma unroll
             for (int x = 0; x < HALVES; ++x) {
-                const int at = x * 128 + lane * 4;
-                if (A.q_vec) {
-                    const uint2 u = at < A.c.d ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0u, 0u);
-                    v[x][0] = bf_lo(u.x); v[x][1] = bf_hi(u.x); v[x][2] = bf_lo(u.y); v[x][3] = bf_hi(u.y);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[x][e] = at + e < A.c.d ? __bfloat162float(q[at + e]) : 0.0f;
-                }
+                four_of(u[i][x], v[x]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[x][e])));
             }

@@ -148,6 +148,34 @@ __device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, i
 // first position of step i of a share that begins at number lo
 __device__ __forceinline__ int step_place(const Seen& seen, int lo, int i) { return (lo + i < seen.lead ? lo + i : seen.from + lo + i - seen.lead) * kStep; }
 
+// N rows of queries as they lie in memory, lane l's coordinates 4 l .. + 3 of each 128; all loads before anything is made of them (a row's after the one before it
+// took 2000 cycles a row).
+template <int N, int KH, class RowAt>
+__device__ __forceinline__ void load_queries(uint2 (&u)[N][KH], const AttendArgs& A, RowAt&& row_at) {
+    const int at = (threadIdx.x & 31) * 4;
+    if (A.q_vec) {
+#pragma unroll
+        for (int y = 0; y < N; ++y) {
+            const bf16* q = row_at(y);
+#pragma unroll
+            for (int x = 0; x < KH; ++x) u[y][x] = x * 128 + at < A.c.d ? *reinterpret_cast<const uint2*>(q + x * 128 + at) : make_uint2(0u, 0u);
+        }
+    } else {
+#pragma unroll
+        for (int y = 0; y < N; ++y) {
+            const unsigned short* q = reinterpret_cast<const unsigned short*>(row_at(y));
+#pragma unroll
+            for (int x = 0; x < KH; ++x) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = x * 128 + at + e < A.c.d ? q[x * 128 + at + e] : 0u;
+                u[y][x] = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+            }
+        }
+    }
+}
+__device__ __forceinline__ void four_of(uint2 u, float (&v)[4]) { v[0] = bf_lo(u.x); v[1] = bf_hi(u.x); v[2] = bf_lo(u.y); v[3] = bf_hi(u.y); }
+
 // What the copying warp leaves beside a stage: the scales of the step's blocks (0: nothing there; the values' sign says whether a block holds a NaN).
 struct StepScales {
     float k[kStepBlocks], v[kStepBlocks];

@@ -186,38 +186,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
         constexpr int AT_ONCE = 8 / KH;      // rows whose loads are on their way together
 #pragma unroll 1
         for (int r0 = warp; r0 < kTileRows; r0 += kTileSoft * AT_ONCE) {
-            float v[AT_ONCE][KH][4];
-#pragma unroll
-            for (int y = 0; y < AT_ONCE; ++y) {
+            uint2 u[AT_ONCE][KH];
+            load_queries<AT_ONCE, KH>(u, A, [&](int y) {
                 const int row = min(row0 + r0 + y * kTileSoft, n * Gq - 1), tok = row / Gq;
-                const bf16* q = static_cast<const bf16*>(A.q) + (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
-#pragma unroll
-                for (int x = 0; x < KH; ++x) {
-                    const int at = x * 128 + lane * 4;
-                    if (A.q_vec) {
-                        const uint2 u = at < A.c.d ? *reinterpret_cast<const uint2*>(q + at) : make_uint2(0u, 0u);
-                        v[y][x][0] = bf_lo(u.x); v[y][x][1] = bf_hi(u.x); v[y][x][2] = bf_lo(u.y); v[y][x][3] = bf_hi(u.y);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[y][x][e] = at + e < A.c.d ? __bfloat162float(q[at + e]) : 0.0f;
-                    }
-                }
-            }
+                return static_cast<const bf16*>(A.q) + (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
+            });
 #pragma unroll
             for (int y = 0; y < AT_ONCE; ++y) {
+                float v[KH][4];
+#pragma unroll
+                for (int x = 0; x < KH; ++x) four_of(u[y][x], v[x]);
                 const int r = r0 + y * kTileSoft;
                 uint32_t top = 0;
 #pragma unroll
                 for (int x = 0; x < KH; ++x)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[y][x][e])));
+                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[x][e])));
                 top = __reduce_max_sync(0xffffffffu, top);
                 const int e = max((int)(top >> 23) - 127, -110);      // (below: rows of less than 2^-110 keep a factor that fp32 holds)
                 const float up = pow2(7 - e);
 #pragma unroll
                 for (int x = 0; x < KH; ++x) {
                     uint32_t hi, rest;
-                    four_equal_parts(half_two(v[y][x][0] * up, v[y][x][1] * up), half_two(v[y][x][2] * up, v[y][x][3] * up), hi, rest);
+                    four_equal_parts(half_two(v[x][0] * up, v[x][1] * up), half_two(v[x][2] * up, v[x][3] * up), hi, rest);
                     *reinterpret_cast<uint32_t*>(Qs + x * (kTileRows * 128) + sw128_byte(r, lane * 4)) = hi;
                     *reinterpret_cast<uint32_t*>(Qs + (KH + x) * (kTileRows * 128) + sw128_byte(r, lane * 4)) = rest;
                 }
@@ -400,39 +391,49 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
 #pragma unroll
         for (int x = 0; x < kTileParts; ++x) total += s_max[0][x][row];
         const int col = v_col + part * kTileCols;
-        if (row < rows && col < A.c.dv && !*stop) {
+        if (col < A.c.dv && !__any_sync(0xffffffffu, *stop)) {
+            const bool mine = row < rows;
             const int tok = t0 + my_row / Gq;
-            if (s_bad) {
+            if (s_bad && mine) {
+                const uint32_t bits = nan_bits(A, W, pos, col);
 #pragma unroll
-                for (int x = 0; x < kTileCols / 32; ++x) {
-                    const uint32_t bits = nan_bits(A, W, pos, col + 32 * x);
-#pragma unroll
-                    for (int c = 0; c < 32; ++c)
-                        if (bits >> c & 1) o[32 * x + c] = __int_as_float(0x7fffffff);
-                }
+                for (int c = 0; c < 32; ++c)
+                    if (bits >> c & 1) o[c] = __int_as_float(0x7fffffff);
             }
             if (A.n_splits > 1) {
+                const int ld = (A.c.dv + 3) / 4 * 4;
                 const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
-                if (col == 0) part_stats(A)[at] = make_float2(m, total);
-                float* to = A.part + at * ((A.c.dv + 3) / 4 * 4) + col;
+                if (mine && col == 0) part_stats(A)[at] = make_float2(m, total);
+                float* to = A.part + at * ld + col;
 #pragma unroll
-                for (int c = 0; c < kTileCols; ++c)
-                    if (col + c < A.c.dv) to[c] = o[c];
+                for (int c = 0; c < kTileCols; c += 4)
+                    if (mine && col + c < ld) *reinterpret_cast<float4*>(to + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
             } else {
-                bf16* to = static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col;
                 // one division a row
                 const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, m);
                 const float f = m == -INFINITY ? 1.0f : exp2_fast(m - M), all = fmaf(total, f, M == -INFINITY ? 0.0f : exp2_fast(sink - M)), r = all == 0.0f ? 1.0f : f / all;
-                if (A.o_vec && !A.gate) {
+                if (A.o_vec == 2 && !A.gate) {
+                    // through shared memory (the ring is done with: the last product was waited for), so that four lanes write a row's 64 bytes: a lane's own row
+                    // a lane, 8 bytes at a time, cost 4000 cycles a block
+                    unsigned char* tile = KV + warp * (32 * 64);
 #pragma unroll
-                    for (int c = 0; c < kTileCols; c += 4)
-                        if (col + c < A.c.dv) {
-                            float v[4];
+                    for (int x = 0; x < 4; ++x) {
+                        uint32_t w[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] = o[c + e] * r * A.out_scale;
-                            *reinterpret_cast<uint2*>(to + c) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-                        }
-                } else {
+                        for (int y = 0; y < 4; ++y) w[y] = pack_bf16(o[8 * x + 2 * y] * r * A.out_scale, o[8 * x + 2 * y + 1] * r * A.out_scale);
+                        *reinterpret_cast<uint4*>(tile + lane * 64 + (x ^ (lane >> 1 & 3)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    __syncwarp();
+                    const int piece = lane & 3;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int l = 8 * x + (lane >> 2), at = row0 + quad * 32 + l, t = at / Gq;
+                        if (quad * 32 + l >= rows || col + piece * 8 >= A.c.dv) continue;
+                        bf16* to = static_cast<bf16*>(A.out) + (size_t)(t0 + t) * A.o_row + (size_t)(g * Gq + at - t * Gq) * A.o_head + col + piece * 8;
+                        *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(tile + l * 64 + (piece ^ (l >> 1 & 3)) * 16);
+                    }
+                } else if (mine) {
+                    bf16* to = static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col;
 #pragma unroll
                     for (int c = 0; c < kTileCols; ++c)
                         if (col + c < A.c.dv) to[c] = __float2bfloat16_rn(finished(A, tok, h, col + c, o[c] * r));
