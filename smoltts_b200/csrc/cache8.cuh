@@ -66,7 +66,7 @@ struct AttendArgs {
     float out_scale;
     float* part;                     // shares of the keys: unnormalised results [T * H][n_splits][dv rounded up to 4], then (maximum, denominator) [T * H][n_splits]
     int n_splits;
-    int q_vec, o_vec;
+    int q_vec, o_vec;                // rows are whole groups of four elements that a load takes (1), of eight on 16-byte boundaries (2)
     int rows_over, rows_most;        // only sequences of more than rows_over and at most rows_most query rows per key/value head
 };
 

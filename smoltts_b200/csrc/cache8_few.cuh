@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         uint2 u[RA / 4][HALVES];
         load_queries<RA / 4, HALVES>(u, A, [&](int y) {
             const int row = min(row0 + warp + 4 * y, n * Gq - 1), tok = row / Gq;
-            return static_cast<const bf16*>(A.q) + (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
+            return (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
         });
 #pragma unroll
         for (int i = 0; i < RA / 4; ++i) {

@@ -149,10 +149,12 @@ __device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, i
 __device__ __forceinline__ int step_place(const Seen& seen, int lo, int i) { return (lo + i < seen.lead ? lo + i : seen.from + lo + i - seen.lead) * kStep; }
 
 // N rows of queries as they lie in memory, lane l's coordinates 4 l .. + 3 of each 128; all loads before anything is made of them (a row's after the one before it
-// took 2000 cycles a row).
-template <int N, int KH, class RowAt>
-__device__ __forceinline__ void load_queries(uint2 (&u)[N][KH], const AttendArgs& A, RowAt&& row_at) {
-    const int at = (threadIdx.x & 31) * 4;
+// took 2000 cycles a row).  Lane y finds row y: offset_of(y), in elements, has a division.
+template <int N, int KH, class OffsetOf>
+__device__ __forceinline__ void load_queries(uint2 (&u)[N][KH], const AttendArgs& A, OffsetOf&& offset_of) {
+    const int lane = threadIdx.x & 31, at = lane * 4;
+    const size_t mine = offset_of(min(lane, N - 1));
+    auto row_at = [&](int y) { return static_cast<const bf16*>(A.q) + __shfl_sync(0xffffffffu, mine, y); };
     if (A.q_vec) {
 #pragma unroll
         for (int y = 0; y < N; ++y) {

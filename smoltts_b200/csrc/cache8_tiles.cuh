@@ -182,38 +182,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             drain_bar(&bars.drained, 0);
         }
     } else if (steps > 0) {
-        // ---- queries into shared memory, a warp per row ----
-        constexpr int AT_ONCE = 8 / KH;      // rows whose loads are on their way together
-#pragma unroll 1
-        for (int r0 = warp; r0 < kTileRows; r0 += kTileSoft * AT_ONCE) {
-            uint2 u[AT_ONCE][KH];
-            load_queries<AT_ONCE, KH>(u, A, [&](int y) {
-                const int row = min(row0 + r0 + y * kTileSoft, n * Gq - 1), tok = row / Gq;
-                return static_cast<const bf16*>(A.q) + (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
-            });
+        // ---- queries into shared memory, eight rows a warp, eight coordinates a lane: all loads before anything is made of them ----
+        {
+            constexpr int LANES = DK / 8, AT_ONCE = 32 / LANES, LOADS = 8 / AT_ONCE;      // of a row; rows of a load; loads
+            const int at = lane % LANES * 8, r0 = warp * 8;
+            size_t off = 0;      // (lane y finds row y, which takes a division)
+            {
+                const int row = min(row0 + r0 + (lane & 7), n * Gq - 1), tok = row / Gq;
+                off = (size_t)(t0 + tok) * A.q_row + (size_t)(g * Gq + row - tok * Gq) * A.q_head;
+            }
+            uint4 u[LOADS];
 #pragma unroll
-            for (int y = 0; y < AT_ONCE; ++y) {
-                float v[KH][4];
-#pragma unroll
-                for (int x = 0; x < KH; ++x) four_of(u[y][x], v[x]);
-                const int r = r0 + y * kTileSoft;
-                uint32_t top = 0;
-#pragma unroll
-                for (int x = 0; x < KH; ++x)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(fabsf(v[x][e])));
-                top = __reduce_max_sync(0xffffffffu, top);
-                const int e = max((int)(top >> 23) - 127, -110);      // (below: rows of less than 2^-110 keep a factor that fp32 holds)
-                const float up = pow2(7 - e);
-#pragma unroll
-                for (int x = 0; x < KH; ++x) {
-                    uint32_t hi, rest;
-                    four_equal_parts(half_two(v[x][0] * up, v[x][1] * up), half_two(v[x][2] * up, v[x][3] * up), hi, rest);
-                    *reinterpret_cast<uint32_t*>(Qs + x * (kTileRows * 128) + sw128_byte(r, lane * 4)) = hi;
-                    *reinterpret_cast<uint32_t*>(Qs + (KH + x) * (kTileRows * 128) + sw128_byte(r, lane * 4)) = rest;
+            for (int y = 0; y < LOADS; ++y) {
+                const bf16* q = static_cast<const bf16*>(A.q) + __shfl_sync(0xffffffffu, off, y * AT_ONCE + lane / LANES);
+                u[y] = make_uint4(0u, 0u, 0u, 0u);
+                if (A.q_vec == 2) {
+                    if (at < A.c.d) u[y] = *reinterpret_cast<const uint4*>(q + at);
+                } else {
+                    auto two_at = [&](int c) {
+                        const unsigned short* w = reinterpret_cast<const unsigned short*>(q);
+                        return (c < A.c.d ? (uint32_t)w[c] : 0u) | (c + 1 < A.c.d ? (uint32_t)w[c + 1] << 16 : 0u);
+                    };
+                    u[y] = make_uint4(two_at(at), two_at(at + 2), two_at(at + 4), two_at(at + 6));
                 }
+            }
+#pragma unroll
+            for (int y = 0; y < LOADS; ++y) {
+                const int r = r0 + y * AT_ONCE + lane / LANES;
+                const uint32_t w[4] = {u[y].x, u[y].y, u[y].z, u[y].w};
+                // the largest magnitude, as bits: a NaN's are above infinity's
+                uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+#pragma unroll
+                for (int x = LANES / 2; x > 0; x >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, x));
+                const uint32_t top = max(most & 0xffffu, most >> 16);
+                const int e = max((int)(top >> 7) - 127, -110);      // (below: rows of less than 2^-110 keep a factor that fp32 holds)
+                const float up = pow2(7 - e);
+                uint32_t hi[2], rest[2];
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+                    four_equal_parts(half_two(bf_lo(w[2 * x]) * up, bf_hi(w[2 * x]) * up), half_two(bf_lo(w[2 * x + 1]) * up, bf_hi(w[2 * x + 1]) * up), hi[x], rest[x]);
+                unsigned char* to = Qs + at / 128 * (kTileRows * 128) + sw128_byte(r, at % 128);
+                *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(to + KH * (kTileRows * 128)) = make_uint2(rest[0], rest[1]);
                 // (a row that is not finite: every score of it is a NaN)
-                if (lane == 0) s_rowmul[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 7) * (A.scale * (BENT ? 1.0f : kLog2e));
+                if (at == 0) s_rowmul[r] = top >= 0x7f80u ? __int_as_float(0x7fffffff) : pow2(e - 7) * (A.scale * (BENT ? 1.0f : kLog2e));
             }
         }
         umma::fence_async_smem();
