@@ -206,10 +206,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                     u[y] = make_uint4(two_at(at), two_at(at + 2), two_at(at + 4), two_at(at + 6));
                 }
             }
-#pragma unroll
-            for (int y = 0; y < LOADS; ++y) {
+#pragma unroll 1
+            for (int y = 0; y < LOADS; ++y) {      // (once a block: code that is fetched for it takes longer than it runs)
                 const int r = r0 + y * AT_ONCE + lane / LANES;
-                const uint32_t w[4] = {u[y].x, u[y].y, u[y].z, u[y].w};
+                const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+                for (int x = 1; x < LOADS; ++x) u[x - 1] = u[x];
                 // the largest magnitude, as bits: a NaN's are above infinity's
                 uint32_t most = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
 #pragma unroll
