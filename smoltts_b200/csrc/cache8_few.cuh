@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     volatile int* stop = &bars.stop;
 
     if (warp == kFewCopies) {
-        copy_steps<HALVES, HALVES, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, 0);
+        copy_steps<HALVES, HALVES, NS, false>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, 0);
     } else if (warp == kFewProducts) {
         if (steps > 0) {
             // ---- products: whichever can be made next, so that neither the keys' waits for the weights nor the values' (and the stage they free) for the
@@ -294,10 +294,10 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), j = j0 + me;
             // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
             wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
-            const float ks = s_scales[st].k[me / kBlock], vs = s_scales[st].v[me / kBlock];
+            const float ks = s_scales[st].of[me / kBlock].x, vs = s_scales[st].of[me / kBlock].y;
             float v_top = 0.0f;
 #pragma unroll
-            for (int x = 0; x < kStepBlocks; ++x) v_top = fmaxf(v_top, fabsf(s_scales[st].v[x]));
+            for (int x = 0; x < kStepBlocks; ++x) v_top = fmaxf(v_top, fabsf(s_scales[st].of[x].y));
             wait_bar(&bars.s_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
             umma::fence_after_sync();

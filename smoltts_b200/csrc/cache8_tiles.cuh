@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
     volatile int* stop = &bars.stop;
 
     if (warp == kTileSoft) {
-        copy_steps<KH, 1, NS>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, v_col);
+        copy_steps<KH, 1, NS, true>(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars.full, bars.empty, stop, v_col);
     } else if (warp == kTileSoft + 1) {
         if (steps > 0) {
             // ---- products ----
@@ -278,19 +278,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), jc = j0 + part * kTileCols;
             // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
             wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
-            float ks[kTileCols / kBlock], vs[kTileCols / kBlock], v_top = 0.0f;
-            bool nans = false, holes = false;      // in the whole step
-#pragma unroll
-            for (int x = 0; x < kStepBlocks; ++x) {
-                const float v = s_scales[st].v[x];
-                v_top = fmaxf(v_top, fabsf(v));
-                nans |= v < 0.0f;
-                holes |= v == 0.0f;
-            }
+            const float v_top = s_scales[st].v_top;
+            const uint32_t marks = s_scales[st].marks;
+            const bool nans = marks & ((1 << kStepBlocks) - 1), holes = marks >> kStepBlocks;      // in the whole step
+            float ks[kTileCols / kBlock], share[kTileCols / kBlock];
 #pragma unroll
             for (int x = 0; x < kTileCols / kBlock; ++x) {
-                ks[x] = s_scales[st].k[part * (kTileCols / kBlock) + x];
-                vs[x] = fabsf(s_scales[st].v[part * (kTileCols / kBlock) + x]);
+                const float2 of = s_scales[st].of[part * (kTileCols / kBlock) + x];
+                ks[x] = of.x;
+                share[x] = of.y;
             }
             wait_bar(&bars.s_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
@@ -370,8 +366,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                     sum = add_two(sum, two(p0, p1));
                     w[y] = half_two(p0, p1);
                 }
-                if (vs[x] != v_top) {
-                    const __half2 ratio = __float2half2_rn(vs[x] / fmaxf(v_top, kLeastScale));      // a power of two (0 below 2^-24)
+                if (share[x] != 1.0f) {
+                    const __half2 ratio = __float2half2_rn(share[x]);      // a power of two (0 below 2^-24)
 #pragma unroll
                     for (int y = 0; y < 8; ++y) {
                         const __half2 t = __hmul2(*reinterpret_cast<const __half2*>(&w[y]), ratio);
