@@ -9,8 +9,8 @@
 // With |x| <= a over the block's new rows the exponent is the smallest E with a <= 448 2^E; a block that an earlier step began keeps the
 // larger of its old exponent and this, and its old codes are requantised only where it grows.
 //
-// What bounds it: the bytes of queries, keys and values.  10671 tokens of 32 query and 8 key/value heads of 128, slices of one projection: 54 us, 4.4 TB/s
-// (four coordinates a lane and the four they go with read again: 228); a token of 12 and 4 heads of 64 3.8 us, which is launch and two dependent loads.
+// What bounds it: the bytes of queries, keys and values.  10671 tokens of 32 query and 8 key/value heads of 128, slices of one projection: 55 us, 4.4 TB/s
+// (four coordinates a lane and the four they go with read again: 228); a token of 12 and 4 heads of 64 3.2 us, which is launch and two dependent loads.
 #pragma once
 
 #include "cache8.cuh"

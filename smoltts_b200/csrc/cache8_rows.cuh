@@ -1,5 +1,4 @@
-// Attention over the 8-bit key/value cache for few query rows per sequence (decoding, short portions), and for every size and type the tiles
-// of cache8_tiles.cuh do not serve.  Included by cache8.cu.
+// Attention over the 8-bit key/value cache for float32 queries, whatever their number, and what the kernels for bf16 share with it.  Included by cache8.cu.
 //
 // One block per (16 query rows of a sequence and key/value head, key/value head, sequence, share of the keys): the rows are the step's tokens
 // times the query heads that share the key/value head, so that a cached row is read once for all of them.  Its four warps take the share's
@@ -10,10 +9,11 @@
 // order of a product's terms is free -- lane c of four takes bytes 16 c .. + 15 of a key row, which is four steps of four coordinates, and the
 // query fragments are laid out to match; for the values a lane holds the same DV / 8 columns of four positions, and the column index of the
 // product's eight columns is the lane's group.  Codes become f16 by moving bits (cache8.cuh); queries are scaled to below 2^15 per row and
-// enter as one f16 part (bf16 queries: exact) or two (float32), weights likewise, as 2^8 exp2(s - m) times the block's value scale over the
+// enter as two f16 parts, weights likewise, as 2^8 exp2(s - m) times the block's value scale over the
 // largest one so far.  Scores, maxima, denominators and results are fp32.
 //
-// What bounds it: the bytes of the cache, as long as enough of them are under way.
+// What bounds it: the instructions of its fragments (legacy mma.sync: f16 products of fp32's width would take three e4m3 parts on tcgen05).  A prompt of 300 tokens, 12
+// and 4 heads of 64, logarithmic penalty: 22 us.
 #pragma once
 
 #include "cache8.cuh"
@@ -92,11 +92,9 @@ struct Bend {
 
 template <class T> struct Elem;
 template <> struct Elem<float> {
-    static __device__ __forceinline__ float get(const float* p) { return *p; }
     static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 };
 template <> struct Elem<bf16> {
-    static __device__ __forceinline__ float get(const bf16* p) { return __bfloat162float(*p); }
     static __device__ __forceinline__ void put(bf16* p, float v) { *p = __float2bfloat16_rn(v); }
 };
 
@@ -154,7 +152,7 @@ struct Join {
 __host__ __device__ constexpr int join_ld(int DV) { return DV + 4; }
 
 // The four warps' maxima, sums and unnormalised results join[(warp * ROWS + row) * LD + column], joined and finished, or written as this share's part.
-template <class T, int ROWS, int LD>
+template <int ROWS, int LD>
 __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, float* join, const Rows& W, int split) {
     if (threadIdx.x < ROWS) {
         const int row = threadIdx.x;
@@ -185,15 +183,15 @@ __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, fl
             if (col == 0) part_stats(A)[at] = make_float2(J.top[row], J.total[row]);
             A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = v;
         } else {
-            Elem<T>::put(static_cast<T*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, J.top[row], J.total[row], v)));
+            static_cast<float*>(A.out)[(size_t)tok * A.o_row + (size_t)h * A.o_head + col] = finished(A, tok, h, col, with_sink(A, h, J.top[row], J.total[row], v));
         }
     }
 }
 
-// T: type of queries and results; PARTS: f16 parts of a query and of a weight; DK, DV: head sizes padded; BENT: soft cap or distance penalties
-template <class T, int DK, int DV, bool BENT>
+// PARTS: f16 parts of a query and of a weight; DK, DV: head sizes padded; BENT: soft cap or distance penalties
+template <int DK, int DV, bool BENT>
 __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs A) {
-    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1, KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
+    constexpr int PARTS = 2, KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
     constexpr bool QS = q_in_smem(DK, PARTS);
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Join<kRowTile> J;
@@ -276,14 +274,14 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     uint32_t qa[QS ? 1 : KS][QS ? 1 : PARTS][4];
     uint4* qs = reinterpret_cast<uint4*>(smem + kRowWarps * NS * SB);
     {
-        const T* q[2];
+        const float* q[2];
         float up[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int row = min(row0 + r + 8 * x, n * Gq - 1);
-            q[x] = static_cast<const T*>(A.q) + (size_t)(t0 + row / Gq) * A.q_row + (size_t)(g * Gq + row % Gq) * A.q_head;
+            q[x] = static_cast<const float*>(A.q) + (size_t)(t0 + row / Gq) * A.q_row + (size_t)(g * Gq + row % Gq) * A.q_head;
             uint32_t top = 0;
-            for (int k = c; k < A.c.d; k += 4) top = max(top, __float_as_uint(fabsf(Elem<T>::get(q[x] + k))));
+            for (int k = c; k < A.c.d; k += 4) top = max(top, __float_as_uint(fabsf(q[x][k])));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // (2^(14 - e) for a largest magnitude of m 2^e: within fp32 for e from -110 to 127; smaller rows are scaled by 2^124)
@@ -298,14 +296,14 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int x = 0; x < 2; ++x) {
                 float v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = at + e < A.c.d ? Elem<T>::get(q[x] + at + e) * up[x] : 0.0f;
+                for (int e = 0; e < 4; ++e) v[e] = at + e < A.c.d ? q[x][at + e] * up[x] : 0.0f;
                 const uint32_t odd = pack_f16(v[1], v[3]), even = pack_f16(v[0], v[2]);
                 part[0][x] = odd;
                 part[0][2 + x] = even;
-                if (PARTS == 2) {
+                {
                     const float2 o = unpack_f16(odd), z = unpack_f16(even);
-                    part[PARTS - 1][x] = pack_f16(v[1] - o.x, v[3] - o.y);
-                    part[PARTS - 1][2 + x] = pack_f16(v[0] - z.x, v[2] - z.y);
+                    part[1][x] = pack_f16(v[1] - o.x, v[3] - o.y);
+                    part[1][2 + x] = pack_f16(v[0] - z.x, v[2] - z.y);
                 }
             }
         };
@@ -432,9 +430,9 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int y = 0; y < 2; ++y) {
                 const float a = p[x][2 * y] * vmul, b = p[x][2 * y + 1] * vmul;
                 pa[0][x + 2 * y] = pack_f16(a, b);
-                if (PARTS == 2) {
+                {
                     const float2 h = unpack_f16(pa[0][x + 2 * y]);
-                    pa[PARTS - 1][x + 2 * y] = pack_f16(a - h.x, b - h.y);
+                    pa[1][x + 2 * y] = pack_f16(a - h.x, b - h.y);
                 }
             }
         }
@@ -492,7 +490,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int t = 0; t < VB; t += 4)
                 *reinterpret_cast<float4*>(to + t) = make_float4(o[t][2 * x + e] * unit, o[t + 1][2 * x + e] * unit, o[t + 2][2 * x + e] * unit, o[t + 3][2 * x + e] * unit);
         }
-    join_rows<T, kRowTile, LD>(A, J, join, W, split);
+    join_rows<kRowTile, LD>(A, J, join, W, split);
 }
 
 // A block of threads per (token, head): joins the shares of the keys, and the sink.  Latency is all there is to it, so everything a warp needs is
