@@ -313,10 +313,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             }
             umma::fence_before_sync();
             arrive(&bars.s_empty[b]);
-            if (BENT) {
-#pragma unroll
-                for (int r = 0; r < RA; ++r) S[r] = bend(A, S[r], (float)(s_pos[r] - j), s_r1[r], s_r2[r], s_slope[r]);
-            }
+            if (BENT) bend(A, S, [&](int r) { return (float)(s_pos[r] - j); }, [&](int r) { return s_r1[r]; }, [&](int r) { return s_r2[r]; }, [&](int r) { return s_slope[r]; });
             const bool whole = j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             bool hidden = ks == 0.0f;      // from some row
             if (!whole || hidden) {

@@ -82,11 +82,24 @@ __device__ __forceinline__ float bent_score(const AttendArgs& A, float s, int di
 struct Bend {
     float in, c;
     __device__ __forceinline__ explicit Bend(const AttendArgs& A) : in(A.softcap > 0.0f ? fminf(2.0f * kLog2e / A.softcap, 3e38f) : 0.0f), c(A.softcap * kLog2e) {}
-    __device__ __forceinline__ float operator()(const AttendArgs& A, float s, float dist, float r1, float r2, float slope) const {
-        if (c > 0.0f) s = fmaf(-2.0f * c, __fdividef(1.0f, exp2_fast(s * in) + 1.0f), c);
-        else s *= kLog2e;
-        if (A.r1) s = fmaf(-r1, log2_fast(fmaf(r2, dist, 1.0f)), s);
-        return fmaf(-slope, dist, s);
+    // N scores; dist(e), r1(e), r2(e), slope(e): of score e.  A loop per option: with the options looked at in every score, a step of the tiles took 7500 cycles.
+    template <int N, class Dist, class R1, class R2, class Slope>
+    __device__ __forceinline__ void operator()(const AttendArgs& A, float (&s)[N], Dist&& dist, R1&& r1, R2&& r2, Slope&& slope) const {
+        if (c > 0.0f) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] = fmaf(-2.0f * c, __fdividef(1.0f, exp2_fast(s[e] * in) + 1.0f), c);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] *= kLog2e;
+        }
+        if (A.r1) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] = fmaf(-r1(e), log2_fast(fmaf(r2(e), dist(e), 1.0f)), s[e]);
+        }
+        if (A.slope) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) s[e] = fmaf(-slope(e), dist(e), s[e]);
+        }
     }
 };
 

@@ -313,11 +313,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
 #pragma unroll
             for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = rowmul * ks[x];
             if (!direct) {
-                const float d0 = (float)(pos - jc);
 #pragma unroll
-                for (int e = 0; e < kTileCols; ++e) {
-                    S[e] *= mul[e / kBlock];
-                    if (BENT) S[e] = bend(A, S[e], d0 - (float)e, r1, r2, slope);
+                for (int e = 0; e < kTileCols; ++e) S[e] *= mul[e / kBlock];
+                if (BENT) {
+                    const float d0 = (float)(pos - jc);
+                    bend(A, S, [&](int e) { return d0 - (float)e; }, [&](int) { return r1; }, [&](int) { return r2; }, [&](int) { return slope; });
                 }
 #pragma unroll
                 for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = 1.0f;
