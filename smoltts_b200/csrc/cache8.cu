@@ -177,10 +177,10 @@ static bool mixed(const AttendArgs& A, bool f32) {
 
 size_t attend_bytes(const AttendArgs& A, bool f32, int n_sms) {
     const int splits = splits_for(A, f32, n_sms);
-    return splits == 1 || joins_in_cluster(A, splits, f32) ? 0 : (part_floats(A, splits) + 2ull * A.b.T * A.H * splits) * sizeof(float);
+    return splits == 1 || joins_in_cluster(A, splits, f32) ? 0 : (part_floats(A, splits) + 4ull * A.b.T * A.H * splits) * sizeof(float);
 }
 // There are shares only while blocks (of at most 128 rows) times shares are no more than the SMs hold, 3 each of at most 16 rows or 1 of 128.
-size_t attend_bytes_most(int dv) { return (size_t)256 * kTileRows * ((dv + 3) / 4 * 4 + 2) * sizeof(float); }
+size_t attend_bytes_most(int dv) { return (size_t)256 * kTileRows * ((dv + 3) / 4 * 4 + 4) * sizeof(float); }
 
 cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* launches, cudaStream_t st) {
     AttendArgs few = A;

@@ -64,7 +64,7 @@ struct AttendArgs {
     const float* gate;               // [T] rows of gate_row floats: the result is multiplied by sigmoid(gate[t][h * dv + c]) (nullptr: not)
     size_t gate_row;
     float out_scale;
-    float* part;                     // shares of the keys: unnormalised results [T * H][n_splits][dv rounded up to 4], then (maximum, denominator) [T * H][n_splits]
+    float* part;                     // shares of the keys: unnormalised results [T * H][n_splits][dv rounded up to 4], then (maximum, denominator, e of the results, which are in units of 2^(maximum + e), -) [T * H][n_splits]
     int n_splits;
     int q_vec, o_vec;                // rows are whole groups of four elements that a load takes (1), of eight on 16-byte boundaries (2)
     int rows_over, rows_most;        // only sequences of more than rows_over and at most rows_most query rows per key/value head
@@ -72,7 +72,7 @@ struct AttendArgs {
 
 constexpr int kMaxSplits = 128;
 __host__ __device__ inline size_t part_floats(const AttendArgs& A, int splits) { return (size_t)A.b.T * A.H * splits * ((A.c.dv + 3) / 4 * 4); }
-__device__ __forceinline__ float2* part_stats(const AttendArgs& A) { return reinterpret_cast<float2*>(A.part + part_floats(A, A.n_splits)); }
+__device__ __forceinline__ float4* part_stats(const AttendArgs& A) { return reinterpret_cast<float4*>(A.part + part_floats(A, A.n_splits)); }
 
 // what a score goes through in either attention kernel is the plain scaled product
 inline bool plain_scores(const AttendArgs& A) { return A.softcap == 0.0f && !A.slope && !A.r1; }

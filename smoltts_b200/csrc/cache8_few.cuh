@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     // a finished row's column, and a column of this block's share of the keys: maximum, denominator, unnormalised result
     auto store = [&](int r, int col, float top, float total, float v) {
         const int tok = t0 + s_pos[r] - pos0, h = s_head[r];
-        Elem<bf16>::put(static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, top, total, v)));
+        Elem<bf16>::put(static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, top, total, 0.0f, v)));
     };
     auto put = [&](int r, int col, float top, float total, float v) {
         if (A.n_splits == 1) {
@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             joint[r * D + col] = v;
         } else {
             const size_t at = ((size_t)(t0 + s_pos[r] - pos0) * A.H + s_head[r]) * A.n_splits + split;
-            if (col == 0) part_stats(A)[at] = make_float2(top, total);
+            if (col == 0) part_stats(A)[at] = make_float4(top, total, 0.0f, 0.0f);
             A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = v;
         }
     };

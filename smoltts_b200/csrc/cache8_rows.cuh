@@ -9,8 +9,13 @@
 // order of a product's terms is free -- lane c of four takes bytes 16 c .. + 15 of a key row, which is four steps of four coordinates, and the
 // query fragments are laid out to match; for the values a lane holds the same DV / 8 columns of four positions, and the column index of the
 // product's eight columns is the lane's group.  Codes become f16 by moving bits (cache8.cuh); queries are scaled to below 2^15 per row and
-// enter as two f16 parts, weights likewise, as 2^8 exp2(s - m) times the block's value scale over the
-// largest one so far.  Scores, maxima, denominators and results are fp32.
+// enter as two f16 parts, weights likewise.  Scores, maxima, denominators and results are fp32.
+//
+// What a row's results are relative to is the largest product of weight and value scale among the keys that it sees: with m about the largest score, and e about the
+// largest (s - m) + log2(scale), a weight that the product multiplies is 2^8 exp2(s - m + log2(scale) - e), so that its last bit is one of the row's own largest term,
+// whatever lies beside.  (With the scale as a factor behind exp2, over the largest scale of all blocks that the tile reads, a value 2^34 larger that a row does not see
+// left nothing of its own.)  The denominator is in units of 2^m, results of 2^(m + e).  Both are whole numbers, so that what goes from one unit to the
+// other is a power of two and rounds nothing.
 //
 // What bounds it: the instructions of its fragments (legacy mma.sync: f16 products of fp32's width would take three e4m3 parts on tcgen05).  A prompt of 300 tokens, 12
 // and 4 heads of 64, logarithmic penalty: 22 us.
@@ -117,11 +122,20 @@ __device__ __forceinline__ float finished(const AttendArgs& A, int t, int h, int
     return v;
 }
 
-// An unnormalised result over its denominator, the sink's part included; nothing visible: no weights, and the result is zero.
-__device__ __forceinline__ float with_sink(const AttendArgs& A, int h, float top, float total, float v) {
-    const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, top);
-    const float f = top == -INFINITY ? 1.0f : exp2_fast(top - M), all = fmaf(total, f, M == -INFINITY ? 0.0f : exp2_fast(sink - M));
-    return all == 0.0f ? v : v * f / all;
+// What a row's unnormalised results, in units of 2^(top + e), are multiplied by: by a, then by b.  The denominator is total, in units of 2^top, and the sink's
+// part.  Nothing visible: no weights, and the result is zero.  (In two steps: 2^e over the sink's part alone may be no fp32 number where result and quotient are.)
+struct Finish {
+    float a, b;
+    __device__ __forceinline__ Finish(const AttendArgs& A, int h, float top, float total, float e) {
+        const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, top);
+        const float all = fmaf(total, top == -INFINITY ? 1.0f : exp2_fast(top - M), M == -INFINITY ? 0.0f : exp2_fast(sink - M));
+        a = top == -INFINITY ? 1.0f : exp2_fast(0.5f * (e + (top - M)));
+        b = all == 0.0f ? 1.0f : a / all;
+    }
+};
+__device__ __forceinline__ float with_sink(const AttendArgs& A, int h, float top, float total, float e, float v) {
+    const Finish f(A, h, top, total, e);
+    return v * f.a * f.b;
 }
 
 // Blocks of scale sign < 0 hold NaN codes, which the products took for 480: a row that sees one of them becomes NaN, all of it where a key holds
@@ -159,7 +173,7 @@ struct Rows {
 };
 template <int ROWS>
 struct Join {
-    float max[kRowWarps][ROWS], sum[kRowWarps][ROWS], weight[kRowWarps][ROWS], top[ROWS], total[ROWS];
+    float max[kRowWarps][ROWS], sum[kRowWarps][ROWS], weight[kRowWarps][ROWS], top[ROWS], total[ROWS], unit[ROWS];      // weight: e of the warps' results, then what these count
     int bad;
 };
 __host__ __device__ constexpr int join_ld(int DV) { return DV + 4; }
@@ -175,11 +189,19 @@ __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, fl
         for (int w = 0; w < kRowWarps; ++w) {
             // a row of NaN scores has no maximum: its sums say so
             const float f = J.max[w][row] == -INFINITY ? (J.sum[w][row] == 0.0f ? 0.0f : J.sum[w][row]) : exp2_fast(J.max[w][row] - M);
-            J.weight[w][row] = f;
             total = fmaf(J.sum[w][row], f, total);
         }
+        float e[kRowWarps], E = -INFINITY;      // (a warp that has seen nothing: -infinity)
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) {
+            e[w] = J.max[w][row] == -INFINITY ? -INFINITY : J.weight[w][row] + (J.max[w][row] - M);
+            E = fmaxf(E, e[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < kRowWarps; ++w) J.weight[w][row] = e[w] == -INFINITY ? 0.0f : exp2_fast(e[w] - E);
         J.top[row] = M;
         J.total[row] = total;
+        J.unit[row] = E;
     }
     __syncthreads();
     if (J.bad) {
@@ -193,10 +215,10 @@ __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, fl
         for (int w = 0; w < kRowWarps; ++w) v = fmaf(join[(w * ROWS + row) * LD + col], J.weight[w][row], v);
         if (A.n_splits > 1) {
             const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
-            if (col == 0) part_stats(A)[at] = make_float2(J.top[row], J.total[row]);
+            if (col == 0) part_stats(A)[at] = make_float4(J.top[row], J.total[row], J.unit[row], 0.0f);
             A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = v;
         } else {
-            static_cast<float*>(A.out)[(size_t)tok * A.o_row + (size_t)h * A.o_head + col] = finished(A, tok, h, col, with_sink(A, h, J.top[row], J.total[row], v));
+            static_cast<float*>(A.out)[(size_t)tok * A.o_row + (size_t)h * A.o_head + col] = finished(A, tok, h, col, with_sink(A, h, J.top[row], J.total[row], J.unit[row], v));
         }
     }
 }
@@ -224,11 +246,12 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     if (threadIdx.x == 0) J.bad = 0;
 
     // where the warp's blocks are: lane i knows block number i of 32 (`now`), and of the 32 that follow
-    struct Place { int page, in_page; float ks, vs; };
+    struct Place { int page, in_page; float ks, lv; };      // lv: log2 of the values' scale (exact for a power of two)
+    bool bad = false;
     auto block_of = [&](int i) { const int x = b_lo + warp + i * kRowWarps; return x < seen.lead ? x : seen.from + x - seen.lead; };
     auto look_up = [&](int i0) {
         Place p;
-        p.page = -1; p.in_page = 0; p.ks = 0.0f; p.vs = 0.0f;
+        p.page = -1; p.in_page = 0; p.ks = 0.0f; p.lv = 0.0f;
         if (i0 + lane < mine) {
             const int j = block_of(i0 + lane) * kBlock, pg = j / A.c.page;
             p.page = pg < A.b.max_pages ? A.b.table[(size_t)s * A.b.max_pages + pg] : -1;
@@ -239,7 +262,9 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             } else {
                 const int at = g * (A.c.page / kBlock) + p.in_page / kBlock;
                 p.ks = A.c.ks[(size_t)p.page * A.c.ks_page + at];
-                p.vs = A.c.vs[(size_t)p.page * A.c.vs_page + at];
+                const float vs = A.c.vs[(size_t)p.page * A.c.vs_page + at];
+                p.lv = log2f(fmaxf(fabsf(vs), 7.5231638e-37f));      // 2^-120: below every scale
+                bad |= p.ks < 0.0f || vs < 0.0f;
             }
         }
         return p;
@@ -344,13 +369,12 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         r2[x] = BENT && A.r1 ? A.r2[h] : 0.0f;
         slope[x] = BENT && A.slope ? A.slope[h] : 0.0f;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, unit = 0.0f;      // unit: the largest value scale so far, what o is in units of
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, unit[2] = {-INFINITY, -INFINITY};      // l is in units of 2^m, o of 2^(m + unit)
     float o[VB][4];
 #pragma unroll
     for (int t = 0; t < VB; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[t][e] = 0.0f;
-    bool bad = false;
 
     for (int i = 0; i < mine; ++i) {
         if (i > 0 && (i & 31) == 0) {
@@ -362,10 +386,9 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             copy_block(ahead, (ahead & ~31) == (i & ~31) ? now : next);
         }
         const int page = __shfl_sync(0xffffffffu, now.page, i & 31);
-        const float ks = __shfl_sync(0xffffffffu, now.ks, i & 31), vs = __shfl_sync(0xffffffffu, now.vs, i & 31);
+        const float ks = __shfl_sync(0xffffffffu, now.ks, i & 31), lv = __shfl_sync(0xffffffffu, now.lv, i & 31);
         copies_left<NS - 1>();
         if (page < 0) continue;
-        bad |= ks < 0.0f || vs < 0.0f;
         const unsigned char* st = smem + warp * (NS * SB) + (i % NS) * SB;
         // ---- scores of 16 rows and 16 positions ----
         float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
@@ -415,33 +438,41 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
             top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 2));
         }
-        const float v_unit = fmaxf(fabsf(vs), 7.5231638e-37f);      // 2^-120: below every scale
-        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1]) || v_unit > unit) {
-            const float grown = fmaxf(unit, v_unit), down = unit / grown;      // powers of two
+        if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1] || (top[0] - m[0]) + lv > unit[0] || (top[1] - m[1]) + lv > unit[1])) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const float mn = fmaxf(m[x], top[x]), corr = mn == -INFINITY ? 1.0f : exp2_fast(m[x] - mn);
+                const float mn = fmaxf(m[x], ceilf(top[x]));
+                if (mn == -INFINITY) continue;
+                const float had = unit[x] + (m[x] - mn), un = fmaxf(had, ceilf((top[x] - mn) + lv)), keep = exp2_fast(had - un);
+                l[x] *= exp2_fast(m[x] - mn);
                 m[x] = mn;
-                l[x] *= corr;
+                unit[x] = un;
 #pragma unroll
                 for (int t = 0; t < VB; ++t) {
-                    o[t][2 * x] *= corr * down;
-                    o[t][2 * x + 1] *= corr * down;
+                    o[t][2 * x] *= keep;
+                    o[t][2 * x + 1] *= keep;
                 }
             }
-            unit = grown;
         }
-        const float vmul = kCodeUnit * (v_unit / unit);
         uint32_t pa[PARTS][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const float base = m[x] == -INFINITY ? 0.0f : m[x];
+            const bool none = m[x] == -INFINITY;
+            const float base = none ? 0.0f : m[x], away = none ? 0.0f : unit[x] - lv;
+            // The denominator's terms are the weights' times 2^away, unless weights that count in it may be too small for an fp32 number (what is lost with them otherwise
+            // is below 2^-62 of it).
+            float sum = 0.0f;
+            if (away > 64.0f) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) p[x][e] = exp2_fast(p[x][e] - base);
-            l[x] += (p[x][0] + p[x][1]) + (p[x][2] + p[x][3]);
+                for (int e = 0; e < 4; ++e) sum += exp2_fast(p[x][e] - base);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) p[x][e] = exp2_fast((p[x][e] - base) - away);
+            if (!(away > 64.0f)) sum = ((p[x][0] + p[x][1]) + (p[x][2] + p[x][3])) * exp2_fast(away);
+            l[x] += sum;
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-                const float a = p[x][2 * y] * vmul, b = p[x][2 * y + 1] * vmul;
+                const float a = p[x][2 * y] * kCodeUnit, b = p[x][2 * y + 1] * kCodeUnit;
                 pa[0][x + 2 * y] = pack_f16(a, b);
                 {
                     const float2 h = unpack_f16(pa[0][x + 2 * y]);
@@ -488,9 +519,10 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         if (c == 0) {
             J.max[warp][r + 8 * x] = m[x];
             J.sum[warp][r + 8 * x] = l[x];
+            J.weight[warp][r + 8 * x] = unit[x];
         }
     }
-    if (bad && lane == 0) J.bad = 1;
+    if (bad) J.bad = 1;
     __syncthreads();      // everybody's copies are used up: the ring becomes the results' place
     constexpr int LD = join_ld(DV);
     float* join = reinterpret_cast<float*>(smem);
@@ -501,7 +533,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             float* to = join + (warp * kRowTile + r + 8 * x) * LD + (2 * c + e) * VB;
 #pragma unroll
             for (int t = 0; t < VB; t += 4)
-                *reinterpret_cast<float4*>(to + t) = make_float4(o[t][2 * x + e] * unit, o[t + 1][2 * x + e] * unit, o[t + 2][2 * x + e] * unit, o[t + 3][2 * x + e] * unit);
+                *reinterpret_cast<float4*>(to + t) = make_float4(o[t][2 * x + e], o[t + 1][2 * x + e], o[t + 2][2 * x + e], o[t + 3][2 * x + e]);
         }
     join_rows<kRowTile, LD>(A, J, join, W, split);
 }
@@ -525,14 +557,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
     const int t0 = A.b.start[lo], t1 = A.b.start[lo + 1];
     if (t < t0 || t >= t1 || t0 < 0 || t1 > A.b.T || t - t0 >= A.b.max_new || (long long)(t1 - t0) * (A.H / A.c.G) <= A.rows_over) return;
     const int pieces = (A.c.dv + 3) / 4;
-    const float2* stat = part_stats(A) + (size_t)unit * A.n_splits;
+    const float4* stat = part_stats(A) + (size_t)unit * A.n_splits;      // maximum, denominator, e of the results
     const float4* part = reinterpret_cast<const float4*>(A.part) + (size_t)unit * A.n_splits * pieces;
-    const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY;
-    float2 st[kMaxSplits / 32];
-    float M = sink;
+    float4 st[kMaxSplits / 32];
+    float M = -INFINITY, E = -INFINITY;
 #pragma unroll
     for (int x = 0; x < kMaxSplits / 32; ++x) {
-        st[x] = lane + 32 * x < A.n_splits ? stat[lane + 32 * x] : make_float2(-INFINITY, 0.0f);
+        st[x] = lane + 32 * x < A.n_splits ? stat[lane + 32 * x] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         M = fmaxf(M, st[x].x);
     }
     M = warp_max(M);
@@ -540,10 +571,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 #pragma unroll
     for (int x = 0; x < kMaxSplits / 32; ++x) {
         // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
-        const float f = st[x].x == -INFINITY ? (st[x].y == 0.0f ? 0.0f : st[x].y) : exp2_fast(st[x].x - M);
-        total = fmaf(st[x].y, f, total);
-        st[x].x = f;
+        total = fmaf(st[x].y, st[x].x == -INFINITY ? (st[x].y == 0.0f ? 0.0f : st[x].y) : exp2_fast(st[x].x - M), total);
+        st[x].z = st[x].x == -INFINITY ? -INFINITY : st[x].z + (st[x].x - M);
+        E = fmaxf(E, st[x].z);
     }
+    E = warp_max(E);
+#pragma unroll
+    for (int x = 0; x < kMaxSplits / 32; ++x) st[x].z = st[x].z == -INFINITY ? 0.0f : exp2_fast(st[x].z - E);
     float4 acc[kMaxDim / 128];
 #pragma unroll
     for (int e = 0; e < kMaxDim / 128; ++e) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -553,7 +587,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 #pragma unroll
         for (int i = 0; i < 32 / kJoinWarps; ++i) {
             const int z = 32 * x + i * kJoinWarps + warp;
-            const float f = __shfl_sync(0xffffffffu, st[x].x, z & 31);
+            const float f = __shfl_sync(0xffffffffu, st[x].z, z & 31);
 #pragma unroll
             for (int e = 0; e < kMaxDim / 128; ++e)
                 if (z < A.n_splits && lane + 32 * e < pieces) {
@@ -568,13 +602,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
 #pragma unroll
     for (int e = 0; e < kMaxDim / 128; ++e) s_acc[warp][lane + 32 * e] = acc[e];
     __syncthreads();
-    total = warp_sum(total) + (M == -INFINITY ? 0.0f : exp2_fast(sink - M));
+    const Finish finish(A, h, M, warp_sum(total), E);
     const float* flat = reinterpret_cast<const float*>(s_acc);
     for (int col = threadIdx.x; col < A.c.dv; col += kJoinWarps * 32) {
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < kJoinWarps; ++w) v += flat[w * kMaxDim + col];
-        Elem<T>::put(static_cast<T*>(A.out) + (size_t)t * A.o_row + (size_t)h * A.o_head + col, finished(A, t, h, col, total == 0.0f ? v : v / total));
+        Elem<T>::put(static_cast<T*>(A.out) + (size_t)t * A.o_row + (size_t)h * A.o_head + col, finished(A, t, h, col, v * finish.a * finish.b));
     }
 }
 

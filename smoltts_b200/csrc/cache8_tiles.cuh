@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             if (A.n_splits > 1) {
                 const int ld = (A.c.dv + 3) / 4 * 4;
                 const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
-                if (mine && col == 0) part_stats(A)[at] = make_float2(m, total);
+                if (mine && col == 0) part_stats(A)[at] = make_float4(m, total, 0.0f, 0.0f);
                 float* to = A.part + at * ld + col;
 #pragma unroll
                 for (int c = 0; c < kTileCols; c += 4)
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             if (col >= A.c.dv) continue;
             if (A.n_splits > 1) {
                 const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
-                if (col == 0) part_stats(A)[at] = make_float2(-INFINITY, 0.0f);
+                if (col == 0) part_stats(A)[at] = make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
                 A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = 0.0f;
             } else {
                 static_cast<bf16*>(A.out)[(size_t)tok * A.o_row + (size_t)h * A.o_head + col] = __float2bfloat16_rn(0.0f);

@@ -1,0 +1,174 @@
+"""The 8-bit key/value cache where magnitudes differ: a row's result depends on what it sees alone, however large or small what lies beside it is."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from cache8_util import BLOCK, ints, tolerance
+from test_gpu_cache8 import cache_of, randn
+
+pytestmark = pytest.mark.gpu
+
+# A weight's last bit, relative to the largest product of a weight and its block's scale that the row sees in the step.  Tiles of many rows: the second e4m3 part
+# has the first one's unit, so half of its least code, 2^-10, on 256.  Few rows: the second part is 16 times finer.  float32: half of f16's least number, 2^-25, on
+# at least 128.
+LEAST_TILES, LEAST_FEW, LEAST_F32 = 2.0 ** -18, 2.0 ** -22, 2.0 ** -32
+
+
+def check(c, table, q, pos0, out, least, scale=None, window=0, first=0, kv_len=None, sink=None, rows=None):
+    """One sequence's rows against 64 bits.  On top of `tolerance`: the weights' last bit times the codes it multiplies; and for bf16 2^-15 of the weights, from three roundings
+    of a sum of a score and a block's exponent of at most 110, each 2^-24 of at most 160 (scores below 50 in units of log2) in units of log2."""
+    n, H, d = q.shape
+    G, page, pages = c.kv_heads, c.page_size, table[0][table[0] >= 0].long()
+    L = pos0 + n
+    k, _ = c.values(pages)
+    k = k.double().transpose(1, 2).reshape(-1, G, d)[:L]
+    codes = c.v.view(torch.uint8)[pages].view(torch.float8_e4m3fn).double().transpose(1, 2).reshape(-1, G, c.v.shape[3])[:L, :, :c.vdim]
+    unit = c.v_scale[pages].abs().double().transpose(1, 2).reshape(-1, G).repeat_interleave(BLOCK, 0)[:L]
+    j = torch.arange(L, device="cuda")
+    dist = torch.arange(pos0, L, device="cuda").view(n, 1) - j
+    seen = dist >= 0
+    if window:
+        seen &= (dist < window) | (j < first)
+    if kv_len is not None:
+        seen &= j < kv_len
+    some = seen.any(1, keepdim=True)
+    for h in range(H):
+        g = h // (H // G)
+        scale_ = d ** -0.5 if scale is None else scale
+        s = (q[:, h].double() @ k[:, g].T * scale_).masked_fill(~seen, -math.inf)
+        size = (q[:, h].double().abs() @ k[:, g].abs().T * scale_).masked_fill(~seen, 0.0).amax(1, keepdim=True)
+        top = s.amax(1, keepdim=True).masked_fill(~some, 0.0)
+        if sink is not None:
+            top = top.clamp(min=sink[h].item())
+        w = torch.exp(s - top)
+        total = w.sum(1, keepdim=True) + (torch.exp(sink[h].double() - top) if sink is not None else 0.0)
+        total = total.masked_fill(total == 0, 1.0)
+        v = codes[:, g] * unit[:, g, None]
+        want, spread = w @ v / total, w @ v.abs() / total
+        floor = (w * unit[:, g]).amax(1, keepdim=True) * (seen.double() @ codes[:, g].abs()) / total
+        tol = tolerance(q.dtype, want, spread, size) + least * floor + (2.0 ** -15 * spread if q.dtype == torch.bfloat16 else 0.0)
+        far = ((out[:, h].double() - want).abs() - tol) / (spread + 1e-30)
+        if rows is not None:
+            far = far[rows]
+        assert far.max().item() <= 0, (h, far.max().item(), (far > 0).any(1).nonzero().flatten().tolist()[:20])
+
+
+def ones_column(q, k, at=8.0, key=0.0):
+    """Coordinate 0 as a score of its own: with a scale of 1/8 a key's is its coordinate."""
+    q[..., 0], k[..., 0] = at, key
+
+
+KERNELS = [(torch.float32, 1, LEAST_F32), (torch.float32, 7, LEAST_F32), (torch.float32, 150, LEAST_F32)]
+
+
+@pytest.mark.parametrize("dtype,n,least", KERNELS)
+@pytest.mark.parametrize("power", [6, 12, 18, 30, 60, 100])
+@pytest.mark.parametrize("where", ["later", "behind_the_window", "behind_kv_len", "little_weight", "infinity", "between"])
+def test_a_row_depends_on_what_it_sees_alone(dtype, n, least, power, where):
+    """Values 2^power larger at positions that some or all rows do not see, or that weigh next to nothing (a score 40 lower, 2^-58)."""
+    H, G, d, pos0 = 4, 2, 64, 246
+    L = pos0 + n
+    c, table = cache_of([L], 32, G, d, d, seed=3)
+    k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2), randn(n, H, d, seed=3)
+    ones_column(q, k)
+    v *= 2.0 ** (-power / 2 if where == "between" else 0.0)
+    big = torch.zeros(L, dtype=torch.bool, device="cuda")
+    options = {}
+    if where in ("later", "infinity"):
+        big[pos0 + 1 if n == 1 else pos0 + n // 2:] = True
+        if n == 1:      # (hidden in the last step all the same)
+            big[pos0 - 10:], options["kv_len"] = True, pos0 - 16
+    elif where == "behind_the_window":
+        big[192:208], options["window"] = True, 40      # (the first row sees one of them)
+        big[272:288] = True
+    elif where == "behind_kv_len":
+        big[240:], options["kv_len"] = True, 240 - 10
+    elif where == "little_weight":
+        big[224:240] = True
+        k[224:240, :, 0] = -40.0
+    else:
+        big[192:208] = True
+    v[big] *= 2.0 ** power
+    if where == "infinity":
+        v[big.nonzero()[-1].item(), :, 5] = math.inf
+    q = q.to(dtype)
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    o = {x: (ints([y]) if x == "kv_len" else y) for x, y in options.items()}
+    out = c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L, **o)
+    check(c, table, q, pos0, out, least, **options)
+    sink = torch.linspace(-1.0, 3.0, H, device="cuda")
+    out = c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L, sink=sink, **o)
+    check(c, table, q, pos0, out, least, sink=sink, **options)
+    c.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,n,least", KERNELS)
+@pytest.mark.parametrize("low", [0.0, 2.0 ** -90])
+def test_blocks_of_zeros_and_of_everything(dtype, n, least, low):
+    """Blocks of zeros (scale 2^-110) or next to nothing beside ordinary ones, and blocks near the largest there is: the denominator counts them all."""
+    H, G, d, pos0 = 4, 2, 64, 250
+    L = pos0 + n
+    c, table = cache_of([L], 32, G, d, d, seed=3)
+    k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2), randn(n, H, d, seed=3).to(dtype)
+    for b in range(0, L, 2 * BLOCK):
+        v[b:b + BLOCK] *= low
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    check(c, table, q, pos0, c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L), least)
+    v[96:112] *= 2.0 ** 88      # (ordinary, tiny and huge in one step)
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    for options in (dict(), dict(window=120)):
+        check(c, table, q, pos0, c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L, **options), least, **options)
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("dtype", [torch.float32])
+def test_shares_of_the_keys_whose_values_differ(dtype, n):
+    """A long context in several shares, joined in a cluster or by a kernel of its own: values grow by 2^20 every 700 positions, scores fall by 12 meanwhile."""
+    H, G, d = 4, 2, 64
+    for L in (2100, 9000 if n == 1 else 3000):
+        pos0 = L - n
+        c, table = cache_of([L], 64, G, d, d, seed=3)
+        k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2), randn(n, H, d, seed=3)
+        ones_column(q, k)
+        steps = (torch.arange(L, device="cuda") // 700).float()
+        k[:, :, 0] = -12.0 * (steps % 4).view(-1, 1)
+        v *= torch.exp2(20.0 * (steps % 4) - 30.0).view(-1, 1, 1)
+        q = q.to(dtype)
+        c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+        out = c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L)
+        check(c, table, q, pos0, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n == 1 else LEAST_TILES)
+
+
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("rise", [30.0, 40.0, 44.0])
+def test_rising_scores_of_large_values(dtype, n, rise):
+    """Scores that rise by 30 to 44 from one step of 128 positions to the next, values near 2^90 and a clamped infinity."""
+    H, G, d, pos0 = 4, 2, 64, 500
+    L = pos0 + n
+    c, table = cache_of([L], 64, G, d, d, seed=3)
+    k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2) * 2.0 ** 88, randn(n, H, d, seed=3)
+    ones_column(q, k)
+    k[:, :, 0] = ((torch.arange(L, device="cuda") // 128).float() * rise - 2 * rise).view(-1, 1)
+    v[400, 0, 3], v[L - 1, 1, 9] = math.inf, -math.inf
+    q = q.to(dtype)
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    out = c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L)
+    assert torch.isfinite(out).all()
+    check(c, table, q, pos0, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n == 1 else LEAST_TILES)
+
+
+def test_a_sink_far_above_the_scores():
+    """Scores 70 below the sink, values of 2^90: what is left is 2^-11."""
+    H, G, d, L = 4, 2, 64, 300
+    for dtype in (torch.float32,):
+        for n in (1, 150):
+            c, table = cache_of([L], 64, G, d, d, seed=3)
+            k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2) * 2.0 ** 90, randn(n, H, d, seed=3).to(dtype)
+            c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+            sink = torch.full((H,), 70.0, device="cuda")
+            out = c.attend(q, ints([0, n]), ints([L - n]), table, max_new=n, max_len=L, sink=sink)
+            check(c, table, q, L - n, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n == 1 else LEAST_TILES, sink=sink)
