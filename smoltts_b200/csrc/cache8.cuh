@@ -106,6 +106,13 @@ __device__ __forceinline__ float log2_fast(float x) {
     return y;
 }
 
+// log2 of a scale, a normal number above 0: its exponent, exactly.  (A scale that is no power of two, which only a caller who makes scales can bring, takes the function.)
+__device__ __forceinline__ float scale_log2(float s) {
+    const uint32_t bits = __float_as_uint(s);
+    if ((bits & 0x7fffffu) != 0) return log2f(s);
+    return __uint_as_float(0x4b000000u | bits >> 23) - (8388608.0f + 127.0f);      // (2^23 and the exponent: fewer instructions than a conversion)
+}
+
 // Launches on `st`; 0 or a CUDA error.  `launches` counts them.
 cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cudaStream_t st);
 // Bytes of workspace attend needs for these sizes, and the most it needs for results of dv columns on any device of up to 256 SMs.

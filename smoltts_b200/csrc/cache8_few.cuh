@@ -9,8 +9,10 @@
 //
 // e4m3 on both sides (kind::f8f6f4).  A query, scaled by a power of two to a largest magnitude in [128, 256), is the sum of two e4m3 parts, the second 16
 // times finer: four bits each and the sign of the remainder hold bf16's eight bits, down to 2^-13 of the row's largest coordinate, and 2^-23 of
-// it below.  A weight exp2(s - m), m being the row's maximum over the step, times its block's value scale over the step's largest, is taken apart the same
-// way, on 256: a relative error of at most 2^-9, as a weight in bf16 would have, or 2^-22 of the step's largest.  Parts are columns of their own.
+// it below.  A weight exp2(s - m + log2(its block's value scale) - e), with the row's largest score m over the step and its largest s - m + log2(scale) e, is taken apart the
+// same way, on 256: a relative error of at most 2^-9, as a weight in bf16 would have, or 2^-22 of the largest weight times scale that the row sees in the step.
+// (With the scale as a factor behind exp2, over the step's largest, a value 2^20 larger that the row does not see halved the bits of its own weights.)  Parts are
+// columns of their own.
 //
 // Roles: a warp that looks pages up and issues the copies (tensor maps, 128-byte swizzle, boxes of up to 128 positions that lie together), a warp
 // that issues the products, four warps for the softmax.  A NaN code is a NaN to the product even under a weight of 0: in steps with positions that
@@ -37,6 +39,40 @@ __host__ __device__ constexpr int few_tmem(int D, int NR) { return 2 * NR * (2 +
 
 // blocks an SM holds: by shared memory (stages of 32 KB or 64) and registers.  Three of four rows instead of two: 64 sequences at up to 8192 positions 145 us, 161
 __host__ __device__ constexpr int few_blocks(int D, int RA) { return D > 128 ? 1 : RA <= 4 ? 3 : 2; }
+
+// What weights and results are relative to.  While the logarithms of all value scales lie within kNear of the first block's (`unit`): weights are relative to the
+// row's largest score + log2(scale) =: m, results are in units of 2^m, and the denominator's terms, in units of 2^(m - unit), are the weights' times
+// 2^(unit - log2(scale)): one exponential and one maximum a score.  (A weight below fp32's range counts for less than 2^-62 there.)  From the first step on that has a
+// scale further away, whoever sees it, the same with an exponential and a maximum each for weights and denominator, and a unit per row: rare, and behind calls, so
+// that the ordinary loop stays as short as it is (with all of it in the loop 64 sequences at up to 8192 positions took 150 us, 142 without).
+constexpr float kNear = 32.0f;      // in units of log2
+
+// the warp's largest score, and largest score - it + log2(scale)
+__device__ __noinline__ float2 apart_maxima(float s, float lv) {
+    const float t = warp_top(s);
+    return make_float2(t, warp_top(s - (t == -INFINITY ? 0.0f : t) + lv));
+}
+// (weight, the denominator's term, the row's largest score, what the weight is relative to on top of it), from the four warps' maxima
+__device__ __noinline__ float4 apart_weight(float s, float lv, const float* tops, const float* fars, int ld) {
+    float top = -INFINITY, e = -INFINITY;
+    for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w * ld]);
+    if (top == -INFINITY) return make_float4(exp2_fast(s), exp2_fast(s), top, 0.0f);      // (0, or NaN)
+    for (int w = 0; w < 4; ++w) e = fmaxf(e, fars[w * ld] + (tops[w * ld] - top));
+    return make_float4(exp2_fast((s - top) + (lv - e)), exp2_fast(s - top), top, e);
+}
+// what results and denominator so far (in units of 2^(m + unit - 8), 2^m) and a step's count when joined
+struct Apart {
+    float keep, add, keep_l, add_l, unit;
+    __device__ __noinline__ Apart(float m, float m_step, float unit_, float unit_step) {
+        const float mn = fmaxf(m, m_step), had = m == -INFINITY ? -INFINITY : unit_ + (m - mn), has = m_step == -INFINITY ? -INFINITY : unit_step + (m_step - mn);
+        unit = mn == -INFINITY ? unit_ : fmaxf(had, has);
+        keep = m == -INFINITY ? 0.0f : exp2_fast(had - unit);
+        add = m_step == -INFINITY ? 0.0f : exp2_fast(has - unit);
+        // (a step, or all before it, of NaN scores has no maximum: its sums say so)
+        keep_l = m == -INFINITY ? 1.0f : exp2_fast(m - mn);
+        add_l = m_step == -INFINITY ? 1.0f : exp2_fast(m_step - mn);
+    }
+};
 
 struct FewBars {
     uint64_t full[3], empty[3];      // stages
@@ -68,6 +104,13 @@ __device__ uint32_t nan_columns(const AttendArgs& A, const Rows& W, int col) {
 }
 
 __device__ __forceinline__ void cluster_sync() { asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 of_rank(const float4* mine, int rank) {
+    uint32_t at;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(umma::s2u(mine)), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
 __device__ __forceinline__ float of_rank(const float* mine, int rank) {      // the same place in another block of the cluster
     uint32_t at;
     float v;
@@ -84,7 +127,10 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     extern __shared__ unsigned char smem_raw[];
     __shared__ FewBars bars;
     __shared__ StepScales s_scales[NS];
-    __shared__ float s_top[2][4][RA], s_rowmul[RA], s_sum[4][RA], s_r1[RA], s_r2[RA], s_slope[RA], s_stat[2][RA];
+    __shared__ float s_top[2][4][RA], s_rowmul[RA], s_sum[4][RA], s_r1[RA], s_r2[RA], s_slope[RA];
+    __shared__ float4 s_stat[RA];      // of this block's share: maximum, denominator, e
+    __shared__ float s_far[2][4][RA], s_step_unit[2][RA], s_unit[2][RA];      // (value scales far apart)
+    __shared__ int s_apart[2];      // some thread has met one: in even and odd steps, so that the next step's is written while this one's is read
     __shared__ int s_pos[RA], s_head[RA], s_bad;
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *KV = base, *Qs = KV + NS * SB, *Ps = Qs + N * D;
@@ -102,7 +148,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&kmap), "l"(&vmap) : "memory");
         bars.stop = 0;
-        s_bad = 0;
+        s_bad = s_apart[0] = s_apart[1] = 0;
     }
     if (warp == kFewProducts) tmem_take<COLS>(&bars.tmem);
     dep_wait();
@@ -118,23 +164,20 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     const int steps = any ? min(lo + share, seen.count) - lo : 0;
     const bool clustered = A.n_splits > 1 && A.n_splits <= kMostCluster;
     float* joint = reinterpret_cast<float*>(KV);      // [row][D], once everything has been multiplied
-    // a finished row's column, and a column of this block's share of the keys: maximum, denominator, unnormalised result
-    auto store = [&](int r, int col, float top, float total, float v) {
+    // a finished row's column, and a column of this block's share of the keys: maximum, denominator, unnormalised result in units of 2^(top + e)
+    auto store = [&](int r, int col, float top, float total, float e, float v) {
         const int tok = t0 + s_pos[r] - pos0, h = s_head[r];
-        Elem<bf16>::put(static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, top, total, 0.0f, v)));
+        Elem<bf16>::put(static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, top, total, e, v)));
     };
-    auto put = [&](int r, int col, float top, float total, float v) {
+    auto put = [&](int r, int col, float top, float total, float e, float v) {
         if (A.n_splits == 1) {
-            store(r, col, top, total, v);
+            store(r, col, top, total, e, v);
         } else if (clustered) {
-            if (col == 0) {
-                s_stat[0][r] = top;
-                s_stat[1][r] = total;
-            }
+            if (col == 0) s_stat[r] = make_float4(top, total, e, 0.0f);
             joint[r * D + col] = v;
         } else {
             const size_t at = ((size_t)(t0 + s_pos[r] - pos0) * A.H + s_head[r]) * A.n_splits + split;
-            if (col == 0) part_stats(A)[at] = make_float4(top, total, 0.0f, 0.0f);
+            if (col == 0) part_stats(A)[at] = make_float4(top, total, e, 0.0f);
             A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = v;
         }
     };
@@ -256,8 +299,10 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         const int me = threadIdx.x;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         const Bend bend(A);
-        float m[RA], l[RA], o[HALVES][RA];              // running maximum, this thread's part of the denominator, results in full
-        float m_step[RA], l_step[RA], unit = 0.0f;      // of the step before, whose product is not yet joined; what it is in units of
+        // (weights are multiplied as 256 times what they are: results are in units of 2^-8 of the reference's)
+        float m[RA], l[RA], o[HALVES][RA];              // largest score + log2(scale), or once apart largest score; this thread's part of the denominator; results in full
+        float m_step[RA], l_step[RA], unit = 0.0f;      // of the step before, whose product is not yet joined; log2 of the first block's scale
+        bool apart = false, apart_step = false;
 #pragma unroll
         for (int r = 0; r < RA; ++r) {
             m[r] = m_step[r] = -INFINITY;
@@ -271,14 +316,25 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             __syncwarp();
             umma::fence_after_sync();
             float keep[RA], add[RA];
+            if (!apart_step) {
 #pragma unroll
-            for (int r = 0; r < RA; ++r) {
-                const float mn = fmaxf(m[r], m_step[r]);
-                keep[r] = m[r] == mn ? 1.0f : exp2_fast(m[r] - mn);
-                add[r] = m_step[r] == -INFINITY ? 0.0f : exp2_fast(m_step[r] - mn);
-                m[r] = mn;
-                l[r] = fmaf(l_step[r], add[r], l[r] * keep[r]);
-                add[r] *= unit;
+                for (int r = 0; r < RA; ++r) {
+                    const float mn = fmaxf(m[r], m_step[r]);
+                    keep[r] = m[r] == mn ? 1.0f : exp2_fast(m[r] - mn);
+                    add[r] = m_step[r] == -INFINITY ? 0.0f : exp2_fast(m_step[r] - mn);
+                    m[r] = mn;
+                    l[r] = fmaf(l_step[r], add[r], l[r] * keep[r]);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < RA; ++r) {
+                    const Apart f(m[r], m_step[r], s_unit[b][r], s_step_unit[b][r]);
+                    if (me == r) s_unit[b ^ 1][r] = f.unit;
+                    keep[r] = f.keep;
+                    add[r] = f.add;
+                    l[r] = fmaf(l_step[r], f.add_l, l[r] * f.keep_l);
+                    m[r] = fmaxf(m[r], m_step[r]);
+                }
             }
 #pragma unroll
             for (int x = 0; x < HALVES; ++x) {
@@ -295,10 +351,9 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), j = j0 + me;
             // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
             wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
-            const float ks = s_scales[st].of[me / kBlock].x, vs = s_scales[st].of[me / kBlock].y;
-            float v_top = 0.0f;
-#pragma unroll
-            for (int x = 0; x < kStepBlocks; ++x) v_top = fmaxf(v_top, fabsf(s_scales[st].of[x].y));
+            const float2 scales = s_scales[st].of[me / kBlock];
+            const float ks = scales.x, vs = scales.y, lv = ks == 0.0f ? 0.0f : scale_log2(fabsf(vs));
+            if (i == 0 && s_scales[0].of[0].x != 0.0f) unit = scale_log2(fabsf(s_scales[0].of[0].y));
             wait_bar(&bars.s_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
             umma::fence_after_sync();
@@ -309,11 +364,15 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                 for (int x = 0; x < N / 8; ++x) umma::tmem_ld8_issue(tmem + b * N + 8 * x + lanes, v[x]);
                 umma::tmem_ld_wait();
 #pragma unroll
-                for (int r = 0; r < RA; ++r) S[r] = fmaf(__uint_as_float(v[(NR + r) / 8][r % 8]), 0.0625f, __uint_as_float(v[r / 8][r % 8])) * (rowmul[r] * ks);
+                for (int r = 0; r < RA; ++r) S[r] = fmaf(fmaf(__uint_as_float(v[(NR + r) / 8][r % 8]), 0.0625f, __uint_as_float(v[r / 8][r % 8])), rowmul[r] * ks, BENT ? 0.0f : lv);
             }
             umma::fence_before_sync();
             arrive(&bars.s_empty[b]);
-            if (BENT) bend(A, S, [&](int r) { return (float)(s_pos[r] - j); }, [&](int r) { return s_r1[r]; }, [&](int r) { return s_r2[r]; }, [&](int r) { return s_slope[r]; });
+            if (BENT) {
+                bend(A, S, [&](int r) { return (float)(s_pos[r] - j); }, [&](int r) { return s_r1[r]; }, [&](int r) { return s_r2[r]; }, [&](int r) { return s_slope[r]; });
+#pragma unroll
+                for (int r = 0; r < RA; ++r) S[r] += lv;
+            }
             const bool whole = j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             bool hidden = ks == 0.0f;      // from some row
             if (!whole || hidden) {
@@ -335,27 +394,60 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                     if (w.x != z.x || w.y != z.y || w.z != z.z || w.w != z.w) at = z;
                 }
             }
-            // ---- the rows' maxima over the step ----
-            float mine = 0.0f, top[RA];
+            // ---- the rows' maxima over the step, of score + log2(scale) ----
+            float mine = 0.0f, top[RA], sums[RA];
 #pragma unroll
             for (int r = 0; r < RA; ++r) {
                 const float t = warp_top(S[r]);
                 mine = lane == r ? t : mine;
             }
             if (lane < RA) s_top[b][warp][lane] = mine;
+            const bool apart_before = apart;
+            if (ks != 0.0f && fabsf(lv - unit) > kNear) s_apart[b] = 1;
             sync4();
+            apart |= s_apart[b] != 0;
+            if (!apart) {
+                const float counts = exp2_fast(unit - lv);
 #pragma unroll
-            for (int r = 0; r < RA; ++r) top[r] = fmaxf(fmaxf(s_top[b][0][r], s_top[b][1][r]), fmaxf(s_top[b][2][r], s_top[b][3][r]));
+                for (int r = 0; r < RA; ++r) {
+                    top[r] = fmaxf(fmaxf(s_top[b][0][r], s_top[b][1][r]), fmaxf(s_top[b][2][r], s_top[b][3][r]));
+                    S[r] = exp2_fast(S[r] - (top[r] == -INFINITY ? 0.0f : top[r]));
+                    sums[r] = S[r] * counts;
+                }
+            } else {
+                if (!apart_before) {
+                    if (me < RA) s_unit[b][me] = unit;
+#pragma unroll
+                    for (int r = 0; r < RA; ++r) {
+                        m[r] -= unit;
+                        m_step[r] -= unit;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < RA; ++r) {
+                    S[r] -= lv;
+                    const float2 most = apart_maxima(S[r], lv);
+                    if (lane == r) {
+                        s_top[b][warp][r] = most.x;
+                        s_far[b][warp][r] = most.y;
+                    }
+                }
+                sync4();
+#pragma unroll
+                for (int r = 0; r < RA; ++r) {
+                    const float4 w = apart_weight(S[r], lv, s_top[b][0] + r, s_far[b][0] + r, RA);
+                    if (me == r) s_step_unit[b][r] = w.w;
+                    S[r] = w.x;
+                    sums[r] = w.y;
+                    top[r] = w.z;
+                }
+            }
             // ---- weights: hi at row r, lo at row NR + r, this position's byte (the product of two steps ago, which read them, has been joined) ----
-            const float vmul = 256.0f * (fabsf(vs) / fmaxf(v_top, kLeastScale));
             unsigned char* P = Ps + b * (N * 128);
-            float sums[RA];
 #pragma unroll
             for (int r = 0; r < RA; r += 2) {
-#pragma unroll
-                for (int e = 0; e < 2; ++e) sums[r + e] = exp2_fast(S[r + e] - (top[r + e] == -INFINITY ? 0.0f : top[r + e]));
                 uint32_t hi, part;
-                two_parts(__floats2half2_rn(sums[r] * vmul, sums[r + 1] * vmul), hi, part);
+                two_parts(__floats2half2_rn(S[r] * 256.0f, S[r + 1] * 256.0f), hi, part);
                 P[sw128_byte(r, me)] = (unsigned char)hi;
                 P[sw128_byte(r + 1, me)] = (unsigned char)(hi >> 8);
                 P[sw128_byte(NR + r, me)] = (unsigned char)part;
@@ -369,8 +461,9 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                 m_step[r] = top[r];
                 l_step[r] = sums[r];
             }
-            unit = v_top * (1.0f / 256.0f);
+            apart_step = apart;
         }
+        if (apart_step) sync4();
         join_product(steps - 1);
         // ---- a column of the result per thread: written, put down as this share's, or left in shared memory for the cluster ----
 #pragma unroll
@@ -387,7 +480,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
 #pragma unroll
             for (int r = 0; r < RA; ++r) {
                 if (r >= rows) break;
-                put(r, col, m[r], (s_sum[0][r] + s_sum[1][r]) + (s_sum[2][r] + s_sum[3][r]), nans >> r & 1 ? __int_as_float(0x7fffffff) : o[x][r]);
+                put(r, col, apart_step ? m[r] : m[r] - unit, (s_sum[0][r] + s_sum[1][r]) + (s_sum[2][r] + s_sum[3][r]), (apart_step ? s_unit[steps & 1][r] : unit) - 8.0f, nans >> r & 1 ? __int_as_float(0x7fffffff) : o[x][r]);
             }
         }
     } else if (any) {
@@ -401,38 +494,47 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         }
         asm volatile("bar.sync 1, 128;" ::: "memory");
         for (int col = threadIdx.x; col < A.c.dv; col += 128)
-            for (int r = 0; r < rows; ++r) put(r, col, -INFINITY, 0.0f, 0.0f);
+            for (int r = 0; r < rows; ++r) put(r, col, -INFINITY, 0.0f, 0.0f, 0.0f);
     }
     __syncwarp();
     if (clustered) {
         cluster_sync();
         if (any && warp < 4 && !*stop)
             for (int r = split; r < rows; r += A.n_splits) {
-                float top[kMostCluster], f[kMostCluster], v[D / 128][kMostCluster];
+                float top[kMostCluster], f[kMostCluster], e[kMostCluster], v[D / 128][kMostCluster];
 #pragma unroll
                 for (int z = 0; z < kMostCluster; ++z) {
                     const bool on = z < A.n_splits;
-                    top[z] = on ? of_rank(&s_stat[0][r], z) : -INFINITY;
-                    f[z] = on ? of_rank(&s_stat[1][r], z) : 0.0f;
+                    const float4 stat = on ? of_rank(&s_stat[r], z) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+                    top[z] = stat.x;
+                    f[z] = stat.y;
+                    e[z] = stat.z;
 #pragma unroll
                     for (int x = 0; x < D / 128; ++x) v[x][z] = on && threadIdx.x + 128 * x < A.c.dv ? of_rank(joint + r * D + threadIdx.x + 128 * x, z) : 0.0f;
                 }
-                float M = -INFINITY, total = 0.0f;
+                float M = -INFINITY, E = -INFINITY, least = INFINITY, total = 0.0f;
 #pragma unroll
-                for (int z = 0; z < kMostCluster; ++z) M = fmaxf(M, top[z]);
+                for (int z = 0; z < kMostCluster; ++z) {
+                    M = fmaxf(M, top[z]);
+                    E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z]);
+                    least = fminf(least, top[z] == -INFINITY ? INFINITY : e[z]);
+                }
+                if (E - least > kNear) {      // (units far apart: not the largest, but that of the largest results)
+                    E = -INFINITY;
+                    for (int z = 0; z < kMostCluster; ++z) E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z] + (top[z] - M));
+                }
 #pragma unroll
                 for (int z = 0; z < kMostCluster; ++z) {
                     // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
-                    const float w = top[z] == -INFINITY ? (f[z] == 0.0f ? 0.0f : f[z]) : exp2_fast(top[z] - M);
-                    total = fmaf(f[z], w, total);
-                    f[z] = w;
+                    total = fmaf(f[z], top[z] == -INFINITY ? (f[z] == 0.0f ? 0.0f : f[z]) : exp2_fast(top[z] - M), total);
+                    e[z] = top[z] == -INFINITY ? 0.0f : exp2_fast((e[z] - E) + (top[z] - M));
                 }
 #pragma unroll
                 for (int x = 0; x < D / 128; ++x) {
                     float sum = 0.0f;
 #pragma unroll
-                    for (int z = 0; z < kMostCluster; ++z) sum = fmaf(v[x][z], f[z], sum);
-                    if (threadIdx.x + 128 * x < A.c.dv) store(r, threadIdx.x + 128 * x, M, total, sum);
+                    for (int z = 0; z < kMostCluster; ++z) sum = fmaf(v[x][z], e[z], sum);
+                    if (threadIdx.x + 128 * x < A.c.dv) store(r, threadIdx.x + 128 * x, M, total, E, sum);
                 }
             }
         cluster_sync();      // nobody leaves while others read

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     if (threadIdx.x == 0) J.bad = 0;
 
     // where the warp's blocks are: lane i knows block number i of 32 (`now`), and of the 32 that follow
-    struct Place { int page, in_page; float ks, lv; };      // lv: log2 of the values' scale (exact for a power of two)
+    struct Place { int page, in_page; float ks, lv; };      // lv: log2 of the values' scale
     bool bad = false;
     auto block_of = [&](int i) { const int x = b_lo + warp + i * kRowWarps; return x < seen.lead ? x : seen.from + x - seen.lead; };
     auto look_up = [&](int i0) {
@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
                 const int at = g * (A.c.page / kBlock) + p.in_page / kBlock;
                 p.ks = A.c.ks[(size_t)p.page * A.c.ks_page + at];
                 const float vs = A.c.vs[(size_t)p.page * A.c.vs_page + at];
-                p.lv = log2f(fmaxf(fabsf(vs), 7.5231638e-37f));      // 2^-120: below every scale
+                p.lv = scale_log2(fmaxf(fabsf(vs), 7.5231638e-37f));      // 2^-120: below every scale
                 bad |= p.ks < 0.0f || vs < 0.0f;
             }
         }

@@ -181,7 +181,7 @@ __device__ __forceinline__ void four_of(uint2 u, float (&v)[4]) { v[0] = bf_lo(u
 // What the copying warp leaves beside a stage: the scales of the step's blocks, keys' and values' (0: nothing there; the values' sign says whether a block
 // holds a NaN).  With SHARES the values' are shares of the step's largest, powers of two, and bit x of marks says that block x holds NaNs among its
 // values, bit 8 + x that there is nothing: 512 threads that each find this out take 2 % of their time, while for few rows, whose copies are what is
-// waited for, it is better left to the threads (64 sequences at up to 8192 positions 142 us, 146 with it).
+// waited for, it is better left to the threads (64 sequences at up to 8192 positions 142 us; 146 with it, 150 with the logarithms and a vote on whether they are near).
 struct StepScales {
     float2 of[kStepBlocks];
     float v_top;
