@@ -179,19 +179,18 @@ __device__ __forceinline__ void load_queries(uint2 (&u)[N][KH], const AttendArgs
 __device__ __forceinline__ void four_of(uint2 u, float (&v)[4]) { v[0] = bf_lo(u.x); v[1] = bf_hi(u.x); v[2] = bf_lo(u.y); v[3] = bf_hi(u.y); }
 
 // What the copying warp leaves beside a stage: the scales of the step's blocks, keys' and values' (0: nothing there; the values' sign says whether a block
-// holds a NaN).  With SHARES the values' are shares of the step's largest, powers of two, and bit x of marks says that block x holds NaNs among its
-// values, bit 8 + x that there is nothing: 512 threads that each find this out take 2 % of their time, while for few rows, whose copies are what is
-// waited for, it is better left to the threads (64 sequences at up to 8192 positions 142 us; 146 with it, 150 with the logarithms and a vote on whether they are near).
+// holds a NaN).  With LOGS the values' are logarithms to base 2, and bit x of marks says that block x holds NaNs among its values, bit 8 + x that there is
+// nothing: 512 threads that each find this out take 2 % of their time, while for few rows, whose copies are what is
+// waited for, it is better left to the threads (64 sequences at up to 8192 positions 142 us; 146 with the marks, 150 with the logarithms and a vote on whether they are near).
 struct StepScales {
     float2 of[kStepBlocks];
-    float v_top;
     uint32_t marks;
 };
 
 // The copying warp: keys and values of every step into a ring of NS stages (keys: KH tiles of 128 positions by 128 bytes, then VH of the values from
 // column v_col on), 128-byte swizzle, in boxes of `box` positions that lie together.  Lane x < 8 looks up block x of a step; entries are loaded two steps ahead and scales one,
 // so that nothing waits for them here.
-template <int KH, int VH, int NS, bool SHARES>
+template <int KH, int VH, int NS, bool LOGS>
 __device__ __forceinline__ void copy_steps(const AttendArgs& A, const CUtensorMap* kmap, const CUtensorMap* vmap, int box, const Rows& W, const Seen& seen, int lo, int steps, int first_pos,
                                            unsigned char* ring, StepScales* scales, uint64_t* full, uint64_t* empty, volatile int* stop, int v_col) {
     constexpr int SB = kStep * 128 * (KH + VH);
@@ -231,13 +230,10 @@ __device__ __forceinline__ void copy_steps(const AttendArgs& A, const CUtensorMa
         if (now.in_page >= 0 && !held) atomicExch(A.c.err, 1);
         const bool mine = held && lane % per == 0;      // a box's first block issues it
         const int live = __popc(__ballot_sync(0xffffffffu, mine));
-        if (SHARES) {
-            float v_top = lane < kStepBlocks ? fabsf(sc.y) : 0.0f;
-#pragma unroll
-            for (int x = kStepBlocks / 2; x > 0; x >>= 1) v_top = fmaxf(v_top, __shfl_xor_sync(0xffffffffu, v_top, x));
+        if (LOGS) {
             const uint32_t marks = __ballot_sync(0xffffffffu, lane < kStepBlocks && sc.y < 0.0f) | __ballot_sync(0xffffffffu, lane < kStepBlocks && sc.x == 0.0f) << kStepBlocks;
-            sc.y = fabsf(sc.y) / fmaxf(v_top, kLeastScale);
-            if (lane == 0) { scales[st].v_top = v_top; scales[st].marks = marks; }
+            if (sc.x != 0.0f) sc.y = scale_log2(fabsf(sc.y));
+            if (lane == 0) scales[st].marks = marks;
         }
         if (lane < kStepBlocks) scales[st].of[lane] = sc;
         __syncwarp();

@@ -5,7 +5,9 @@
 // portion fills a tile.  128 positions a step.  As for few rows (cache8_few.cuh) the codes go to the tensor cores as they are, and queries and
 // weights are the sum of two e4m3 parts; here both parts have one unit and one accumulator, so that a product is eight instructions for 128 terms,
 // as many cycles as bf16 operands would take.  That leaves a query's coordinates exact down to 2^-10 of the row's largest and 2^-18 of it
-// below, and a weight's error at 2^-9, or 2^-18 of the row's largest in the step.
+// below, and a weight's error at 2^-9, or 2^-18 of the largest weight times value scale that the row sees in the step: as for few rows the scale's logarithm is part of what is
+// raised, exp2(s - m + log2(scale) - e).  (With the scale as a factor behind it, over the step's largest, a value 2^12 larger at a later position cost a row 5 %, one
+// 2^18 larger all of it.)  Results are in units of 2^(m + e), the denominator, the weights' sums per block times 2^(e - log2(scale)), in units of 2^m.
 //
 // Roles: a warp that copies, one that issues the products, sixteen warps for the softmax: four threads per row, 32 columns of the scores and of
 // the result each.  Scores are double-buffered in tensor memory, so that the next step's are multiplied while this step's are worked on, and weights
@@ -100,7 +102,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
     __shared__ StepScales s_scales[NS];
-    __shared__ float s_max[2][kTileParts][kTileRows], s_rowmul[kTileRows];
+    __shared__ float2 s_max[2][kTileParts][kTileRows];      // a part's largest score, and largest score - it + log2(value scale)
+    __shared__ float s_rowmul[kTileRows];
     __shared__ int s_bad;
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *KV = base, *Qs = KV + NS * SB;      // Qs: first parts, then second parts
@@ -247,7 +250,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
         const float rowmul = s_rowmul[row], r1 = BENT && A.r1 ? A.r1[h] : 0.0f, r2 = BENT && A.r1 ? A.r2[h] : 0.0f, slope = BENT && A.slope ? A.slope[h] * kLog2e : 0.0f;
         const Bend bend(A);
         auto row_barrier = [&] { asm volatile("bar.sync %0, %1;" ::"r"(quad + 1), "n"(kTileParts * 32) : "memory"); };
-        float m = -INFINITY, l = 0.0f, m_step = -INFINITY, l_step = 0.0f, unit = 0.0f, o[kTileCols];
+        float m = -INFINITY, unit = 0.0f, l = 0.0f, m_step = -INFINITY, unit_step = 0.0f, l_step = 0.0f, o[kTileCols];      // l in units of 2^m, o of 2^(m + unit)
 #pragma unroll
         for (int c = 0; c < kTileCols; ++c) o[c] = 0.0f;
         auto join_product = [&](int i) {
@@ -255,17 +258,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             wait_bar(&bars.o_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
             umma::fence_after_sync();
-            // m is what results and denominator are relative to: the first step's maximum, and a later one's only where fp32 would come near its end
-            if (__any_sync(0xffffffffu, m_step > m + kFarAbove)) {
-                const float mn = m_step > m + kFarAbove ? m_step : m, keep = m == mn ? 1.0f : exp2_fast(m - mn);
+            // what results and denominator are relative to is the first step's, and a later one's only where they would come near fp32's end (they are below 2^90)
+            if (__any_sync(0xffffffffu, m_step > m + kFarAbove || (m_step - m) + unit_step > unit + kFarAbove)) {
+                const float mn = m_step > m + kFarAbove ? m_step : m, had = unit + (m - mn), has = unit_step + (m_step - mn), un = m == -INFINITY || has > had + kFarAbove ? has : had;
+                const bool some = mn != -INFINITY;
+                const float keep = !some || had == un ? 1.0f : m == -INFINITY ? 0.0f : exp2_fast(had - un);
+                l *= !some || m == mn ? 1.0f : exp2_fast(m - mn);
                 m = mn;
-                l *= keep;
+                unit = some ? un : unit;
 #pragma unroll
                 for (int c = 0; c < kTileCols; ++c) o[c] *= keep;
             }
-            float add = m_step == -INFINITY ? 0.0f : exp2_fast(m_step - m);
-            l = fmaf(l_step, add, l);
-            add *= unit;
+            l = fmaf(l_step, m_step == -INFINITY ? 0.0f : exp2_fast(m_step - m), l);
+            const float add = m_step == -INFINITY ? 0.0f : exp2_fast((m_step - m) + (unit_step - unit)) * (1.0f / 256.0f);
 #pragma unroll
             for (int x = 0; x < kTileCols / 32; ++x) {
                 uint32_t v[4][8];
@@ -284,15 +289,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), jc = j0 + part * kTileCols;
             // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
             wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
-            const float v_top = s_scales[st].v_top;
             const uint32_t marks = s_scales[st].marks;
             const bool nans = marks & ((1 << kStepBlocks) - 1), holes = marks >> kStepBlocks;      // in the whole step
-            float ks[kTileCols / kBlock], share[kTileCols / kBlock];
+            float ks[kTileCols / kBlock], lv[kTileCols / kBlock];
 #pragma unroll
             for (int x = 0; x < kTileCols / kBlock; ++x) {
                 const float2 of = s_scales[st].of[part * (kTileCols / kBlock) + x];
                 ks[x] = of.x;
-                share[x] = of.y;
+                lv[x] = of.y;
             }
             wait_bar(&bars.s_full[b], (i >> 1) & 1, stop, A.c.err);
             __syncwarp();
@@ -338,48 +342,67 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                     if (w.x != z.x || w.y != z.y || w.z != z.z || w.w != z.w) at = z;
                 }
             }
-            // ---- the row's maximum over the step ----
-            float top = -INFINITY;
+            // ---- the row's maxima over the step: of its scores, and of score + log2(scale) from there ----
+            float most[kTileCols / kBlock], top = -INFINITY, e = -INFINITY;
 #pragma unroll
             for (int x = 0; x < kTileCols / kBlock; ++x) {
                 float t[4] = {S[16 * x], S[16 * x + 1], S[16 * x + 2], S[16 * x + 3]};
 #pragma unroll
-                for (int e = 4; e < 16; ++e) t[e % 4] = fmaxf(t[e % 4], S[16 * x + e]);
-                top = fmaxf(top, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * mul[x]);
+                for (int c = 4; c < 16; ++c) t[c % 4] = fmaxf(t[c % 4], S[16 * x + c]);
+                most[x] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * mul[x];
+                top = fmaxf(top, most[x]);
             }
-            s_max[b][part][row] = top;
-            row_barrier();
 #pragma unroll
-            for (int x = 0; x < kTileParts; ++x) top = fmaxf(top, s_max[b][x][row]);
-            // ---- weights, times 256 and the block's share of the largest value scale ----
-            const float under = (top == -INFINITY ? 0.0f : top) - 8.0f;
+            for (int x = 0; x < kTileCols / kBlock; ++x) e = fmaxf(e, top == -INFINITY ? -INFINITY : (most[x] - top) + lv[x]);
+            s_max[b][part][row] = make_float2(top, e);
+            row_barrier();
+            {
+                float2 t[kTileParts];
+#pragma unroll
+                for (int x = 0; x < kTileParts; ++x) {
+                    t[x] = s_max[b][x][row];
+                    top = fmaxf(top, t[x].x);
+                }
+#pragma unroll
+                for (int x = 0; x < kTileParts; ++x) e = x == 0 ? t[x].y + (t[x].x - top) : fmaxf(e, t[x].y + (t[x].x - top));
+            }
+            const bool none = top == -INFINITY;
+            if (none) e = 0.0f;
+            const float base = none ? 0.0f : top;
+            float total = 0.0f;      // the denominator's terms
+            // (value scales so far apart that weights which count there may be too small for an fp32 number; what is lost with them otherwise is below 2^-62)
+            bool far = false;
+#pragma unroll
+            for (int x = 0; x < kTileCols / kBlock; ++x) far |= e - lv[x] > kFarAbove;
+            far = __any_sync(0xffffffffu, far && !none);
+            if (far) {
+#pragma unroll
+                for (int c = 0; c < kTileCols; ++c) total += exp2_fast(fmaf(S[c], mul[c / kBlock], -base));
+            }
+            // ---- weights, times 256 ----
             // (behind the barrier all of the row's scores are in registers: weights go where they were, first parts into the first 32 columns, second parts into the next)
             const uint32_t P = tmem + b * kStep + part * (kTileCols / 4) + lanes;
-            const uint64_t under2 = two(-under, -under);
-            uint64_t sum = two(0.0f, 0.0f);
             uint32_t hi[8], rest[8];
             static_assert(kTileCols == 32, "eight columns of weights a thread");
 #pragma unroll
             for (int x = 0; x < kTileCols / kBlock; ++x) {
-                const uint64_t mul2 = two(mul[x], mul[x]);
+                // (rounded down: not above 256 however large the scores)
+                const float over = __fadd_rd((lv[x] - e) + 8.0f, -base);
+                const uint64_t mul2 = two(mul[x], mul[x]), over2 = two(over, over);
+                uint64_t sum = two(0.0f, 0.0f);
                 uint32_t w[8];
 #pragma unroll
                 for (int y = 0; y < 8; ++y) {
                     float p0, p1;
-                    of_two(fma_two(two(S[16 * x + 2 * y], S[16 * x + 2 * y + 1]), mul2, under2), p0, p1);
+                    of_two(fma_two(two(S[16 * x + 2 * y], S[16 * x + 2 * y + 1]), mul2, over2), p0, p1);
                     p0 = exp2_fast(p0);
                     p1 = exp2_fast(p1);
                     sum = add_two(sum, two(p0, p1));
                     w[y] = half_two(p0, p1);
                 }
-                if (share[x] != 1.0f) {
-                    const __half2 ratio = __float2half2_rn(share[x]);      // a power of two (0 below 2^-24)
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        const __half2 t = __hmul2(*reinterpret_cast<const __half2*>(&w[y]), ratio);
-                        w[y] = *reinterpret_cast<const uint32_t*>(&t);
-                    }
-                }
+                float sum0, sum1;
+                of_two(sum, sum0, sum1);
+                if (!far) total = fmaf(sum0 + sum1, exp2_fast((e - lv[x]) - 8.0f), total);
 #pragma unroll
                 for (int y = 0; y < 4; ++y) four_equal_parts(w[2 * y], w[2 * y + 1], hi[4 * x + y], rest[4 * x + y]);
             }
@@ -393,19 +416,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             if (lane == 0) arrive(&bars.p_full[b]);
             if (i > 0) join_product(i - 1);
             m_step = top;
-            float sum0, sum1;
-            of_two(sum, sum0, sum1);
-            l_step = (sum0 + sum1) * (1.0f / 256.0f);
-            unit = v_top * (1.0f / 256.0f);
+            unit_step = e;
+            l_step = total;
         }
         join_product(steps - 1);
         // ---- the row's denominator, then 32 columns a thread ----
         row_barrier();
-        s_max[0][part][row] = l;
+        s_max[0][part][row].x = l;
         row_barrier();
         float total = 0.0f;
 #pragma unroll
-        for (int x = 0; x < kTileParts; ++x) total += s_max[0][x][row];
+        for (int x = 0; x < kTileParts; ++x) total += s_max[0][x][row].x;
         const int col = v_col + part * kTileCols;
         if (col < A.c.dv && !__any_sync(0xffffffffu, *stop)) {
             const bool mine = row < rows;
@@ -419,15 +440,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             if (A.n_splits > 1) {
                 const int ld = (A.c.dv + 3) / 4 * 4;
                 const size_t at = ((size_t)tok * A.H + h) * A.n_splits + split;
-                if (mine && col == 0) part_stats(A)[at] = make_float4(m, total, 0.0f, 0.0f);
+                if (mine && col == 0) part_stats(A)[at] = make_float4(m, total, unit, 0.0f);
                 float* to = A.part + at * ld + col;
 #pragma unroll
                 for (int c = 0; c < kTileCols; c += 4)
                     if (mine && col + c < ld) *reinterpret_cast<float4*>(to + c) = make_float4(o[c], o[c + 1], o[c + 2], o[c + 3]);
             } else {
-                // one division a row
-                const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, m);
-                const float f = m == -INFINITY ? 1.0f : exp2_fast(m - M), all = fmaf(total, f, M == -INFINITY ? 0.0f : exp2_fast(sink - M)), r = all == 0.0f ? 1.0f : f / all;
+                const Finish f(A, h, m, total, unit);      // (one division a row)
                 if (A.o_vec == 2 && !A.gate) {
                     // through shared memory (the ring is done with: the last product was waited for), so that four lanes write a row's 64 bytes: a lane's own row
                     // a lane, 8 bytes at a time, cost 4000 cycles a block
@@ -436,7 +455,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                     for (int x = 0; x < 4; ++x) {
                         uint32_t w[4];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) w[y] = pack_bf16(o[8 * x + 2 * y] * r * A.out_scale, o[8 * x + 2 * y + 1] * r * A.out_scale);
+                        for (int y = 0; y < 4; ++y) w[y] = pack_bf16(o[8 * x + 2 * y] * f.a * f.b * A.out_scale, o[8 * x + 2 * y + 1] * f.a * f.b * A.out_scale);
                         *reinterpret_cast<uint4*>(tile + lane * 64 + (x ^ (lane >> 1 & 3)) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                     __syncwarp();
@@ -452,7 +471,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                     bf16* to = static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col;
 #pragma unroll
                     for (int c = 0; c < kTileCols; ++c)
-                        if (col + c < A.c.dv) to[c] = __float2bfloat16_rn(finished(A, tok, h, col + c, o[c] * r));
+                        if (col + c < A.c.dv) to[c] = __float2bfloat16_rn(finished(A, tok, h, col + c, o[c] * f.a * f.b));
                 }
             }
         }

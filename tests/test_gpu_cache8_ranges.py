@@ -61,7 +61,8 @@ def ones_column(q, k, at=8.0, key=0.0):
     q[..., 0], k[..., 0] = at, key
 
 
-KERNELS = [(torch.bfloat16, 1, LEAST_FEW), (torch.bfloat16, 7, LEAST_FEW), (torch.float32, 1, LEAST_F32), (torch.float32, 7, LEAST_F32), (torch.float32, 150, LEAST_F32)]
+KERNELS = [(torch.bfloat16, 1, LEAST_FEW), (torch.bfloat16, 7, LEAST_FEW), (torch.bfloat16, 150, LEAST_TILES), (torch.float32, 1, LEAST_F32),
+           (torch.float32, 7, LEAST_F32), (torch.float32, 150, LEAST_F32)]
 
 
 @pytest.mark.parametrize("dtype,n,least", KERNELS)
@@ -123,7 +124,8 @@ def test_blocks_of_zeros_and_of_everything(dtype, n, least, low):
         check(c, table, q, pos0, c.attend(q, ints([0, n]), ints([pos0]), table, max_new=n, max_len=L, **options), least, **options)
 
 
-@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 1), (torch.bfloat16, 7), (torch.float32, 1), (torch.float32, 40)])
+@pytest.mark.parametrize("n", [1, 7, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_shares_of_the_keys_whose_values_differ(dtype, n):
     """A long context in several shares, joined in a cluster or by a kernel of its own: values grow by 2^20 every 700 positions, scores fall by 12 meanwhile."""
     H, G, d = 4, 2, 64
@@ -141,7 +143,8 @@ def test_shares_of_the_keys_whose_values_differ(dtype, n):
         check(c, table, q, pos0, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n < 9 else LEAST_TILES)
 
 
-@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 1), (torch.float32, 1), (torch.float32, 150)])
+@pytest.mark.parametrize("n", [1, 150])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("rise", [30.0, 40.0, 44.0])
 def test_rising_scores_of_large_values(dtype, n, rise):
     """Scores that rise by 30 to 44 from one step of 128 positions to the next, values near 2^90 and a clamped infinity."""
@@ -163,7 +166,7 @@ def test_a_sink_far_above_the_scores():
     """Scores 70 below the sink, values of 2^90: what is left is 2^-11."""
     H, G, d, L = 4, 2, 64, 300
     for dtype in (torch.bfloat16, torch.float32):
-        for n in (1, 150) if dtype == torch.float32 else (1,):
+        for n in (1, 150):
             c, table = cache_of([L], 64, G, d, d, seed=3)
             k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2) * 2.0 ** 90, randn(n, H, d, seed=3).to(dtype)
             c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
