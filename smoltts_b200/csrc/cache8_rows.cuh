@@ -84,13 +84,25 @@ __device__ __forceinline__ float bent_score(const AttendArgs& A, float s, int di
 }
 // The same with the hardware's (bf16): cap tanh(s / cap) log2 e = c - 2 c / (2^(s in) + 1) with c = cap log2 e and in = 2 log2 e / cap, and r ln(x) log2 e = r log2(x);
 // slope comes in units of log2.  (Of a distance below zero, that is hidden anyway, a NaN is made.)
+// That difference is off by some 2^-22 of the cap however small the score is: 6e-5 of a weight at a cap of 256, little beside a weight's own 2^-9, but 0.1 at 1e6.
+// Above, scores below a quarter of the cap take tanh's series, cap tanh(x) = s (1 - x^2 / 3 + 2 x^4 / 15 - 17 x^6 / 315 + 62 x^8 / 2835) with x = s / cap, whose next
+// term is below 2^-25 there; the others are off by at most 2^-20 of themselves either way.
+constexpr float kCapOfDifference = 256.0f;
 struct Bend {
     float in, c;
-    __device__ __forceinline__ explicit Bend(const AttendArgs& A) : in(A.softcap > 0.0f ? fminf(2.0f * kLog2e / A.softcap, 3e38f) : 0.0f), c(A.softcap * kLog2e) {}
+    __device__ __forceinline__ explicit Bend(const AttendArgs& A) : in(A.softcap > 0.0f ? fminf(2.0f * kLog2e / A.softcap, 3e38f) : 0.0f), c(fminf(A.softcap * kLog2e, 3.4e38f)) {}
     // N scores; dist(e), r1(e), r2(e), slope(e): of score e.  A loop per option: with the options looked at in every score, a step of the tiles took 7500 cycles.
     template <int N, class Dist, class R1, class R2, class Slope>
     __device__ __forceinline__ void operator()(const AttendArgs& A, float (&s)[N], Dist&& dist, R1&& r1, R2&& r2, Slope&& slope) const {
-        if (c > 0.0f) {
+        if (A.softcap > kCapOfDifference) {
+            const float inv = 1.0f / A.softcap;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float x = s[e] * inv, t = x * x, far = c * fmaf(-2.0f, __fdividef(1.0f, exp2_fast(s[e] * in) + 1.0f), 1.0f), l = s[e] * kLog2e;
+                const float p = fmaf(fmaf(fmaf(62.0f / 2835.0f, t, -17.0f / 315.0f), t, 2.0f / 15.0f), t, -1.0f / 3.0f);
+                s[e] = t < 0.0625f ? fmaf(l * t, p, l) : far;
+            }
+        } else if (c > 0.0f) {
 #pragma unroll
             for (int e = 0; e < N; ++e) s[e] = fmaf(-2.0f * c, __fdividef(1.0f, exp2_fast(s[e] * in) + 1.0f), c);
         } else {

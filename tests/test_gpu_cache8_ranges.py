@@ -17,7 +17,7 @@ pytestmark = pytest.mark.gpu
 LEAST_TILES, LEAST_FEW, LEAST_F32 = 2.0 ** -18, 2.0 ** -22, 2.0 ** -32
 
 
-def check(c, table, q, pos0, out, least, scale=None, window=0, first=0, kv_len=None, sink=None, rows=None):
+def check(c, table, q, pos0, out, least, scale=None, window=0, first=0, kv_len=None, sink=None, softcap=0.0):
     """One sequence's rows against 64 bits.  On top of `tolerance`: the weights' last bit times the codes it multiplies; and for bf16 2^-15 of the weights, from three roundings
     of a sum of a score and a block's exponent of at most 110, each 2^-24 of at most 160 (scores below 50 in units of log2) in units of log2."""
     n, H, d = q.shape
@@ -38,7 +38,8 @@ def check(c, table, q, pos0, out, least, scale=None, window=0, first=0, kv_len=N
     for h in range(H):
         g = h // (H // G)
         scale_ = d ** -0.5 if scale is None else scale
-        s = (q[:, h].double() @ k[:, g].T * scale_).masked_fill(~seen, -math.inf)
+        s = q[:, h].double() @ k[:, g].T * scale_
+        s = (softcap * torch.tanh(s / softcap) if softcap else s).masked_fill(~seen, -math.inf)
         size = (q[:, h].double().abs() @ k[:, g].abs().T * scale_).masked_fill(~seen, 0.0).amax(1, keepdim=True)
         top = s.amax(1, keepdim=True).masked_fill(~some, 0.0)
         if sink is not None:
@@ -51,8 +52,6 @@ def check(c, table, q, pos0, out, least, scale=None, window=0, first=0, kv_len=N
         floor = (w * unit[:, g]).amax(1, keepdim=True) * (seen.double() @ codes[:, g].abs()) / total
         tol = tolerance(q.dtype, want, spread, size) + least * floor + (2.0 ** -15 * spread if q.dtype == torch.bfloat16 else 0.0)
         far = ((out[:, h].double() - want).abs() - tol) / (spread + 1e-30)
-        if rows is not None:
-            far = far[rows]
         assert far.max().item() <= 0, (h, far.max().item(), (far > 0).any(1).nonzero().flatten().tolist()[:20])
 
 
@@ -173,3 +172,17 @@ def test_a_sink_far_above_the_scores():
             sink = torch.full((H,), 70.0, device="cuda")
             out = c.attend(q, ints([0, n]), ints([L - n]), table, max_new=n, max_len=L, sink=sink)
             check(c, table, q, L - n, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n == 1 else LEAST_TILES, sink=sink)
+
+
+@pytest.mark.parametrize("n", [1, 7, 150])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("cap", [300.0, 1e3, 1e4, 1e6, 1e8, 1e9, 1e20, 3.4e38])
+@pytest.mark.parametrize("scale", [0.125, 3.0, 60.0])
+def test_soft_caps_far_above_the_scores(dtype, n, cap, scale):
+    """Scores of up to 10, 250 and 5000 under caps from below them to fp32's end: what a cap adds to a score's error is 2^-20 of the score, an eighth of what its size is given."""
+    H, G, d, L = 4, 2, 64, 400
+    c, table = cache_of([L], 32, G, d, d, seed=5)
+    k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2), randn(n, H, d, seed=3).to(dtype)
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    out = c.attend(q, ints([0, n]), ints([L - n]), table, max_new=n, max_len=L, scale=scale, softcap=cap)
+    check(c, table, q, L - n, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n < 9 else LEAST_TILES, scale=scale, softcap=cap)
