@@ -385,7 +385,8 @@ int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const SmolLmCache8
 int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, void* workspace, size_t workspace_bytes, void* stream);
 
 int64_t smol_lm_launch_count(const SmolLm* m);
-int32_t* smol_lm_error_word(SmolLm* m);           /* device word, nonzero after a step that addressed outside its pools */
+int32_t* smol_lm_error_word(SmolLm* m);           /* device word, nonzero after a step that addressed outside its pools (1: a page, 2: a slot) or
+                                                     in which a wait inside a kernel ran out (3: results are missing) */
 
 #ifdef __cplusplus
 }

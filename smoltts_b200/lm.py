@@ -41,7 +41,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from . import _capi_lm
-from ._errors import SMOL_ERR_CAPACITY, SmolError
+from ._errors import SMOL_ERR_CAPACITY, SMOL_ERR_CUDA, SmolError
 from .lm_config import (ACT_CLAMPED, ACT_GELU_TANH, ACT_RELU_SQUARED, ACT_SILU, BLOCK_OUTNORM, BLOCK_PARALLEL, BLOCK_POSTNORM, BLOCK_PRENORM, BLOCK_SANDWICH,
                         MAFERAX_MLP_KINDS, MIXER_KINDS, MLP_KINDS, NORM_DYT, NORM_LAYER, ROUTE_CHOSEN, ROUTE_SIGMOID, RUN_ADD_EMBED, RUN_MERGE_EMBED,
                         BizulixConfig, GuniraxConfig, MaferaxConfig, PamasunConfig, SunutarConfig, VirusunConfig)
@@ -341,10 +341,12 @@ class HybridLM:
         return y
 
     def check_device_errors(self) -> None:
-        """Raises if a step addressed a page or slot outside the pools (reads the device-side error word; synchronises)."""
+        """Raises if a step addressed a page or slot outside the pools, or a wait inside a kernel ran out (reads the device-side error word; synchronises)."""
         ptr = self.lib.smol_lm_error_word(self._h)
         off = ptr - self._workspace.data_ptr()
         word = int(self._workspace[off:off + 4].view(torch.int32).item())
+        if word == 3:
+            raise SmolError(SMOL_ERR_CUDA, "device-side error word 3: a wait inside a kernel ran out, results of that step are missing")
         if word:
             raise SmolError(SMOL_ERR_CAPACITY, f"device-side error word {word}: a step addressed outside its pools")
 
