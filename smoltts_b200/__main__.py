@@ -8,6 +8,7 @@
 from __future__ import annotations
 
 import argparse
+import inspect
 import json
 import os
 import sys
@@ -19,8 +20,25 @@ def _dtype(name: str):
     return {"bfloat16": torch.bfloat16, "float32": torch.float32}[name]
 
 
-def _cache(a) -> dict:
-    return {"kv_bits": 8, "first_tokens": a.first_tokens} if a.kv_bits == 8 else {}
+def _load(a, max_tokens: int):
+    """The engine of ``--model``; None, with the reason on standard error, where its design cannot serve ``--kv-bits 8``."""
+    from ._errors import SMOL_ERR_UNSUPPORTED, SmolError
+    from .registry import design_of, load_model, model_class
+
+    if a.kv_bits != 8:
+        return load_model(a.model, dtype=_dtype(a.dtype), max_tokens=max_tokens, max_seqs=a.max_seqs)
+    design = design_of(a.model)
+    known = inspect.signature(model_class(design).__init__).parameters.values()
+    if not any(p.name == "kv_bits" or p.kind is p.VAR_KEYWORD for p in known):
+        print(f"--kv-bits 8: the engine of design {design!r} has no 8-bit cache", file=sys.stderr)
+        return None
+    try:
+        return load_model(a.model, dtype=_dtype(a.dtype), max_tokens=max_tokens, max_seqs=a.max_seqs, kv_bits=8, first_tokens=a.first_tokens)
+    except SmolError as e:
+        if e.code != SMOL_ERR_UNSUPPORTED:
+            raise
+        print(f"--kv-bits 8: design {design!r}: {e}", file=sys.stderr)
+        return None
 
 
 def _cache_arguments(p) -> None:
@@ -29,12 +47,13 @@ def _cache_arguments(p) -> None:
 
 
 def cmd_generate(a) -> int:
-    from .registry import load_model
     from .serving import TokenBatcher
 
     prompts = [[int(t) for t in p.split(",")] for p in a.prompt]
     longest = max(len(p) for p in prompts) + a.max_new_tokens
-    model = load_model(a.model, dtype=_dtype(a.dtype), max_tokens=a.max_tokens or 4 * (longest + 64), max_seqs=a.max_seqs, **_cache(a))
+    model = _load(a, a.max_tokens or 4 * (longest + 64))
+    if model is None:
+        return 4
     batcher = TokenBatcher(model, temp=a.temp, top_k=a.top_k, top_p=a.top_p, min_p=a.min_p, seed=a.seed, eos_id=a.eos)
     for p, out in zip(prompts, batcher.generate(prompts, a.max_new_tokens)):
         print(json.dumps({"prompt": p, "tokens": out}))
@@ -46,13 +65,14 @@ def cmd_trace(a) -> int:
     with wanted places, writes <out>/<step>.f32 (little-endian fp32 [wanted, vocab], entries' order); prints 'done <step>'."""
     import torch
 
-    from .registry import load_model
     from .serving import TokenBatcher
 
     try:
-        model = load_model(a.model, dtype=_dtype(a.dtype), max_tokens=a.max_tokens, max_seqs=a.max_seqs, **_cache(a))
+        model = _load(a, a.max_tokens)
     except TypeError:
         print("this design's engine does not take explicit-token steps", file=sys.stderr)
+        return 4
+    if model is None:
         return 4
     batcher = TokenBatcher(model)
     os.makedirs(a.out, exist_ok=True)

@@ -29,3 +29,44 @@ def test_the_engine_tells_a_wait_that_ran_out_from_a_bad_page(word, code, text):
     with pytest.raises(SmolError, match=text) as e:
         model.check_device_errors()
     assert e.value.code == code
+
+
+class Plain:
+    """An engine that knows no 8-bit cache."""
+
+    def __init__(self, config, dtype=None, max_tokens=0, max_seqs=0):
+        pass
+
+
+class Coded:
+    def __init__(self, config, dtype=None, max_tokens=0, max_seqs=0, kv_bits=16, first_tokens=0):
+        pass
+
+
+@pytest.mark.parametrize("command", [["generate", "--prompt", "1,2"], ["trace", "--out", "unused", "--max-tokens", "64"]])
+def test_the_command_line_says_why_a_design_cannot_have_the_cache(monkeypatch, capsys, command):
+    """Both commands end with status 4 and the reason, whether the class does not know the option or its layers are refused; other errors are not taken for one."""
+    from smoltts_b200 import __main__ as cli
+    from smoltts_b200 import registry
+    from smoltts_b200._errors import SMOL_ERR_UNSUPPORTED
+
+    def refuse(code):
+        def load(path, **kw):
+            assert kw["kv_bits"] == 8 and kw["first_tokens"] == 3
+            raise SmolError(code, "8-bit cache: softmax attention over keys and values only")
+        return load
+
+    argv = command + ["--model", "somewhere", "--kv-bits", "8", "--first-tokens", "3"]
+    monkeypatch.setattr(registry, "design_of", lambda path: "Some")
+    monkeypatch.setattr(registry, "model_class", lambda name: Plain)
+    monkeypatch.setattr(registry, "load_model", lambda path, **kw: Plain(None, **kw))
+    assert cli.main(argv) == 4
+    assert "'Some' has no 8-bit cache" in capsys.readouterr().err
+    monkeypatch.setattr(registry, "model_class", lambda name: Coded)
+    monkeypatch.setattr(registry, "load_model", refuse(SMOL_ERR_UNSUPPORTED))
+    assert cli.main(argv) == 4
+    said = capsys.readouterr().err
+    assert "softmax attention over keys and values only" in said and "explicit-token" not in said
+    monkeypatch.setattr(registry, "load_model", refuse(SMOL_ERR_CUDA))
+    with pytest.raises(SmolError):
+        cli.main(argv)
