@@ -337,6 +337,7 @@ typedef struct SmolLmCache8 {
 } SmolLmCache8;
 
 /* Rows seq_start[s] .. seq_start[s + 1] - 1 are the positions seq_pos0[s], + 1, ... of sequence s; rows outside every sequence are left alone.
+ * Positions are below 2^31 - 128; what the arrays say is looked at on the device, and a sequence that does not fit is left out and reported (err).
  * max_new: most rows of a sequence; max_len: most positions of a sequence, these rows included (attention only: sizes its grid; longer ones are
  * attended to as a whole all the same). */
 typedef struct SmolLmCache8Batch {

@@ -229,6 +229,7 @@ void note_alignment(AppendArgs& A, bool f32) {
 void note_alignment(AttendArgs& A, bool f32) {
     A.q_vec = whole_eights(A.q, A.q_row, A.q_head, A.c.d, f32) ? 2 : whole_fours(A.q, A.q_row, A.q_head, A.c.d, f32) ? 1 : 0;
     A.o_vec = whole_eights(A.out, A.o_row, A.o_head, A.c.dv, f32) ? 2 : whole_fours(A.out, A.o_row, A.o_head, A.c.dv, f32) ? 1 : 0;
+    A.held = (int)std::min<long long>((long long)A.b.max_pages * A.c.page, kPositions);
 }
 
 static int cache_of(const SmolLmCache8* s, Cache& c, const char* me) {

@@ -22,6 +22,7 @@ constexpr int kLeastExp = -110, kMostExp = 92;   // exponents of a scale: a code
 constexpr float kMostValue = 1.2676506e30f;      // 2^100: magnitudes above are clamped
 constexpr int kMaxDim = 256;
 constexpr int kMaxPairs = 128;
+constexpr int kPositions = 0x7fffffff - 127;     // positions are below this: a step of 128 rounded up from there is still an int
 
 struct Cache {
     uint8_t *k, *v;                  // codes: page * k_page + (head * page_size + position) * ldk + coordinate
@@ -37,6 +38,17 @@ struct Batch {
     const int32_t *start, *pos0, *table;
     const int32_t* kv_len;           // attention: keys of the sequence (nullptr: up to the row's own position)
     int S, T, max_pages, max_new, max_len;
+};
+// Sequence s as the arrays have it, which are looked at here before anything is made of them: rows that lie in the step, positions that are numbers.  Otherwise it has
+// no rows, and the batch's error is reported.
+struct Sequence {
+    int t0, n, pos0;
+    __device__ __forceinline__ Sequence(const Batch& b, int s, int32_t* err) : t0(b.start[s]), pos0(b.pos0[s]) {
+        const int t1 = b.start[s + 1];
+        const bool fits = t0 >= 0 && t1 >= t0 && t1 <= b.T && pos0 <= kPositions - (t1 - t0);
+        n = fits ? t1 - t0 : 0;
+        if (!fits && threadIdx.x == 0) atomicExch(err, 2);
+    }
 };
 
 struct AppendArgs {
@@ -67,6 +79,7 @@ struct AttendArgs {
     float* part;                     // shares of the keys: unnormalised results [T * H][n_splits][dv rounded up to 4], then (maximum, denominator, e of the results, which are in units of 2^(maximum + e), -) [T * H][n_splits]
     int n_splits;
     int q_vec, o_vec;                // rows are whole groups of four elements that a load takes (1), of eight on 16-byte boundaries (2)
+    int held;                        // positions that a row of the block table names
     int rows_over, rows_most;        // only sequences of more than rows_over and at most rows_most query rows per key/value head
 };
 
@@ -119,7 +132,7 @@ cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cuda
 size_t attend_bytes(const AttendArgs& A, bool f32, int n_sms);
 size_t attend_bytes_most(int dv);
 cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* launches, cudaStream_t st);
-// What a caller that fills the structs itself leaves to be worked out: whether rows are whole, aligned pieces.
+// What a caller that fills the structs itself leaves to be worked out: whether rows are whole, aligned pieces; the positions that a block table's row names.
 void note_alignment(AppendArgs& A, bool f32);
 void note_alignment(AttendArgs& A, bool f32);
 

@@ -135,14 +135,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     __shared__ __align__(16) float turn[2][kBlock][kMaxPairs + 4];
     dep_wait();
     dep_go();
-    const int s = blockIdx.y, t0 = A.b.start[s], n = A.b.start[s + 1] - t0, pos0 = A.b.pos0[s];
-    const int block = pos0 / kBlock + blockIdx.x, p0 = block * kBlock;
-    if (n <= 0) return;
-    if (pos0 < 0 || t0 < 0 || t0 + n > A.b.T || n > A.b.max_new) {
+    const int s = blockIdx.y;
+    const Sequence Q(A.b, s, A.c.err);
+    const int t0 = Q.t0, n = Q.n, pos0 = Q.pos0, block = pos0 / kBlock + blockIdx.x;
+    if (n == 0) return;
+    if (pos0 < 0 || n > A.b.max_new) {
         if (threadIdx.x == 0) atomicExch(A.c.err, 2);
         return;
     }
-    if (p0 >= pos0 + n) return;
+    if (block > (pos0 + n - 1) / kBlock) return;      // (before there is a position: behind the last it may be no number)
+    const int p0 = block * kBlock;
     const int lo = max(pos0 - p0, 0), hi = min(pos0 + n - p0, kBlock);      // new rows of the block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % LANES, sub = lane / LANES;
     const int pg = p0 / A.c.page, page = pg < A.b.max_pages ? A.b.table[(size_t)s * A.b.max_pages + pg] : -1, in_page = p0 - pg * A.c.page;

@@ -153,11 +153,12 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     if (warp == kFewProducts) tmem_take<COLS>(&bars.tmem);
     dep_wait();
     const int s = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / A.n_splits, split = blockIdx.x % A.n_splits;
-    const int t0 = A.b.start[s], n_all = A.b.start[s + 1] - t0, n = min(n_all, A.b.max_new), pos0 = A.b.pos0[s];
+    const Sequence Q(A.b, s, A.c.err);
+    const int t0 = Q.t0, n_all = Q.n, n = min(n_all, A.b.max_new), pos0 = Q.pos0;
     const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
     const int Gq = A.H / A.c.G, row0 = tile * RA, rows = min(n * Gq - row0, RA);
-    const bool any = rows > 0 && t0 >= 0 && t0 + n_all <= A.b.T && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most;
-    const int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq;
+    const bool any = rows > 0 && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most;
+    const int first_pos = pos0 + row0 / Gq, last_pos = any ? pos0 + (row0 + rows - 1) / Gq : -1;
     Seen seen = seen_steps(A, first_pos, last_pos, kv_len);
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
     const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = min(split * share, seen.count);

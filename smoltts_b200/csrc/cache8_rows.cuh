@@ -62,11 +62,19 @@ __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_gro
 struct Seen {
     int lead, from, count, end;      // end: one behind the last visible key
 };
+// one behind the last key that a row at last_pos sees; positions behind the block table's last page are reported as a page that is not there, and not walked
+__device__ __forceinline__ int last_visible(const AttendArgs& A, int last_pos, int kv_len) {
+    const int end = max(min(kv_len, last_pos + 1), 0);
+    if (end > A.held && threadIdx.x == 0) atomicExch(A.c.err, 1);
+    return min(end, A.held);
+}
+// first position in the window of a row at pos (below 0: all)
+__device__ __forceinline__ int window_from(const AttendArgs& A, int pos) { return pos - A.window + 1; }
 __device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
     Seen x;
-    x.end = max(min(kv_len, last_pos + 1), 0);
+    x.end = last_visible(A, last_pos, kv_len);
     const int blocks = (x.end + kBlock - 1) / kBlock;
-    x.from = A.window > 0 ? min(max(first_pos - A.window + 1, 0) / kBlock, blocks) : 0;
+    x.from = A.window > 0 ? min(max(window_from(A, first_pos), 0) / kBlock, blocks) : 0;
     x.lead = A.window > 0 ? min(A.first / kBlock + (A.first % kBlock > 0), x.from) : 0;
     x.count = x.lead + blocks - x.from;
     return x;
@@ -245,9 +253,10 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     dep_wait();
     dep_go();
     const int s = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / A.n_splits, split = blockIdx.x % A.n_splits;
-    const int t0 = A.b.start[s], n_all = A.b.start[s + 1] - t0, n = min(n_all, A.b.max_new), pos0 = A.b.pos0[s];
+    const Sequence Q(A.b, s, A.c.err);
+    const int t0 = Q.t0, n = min(Q.n, A.b.max_new), pos0 = Q.pos0;
     const int Gq = A.H / A.c.G, row0 = tile * kRowTile, rows = min(n * Gq - row0, kRowTile);
-    if (rows <= 0 || t0 < 0 || t0 + n_all > A.b.T) return;
+    if (rows <= 0) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
     const int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq;
@@ -566,8 +575,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
         if (A.b.start[mid] <= t) lo = mid;
         else hi = mid;
     }
-    const int t0 = A.b.start[lo], t1 = A.b.start[lo + 1];
-    if (t < t0 || t >= t1 || t0 < 0 || t1 > A.b.T || t - t0 >= A.b.max_new || (long long)(t1 - t0) * (A.H / A.c.G) <= A.rows_over) return;
+    const Sequence Q(A.b, lo, A.c.err);
+    if (t < Q.t0 || t - Q.t0 >= min(Q.n, A.b.max_new) || (long long)Q.n * (A.H / A.c.G) <= A.rows_over) return;
     const int pieces = (A.c.dv + 3) / 4;
     const float4* stat = part_stats(A) + (size_t)unit * A.n_splits;      // maximum, denominator, e of the results
     const float4* part = reinterpret_cast<const float4*>(A.part) + (size_t)unit * A.n_splits * pieces;

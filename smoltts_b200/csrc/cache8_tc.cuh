@@ -138,9 +138,9 @@ constexpr int kStep = 128, kStepBlocks = kStep / kBlock;
 // `from` up to the last visible key.
 __device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
     Seen x;
-    x.end = max(min(kv_len, last_pos + 1), 0);
+    x.end = last_visible(A, last_pos, kv_len);
     const int steps = (x.end + kStep - 1) / kStep;
-    x.from = A.window > 0 ? min(max(first_pos - A.window + 1, 0) / kStep, steps) : 0;
+    x.from = A.window > 0 ? min(max(window_from(A, first_pos), 0) / kStep, steps) : 0;
     x.lead = A.window > 0 ? min(A.first / kStep + (A.first % kStep > 0), x.from) : 0;
     x.count = x.lead + steps - x.from;
     return x;
@@ -196,7 +196,7 @@ __device__ __forceinline__ void copy_steps(const AttendArgs& A, const CUtensorMa
     constexpr int SB = kStep * 128 * (KH + VH);
     const int lane = threadIdx.x & 31, per = box / kBlock;
     struct Entry { int page, in_page, seen; };      // in_page < 0: nobody sees the block's box; seen: the block itself
-    auto near = [&](int j, int n) { return j < seen.end && (A.window == 0 || j + n > first_pos - A.window + 1 || j < A.first); };
+    auto near = [&](int j, int n) { return j < seen.end && (A.window == 0 || j + n > window_from(A, first_pos) || j < A.first); };
     auto entry = [&](int i) {
         Entry e{-1, -1, 0};
         if (i < steps && lane < kStepBlocks) {

@@ -127,11 +127,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
     const int Gq = A.H / A.c.G, v_halves = (A.c.dv + 127) / 128, tiles = gridDim.x / (A.n_splits * v_halves);
     const int split = blockIdx.x % A.n_splits, v_col = blockIdx.x / A.n_splits % v_halves * 128, tile = tiles - 1 - blockIdx.x / (A.n_splits * v_halves);      // the tiles with the most keys first
     const int s = blockIdx.z, g = blockIdx.y;
-    const int t0 = A.b.start[s], n_all = A.b.start[s + 1] - t0, n = min(n_all, A.b.max_new), pos0 = A.b.pos0[s];
+    const Sequence Q(A.b, s, A.c.err);
+    const int t0 = Q.t0, n_all = Q.n, n = min(n_all, A.b.max_new), pos0 = Q.pos0;
     const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
     const int row0 = tile * kTileRows, rows = min(n * Gq - row0, kTileRows);
-    const bool any = rows > 0 && t0 >= 0 && t0 + n_all <= A.b.T && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most;
-    const int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq;
+    const bool any = rows > 0 && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most;
+    const int first_pos = pos0 + row0 / Gq, last_pos = any ? pos0 + (row0 + rows - 1) / Gq : -1;
     const Seen seen = seen_steps(A, first_pos, last_pos, kv_len);
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
     const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = min(split * share, seen.count);

@@ -186,3 +186,65 @@ def test_soft_caps_far_above_the_scores(dtype, n, cap, scale):
     c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
     out = c.attend(q, ints([0, n]), ints([L - n]), table, max_new=n, max_len=L, scale=scale, softcap=cap)
     check(c, table, q, L - n, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n < 9 else LEAST_TILES, scale=scale, softcap=cap)
+
+
+END = 2 ** 31 - 128      # positions are below this
+BAD = [([0, 3], [2 ** 31 - 1]), ([0, 3], [2 ** 31 - 10]), ([0, 3], [END - 2]), ([2, 0], [5]), ([-1, 2], [5]), ([2 ** 31 - 1, -2 ** 31], [5]), ([1, 4], [5]), ([-2 ** 31, 3], [5])]
+
+
+@pytest.mark.parametrize("start,pos0", BAD)
+def test_append_to_arrays_that_do_not_fit(start, pos0):
+    """Positions and rows outside their ranges, those whose sums pass 32 bits among them: reported, and nothing is written."""
+    from smoltts_b200._errors import SmolError
+
+    c, table = cache_of([40], 32, 2, 64, 64)
+    before = [x.view(torch.uint8).clone() for x in (c.k, c.v, c.k_scale, c.v_scale)]
+    k, v, q = randn(3, 2, 64, seed=1), randn(3, 2, 64, seed=2), randn(3, 4, 64, seed=3)
+    out = torch.full((3, 4, 64), 7.0, device="cuda")
+    c.append(k, v, ints(start), ints(pos0), table, max_new=3, q=q, q_out=out)
+    assert all(torch.equal(a, b.view(torch.uint8)) for a, b in zip(before, (c.k, c.v, c.k_scale, c.v_scale))) and (out == 7).all()
+    with pytest.raises(SmolError, match="do not fit"):
+        c.check_device_errors()
+
+
+def test_append_behind_the_table():
+    from smoltts_b200._errors import SmolError
+
+    c, table = cache_of([40], 32, 2, 64, 64)
+    k = randn(3, 2, 64, seed=1)
+    before = c.k.view(torch.uint8).clone()
+    c.append(k, k, ints([0, 3]), ints([END - 3]), table, max_new=3)
+    assert torch.equal(before, c.k.view(torch.uint8))
+    with pytest.raises(SmolError, match="page outside"):
+        c.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 3), (torch.bfloat16, 3), (torch.bfloat16, 40)])
+@pytest.mark.parametrize("L", [64, 3000])
+def test_attention_of_arrays_that_do_not_fit(dtype, n, L):
+    """A sequence that does not fit is left out, the other is served; positions behind the table are reported and the held ones attended to, without walking to them."""
+    from smoltts_b200._errors import SmolError
+
+    H, G, d = 4, 2, 64
+    c, table = cache_of([L, L], 32, G, d, d)
+    k, v = randn(2 * L, G, d, seed=1), randn(2 * L, G, d, seed=2)
+    c.append(k, v, ints([0, L, 2 * L]), ints([0, 0]), table, max_new=L)
+    q = randn(2 * n, H, d, seed=3).to(dtype)
+    want = c.attend(q, ints([0, n, 2 * n]), ints([L - n, L - n]), table, max_new=n, max_len=L)
+    c.check_device_errors()
+    for first, pos in ((n, 2 ** 31 - 1), (n, 2 ** 31 - 10), (n, END - n + 1), (2 * n + 5, L - n)):
+        out = torch.full((2 * n, H, d), 7.0, device="cuda", dtype=dtype)
+        c.attend(q, ints([0, n, first + n if first == n else first]), ints([L - n, pos]), table, max_new=n, max_len=L, out=out)
+        assert torch.equal(out[:n], want[:n]) and (out[n:] == 7).all()
+        with pytest.raises(SmolError, match="do not fit"):
+            c.check_device_errors()
+        c._err.zero_()
+    held = table.shape[1] * 32
+    every = c.attend(q[n:], ints([0, n]), ints([held - n]), table[1:], max_new=n, max_len=L, kv_len=ints([held - n]))
+    c.check_device_errors()
+    far = c.attend(q[n:], ints([0, n]), ints([2 ** 30]), table[1:], max_new=n, max_len=L, kv_len=ints([held - n]))
+    torch.testing.assert_close(far, every, rtol=0.0, atol=0.0, equal_nan=True)      # (behind the last held position lies what an earlier user left, NaNs too)
+    c.check_device_errors()      # (hidden: nobody asks for the pages)
+    c.attend(q[n:], ints([0, n]), ints([2 ** 30]), table[1:], max_new=n, max_len=L)
+    with pytest.raises(SmolError, match="page outside"):
+        c.check_device_errors()
