@@ -68,8 +68,8 @@ __device__ __forceinline__ int last_visible(const AttendArgs& A, int last_pos, i
     if (end > A.held && threadIdx.x == 0) atomicExch(A.c.err, 1);
     return min(end, A.held);
 }
-// first position in the window of a row at pos (below 0: all)
-__device__ __forceinline__ int window_from(const AttendArgs& A, int pos) { return pos - A.window + 1; }
+// first position in the window of a row at pos (below 0: all; a row in front of the sequence's first position sees nothing, and pos - window may be no number)
+__device__ __forceinline__ int window_from(const AttendArgs& A, int pos) { return max(pos, 0) - A.window + 1; }
 __device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
     Seen x;
     x.end = last_visible(A, last_pos, kv_len);

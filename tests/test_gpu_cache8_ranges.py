@@ -248,3 +248,15 @@ def test_attention_of_arrays_that_do_not_fit(dtype, n, L):
     c.attend(q[n:], ints([0, n]), ints([2 ** 30]), table[1:], max_new=n, max_len=L)
     with pytest.raises(SmolError, match="page outside"):
         c.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype,n", [(torch.float32, 8), (torch.bfloat16, 8), (torch.bfloat16, 40)])
+def test_the_largest_window_and_rows_in_front_of_the_first_position(dtype, n):
+    H, G, d, L = 4, 2, 64, n - 5
+    c, table = cache_of([64], 32, G, d, d)
+    k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2), randn(n, H, d, seed=3).to(dtype)
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    want = c.attend(q, ints([0, n]), ints([-5]), table, max_new=n, max_len=L)
+    assert (want[:5] == 0).all() and (want[5:] != 0).any()
+    for window in (2 ** 31 - 1, 2 ** 31 - 4):
+        assert torch.equal(c.attend(q, ints([0, n]), ints([-5]), table, max_new=n, max_len=L, window=window), want)
