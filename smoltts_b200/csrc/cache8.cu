@@ -97,15 +97,24 @@ static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new 
 
 // shares of the keys: one block of threads each
 static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
-    const long long base = (long long)A.b.S * A.c.G * row_tiles(A, f32);
+    const bool tiles = tiles_serve(A, f32);
+    const long long halves = tiles ? (A.c.dv + 127) / 128 : 1, base = (long long)A.b.S * A.c.G * row_tiles(A, f32) * halves;      // blocks of a share
     long long keys = A.b.max_len;
     if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
     // as many shares as the SMs hold blocks at once, none of less than 256 keys (a share of 128 is one step: 15.1 us against 15.7 for a token of 12 heads
     // at 2048 positions, appended and attended to, but twice the blocks; of 512 17.7).  More blocks than are held at once wait for whole others: 64
     // sequences at up to 8192 positions, 512 blocks, 145 us in one share, 181 in two; one at 131072 33 us in 111 shares, 42 in 128 and more.
-    const int held = f32 ? 2 : tiles_serve(A, f32) ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
-    const long long want = std::min((long long)held * n_sms / base, (keys + 255) / 256);
-    return (int)std::max(1ll, std::min(want, (long long)kMaxSplits));
+    const int held = f32 ? 2 : tiles ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
+    const long long slots = (long long)held * n_sms;
+    auto at_once = [&](long long blocks) { return std::max(1ll, std::min({slots / blocks, (keys + 255) / 256, (long long)kMaxSplits})); };
+    const long long want = at_once(base);
+    if (halves == 1) return (int)want;
+    // Values of more than 128 columns take two blocks a tile, and so at most half as many shares at once: often fewer SMs at work, where two rounds of shorter shares may
+    // take less time for all that they and their join cost.  In keys, with a block's own start at 512 and the join at 2048: 300 rows of 16 and 8 heads, 80 blocks, one share /
+    // three at 4000 positions 75 / 90 us, at 6000 107 / 110, at 8000 134 / 127, at 20000 316 / 247; 420 rows, 112 blocks, one / two at 8000 134 / 176, at 32000 488 / 530.
+    auto walk = [&](long long shares) { return (base * shares + slots - 1) / slots * ((keys + shares - 1) / shares + 512) + (shares > 1 ? 2048 : 0); };
+    const long long more = at_once(base / halves);
+    return (int)(walk(more) < walk(want) ? more : want);
 }
 
 // Rows of a head's codes, page by page: boxes of 128 bytes by `box` positions; bytes behind the row read as zeros.

@@ -260,3 +260,26 @@ def test_the_largest_window_and_rows_in_front_of_the_first_position(dtype, n):
     assert (want[:5] == 0).all() and (want[5:] != 0).any()
     for window in (2 ** 31 - 1, 2 ** 31 - 4):
         assert torch.equal(c.attend(q, ints([0, n]), ints([-5]), table, max_new=n, max_len=L, window=window), want)
+
+
+@pytest.mark.parametrize("n,context", [(300, 1000), (300, 12000), (420, 2000)])
+def test_two_column_halves_share_the_keys(n, context):
+    """Values of 200 columns take two blocks a tile: shares of the keys are counted for both, and few keys are not shared out beyond what the SMs hold."""
+    H, G, d, dv, L = 4, 2, 128, 200, context + n
+    c, table = cache_of([L], 64, G, d, dv, seed=3)
+    k, v, q = randn(L, G, d, seed=1), randn(L, G, dv, seed=2), randn(n, H, d, seed=3).to(torch.bfloat16)
+    c.append(k, v, ints([0, L]), ints([0]), table, max_new=L)
+    out = c.attend(q, ints([0, n]), ints([context]), table, max_new=n, max_len=L)
+    check(c, table, q, context, out, LEAST_TILES)
+
+
+def test_shares_of_two_column_halves_fit_the_device():
+    """A portion of 280 tokens of 16 and 8 heads: 40 tiles, 80 blocks with 200 columns.  Three shares of 80 would wait for one another; the keys are too few for that."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    H, G, d, L, n = 16, 8, 128, 1000, 280
+    c, table = cache_of([L], 64, G, d, 200)
+    c.append(randn(L, G, d, seed=1), randn(L, G, 200, seed=2), ints([0, L]), ints([0]), table, max_new=L)
+    c.attend(randn(n, H, d, seed=3).to(torch.bfloat16), ints([0, n]), ints([L - n]), table, max_new=n, max_len=L)
+    (need,) = c._need.values()
+    shares = need // (n * H * (200 + 4) * 4) if need else 1
+    assert shares * 80 <= sms
