@@ -246,6 +246,7 @@ static int cache_of(const SmolLmCache8* s, Cache& c, const char* me) {
     if (s->n_pages < 1 || s->page_size < kBlock || s->page_size % kBlock) return report(SMOL_ERR_INVALID, me, "page_size must be a multiple of 16, with at least one page");
     if (s->kv_heads < 1 || s->dim < 1 || s->vdim < 1) return report(SMOL_ERR_INVALID, me, "kv_heads, dim and vdim must be positive");
     if (s->dim > kMaxDim || s->vdim > kMaxDim) return report(SMOL_ERR_UNSUPPORTED, me, "head sizes above 256");
+    if ((long long)s->kv_heads * s->page_size > 0x7fffffffll) return report(SMOL_ERR_UNSUPPORTED, me, "a page of more than 2^31 - 1 rows");      // (heads times positions: coordinates of the copies)
     if (s->kv_heads > 65535) return report(SMOL_ERR_UNSUPPORTED, me, "more than 65535 key/value heads");
     c.ldk = (s->dim + 15) / 16 * 16;
     c.ldv = (s->vdim + 15) / 16 * 16;

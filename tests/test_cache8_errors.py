@@ -70,3 +70,17 @@ def test_the_command_line_says_why_a_design_cannot_have_the_cache(monkeypatch, c
     monkeypatch.setattr(registry, "load_model", refuse(SMOL_ERR_CUDA))
     with pytest.raises(SmolError):
         cli.main(argv)
+
+
+def test_pages_whose_rows_pass_32_bits_are_refused():
+    import ctypes
+
+    from smoltts_b200 import _capi_lm as cl
+
+    lib, p = cl.load(), 1 << 20
+    cache = cl.SmolLmCache8(k=p, v=p, k_scale=p, v_scale=p, n_pages=1, page_size=1 << 21, kv_heads=1024, dim=16, vdim=16, err=p)
+    batch = cl.SmolLmCache8Batch(n_tokens=1, n_seqs=1, max_pages=1, max_new=1, max_len=40, seq_start=p, seq_pos0=p, block_table=p)
+    app = cl.SmolLmCache8Append(dtype=0, k=p, v=p, k_row=128, k_head=64, v_row=96, v_head=48, rot_mult=1.0)
+    att = cl.SmolLmCache8Attend(dtype=0, heads=1024, q=p, out=p, q_row=16384, q_head=16, out_row=16384, out_head=16, scale=0.1, out_scale=1.0)
+    assert lib.smol_lm_cache8_append(ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(app), None) == -4
+    assert lib.smol_lm_cache8_attend(ctypes.byref(cache), ctypes.byref(batch), ctypes.byref(att), None, 0, None) == -4
