@@ -99,8 +99,8 @@ class HybridLM:
             raise ValueError("kv_bits must be 8 or 16")
         if kv_bits == 8 and page_size % 16:
             raise ValueError("an 8-bit cache needs a page_size that is a multiple of 16")
-        if first_tokens < 0 or (first_tokens and kv_bits != 8):
-            raise ValueError("first_tokens needs kv_bits=8 and must not be negative")
+        if not 0 <= first_tokens < 1 << 31 or (first_tokens and kv_bits != 8):
+            raise ValueError("first_tokens needs kv_bits=8 and must be neither negative nor above 2^31 - 1")
         self.kv_bits = kv_bits
         self.first_tokens = first_tokens
         self.lib = _capi_lm.load()

@@ -72,6 +72,16 @@ def test_the_command_line_says_why_a_design_cannot_have_the_cache(monkeypatch, c
         cli.main(argv)
 
 
+@pytest.mark.parametrize("first", [-1, 2 ** 31, 2 ** 32 + 4])
+def test_first_tokens_outside_32_bits_are_refused(monkeypatch, first):
+    """(ctypes would keep the low bits.)"""
+    from smoltts_b200.lm import HybridLM
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    with pytest.raises(ValueError, match="first_tokens"):
+        HybridLM(None, kv_bits=8, first_tokens=first)
+
+
 def test_pages_whose_rows_pass_32_bits_are_refused():
     import ctypes
 
