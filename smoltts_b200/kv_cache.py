@@ -30,6 +30,14 @@ for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCa
     assert _s.size == C.sizeof(_m)
 
 
+def _pack(layout: struct.Struct, *fields) -> bytes:
+    """The fields in their native types; a number that its type does not hold is the caller's."""
+    try:
+        return layout.pack(*fields)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"a number outside its range (32-bit integers and floats): {e}") from e
+
+
 def _padded(n: int) -> int:
     return (n + 15) // 16 * 16
 
@@ -129,8 +137,8 @@ class KVCache8:
         n, pages = block_table.shape
         if tokens < 1 or n < 1 or pages < 1 or max_new < 1 or max_len < 1:
             raise ValueError("a batch needs at least one row, sequence and page, max_new and max_len at least 1")
-        return _BATCH.pack(tokens, n, pages, max_new, max_len, self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"),
-                           self._ints(block_table, (n, pages), "block_table"), 0 if kv_len is None else self._ints(kv_len, (n,), "kv_len"))
+        return _pack(_BATCH, tokens, n, pages, max_new, max_len, self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"),
+                     self._ints(block_table, (n, pages), "block_table"), 0 if kv_len is None else self._ints(kv_len, (n,), "kv_len"))
 
     def _call(self, call, *args) -> None:
         """On the cache's device and its current stream."""
@@ -180,8 +188,8 @@ class KVCache8:
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
-        self._call(self._append, batch, _APPEND.pack(_DTYPES[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, heads, q_ptr, out_ptr, q_row, q_head,
-                                                     out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, rot_mult))
+        self._call(self._append, batch, _pack(_APPEND, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, heads, q_ptr, out_ptr, q_row, q_head,
+                                              out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, rot_mult))
         return q_out
 
     def attend(self, q: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, max_new: int, max_len: int,
@@ -215,8 +223,8 @@ class KVCache8:
         r1 = r2 = 0
         if penalty is not None:
             r1, r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
-        a = _ATTEND.pack(_DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else scale, softcap, 1.0,
-                         window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0)
+        a = _pack(_ATTEND, _DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else scale, softcap, 1.0,
+                  window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0)
         key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first)
         need = self._need.get(key)
         if need is None:

@@ -283,3 +283,14 @@ def test_shares_of_two_column_halves_fit_the_device():
     (need,) = c._need.values()
     shares = need // (n * H * (200 + 4) * 4) if need else 1
     assert shares * 80 <= sms
+
+
+def test_numbers_that_their_types_do_not_hold_are_refused():
+    c, table = cache_of([64], 32, 2, 64, 64)
+    q, k, start, pos0 = randn(1, 4, 64), randn(1, 2, 64), ints([0, 1]), ints([63])
+    for bad in (dict(window=2 ** 31), dict(first=2 ** 40), dict(max_len=2 ** 31), dict(max_new=2 ** 31), dict(scale=1e39), dict(softcap=1e39), dict(window=3.5)):
+        with pytest.raises(ValueError, match="range"):
+            c.attend(q, start, pos0, table, **{"max_new": 1, "max_len": 64, **bad})
+    for bad in (dict(max_new=2 ** 31), dict(rot_mult=1e39, freq=torch.ones(4, device="cuda"))):
+        with pytest.raises(ValueError, match="range"):
+            c.append(k, k, start, pos0, table, **{"max_new": 1, **bad})
