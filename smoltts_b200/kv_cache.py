@@ -31,11 +31,17 @@ for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCa
 
 
 def _pack(layout: struct.Struct, *fields) -> bytes:
-    """The fields in their native types; a number that its type does not hold is the caller's."""
+    """The fields in their native types; an integer that its type does not hold is the caller's."""
     try:
         return layout.pack(*fields)
-    except (struct.error, OverflowError) as e:
-        raise ValueError(f"a number outside its range (32-bit integers and floats): {e}") from e
+    except struct.error as e:
+        raise ValueError(f"an integer outside its range: {e}") from e
+
+
+def _float(x: float, what: str) -> float:
+    if not abs(x) <= 3.4028234663852886e38:      # (packing would make an infinity of it)
+        raise ValueError(f"{what} {x} is outside the range of float32")
+    return x
 
 
 def _padded(n: int) -> int:
@@ -189,7 +195,7 @@ class KVCache8:
         elif q_out is not None:
             raise ValueError("q_out without q")
         self._call(self._append, batch, _pack(_APPEND, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, heads, q_ptr, out_ptr, q_row, q_head,
-                                              out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, rot_mult))
+                                              out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, _float(rot_mult, "rot_mult")))
         return q_out
 
     def attend(self, q: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, max_new: int, max_len: int,
@@ -223,7 +229,7 @@ class KVCache8:
         r1 = r2 = 0
         if penalty is not None:
             r1, r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
-        a = _pack(_ATTEND, _DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else scale, softcap, 1.0,
+        a = _pack(_ATTEND, _DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else _float(scale, "scale"), _float(softcap, "softcap"), 1.0,
                   window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0)
         key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first)
         need = self._need.get(key)
