@@ -151,7 +151,7 @@ static cudaError_t attend_few(const AttendArgs& A, cudaStream_t st) { return std
 template <int D, bool BENT>
 static cudaError_t rows_as(const AttendArgs& A, cudaStream_t st) {
     static std::atomic<uint64_t> asked{0};
-    constexpr int bytes = row_smem(D, D, 2);
+    constexpr int bytes = row_smem(D, D);
     if (cudaError_t e = more_smem(attend_rows_kernel<D, D, BENT>, bytes, asked)) return e;
     return launch(attend_rows_kernel<D, D, BENT>, dim3(row_tiles(A, true) * A.n_splits, A.c.G, A.b.S), kRowThreads, bytes, st, A);
 }

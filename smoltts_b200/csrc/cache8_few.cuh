@@ -32,9 +32,9 @@ namespace c8 {
 
 constexpr int kFewThreads = 192, kFewCopies = 4, kFewProducts = 5;      // warps of the copies and of the products
 __host__ __device__ constexpr int few_rows(int RA) { return RA < 8 ? 8 : RA; }      // the instruction has at least 16 columns: two parts of eight rows
-__host__ __device__ constexpr int few_stages(int D) { return 2; }
+constexpr int kFewStages = 2;
 __host__ __device__ constexpr int few_stage_bytes(int D) { return kStep * 2 * D; }
-__host__ __device__ constexpr int few_smem(int D, int RA) { return 1024 + 2 * few_rows(RA) * (D + 2 * 128) + few_stages(D) * few_stage_bytes(D); }
+__host__ __device__ constexpr int few_smem(int D, int RA) { return 1024 + 2 * few_rows(RA) * (D + 2 * 128) + kFewStages * few_stage_bytes(D); }
 __host__ __device__ constexpr int few_tmem(int D, int NR) { return 2 * NR * (2 + 2 * (D / 128)) <= 64 ? 64 : 2 * NR * (2 + 2 * (D / 128)) <= 128 ? 128 : 256; }
 
 // blocks an SM holds: by shared memory (stages of 32 KB or 64) and registers.  Three of four rows instead of two: 64 sequences at up to 8192 positions 145 us, 161
@@ -75,7 +75,7 @@ struct Apart {
 };
 
 struct FewBars {
-    uint64_t full[3], empty[3];      // stages
+    uint64_t full[kFewStages], empty[kFewStages];      // stages
     uint64_t s_full[2], s_empty[2];  // scores in tensor memory
     uint64_t p_full[2], o_full[2];   // weights in shared memory; their product in tensor memory
     uint64_t q_full, drained;
@@ -123,7 +123,7 @@ constexpr int kMostCluster = 8;      // shares of the keys that are joined insid
 // D: head sizes padded (both); RA: query rows
 template <int D, int RA, bool BENT>
 __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
-    constexpr int NR = few_rows(RA), NS = few_stages(D), SB = few_stage_bytes(D), N = 2 * NR, HALVES = D / 128, COLS = few_tmem(D, NR);
+    constexpr int NR = few_rows(RA), NS = kFewStages, SB = few_stage_bytes(D), N = 2 * NR, HALVES = D / 128, COLS = few_tmem(D, NR);
     extern __shared__ unsigned char smem_raw[];
     __shared__ FewBars bars;
     __shared__ StepScales s_scales[NS];
@@ -336,6 +336,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
                     l[r] = fmaf(l_step[r], f.add_l, l[r] * f.keep_l);
                     m[r] = fmaxf(m[r], m_step[r]);
                 }
+                __syncwarp();
             }
 #pragma unroll
             for (int x = 0; x < HALVES; ++x) {

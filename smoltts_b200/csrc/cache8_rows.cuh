@@ -30,11 +30,12 @@ constexpr int kRowWarps = 4, kRowTile = 16, kRowThreads = kRowWarps * 32;
 
 __host__ __device__ constexpr int row_stage_bytes(int DK, int DV) { return kBlock * (DK + DV); }
 __host__ __device__ constexpr int row_stages(int DK, int DV) { return DK + DV <= 256 ? 4 : 3; }
-__host__ __device__ constexpr bool q_in_smem(int DK, int PARTS) { return DK * PARTS > 128; }
-__host__ __device__ constexpr int row_q_bytes(int DK, int PARTS) { return q_in_smem(DK, PARTS) ? DK / 16 * PARTS * 512 : 0; }
+constexpr int kParts = 2;      // f16 parts of a query and of a weight
+__host__ __device__ constexpr bool q_in_smem(int DK) { return DK * kParts > 128; }
+__host__ __device__ constexpr int row_q_bytes(int DK) { return q_in_smem(DK) ? DK / 16 * kParts * 512 : 0; }
 __host__ __device__ constexpr int row_join_bytes(int DV) { return kRowWarps * kRowTile * (DV + 4) * 4; }
-__host__ __device__ constexpr int row_smem(int DK, int DV, int PARTS) {
-    const int ring = kRowWarps * row_stages(DK, DV) * row_stage_bytes(DK, DV) + row_q_bytes(DK, PARTS), join = row_join_bytes(DV);
+__host__ __device__ constexpr int row_smem(int DK, int DV) {
+    const int ring = kRowWarps * row_stages(DK, DV) * row_stage_bytes(DK, DV) + row_q_bytes(DK), join = row_join_bytes(DV);
     return ring > join ? ring : join;
 }
 
@@ -149,8 +150,9 @@ struct Finish {
     __device__ __forceinline__ Finish(const AttendArgs& A, int h, float top, float total, float e) {
         const float sink = A.sink ? A.sink[h] * kLog2e : -INFINITY, M = fmaxf(sink, top);
         const float all = fmaf(total, top == -INFINITY ? 1.0f : exp2_fast(top - M), M == -INFINITY ? 0.0f : exp2_fast(sink - M));
-        a = top == -INFINITY ? 1.0f : exp2_fast(0.5f * (e + (top - M)));
-        b = all == 0.0f ? 1.0f : a / all;
+        const float x = top == -INFINITY ? 0.0f : e + (top - M), half = floorf(0.5f * x);      // (whole numbers stay whole: their powers are exact)
+        a = exp2_fast(half);
+        b = all == 0.0f ? 1.0f : exp2_fast(x - half) / all;
     }
 };
 __device__ __forceinline__ float with_sink(const AttendArgs& A, int h, float top, float total, float e, float v) {
@@ -243,11 +245,11 @@ __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, fl
     }
 }
 
-// PARTS: f16 parts of a query and of a weight; DK, DV: head sizes padded; BENT: soft cap or distance penalties
+// DK, DV: head sizes padded; BENT: soft cap or distance penalties
 template <int DK, int DV, bool BENT>
 __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs A) {
-    constexpr int PARTS = 2, KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
-    constexpr bool QS = q_in_smem(DK, PARTS);
+    constexpr int KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
+    constexpr bool QS = q_in_smem(DK);
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Join<kRowTile> J;
     dep_wait();
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
 
     // ---- queries: fragments of rows r and r + 8, scaled so that the largest magnitude lies in [2^14, 2^15) ----
     float rowmul[2];
-    uint32_t qa[QS ? 1 : KS][QS ? 1 : PARTS][4];
+    uint32_t qa[QS ? 1 : KS][QS ? 1 : kParts][4];
     uint4* qs = reinterpret_cast<uint4*>(smem + kRowWarps * NS * SB);
     {
         const float* q[2];
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             up[x] = pow2(14 - e);
             rowmul[x] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 14) * (A.scale * kCodeUnit * (BENT ? 1.0f : kLog2e));
         }
-        auto fragment = [&](int k, uint32_t (&part)[PARTS][4]) {
+        auto fragment = [&](int k, uint32_t (&part)[kParts][4]) {
             // step k: word k % 4 of the lane's piece c + 4 (k / 4); its bytes 1 and 3, then 0 and 2
             const int at = ((k / 4) * 4 + c) * 16 + (k % 4) * 4;
 #pragma unroll
@@ -368,10 +370,10 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         };
         if constexpr (QS) {
             for (int k = warp; k < KS; k += kRowWarps) {
-                uint32_t part[PARTS][4];
+                uint32_t part[kParts][4];
                 fragment(k, part);
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) qs[(k * PARTS + p) * 32 + lane] = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
+                for (int p = 0; p < kParts; ++p) qs[(k * kParts + p) * 32 + lane] = make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
             }
         } else {
 #pragma unroll
@@ -420,11 +422,11 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int x = 0; x < 2; ++x) w[x] = *reinterpret_cast<const uint4*>(st + (x * KP + y) * 512 + lane * 16);
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
-                uint32_t a[PARTS][4];
+                uint32_t a[kParts][4];
 #pragma unroll
-                for (int p = 0; p < PARTS; ++p) {
+                for (int p = 0; p < kParts; ++p) {
                     if constexpr (QS) {
-                        const uint4 u = qs[((y * 4 + z) * PARTS + p) * 32 + lane];
+                        const uint4 u = qs[((y * 4 + z) * kParts + p) * 32 + lane];
                         a[p][0] = u.x; a[p][1] = u.y; a[p][2] = u.z; a[p][3] = u.w;
                     } else {
 #pragma unroll
@@ -436,7 +438,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
                     const uint32_t word = z == 0 ? w[x].x : z == 1 ? w[x].y : z == 2 ? w[x].z : w[x].w;
                     const uint32_t b0 = odd_codes(word), b1 = even_codes(word);
 #pragma unroll
-                    for (int p = 0; p < PARTS; ++p) mma_f16_16816(sc[x], a[p][0], a[p][1], a[p][2], a[p][3], b0, b1);
+                    for (int p = 0; p < kParts; ++p) mma_f16_16816(sc[x], a[p][0], a[p][1], a[p][2], a[p][3], b0, b1);
                 }
             }
         }
@@ -475,7 +477,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
                 }
             }
         }
-        uint32_t pa[PARTS][4];
+        uint32_t pa[kParts][4];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const bool none = m[x] == -INFINITY;
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
                 const uint32_t b01 = __byte_perm(w[2][z], w[3][z], 0x4501), b23 = __byte_perm(w[2][z], w[3][z], 0x6723);
                 const int t = (y + z) * 4;
 #pragma unroll
-                for (int pp = 0; pp < PARTS; ++pp) {
+                for (int pp = 0; pp < kParts; ++pp) {
                     mma_f16_16816(o[t], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], odd_codes(a01), odd_codes(b01));
                     mma_f16_16816(o[t + 1], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], even_codes(a01), even_codes(b01));
                     mma_f16_16816(o[t + 2], pa[pp][0], pa[pp][1], pa[pp][2], pa[pp][3], odd_codes(a23), odd_codes(b23));
