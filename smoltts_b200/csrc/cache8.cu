@@ -78,9 +78,9 @@ cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cuda
 }
 
 // Query rows of a sequence and key/value head up to which the kernel for few rows takes them: it reads the keys once per 16 rows and shares them out finely, the
-// tiles pay for 128 rows whatever they hold.  Both measured, few rows / tiles, 8 heads of 128: 16 sequences at 4096 positions with 16 rows 51 / 69 us,
-// 24 rows 82 / 69, 32 rows 81 / 69; 64 at 2048 92 / 160, 187 / 162, 180 / 162; one at 32768 27 / 42, 44 / 44, 45 / 45.  Where all of it is too little
-// to fill the GPU the keys' shares are what counts: one at 2048 with 32 rows 15.9 / 18.1, with 64 17.0 / 22.3, with 96 32 / 25.
+// tiles pay for 128 rows whatever they hold.  Both measured, few rows / tiles, 8 heads of 128: 16 sequences at 4096 positions with 16 rows 54 / 72 us,
+// 24 rows 86 / 74, 32 rows 88 / 74; 64 at 2048 84 / 140, 164 / 141, 161 / 143; one at 32768 30 / 43, 49 / 44, 50 / 44.  Where all of it is too little
+// to fill the GPU the keys' shares are what counts: one at 2048 with 32 rows 16.6 / 16.6, with 64 18.1 / 19.6, with 96 33 / 21.
 constexpr int kFewMost = 16, kFewMostSmall = 64;
 constexpr long long kSmall = 1 << 16;      // sequences times heads times positions (16384: the last of these; 262144: the one at 32768)
 bool tiles_serve(const AttendArgs& A, bool f32) {
@@ -101,9 +101,9 @@ static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     const long long halves = tiles ? (A.c.dv + 127) / 128 : 1, base = (long long)A.b.S * A.c.G * row_tiles(A, f32) * halves;      // blocks of a share
     long long keys = A.b.max_len;
     if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
-    // as many shares as the SMs hold blocks at once, none of less than 256 keys (a share of 128 is one step: 15.1 us against 15.7 for a token of 12 heads
-    // at 2048 positions, appended and attended to, but twice the blocks; of 512 17.7).  More blocks than are held at once wait for whole others: 64
-    // sequences at up to 8192 positions, 512 blocks, 145 us in one share, 181 in two; one at 131072 33 us in 111 shares, 42 in 128 and more.
+    // as many shares as the SMs hold blocks at once, none of less than 256 keys (a token of 12 heads at 2048 positions, appended and
+    // attended to: 10.9 us; with shares of 128, which are one step, 11.5; of 512 12.7).  More blocks than are held at once wait for whole others: one sequence at
+    // 131072 34 us in 111 shares, 43 in 128.
     const int held = f32 ? 2 : tiles ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
     const long long slots = (long long)held * n_sms;
     auto at_once = [&](long long blocks) { return std::max(1ll, std::min({slots / blocks, (keys + 255) / 256, (long long)kMaxSplits})); };

@@ -19,8 +19,8 @@
 // some row does not see, and in blocks that hold a NaN, the value codes are cleaned of them in shared memory; at the end nan_columns finds the
 // results that see one.
 //
-// What bounds it: the bytes of the cache.  64 sequences at up to 8192 positions, 32 and 8 heads of 128: 142 us, 5.7 TB/s; one of 12 and 4 heads at 131072
-// 33 us, 4.1 TB/s; 32 behind windows of 1024 18 us, and 2048 positions of 12 and 4 heads of 64 7 us, which are launch, page lookups and the join.  On the registers' way (mma.sync, e4m3 operands made f16 by the compiler's expansion) 32 positions took 965
+// What bounds it: the bytes of the cache.  64 sequences at up to 8192 positions, 32 and 8 heads of 128: 147 us, 5.5 TB/s; one of 12 and 4 heads at 131072
+// 34 us, 3.9 TB/s; 32 behind windows of 1024 19 us, and 2048 positions of 12 and 4 heads of 64 8 us, which are launch, page lookups and the join.  On the registers' way (mma.sync, e4m3 operands made f16 by the compiler's expansion) 32 positions took 965
 // instructions of a warp and 64 sequences at up to 8192 positions 227 us.
 #pragma once
 
@@ -37,14 +37,14 @@ __host__ __device__ constexpr int few_stage_bytes(int D) { return kStep * 2 * D;
 __host__ __device__ constexpr int few_smem(int D, int RA) { return 1024 + 2 * few_rows(RA) * (D + 2 * 128) + kFewStages * few_stage_bytes(D); }
 __host__ __device__ constexpr int few_tmem(int D, int NR) { return 2 * NR * (2 + 2 * (D / 128)) <= 64 ? 64 : 2 * NR * (2 + 2 * (D / 128)) <= 128 ? 128 : 256; }
 
-// blocks an SM holds: by shared memory (stages of 32 KB or 64) and registers.  Three of four rows instead of two: 64 sequences at up to 8192 positions 145 us, 161
+// blocks an SM holds: by shared memory (stages of 32 KB or 64) and registers.  Three of four rows instead of two: 64 sequences at up to 8192 positions 147 us, 160
 __host__ __device__ constexpr int few_blocks(int D, int RA) { return D > 128 ? 1 : RA <= 4 ? 3 : 2; }
 
 // What weights and results are relative to.  While the logarithms of all value scales lie within kNear of the first block's (`unit`): weights are relative to the
 // row's largest score + log2(scale) =: m, results are in units of 2^m, and the denominator's terms, in units of 2^(m - unit), are the weights' times
 // 2^(unit - log2(scale)): one exponential and one maximum a score.  (A weight below fp32's range counts for less than 2^-62 there.)  From the first step on that has a
 // scale further away, whoever sees it, the same with an exponential and a maximum each for weights and denominator, and a unit per row: rare, and behind calls, so
-// that the ordinary loop stays as short as it is (with all of it in the loop 64 sequences at up to 8192 positions took 150 us, 142 without).
+// that the ordinary loop stays as short as it is (64 sequences at up to 8192 positions: 147 us, 158 with all of it in the loop, 143 without any).
 constexpr float kNear = 32.0f;      // in units of log2
 
 // the warp's largest score, and largest score - it + log2(scale)

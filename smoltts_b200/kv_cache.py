@@ -4,7 +4,8 @@ attends to them.
 
 Half the bytes of a bf16 cache: twice the positions in the same pool, and half the traffic of decoding.  Pages are the
 indices of a ``pool.PagePool``; a batch is ragged, as in an engine step: sequence ``s`` brings the rows ``seq_start[s] ..
-seq_start[s + 1] - 1``, which are its positions ``seq_pos0[s], seq_pos0[s] + 1, ...``.  Everything runs on the current stream
+seq_start[s + 1] - 1``, which are its positions ``seq_pos0[s], seq_pos0[s] + 1, ...`` (below 2^31 - 128).  The arrays are looked at on the device: a sequence
+whose rows or positions do not fit is left out, a page outside the cache not touched, and ``check_device_errors`` tells.  Everything runs on the current stream
 of the cache's device and nothing synchronises, so that calls can be captured into a CUDA graph; results carry no gradient.  ``lm.HybridLM`` serves
 its softmax attention layers from such a cache with ``kv_bits=8``.
 """
