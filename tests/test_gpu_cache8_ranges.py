@@ -65,7 +65,7 @@ KERNELS = [(torch.bfloat16, 1, LEAST_FEW), (torch.bfloat16, 7, LEAST_FEW), (torc
 
 
 @pytest.mark.parametrize("dtype,n,least", KERNELS)
-@pytest.mark.parametrize("power", [6, 12, 18, 30, 60, 100])
+@pytest.mark.parametrize("power", [12, 30, 100])
 @pytest.mark.parametrize("where", ["later", "behind_the_window", "behind_kv_len", "little_weight", "infinity", "between"])
 def test_a_row_depends_on_what_it_sees_alone(dtype, n, least, power, where):
     """Values 2^power larger at positions that some or all rows do not see, or that weigh next to nothing (a score 40 lower, 2^-58)."""
@@ -174,12 +174,11 @@ def test_a_sink_far_above_the_scores():
             check(c, table, q, L - n, out, LEAST_F32 if dtype == torch.float32 else LEAST_FEW if n == 1 else LEAST_TILES, sink=sink)
 
 
-@pytest.mark.parametrize("n", [1, 7, 150])
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("cap", [300.0, 1e3, 1e4, 1e6, 1e8, 1e9, 1e20, 3.4e38])
-@pytest.mark.parametrize("scale", [0.125, 3.0, 60.0])
+@pytest.mark.parametrize("dtype,n", [(torch.bfloat16, 1), (torch.bfloat16, 150), (torch.float32, 150)])
+@pytest.mark.parametrize("cap", [300.0, 1e4, 1e6, 1e9, 3.4e38])
+@pytest.mark.parametrize("scale", [0.125, 60.0])
 def test_soft_caps_far_above_the_scores(dtype, n, cap, scale):
-    """Scores of up to 10, 250 and 5000 under caps from below them to fp32's end: what a cap adds to a score's error is 2^-20 of the score, an eighth of what its size is given."""
+    """Scores of up to 10 and 5000 under caps from below them to fp32's end: what a cap adds to a score's error is 2^-20 of the score, an eighth of what its size is given."""
     H, G, d, L = 4, 2, 64, 400
     c, table = cache_of([L], 32, G, d, d, seed=5)
     k, v, q = randn(L, G, d, seed=1), randn(L, G, d, seed=2), randn(n, H, d, seed=3).to(dtype)
