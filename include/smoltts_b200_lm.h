@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define SMOL_LM_ABI_VERSION 7
+#define SMOL_LM_ABI_VERSION 8
 
 enum { SMOL_LM_BF16 = 0, SMOL_LM_F32 = 1 };
 /* token mixers */
@@ -298,7 +298,7 @@ typedef struct SmolLm SmolLm;
 
 int smol_lm_abi_version(void);
 size_t smol_lm_struct_bytes(int which);          /* sizeof of SmolLmLayer (0), SmolLmConfig (1), SmolLmGlobals (2), SmolLmStep (3), SmolLmCache8 (4), SmolLmCache8Batch (5),
-                                                    SmolLmCache8Append (6), SmolLmCache8Attend (7): a binding checks its mirror */
+                                                    SmolLmCache8Append (6), SmolLmCache8Attend (7), SmolLmCache8Keep (8): a binding checks its mirror */
 const char* smol_lm_last_error(void);
 
 /* layers / run_layer are HOST arrays, copied.  run_layer[n] = index of the layer that run n executes. */
@@ -362,11 +362,19 @@ typedef struct SmolLmCache8Append {
     int32_t rot_dims, rot_half;
     const float* freq;           /* device [rot_dims / 2] */
     float rot_mult;
+    const int32_t* positions;    /* device [n_axes][n_tokens]: the rows' rotary positions, one per axis (NULL: where the rows lie, seq_pos0 + ...) */
+    const int32_t* axis;         /* device [rot_dims / 2]: the axis of every pair, 0 .. n_axes - 1 (NULL: the first).  Another one is reported (2), and the first is taken */
+    int32_t n_axes;              /* 0 without positions */
 } SmolLmCache8Append;
 
 /* Softmax attention of the rows over the cache.  A row at position i sees the keys j <= i with window == 0 or i - j < window or j < first;
  * s = scale q.k, bent to softcap tanh(s / softcap) where softcap > 0, less dist_r1 ln(1 + dist_r2 (i - j)), less dist_slope (i - j); the sink logit
- * joins the denominator.  A row that sees no key gives zeros.  The result times out_scale, and times sigmoid(gate). */
+ * joins the denominator.  A row that sees no key gives zeros.  The result times out_scale, and times sigmoid(gate).
+ *
+ * With tree_positions and tree_sees the rows are those of a tree (smol_lm_cache8_tree makes both from parents; any others will do): row t stands at position
+ * tree_positions[t], from 0 to 2^31 - 129 (others count as the nearest), and sees every key in front of its sequence's rows, whose position is its place, and of the sequence's rows
+ * those that its bits name: bit i % 32 of word i / 32 of tree_sees[t] is row i.  Rows behind the last bit are seen by nobody.  A window hides keys whose
+ * position is `window` or more in front of the row's own and not below `first`; distances below 0 count as 0. */
 typedef struct SmolLmCache8Attend {
     int32_t dtype;               /* of queries and results */
     int32_t heads;               /* a multiple of kv_heads */
@@ -378,12 +386,34 @@ typedef struct SmolLmCache8Attend {
     const float *sink, *dist_slope, *dist_r1, *dist_r2;     /* device [heads], each NULL: none */
     const float* gate;           /* device, row t at gate + t * gate_row: [heads * vdim] (NULL: none) */
     size_t gate_row;
+    const int32_t* tree_positions;      /* device [n_tokens] (NULL: no tree) */
+    const uint32_t* tree_sees;          /* device [n_tokens][tree_words] */
+    int32_t tree_words;
 } SmolLmCache8Attend;
+
+/* Rows that stay: rows[s][0] < rows[s][1] < ... < rows[s][counts[s] - 1] of sequence s, counted from position seq_pos0[s]. */
+typedef struct SmolLmCache8Keep {
+    int32_t n_seqs, max_pages, max_keep;
+    const int32_t *seq_pos0, *block_table;      /* device: [n_seqs], [n_seqs][max_pages] */
+    const int32_t *rows, *counts;               /* device: [n_seqs][max_keep], [n_seqs] */
+} SmolLmCache8Keep;
 
 int smol_lm_cache8_append(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Append* a, void* stream);
 /* bytes of workspace the call below needs on the current device (often 0) */
 int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, size_t* bytes);
 int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A tree of rows, from every row's parent among the rows of its sequence (-1: the row follows what the sequence holds already; a parent comes in front of its
+ * children): positions[t] = seq_pos0 + the row's depth, and the bits sees[t][words] of the row itself and of those on its way up.  Rows outside every sequence are left alone; a
+ * sequence of more than max_new (at most 4096) rows is left out and reported, a parent that cannot be one counts as -1 and is reported (err: 2). */
+int smol_lm_cache8_tree(int32_t n_tokens, int32_t n_seqs, int32_t max_new, const int32_t* seq_start, const int32_t* seq_pos0, const int32_t* parents, int32_t* positions,
+                        uint32_t* sees, int32_t words, int32_t* err, void* stream);
+/* The rows that stay move together, in every one of `caches` (HOST array, all of one shape, none twice): row rows[s][i] becomes the row at position seq_pos0[s] + i, as if its
+ * values, as the cache holds them, were appended there; what lies behind the last of them is as it was, or as it was with another scale.  A sequence whose arrays do not fit is left
+ * as it is and reported in the caches' err (1: a page outside the cache, 2: rows not in order). */
+int smol_lm_cache8_keep(const SmolLmCache8* caches, int32_t n_caches, const SmolLmCache8Keep* a, void* stream);
+/* Pages src[i] into pages dst[i], codes and scales, in every one of `caches`.  src and dst are HOST arrays, copied by the call: no page may be written twice, nor read and written. */
+int smol_lm_cache8_copy_pages(const SmolLmCache8* caches, int32_t n_caches, const int32_t* src, const int32_t* dst, int32_t n_pairs, void* stream);
 
 int64_t smol_lm_launch_count(const SmolLm* m);
 int32_t* smol_lm_error_word(SmolLm* m);           /* device word, nonzero after a step that addressed outside its pools (1: a page, 2: a slot) or

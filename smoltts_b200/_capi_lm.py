@@ -11,7 +11,7 @@ import os
 from . import build as _build
 from ._errors import SMOL_OK, SmolError
 
-SMOL_LM_ABI_VERSION = 7
+SMOL_LM_ABI_VERSION = 8
 SMOL_LM_BF16, SMOL_LM_F32 = 0, 1
 
 
@@ -76,14 +76,18 @@ class SmolLmCache8Batch(C.Structure):
 class SmolLmCache8Append(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_size_t) for n in ("k_row", "k_head", "v_row", "v_head")] + [
         ("heads", C.c_int32), ("q", C.c_void_p), ("q_out", C.c_void_p)] + [(n, C.c_size_t) for n in ("q_row", "q_head", "q_out_row", "q_out_head")] + [
-        ("rot_dims", C.c_int32), ("rot_half", C.c_int32), ("freq", C.c_void_p), ("rot_mult", C.c_float)]
+        ("rot_dims", C.c_int32), ("rot_half", C.c_int32), ("freq", C.c_void_p), ("rot_mult", C.c_float), ("positions", C.c_void_p), ("axis", C.c_void_p), ("n_axes", C.c_int32)]
 
 
 class SmolLmCache8Attend(C.Structure):
     _fields_ = [("dtype", C.c_int32), ("heads", C.c_int32), ("q", C.c_void_p), ("out", C.c_void_p)] + [
         (n, C.c_size_t) for n in ("q_row", "q_head", "out_row", "out_head")] + [(n, C.c_float) for n in ("scale", "softcap", "out_scale")] + [
         ("window", C.c_int32), ("first", C.c_int32)] + [(n, C.c_void_p) for n in ("sink", "dist_slope", "dist_r1", "dist_r2", "gate")] + [
-        ("gate_row", C.c_size_t)]
+        ("gate_row", C.c_size_t), ("tree_positions", C.c_void_p), ("tree_sees", C.c_void_p), ("tree_words", C.c_int32)]
+
+
+class SmolLmCache8Keep(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "max_pages", "max_keep")] + [(n, C.c_void_p) for n in ("seq_pos0", "block_table", "rows", "counts")]
 
 
 PROTOTYPES = {
@@ -105,6 +109,9 @@ PROTOTYPES = {
                                                  C.POINTER(C.c_size_t)]),
     "smol_lm_cache8_attend": (C.c_int, [C.POINTER(SmolLmCache8), C.POINTER(SmolLmCache8Batch), C.POINTER(SmolLmCache8Attend), C.c_void_p,
                                         C.c_size_t, C.c_void_p]),
+    "smol_lm_cache8_tree": (C.c_int, [C.c_int32, C.c_int32, C.c_int32] + [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_void_p]),
+    "smol_lm_cache8_keep": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(SmolLmCache8Keep), C.c_void_p]),
+    "smol_lm_cache8_copy_pages": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
     "smol_lm_launch_count": (C.c_int64, [C.c_void_p]),
     "smol_lm_error_word": (C.c_void_p, [C.c_void_p]),
 }
@@ -129,7 +136,7 @@ def load() -> C.CDLL:
         fn.argtypes = args
     if lib.smol_lm_abi_version() != SMOL_LM_ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {lib.smol_lm_abi_version()} != {SMOL_LM_ABI_VERSION}")
-    for which, mirror in enumerate((SmolLmLayer, SmolLmConfig, SmolLmGlobals, SmolLmStep, SmolLmCache8, SmolLmCache8Batch, SmolLmCache8Append, SmolLmCache8Attend)):
+    for which, mirror in enumerate((SmolLmLayer, SmolLmConfig, SmolLmGlobals, SmolLmStep, SmolLmCache8, SmolLmCache8Batch, SmolLmCache8Append, SmolLmCache8Attend, SmolLmCache8Keep)):
         if lib.smol_lm_struct_bytes(which) != C.sizeof(mirror):
             raise RuntimeError(f"{path}: {mirror.__name__} is {lib.smol_lm_struct_bytes(which)} bytes in the library, {C.sizeof(mirror)} in the binding")
     _lib = lib

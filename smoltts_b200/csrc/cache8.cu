@@ -1,16 +1,12 @@
 // The 8-bit key/value cache: launches and the C entries of include/smoltts_b200_lm.h.
 #include <algorithm>
 #include <atomic>
-#include <utility>
 
 #include "../../include/smoltts_b200_lm.h"
 #include "cache8.cuh"
 #include "cache8_append.cuh"
-#include "cache8_few.cuh"
-#include "cache8_tiles.cuh"
-#include "cache8_rows.cuh"
+#include "cache8_launch.cuh"
 #include "lm_report.h"
-#include "tmap_host.h"
 
 #define SMOL_OK 0
 #define SMOL_ERR_INVALID (-1)
@@ -22,41 +18,6 @@ namespace smol {
 namespace c8 {
 
 using lm::report;
-
-// Every kernel here begins with the wait for the kernel in front of it, so all of them may be set up early.
-template <class... P, class... X>
-static cudaError_t launch_cluster(int cluster, void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, X&&... args) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = cluster;
-    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(std::forward<X>(args))...);
-}
-template <class... P, class... X>
-static cudaError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, X&&... args) {
-    return launch_cluster(1, kernel, grid, block, smem, st, std::forward<X>(args)...);
-}
-
-// Shared memory above 48 KB, a few of which are static, is asked for once per kernel and device.
-template <class K>
-static cudaError_t more_smem(K kernel, int bytes, std::atomic<uint64_t>& asked) {
-    if (bytes <= 40 * 1024) return cudaSuccess;
-    int dev = 0;
-    if (cudaError_t e = cudaGetDevice(&dev)) return e;
-    if (dev < 64 && (asked.load() >> dev & 1)) return cudaSuccess;
-    if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
-    if (dev < 64) asked.fetch_or(1ull << dev);
-    return cudaSuccess;
-}
 
 template <class T, int PASSES>
 static cudaError_t append_of(const AppendArgs& A, dim3 grid, cudaStream_t st) {
@@ -76,24 +37,6 @@ cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cuda
     *launches += 1;
     return f32 ? append_as<float>(A, n_sms, st) : append_as<bf16>(A, n_sms, st);
 }
-
-// Query rows of a sequence and key/value head up to which the kernel for few rows takes them: it reads the keys once per 16 rows and shares them out finely, the
-// tiles pay for 128 rows whatever they hold.  Both measured, few rows / tiles, 8 heads of 128: 16 sequences at 4096 positions with 16 rows 54 / 72 us,
-// 24 rows 86 / 74, 32 rows 88 / 74; 64 at 2048 84 / 140, 164 / 141, 161 / 143; one at 32768 30 / 43, 49 / 44, 50 / 44.  Where all of it is too little
-// to fill the GPU the keys' shares are what counts: one at 2048 with 32 rows 16.6 / 16.6, with 64 18.1 / 19.6, with 96 33 / 21.
-constexpr int kFewMost = 16, kFewMostSmall = 64;
-constexpr long long kSmall = 1 << 16;      // sequences times heads times positions (16384: the last of these; 262144: the one at 32768)
-bool tiles_serve(const AttendArgs& A, bool f32) {
-    const long long rows = A.b.max_new * (long long)(A.H / A.c.G), most = (long long)A.b.S * A.c.G * A.b.max_len <= kSmall ? kFewMostSmall : kFewMost;
-    return !f32 && rows > most;
-}
-
-// query rows of a block of threads
-static int row_tile(const AttendArgs& A, bool f32) {
-    const long long rows = A.b.max_new * (long long)(A.H / A.c.G);
-    return f32 ? kRowTile : rows <= 4 ? 4 : rows <= 8 ? 8 : tiles_serve(A, f32) ? kTileRows : 16;
-}
-static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new * (long long)(A.H / A.c.G) + row_tile(A, f32) - 1) / row_tile(A, f32)); }
 
 // shares of the keys: one block of threads each
 static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
@@ -117,66 +60,6 @@ static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     return (int)(walk(more) < walk(want) ? more : want);
 }
 
-// Rows of a head's codes, page by page: boxes of 128 bytes by `box` positions; bytes behind the row read as zeros.
-static bool codes_map(CUtensorMap* map, const uint8_t* base, int ld, size_t page_bytes, const Cache& c, int box) {
-    TensorMapEncodeTiledFn encode = tensor_map_encoder();
-    if (!encode) return false;
-    const cuuint64_t dims[3] = {(cuuint64_t)ld, (cuuint64_t)c.G * c.page, (cuuint64_t)c.n_pages}, strides[2] = {(cuuint64_t)ld, (cuuint64_t)page_bytes};
-    const cuuint32_t boxes[3] = {128u, (cuuint32_t)box, 1u}, ones[3] = {1u, 1u, 1u};
-    return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(base), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-// positions that lie together and begin at a multiple of themselves: the largest power of two that divides the page, at most a step's
-static int box_of(const Cache& c) { return std::min(c.page & -c.page, kStep); }
-
-static bool joins_in_cluster(const AttendArgs& A, int splits, bool f32) { return !f32 && !tiles_serve(A, f32) && splits > 1 && splits <= kMostCluster; }
-
-template <int D, int RA, bool BENT>
-static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
-    static std::atomic<uint64_t> asked{0};
-    constexpr int bytes = few_smem(D, RA);
-    if (cudaError_t e = more_smem(attend_few_kernel<D, RA, BENT>, bytes, asked)) return e;
-    CUtensorMap kmap, vmap;
-    const int box = box_of(A.c);
-    if (!codes_map(&kmap, A.c.k, A.c.ldk, A.c.k_page, A.c, box) || !codes_map(&vmap, A.c.v, A.c.ldv, A.c.v_page, A.c, box)) return cudaErrorInvalidValue;
-    return launch_cluster(joins_in_cluster(A, A.n_splits, false) ? A.n_splits : 1, attend_few_kernel<D, RA, BENT>, dim3(row_tiles(A, false) * A.n_splits, A.c.G, A.b.S), kFewThreads, bytes, st, A, kmap,
-                          vmap, box);
-}
-template <int D, int RA>
-static cudaError_t few_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? few_as<D, RA, false>(A, st) : few_as<D, RA, true>(A, st); }
-template <int D>
-static cudaError_t few_rows(const AttendArgs& A, cudaStream_t st) { return row_tile(A, false) == 4 ? few_of<D, 4>(A, st) : row_tile(A, false) == 8 ? few_of<D, 8>(A, st) : few_of<D, 16>(A, st); }
-static cudaError_t attend_few(const AttendArgs& A, cudaStream_t st) { return std::max(A.c.d, A.c.dv) <= 128 ? few_rows<128>(A, st) : few_rows<256>(A, st); }
-
-template <int D, bool BENT>
-static cudaError_t rows_as(const AttendArgs& A, cudaStream_t st) {
-    static std::atomic<uint64_t> asked{0};
-    constexpr int bytes = row_smem(D, D);
-    if (cudaError_t e = more_smem(attend_rows_kernel<D, D, BENT>, bytes, asked)) return e;
-    return launch(attend_rows_kernel<D, D, BENT>, dim3(row_tiles(A, true) * A.n_splits, A.c.G, A.b.S), kRowThreads, bytes, st, A);
-}
-template <int D>
-static cudaError_t rows_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? rows_as<D, false>(A, st) : rows_as<D, true>(A, st); }
-static cudaError_t attend_rows(const AttendArgs& A, cudaStream_t st) {
-    const int d = std::max(A.c.d, A.c.dv);
-    return d <= 64 ? rows_of<64>(A, st) : d <= 128 ? rows_of<128>(A, st) : rows_of<256>(A, st);
-}
-
-template <int DK, bool BENT>
-static cudaError_t tiles_as(const AttendArgs& A, cudaStream_t st) {
-    static std::atomic<uint64_t> asked{0};
-    constexpr int bytes = tile_smem(DK);
-    if (cudaError_t e = more_smem(attend_tiles_kernel<DK, BENT>, bytes, asked)) return e;
-    CUtensorMap kmap, vmap;
-    const int box = box_of(A.c);
-    if (!codes_map(&kmap, A.c.k, A.c.ldk, A.c.k_page, A.c, box) || !codes_map(&vmap, A.c.v, A.c.ldv, A.c.v_page, A.c, box)) return cudaErrorInvalidValue;
-    return launch(attend_tiles_kernel<DK, BENT>, dim3(row_tiles(A, false) * ((A.c.dv + 127) / 128) * A.n_splits, A.c.G, A.b.S), kTileThreads, bytes, st, A, kmap, vmap, box);
-}
-static cudaError_t attend_tiles(const AttendArgs& A, cudaStream_t st) {
-    if (A.c.d <= 128) return plain_scores(A) ? tiles_as<128, false>(A, st) : tiles_as<128, true>(A, st);
-    return plain_scores(A) ? tiles_as<256, false>(A, st) : tiles_as<256, true>(A, st);
-}
-
 // A batch whose sequences may bring anything from one row to many: those of few rows go to the kernel for few rows, which shares their keys out.  With short
 // contexts (a tile walks 2048 positions in 35 us), one sequence, or as many rows as if all brought max_new, that is not worth a launch (8 us of 77 where it finds
 // nothing to do: 16 sequences of 6 rows at 4096 positions).
@@ -197,7 +80,9 @@ cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* laun
     if (two) A.rows_over = kFewMost;
     A.n_splits = splits_for(A, f32, n_sms);
     A.part = static_cast<float*>(workspace);
-    if (cudaError_t e = f32 ? attend_rows(A, st) : tiles_serve(A, f32) ? attend_tiles(A, st) : attend_few(A, st)) return e;
+    if (cudaError_t e = A.tree_pos ? (f32 ? attend_tree_rows(A, st) : tiles_serve(A, f32) ? attend_tree_tiles(A, st) : attend_tree_few(A, st))
+                                   : (f32 ? attend_rows<false>(A, st) : tiles_serve(A, f32) ? attend_tiles<false>(A, st) : attend_few<false>(A, st)))
+        return e;
     *launches += 1;
     if (A.n_splits > 1 && !joins_in_cluster(A, A.n_splits, f32)) {
         *launches += 1;
@@ -209,7 +94,7 @@ cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* laun
     few.n_splits = std::min(splits_for(few, f32, n_sms), kMostCluster);      // (joined without the workspace, which the tiles' shares may be in)
     few.part = nullptr;
     *launches += 1;
-    return attend_few(few, st);
+    return A.tree_pos ? attend_tree_few(few, st) : attend_few<false>(few, st);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -241,7 +126,7 @@ void note_alignment(AttendArgs& A, bool f32) {
     A.held = (int)std::min<long long>((long long)A.b.max_pages * A.c.page, kPositions);
 }
 
-static int cache_of(const SmolLmCache8* s, Cache& c, const char* me) {
+int cache_of(const SmolLmCache8* s, Cache& c, const char* me) {
     if (!s->k || !s->v || !s->k_scale || !s->v_scale || !s->err) return report(SMOL_ERR_INVALID, me, "null pointer in the cache");
     if (s->n_pages < 1 || s->page_size < kBlock || s->page_size % kBlock) return report(SMOL_ERR_INVALID, me, "page_size must be a multiple of 16, with at least one page");
     if (s->kv_heads < 1 || s->dim < 1 || s->vdim < 1) return report(SMOL_ERR_INVALID, me, "kv_heads, dim and vdim must be positive");
@@ -288,6 +173,9 @@ static int attend_of(const SmolLmCache8* c, const SmolLmCache8Batch* b, const Sm
     A.sink = a->sink; A.slope = a->dist_slope; A.r1 = a->dist_r1; A.r2 = a->dist_r2; A.gate = a->gate; A.gate_row = a->gate_row; A.out_scale = a->out_scale;
     A.part = nullptr; A.n_splits = 1;
     A.rows_over = 0; A.rows_most = 0x7fffffff;
+    A.tree_pos = a->tree_positions; A.tree_sees = a->tree_sees; A.tree_words = a->tree_words;
+    if (!A.tree_pos != !A.tree_sees) return report(SMOL_ERR_INVALID, me, "tree_positions and tree_sees come together");
+    if (A.tree_pos && A.tree_words < 1) return report(SMOL_ERR_INVALID, me, "a tree needs words of bits");
     note_alignment(A, f32);
     return SMOL_OK;
 }
@@ -312,6 +200,8 @@ extern "C" int smol_lm_cache8_append(const SmolLmCache8* cache, const SmolLmCach
     A.k_row = a->k_row; A.k_head = a->k_head; A.v_row = a->v_row; A.v_head = a->v_head;
     A.q_row = a->q_row; A.q_head = a->q_head; A.o_row = a->q_out_row; A.o_head = a->q_out_head;
     A.H = a->q ? a->heads : 0; A.freq = a->freq; A.pairs = a->rot_dims / 2; A.half = a->rot_half; A.mult = a->rot_mult;
+    if (a->n_axes < 0 || (a->positions ? a->n_axes < 1 : a->n_axes > 0 || a->axis)) return report(SMOL_ERR_INVALID, me, "positions come with the number of their axes, and axes with positions");
+    A.places = a->positions; A.axis = a->axis; A.n_axes = a->n_axes;
     note_alignment(A, f32);
     int n_sms = 0, launches = 0;
     if (int rc = n_sms_of_device(&n_sms)) return rc;

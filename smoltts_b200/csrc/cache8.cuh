@@ -14,6 +14,8 @@
 
 #include "common.cuh"
 
+struct SmolLmCache8;
+
 namespace smol {
 namespace c8 {
 
@@ -61,6 +63,8 @@ struct AppendArgs {
     const float* freq;
     int pairs, half;
     float mult;
+    const int32_t *places, *axis;    // rotary positions [n_axes][T] (nullptr: where the rows lie in the cache); the axis of every pair (nullptr: the first)
+    int n_axes;
     int k_vec, v_vec, q_vec;         // rows are whole groups of eight elements, on 16-byte boundaries
 };
 
@@ -81,6 +85,9 @@ struct AttendArgs {
     int q_vec, o_vec;                // rows are whole groups of four elements that a load takes (1), of eight on 16-byte boundaries (2)
     int held;                        // positions that a row of the block table names
     int rows_over, rows_most;        // only sequences of more than rows_over and at most rows_most query rows per key/value head
+    const int32_t* tree_pos;         // rows of a tree: their positions [T] (nullptr: no tree, a row's position is its place in the cache) ...
+    const uint32_t* tree_sees;       // ... and which of their sequence's rows they see [T][tree_words], a bit each
+    int tree_words;
 };
 
 constexpr int kMaxSplits = 128;
@@ -132,9 +139,16 @@ cudaError_t append(const AppendArgs& A, bool f32, int n_sms, int* launches, cuda
 size_t attend_bytes(const AttendArgs& A, bool f32, int n_sms);
 size_t attend_bytes_most(int dv);
 cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* launches, cudaStream_t st);
+// The kernels for rows of a tree (cache8_drafts.cu).
+cudaError_t attend_tree_few(const AttendArgs& A, cudaStream_t st);
+cudaError_t attend_tree_tiles(const AttendArgs& A, cudaStream_t st);
+cudaError_t attend_tree_rows(const AttendArgs& A, cudaStream_t st);
 // What a caller that fills the structs itself leaves to be worked out: whether rows are whole, aligned pieces; the positions that a block table's row names.
 void note_alignment(AppendArgs& A, bool f32);
 void note_alignment(AttendArgs& A, bool f32);
+
+// The cache of a C entry's argument, checked; SMOL_OK or the error it has reported for `me`.
+int cache_of(const SmolLmCache8* s, Cache& c, const char* me);
 
 constexpr float kLog2e = 1.4426950408889634f;
 

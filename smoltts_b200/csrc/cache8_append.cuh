@@ -150,7 +150,16 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendArgs
     const int pg = p0 / A.c.page, page = pg < A.b.max_pages ? A.b.table[(size_t)s * A.b.max_pages + pg] : -1, in_page = p0 - pg * A.c.page;
     for (int i = threadIdx.x; i < (hi - lo) * A.pairs; i += kAppendThreads) {
         const int r = lo + i / A.pairs, j = i % A.pairs;
-        const double half_turns = (double)(p0 + r) * (double)A.freq[j] * 0.3183098861837906715;      // the angle over pi
+        int place = p0 + r;
+        if (A.places) {
+            int a = A.axis ? A.axis[j] : 0;
+            if (a < 0 || a >= A.n_axes) {
+                atomicExch(A.c.err, 2);
+                a = 0;
+            }
+            place = A.places[(size_t)a * A.b.T + (t0 + p0 + r - pos0)];
+        }
+        const double half_turns = (double)place * (double)A.freq[j] * 0.3183098861837906715;      // the angle over pi
         const double at = half_turns - 2.0 * rint(0.5 * half_turns);
         const float near = (float)at, rest = (float)((at - (double)near) * 3.141592653589793);      // (a rounding of the angle of up to 2^-25 pi is twice that of the cosine)
         float sn, cs;

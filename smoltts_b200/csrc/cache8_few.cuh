@@ -48,12 +48,12 @@ __host__ __device__ constexpr int few_blocks(int D, int RA) { return D > 128 ? 1
 constexpr float kNear = 32.0f;      // in units of log2
 
 // the warp's largest score, and largest score - it + log2(scale)
-__device__ __noinline__ float2 apart_maxima(float s, float lv) {
+static __device__ __noinline__ float2 apart_maxima(float s, float lv) {
     const float t = warp_top(s);
     return make_float2(t, warp_top(s - (t == -INFINITY ? 0.0f : t) + lv));
 }
 // (weight, the denominator's term, the row's largest score, what the weight is relative to on top of it), from the four warps' maxima
-__device__ __noinline__ float4 apart_weight(float s, float lv, const float* tops, const float* fars, int ld) {
+static __device__ __noinline__ float4 apart_weight(float s, float lv, const float* tops, const float* fars, int ld) {
     float top = -INFINITY, e = -INFINITY;
     for (int w = 0; w < 4; ++w) top = fmaxf(top, tops[w * ld]);
     if (top == -INFINITY) return make_float4(exp2_fast(s), exp2_fast(s), top, 0.0f);      // (0, or NaN)
@@ -84,7 +84,7 @@ struct FewBars {
 };
 
 // Rows (a bit each) that see a NaN in column col of the values: blocks whose scale is negative hold them.  Rare, and slow.
-template <int ROWS>
+template <int ROWS, bool TREE>
 __device__ uint32_t nan_columns(const AttendArgs& A, const Rows& W, int col) {
     uint32_t rows = 0;
     for (int b = 0; b * kBlock < W.end; ++b) {
@@ -96,8 +96,10 @@ __device__ uint32_t nan_columns(const AttendArgs& A, const Rows& W, int col) {
         for (int i = 0; i < kBlock; ++i) {
             const uint8_t code = A.c.v[(size_t)page * A.c.v_page + ((size_t)W.g * A.c.page + in_page + i) * A.c.ldv + col];
             if ((code & 0x7f) != 0x7f) continue;
-            for (int r = 0; r < min(W.rows, ROWS); ++r)
-                if (sees(A, W.pos0 + (W.row0 + r) / W.Gq, b * kBlock + i, W.end)) rows |= 1u << r;
+            for (int r = 0; r < min(W.rows, ROWS); ++r) {
+                const int t = (W.row0 + r) / W.Gq;
+                if (TREE ? tree_sees(A, W.t0, W.pos0, W.t0 + t, tree_position(A, W.t0 + t), b * kBlock + i, W.end) : sees(A, W.pos0 + t, b * kBlock + i, W.end)) rows |= 1u << r;
+            }
         }
     }
     return rows;
@@ -120,8 +122,8 @@ __device__ __forceinline__ float of_rank(const float* mine, int rank) {      // 
 }
 constexpr int kMostCluster = 8;      // shares of the keys that are joined inside a cluster of blocks; more go through memory and attend_join_kernel
 
-// D: head sizes padded (both); RA: query rows
-template <int D, int RA, bool BENT>
+// D: head sizes padded (both); RA: query rows; BENT: soft cap or distance penalties; TREE: rows of a tree
+template <int D, int RA, bool BENT, bool TREE>
 __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
     constexpr int NR = few_rows(RA), NS = kFewStages, SB = few_stage_bytes(D), N = 2 * NR, HALVES = D / 128, COLS = few_tmem(D, NR);
     extern __shared__ unsigned char smem_raw[];
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     __shared__ float4 s_stat[RA];      // of this block's share: maximum, denominator, e
     __shared__ float s_far[2][4][RA], s_step_unit[2][RA], s_unit[2][RA];      // (value scales far apart)
     __shared__ int s_apart[2];      // some thread has met one: in even and odd steps, so that the next step's is written while this one's is read
-    __shared__ int s_pos[RA], s_head[RA], s_bad;
+    __shared__ int s_pos[RA], s_row[RA], s_head[RA], s_bad;      // positions; the step's rows; heads
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     unsigned char *KV = base, *Qs = KV + NS * SB, *Ps = Qs + N * D;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -157,9 +159,13 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     const int t0 = Q.t0, n_all = Q.n, n = min(n_all, A.b.max_new), pos0 = Q.pos0;
     const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
     const int Gq = A.H / A.c.G, row0 = tile * RA, rows = min(n * Gq - row0, RA);
-    const bool any = rows > 0 && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most;
-    const int first_pos = pos0 + row0 / Gq, last_pos = any ? pos0 + (row0 + rows - 1) / Gq : -1;
-    Seen seen = seen_steps(A, first_pos, last_pos, kv_len);
+    const bool any = rows > 0 && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most && (!TREE || tree_fits(A, pos0, n_all));
+    int first_pos = pos0 + row0 / Gq, last_pos = any ? pos0 + (row0 + rows - 1) / Gq : -1, behind = last_pos + 1, clear = first_pos + 1;      // clear: every row sees what is in front of it, but for the window
+    if (TREE && any) {
+        const TreeSpan span(A, t0 + row0 / Gq, (row0 + rows - 1) / Gq - row0 / Gq + 1, n_all, pos0);
+        first_pos = span.first_pos; last_pos = span.last_pos; behind = span.behind; clear = pos0;
+    }
+    const Seen seen = seen_steps(A, first_pos, behind, kv_len);
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
     const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = min(split * share, seen.count);
     const int steps = any ? min(lo + share, seen.count) - lo : 0;
@@ -167,7 +173,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     float* joint = reinterpret_cast<float*>(KV);      // [row][D], once everything has been multiplied
     // a finished row's column, and a column of this block's share of the keys: maximum, denominator, unnormalised result in units of 2^(top + e)
     auto store = [&](int r, int col, float top, float total, float e, float v) {
-        const int tok = t0 + s_pos[r] - pos0, h = s_head[r];
+        const int tok = s_row[r], h = s_head[r];
         Elem<bf16>::put(static_cast<bf16*>(A.out) + (size_t)tok * A.o_row + (size_t)h * A.o_head + col, finished(A, tok, h, col, with_sink(A, h, top, total, e, v)));
     };
     auto put = [&](int r, int col, float top, float total, float e, float v) {
@@ -177,7 +183,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             if (col == 0) s_stat[r] = make_float4(top, total, e, 0.0f);
             joint[r * D + col] = v;
         } else {
-            const size_t at = ((size_t)(t0 + s_pos[r] - pos0) * A.H + s_head[r]) * A.n_splits + split;
+            const size_t at = ((size_t)s_row[r] * A.H + s_head[r]) * A.n_splits + split;
             if (col == 0) part_stats(A)[at] = make_float4(top, total, e, 0.0f);
             A.part[at * ((A.c.dv + 3) / 4 * 4) + col] = v;
         }
@@ -273,7 +279,8 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             if (lane == 0) {
                 // (a row that is not finite: every score of it is a NaN)
                 s_rowmul[r] = top >= 0x7f800000u ? __int_as_float(0x7fffffff) : pow2(e - 7) * (A.scale * (BENT ? 1.0f : kLog2e));
-                s_pos[r] = pos0 + row / Gq;
+                s_row[r] = t0 + row / Gq;
+                s_pos[r] = TREE ? tree_position(A, t0 + row / Gq) : pos0 + row / Gq;
                 s_head[r] = h;
                 if (BENT) {
                     s_r1[r] = A.r1 ? A.r1[h] : 0.0f;
@@ -351,6 +358,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         };
         for (int i = 0; i < steps; ++i) {
             const int b = i & 1, st = i % NS, j0 = step_place(seen, lo, i), j = j0 + me;
+            const int key = TREE && j >= pos0 && j < seen.end && (BENT || A.window > 0) ? tree_position(A, t0 + j - pos0) : j;      // the key's position
             // (a wait that has run out is not waited for again: the steps that are left go by, and nothing is written)
             wait_bar(&bars.full[st], (i / NS) & 1, stop, A.c.err);
             const float2 scales = s_scales[st].of[me / kBlock];
@@ -371,16 +379,17 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             umma::fence_before_sync();
             arrive(&bars.s_empty[b]);
             if (BENT) {
-                bend(A, S, [&](int r) { return (float)(s_pos[r] - j); }, [&](int r) { return s_r1[r]; }, [&](int r) { return s_r2[r]; }, [&](int r) { return s_slope[r]; });
+                bend(A, S, [&](int r) { return TREE ? fmaxf((float)(s_pos[r] - key), 0.0f) : (float)(s_pos[r] - j); }, [&](int r) { return s_r1[r]; }, [&](int r) { return s_r2[r]; }, [&](int r) { return s_slope[r]; });
 #pragma unroll
                 for (int r = 0; r < RA; ++r) S[r] += lv;
             }
-            const bool whole = j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
+            const bool whole = j0 + kStep <= min(clear, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             bool hidden = ks == 0.0f;      // from some row
             if (!whole || hidden) {
 #pragma unroll
                 for (int r = 0; r < RA; ++r) {
-                    const bool on = ks != 0.0f && sees(A, s_pos[r], j, seen.end);
+                    bool on = ks != 0.0f && (TREE ? j < seen.end && (A.window == 0 || s_pos[r] - key < A.window || key < A.first) : sees(A, s_pos[r], j, seen.end));
+                    if (TREE && on && j >= pos0) on = A.tree_sees[(size_t)s_row[r] * A.tree_words + ((j - pos0) >> 5)] >> ((j - pos0) & 31) & 1u;
                     hidden |= !on;
                     S[r] = on ? S[r] : -INFINITY;
                 }
@@ -478,7 +487,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         for (int x = 0; x < HALVES; ++x) {
             const int col = x * 128 + me;
             if (col >= A.c.dv || *stop) continue;
-            const uint32_t nans = s_bad ? nan_columns<RA>(A, W, col) : 0u;
+            const uint32_t nans = s_bad ? nan_columns<RA, TREE>(A, W, col) : 0u;
 #pragma unroll
             for (int r = 0; r < RA; ++r) {
                 if (r >= rows) break;
@@ -490,7 +499,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         for (int r = warp; r < RA; r += 4) {
             const int row = min(row0 + r, n * Gq - 1);
             if (lane == 0) {
-                s_pos[r] = pos0 + row / Gq;
+                s_row[r] = t0 + row / Gq;
                 s_head[r] = g * Gq + row % Gq;
             }
         }

@@ -58,22 +58,22 @@ __device__ __forceinline__ void copy8(uint32_t to, const void* from, bool in) {
 template <int N> __device__ __forceinline__ void copies_left() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
-// The blocks of 16 positions that rows at positions first_pos .. last_pos see: `lead` of them from the sequence's start (the first tokens, in
+// The blocks of 16 positions that rows at positions from first_pos on see, which see no key from `behind` on: `lead` of them from the sequence's start (the first tokens, in
 // front of the window), then those from `from` up to the last visible key.
 struct Seen {
     int lead, from, count, end;      // end: one behind the last visible key
 };
-// one behind the last key that a row at last_pos sees; positions behind the block table's last page are reported as a page that is not there, and not walked
-__device__ __forceinline__ int last_visible(const AttendArgs& A, int last_pos, int kv_len) {
-    const int end = max(min(kv_len, last_pos + 1), 0);
+// one behind the last key that rows see which see no key from `behind` on; positions behind the block table's last page are reported as a page that is not there, and not walked
+__device__ __forceinline__ int last_visible(const AttendArgs& A, int behind, int kv_len) {
+    const int end = max(min(kv_len, behind), 0);
     if (end > A.held && threadIdx.x == 0) atomicExch(A.c.err, 1);
     return min(end, A.held);
 }
 // first position in the window of a row at pos (below 0: all; a row in front of the sequence's first position sees nothing, and pos - window may be no number)
 __device__ __forceinline__ int window_from(const AttendArgs& A, int pos) { return max(pos, 0) - A.window + 1; }
-__device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
+__device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, int behind, int kv_len) {
     Seen x;
-    x.end = last_visible(A, last_pos, kv_len);
+    x.end = last_visible(A, behind, kv_len);
     const int blocks = (x.end + kBlock - 1) / kBlock;
     x.from = A.window > 0 ? min(max(window_from(A, first_pos), 0) / kBlock, blocks) : 0;
     x.lead = A.window > 0 ? min(A.first / kBlock + (A.first % kBlock > 0), x.from) : 0;
@@ -82,6 +82,48 @@ __device__ __forceinline__ Seen seen_blocks(const AttendArgs& A, int first_pos, 
 }
 __device__ __forceinline__ bool sees(const AttendArgs& A, int pos, int j, int end) {
     return j <= pos && j < end && (A.window == 0 || pos - j < A.window || j < A.first);
+}
+
+// ---- rows of a tree.  What lies in the cache in front of the sequence's rows is the context, which all of them see; of the rows themselves a row sees those that its bits
+// name.  Distances (window, penalties) are between positions, which are the rows' own (a key's of the context is its place); one below zero counts as zero. ----
+__device__ __forceinline__ int tree_position(const AttendArgs& A, int tok) { return min(max(A.tree_pos[tok], 0), kPositions - 1); }
+// smallest and largest position of rows tok .. tok + n - 1; by a whole warp
+__device__ __forceinline__ int2 tree_span(const AttendArgs& A, int tok, int n) {
+    int lo = kPositions, hi = 0;
+    for (int i = threadIdx.x & 31; i < n; i += 32) {
+        const int p = tree_position(A, tok + i);
+        lo = min(lo, p);
+        hi = max(hi, p);
+    }
+    return make_int2(__reduce_min_sync(0xffffffffu, lo), __reduce_max_sync(0xffffffffu, hi));
+}
+// What a block of threads with rows tok .. + n - 1 of a sequence of n_all rows behind pos0 sees: every place up to `behind`, from where the window of a row at `first_pos` begins
+// (no later than the rows themselves, whose positions may be anywhere); `last_pos` is the largest position.  All of it within `whole`.
+struct TreeSpan {
+    int first_pos, last_pos, behind;
+    __device__ __forceinline__ TreeSpan(const AttendArgs& A, int tok, int n, int n_all, int pos0) : first_pos(pos0), last_pos(pos0) {
+        behind = pos0 + (int)min((long long)n_all, 32ll * A.tree_words);
+        if (A.window == 0) return;
+        const int2 span = tree_span(A, tok, n);
+        first_pos = (int)min((long long)span.x, (long long)pos0 + A.window - 1);
+        last_pos = span.y;
+    }
+};
+// position of the key at place j, below `behind`
+__device__ __forceinline__ int tree_key(const AttendArgs& A, int t0, int pos0, int j) { return j < pos0 ? j : tree_position(A, t0 + j - pos0); }
+__device__ __forceinline__ bool tree_sees(const AttendArgs& A, int t0, int pos0, int tok, int pos, int j, int end) {
+    if (j >= end) return false;
+    const int i = j - pos0;
+    if (i >= 0 && (A.tree_sees[(size_t)tok * A.tree_words + (i >> 5)] >> (i & 31) & 1u) == 0u) return false;
+    if (A.window == 0) return true;
+    const int key = tree_key(A, t0, pos0, j);
+    return pos - key < A.window || key < A.first;
+}
+// Sequences of a tree lie behind a context of no fewer than zero positions.
+__device__ __forceinline__ bool tree_fits(const AttendArgs& A, int pos0, int n) {
+    if (pos0 >= 0) return true;
+    if (n > 0 && threadIdx.x == 0) atomicExch(A.c.err, 2);
+    return false;
 }
 
 // What follows the scaled product, in units of log2: soft cap and distance penalties, with the library's functions (float32).
@@ -162,10 +204,10 @@ __device__ __forceinline__ float with_sink(const AttendArgs& A, int h, float top
 
 // Blocks of scale sign < 0 hold NaN codes, which the products took for 480: a row that sees one of them becomes NaN, all of it where a key holds
 // one, the value's column otherwise (mark(row, column)).  Rare, and slow.
-template <class Mark>
-__device__ void mark_nans(const AttendArgs& A, int s, int g, int row0, int rows, int pos0, int Gq, int kv_len, Mark mark) {
+template <bool TREE, class Mark>
+__device__ void mark_nans(const AttendArgs& A, int s, int g, int t0, int row0, int rows, int pos0, int Gq, int kv_len, Mark mark) {
     for (int r = 0; r < rows; ++r) {
-        const int pos = pos0 + (row0 + r) / Gq, end = min(kv_len, pos + 1);
+        const int tok = t0 + (row0 + r) / Gq, pos = TREE ? tree_position(A, tok) : pos0 + (row0 + r) / Gq, end = TREE ? kv_len : min(kv_len, pos + 1);
         for (int b = 0; b * kBlock < end; ++b) {
             const int pg = b * kBlock / A.c.page;
             const int page = pg < A.b.max_pages ? A.b.table[(size_t)s * A.b.max_pages + pg] : -1;
@@ -174,7 +216,7 @@ __device__ void mark_nans(const AttendArgs& A, int s, int g, int row0, int rows,
             const bool kbad = A.c.ks[(size_t)page * A.c.ks_page + at] < 0.0f, vbad = A.c.vs[(size_t)page * A.c.vs_page + at] < 0.0f;
             if (!kbad && !vbad) continue;
             for (int i = 0; i < kBlock; ++i) {
-                if (!sees(A, pos, b * kBlock + i, kv_len)) continue;
+                if (TREE ? !tree_sees(A, t0, pos0, tok, pos, b * kBlock + i, kv_len) : !sees(A, pos, b * kBlock + i, kv_len)) continue;
                 const size_t row = (size_t)g * A.c.page + in_page + i;
                 const uint8_t *k = A.c.k + (size_t)page * A.c.k_page + row * A.c.ldk, *v = A.c.v + (size_t)page * A.c.v_page + row * A.c.ldv;
                 if (kbad)
@@ -201,7 +243,7 @@ struct Join {
 __host__ __device__ constexpr int join_ld(int DV) { return DV + 4; }
 
 // The four warps' maxima, sums and unnormalised results join[(warp * ROWS + row) * LD + column], joined and finished, or written as this share's part.
-template <int ROWS, int LD>
+template <int ROWS, int LD, bool TREE>
 __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, float* join, const Rows& W, int split) {
     if (threadIdx.x < ROWS) {
         const int row = threadIdx.x;
@@ -227,7 +269,7 @@ __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, fl
     }
     __syncthreads();
     if (J.bad) {
-        mark_nans(A, W.s, W.g, W.row0, W.rows, W.pos0, W.Gq, min(W.kv_len, W.end), [&](int row, int col) { join[row * LD + col] = __int_as_float(0x7fffffff); });      // (times whatever weight: NaN)
+        mark_nans<TREE>(A, W.s, W.g, W.t0, W.row0, W.rows, W.pos0, W.Gq, min(W.kv_len, W.end), [&](int row, int col) { join[row * LD + col] = __int_as_float(0x7fffffff); });      // (times whatever weight: NaN)
         __syncthreads();
     }
     for (int i = threadIdx.x; i < W.rows * A.c.dv; i += kRowThreads) {
@@ -245,8 +287,8 @@ __device__ __forceinline__ void join_rows(const AttendArgs& A, Join<ROWS>& J, fl
     }
 }
 
-// DK, DV: head sizes padded; BENT: soft cap or distance penalties
-template <int DK, int DV, bool BENT>
+// DK, DV: head sizes padded; BENT: soft cap or distance penalties; TREE: rows of a tree
+template <int DK, int DV, bool BENT, bool TREE>
 __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendArgs A) {
     constexpr int KP = DK / 64, VB = DV / 8, NS = row_stages(DK, DV), SB = row_stage_bytes(DK, DV), KS = DK / 16;
     constexpr bool QS = q_in_smem(DK);
@@ -258,11 +300,15 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     const Sequence Q(A.b, s, A.c.err);
     const int t0 = Q.t0, n = min(Q.n, A.b.max_new), pos0 = Q.pos0;
     const int Gq = A.H / A.c.G, row0 = tile * kRowTile, rows = min(n * Gq - row0, kRowTile);
-    if (rows <= 0) return;
+    if (rows <= 0 || (TREE && !tree_fits(A, pos0, n))) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
-    const int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq;
-    const Seen seen = seen_blocks(A, first_pos, last_pos, kv_len);
+    int first_pos = pos0 + row0 / Gq, last_pos = pos0 + (row0 + rows - 1) / Gq, behind = last_pos + 1, clear = first_pos + 1;      // clear: every row sees what is in front of it, but for the window
+    if (TREE) {
+        const TreeSpan span(A, t0 + row0 / Gq, (row0 + rows - 1) / Gq - row0 / Gq + 1, Q.n, pos0);
+        first_pos = span.first_pos; last_pos = span.last_pos; behind = span.behind; clear = pos0;
+    }
+    const Seen seen = seen_blocks(A, first_pos, behind, kv_len);
     const int share = (seen.count + A.n_splits - 1) / A.n_splits, b_lo = min(split * share, seen.count), b_hi = min(b_lo + share, seen.count);
     const int mine = b_hi - b_lo > warp ? (b_hi - b_lo - warp + kRowWarps - 1) / kRowWarps : 0;      // blocks of this warp: b_lo + warp, + 4, ...
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
@@ -387,7 +433,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int row = min(row0 + r + 8 * x, n * Gq - 1), h = g * Gq + row % Gq;
-        pos[x] = pos0 + row / Gq;
+        pos[x] = TREE ? tree_position(A, t0 + row / Gq) : pos0 + row / Gq;
         r1[x] = BENT && A.r1 ? A.r1[h] : 0.0f;
         r2[x] = BENT && A.r1 ? A.r2[h] : 0.0f;
         slope[x] = BENT && A.slope ? A.slope[h] : 0.0f;
@@ -445,7 +491,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         // ---- running softmax, in units of log2; a lane has positions 2c, 2c + 1, 2c + 8, 2c + 9 of rows r and r + 8 ----
         const int j0 = block_of(i) * kBlock + 2 * c;
         const float km = fabsf(ks);
-        const bool whole = j0 - 2 * c + kBlock <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 - 2 * c > last_pos - A.window || j0 - 2 * c + kBlock <= A.first);
+        const bool whole = j0 - 2 * c + kBlock <= min(clear, seen.end) && (A.window == 0 || j0 - 2 * c > last_pos - A.window || j0 - 2 * c + kBlock <= A.first);
         float p[2][4], top[2];
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -454,8 +500,8 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int e = 0; e < 4; ++e) {
                 const int j = j0 + (e & 1) + 8 * (e >> 1);
                 float v = sc[e >> 1][2 * x + (e & 1)] * mul;
-                if (BENT) v = bent_score(A, v, pos[x] - j, r1[x], r2[x], slope[x]);
-                p[x][e] = whole || sees(A, pos[x], j, seen.end) ? v : -INFINITY;
+                if (BENT) v = bent_score(A, v, pos[x] - (TREE && j >= pos0 && j < seen.end ? tree_key(A, t0, pos0, j) : j), r1[x], r2[x], slope[x]);
+                p[x][e] = whole || (TREE ? tree_sees(A, t0, pos0, t0 + min(row0 + r + 8 * x, n * Gq - 1) / Gq, pos[x], j, seen.end) : sees(A, pos[x], j, seen.end)) ? v : -INFINITY;
             }
             top[x] = fmaxf(fmaxf(p[x][0], p[x][1]), fmaxf(p[x][2], p[x][3]));
             top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
@@ -558,7 +604,7 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int t = 0; t < VB; t += 4)
                 *reinterpret_cast<float4*>(to + t) = make_float4(o[t][2 * x + e], o[t + 1][2 * x + e], o[t + 2][2 * x + e], o[t + 3][2 * x + e]);
         }
-    join_rows<kRowTile, LD>(A, J, join, W, split);
+    join_rows<kRowTile, LD, TREE>(A, J, join, W, split);
 }
 
 // A block of threads per (token, head): joins the shares of the keys, and the sink.  Latency is all there is to it, so everything a warp needs is

@@ -31,7 +31,7 @@ __device__ __forceinline__ bool has_passed(uint64_t* bar, uint32_t parity) {
         : "=r"(ok) : "r"(umma::s2u(bar)), "r"(parity) : "memory");
     return ok != 0;
 }
-__device__ __noinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* stop, int32_t* err) {
+static __device__ __noinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* stop, int32_t* err) {
     const long long begin = clock64();
 #pragma unroll 1
     while (clock64() - begin < kWaitCycles) {
@@ -52,7 +52,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
     return ok;
 }
 // the same for what is still in flight when a block ends
-__device__ __noinline__ void drain_bar(uint64_t* bar, uint32_t parity) {
+static __device__ __noinline__ void drain_bar(uint64_t* bar, uint32_t parity) {
     const long long begin = clock64();
 #pragma unroll 1
     while (!passed(bar, parity) && clock64() - begin < kWaitCycles) {}
@@ -134,11 +134,11 @@ __device__ __forceinline__ float warp_top(float v) {
 // ---- steps of 128 positions ----
 constexpr int kStep = 128, kStepBlocks = kStep / kBlock;
 
-// The steps that rows first_pos .. last_pos see: `lead` of them from the sequence's start (the first tokens, in front of the window), then those from
+// The steps that rows from first_pos on see, which see no key from `behind` on: `lead` of them from the sequence's start (the first tokens, in front of the window), then those from
 // `from` up to the last visible key.
-__device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, int last_pos, int kv_len) {
+__device__ __forceinline__ Seen seen_steps(const AttendArgs& A, int first_pos, int behind, int kv_len) {
     Seen x;
-    x.end = last_visible(A, last_pos, kv_len);
+    x.end = last_visible(A, behind, kv_len);
     const int steps = (x.end + kStep - 1) / kStep;
     x.from = A.window > 0 ? min(max(window_from(A, first_pos), 0) / kStep, steps) : 0;
     x.lead = A.window > 0 ? min(A.first / kStep + (A.first % kStep > 0), x.from) : 0;

@@ -75,16 +75,17 @@ __device__ __forceinline__ uint32_t half_two(float a, float b) {
 }
 
 // Columns col .. col + 31 (a bit each) of the values in which a row at `pos` sees a NaN.  Rare, and slow.
-__device__ __noinline__ uint32_t nan_bits(const AttendArgs& A, const Rows& W, int pos, int col) {
+template <bool TREE>
+__device__ __noinline__ uint32_t nan_bits(const AttendArgs& A, const Rows& W, int tok, int pos, int col) {
     uint32_t bits = 0;
-    for (int b = 0; b * kBlock < min(W.end, pos + 1); ++b) {
+    for (int b = 0; b * kBlock < (TREE ? W.end : min(W.end, pos + 1)); ++b) {
         const int pg = b * kBlock / A.c.page;
         const int page = pg < A.b.max_pages ? A.b.table[(size_t)W.s * A.b.max_pages + pg] : -1;
         if (page < 0 || page >= A.c.n_pages) continue;
         const int in_page = b * kBlock - pg * A.c.page;
         if (A.c.vs[(size_t)page * A.c.vs_page + W.g * (A.c.page / kBlock) + in_page / kBlock] >= 0.0f) continue;
         for (int i = 0; i < kBlock; ++i) {
-            if (!sees(A, pos, b * kBlock + i, W.end)) continue;
+            if (TREE ? !tree_sees(A, W.t0, W.pos0, tok, pos, b * kBlock + i, W.end) : !sees(A, pos, b * kBlock + i, W.end)) continue;
             const uint8_t* v = A.c.v + (size_t)page * A.c.v_page + ((size_t)W.g * A.c.page + in_page + i) * A.c.ldv + col;
             for (int c = 0; c < 32 && col + c < A.c.dv; ++c)
                 if ((v[c] & 0x7f) == 0x7f) bits |= 1u << c;
@@ -95,8 +96,8 @@ __device__ __noinline__ uint32_t nan_bits(const AttendArgs& A, const Rows& W, in
 
 constexpr float kFarAbove = 64.0f;      // in units of log2
 
-// DK: key size padded
-template <int DK, bool BENT>
+// DK: key size padded; BENT: soft cap or distance penalties; TREE: rows of a tree
+template <int DK, bool BENT, bool TREE>
 __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
     constexpr int NS = tile_stages(DK), SB = tile_stage_bytes(DK), KH = DK / 128;
     extern __shared__ unsigned char smem_raw[];
@@ -131,9 +132,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
     const int t0 = Q.t0, n_all = Q.n, n = min(n_all, A.b.max_new), pos0 = Q.pos0;
     const int kv_len = A.b.kv_len ? A.b.kv_len[s] : 0x7fffffff;
     const int row0 = tile * kTileRows, rows = min(n * Gq - row0, kTileRows);
-    const bool any = rows > 0 && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most;
-    const int first_pos = pos0 + row0 / Gq, last_pos = any ? pos0 + (row0 + rows - 1) / Gq : -1;
-    const Seen seen = seen_steps(A, first_pos, last_pos, kv_len);
+    const bool any = rows > 0 && (long long)n_all * Gq > A.rows_over && (long long)n_all * Gq <= A.rows_most && (!TREE || tree_fits(A, pos0, n_all));
+    int first_pos = pos0 + row0 / Gq, last_pos = any ? pos0 + (row0 + rows - 1) / Gq : -1, behind = last_pos + 1, clear = first_pos + 1;      // clear: every row sees what is in front of it, but for the window
+    if (TREE && any) {
+        const TreeSpan span(A, t0 + row0 / Gq, (row0 + rows - 1) / Gq - row0 / Gq + 1, n_all, pos0);
+        first_pos = span.first_pos; last_pos = span.last_pos; behind = span.behind; clear = pos0;
+    }
+    const Seen seen = seen_steps(A, first_pos, behind, kv_len);
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
     const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = min(split * share, seen.count);
     const int steps = any ? min(lo + share, seen.count) - lo : 0;
@@ -246,7 +251,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
         asm volatile("bar.sync 5, %0;" ::"n"(kTileSoft * 32) : "memory");
 
         // ---- softmax: warps q, q + 4, q + 8, q + 12 share rows 32 q .. + 31; part p has columns 32 p .. + 31 of the scores and of the result ----
-        const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane, my_row = min(row0 + row, n * Gq - 1), pos = pos0 + my_row / Gq, h = g * Gq + my_row % Gq;
+        const int quad = warp & 3, part = warp >> 2, row = quad * 32 + lane, my_row = min(row0 + row, n * Gq - 1), pos = TREE ? tree_position(A, t0 + my_row / Gq) : pos0 + my_row / Gq, h = g * Gq + my_row % Gq;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         const float rowmul = s_rowmul[row], r1 = BENT && A.r1 ? A.r1[h] : 0.0f, r2 = BENT && A.r1 ? A.r2[h] : 0.0f, slope = BENT && A.slope ? A.slope[h] * kLog2e : 0.0f;
         const Bend bend(A);
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
 #pragma unroll
                 for (int e = 0; e < kTileCols; ++e) S[e] = __uint_as_float(v[e / 8][e % 8]);
             }
-            const bool whole = !holes && j0 + kStep <= min(first_pos + 1, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
+            const bool whole = !holes && j0 + kStep <= min(clear, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             // scores in units of log2: S times mul
             const bool direct = !BENT && whole && A.scale > 0.0f;
             float mul[kTileCols / kBlock];
@@ -322,12 +327,33 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
                 for (int e = 0; e < kTileCols; ++e) S[e] *= mul[e / kBlock];
                 if (BENT) {
                     const float d0 = (float)(pos - jc);
-                    bend(A, S, [&](int e) { return d0 - (float)e; }, [&](int) { return r1; }, [&](int) { return r2; }, [&](int) { return slope; });
+                    if (TREE && jc + kTileCols > pos0)      // (some keys are rows of the tree)
+                        bend(A, S, [&](int e) { return fmaxf((float)(pos - (jc + e < seen.end ? tree_key(A, t0, pos0, jc + e) : jc + e)), 0.0f); }, [&](int) { return r1; }, [&](int) { return r2; },
+                             [&](int) { return slope; });
+                    else
+                        bend(A, S, [&](int e) { return TREE ? fmaxf(d0 - (float)e, 0.0f) : d0 - (float)e; }, [&](int) { return r1; }, [&](int) { return r2; }, [&](int) { return slope; });
                 }
 #pragma unroll
                 for (int x = 0; x < kTileCols / kBlock; ++x) mul[x] = 1.0f;
             }
-            if (!whole) {
+            if (TREE && !whole) {
+                // which of the thread's keys the row's bits name (the context's all)
+                const int i0 = jc - pos0, w = i0 >> 5;      // (rounded down)
+                const uint32_t* bits = A.tree_sees + (size_t)(t0 + my_row / Gq) * A.tree_words;
+                const uint32_t low = w < 0 ? 0xffffffffu : w < A.tree_words ? bits[w] : 0u, high = w + 1 < 0 ? 0xffffffffu : w + 1 < A.tree_words ? bits[w + 1] : 0u;
+                const uint32_t named = __funnelshift_r(low, high, i0 & 31);
+                const int last = seen.end - jc;
+#pragma unroll
+                for (int e = 0; e < kTileCols; ++e)
+                    if (e >= last || ks[e / kBlock] == 0.0f || !(named >> e & 1u)) S[e] = -INFINITY;
+                if (A.window > 0) {
+#pragma unroll
+                    for (int e = 0; e < kTileCols; ++e) {
+                        const int key = e < last ? tree_key(A, t0, pos0, jc + e) : 0;
+                        if (pos - key >= A.window && key >= A.first) S[e] = -INFINITY;
+                    }
+                }
+            } else if (!whole) {
                 const int far = A.window > 0 ? A.window : 0x7fffffff, last = min(pos + 1, seen.end) - jc, lead = A.first - jc, dist = pos - jc;
 #pragma unroll
                 for (int e = 0; e < kTileCols; ++e)
@@ -433,7 +459,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const Att
             const bool mine = row < rows;
             const int tok = t0 + my_row / Gq;
             if (s_bad && mine) {
-                const uint32_t bits = nan_bits(A, W, pos, col);
+                const uint32_t bits = nan_bits<TREE>(A, W, tok, pos, col);
 #pragma unroll
                 for (int c = 0; c < 32; ++c)
                     if (bits >> c & 1) o[c] = __int_as_float(0x7fffffff);

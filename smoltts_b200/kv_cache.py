@@ -8,26 +8,39 @@ seq_start[s + 1] - 1``, which are its positions ``seq_pos0[s], seq_pos0[s] + 1, 
 whose rows or positions do not fit is left out, a page outside the cache not touched, and ``check_device_errors`` tells.  Everything runs on the current stream
 of the cache's device and nothing synchronises, so that calls can be captured into a CUDA graph; results carry no gradient.  ``lm.HybridLM`` serves
 its softmax attention layers from such a cache with ``kv_bits=8``.
+
+Drafted tokens may form a tree: ``draft_tree`` lays it out once per step, every layer's cache appends the rows at the positions that their depths give
+them (``append(positions=)``, which also takes the several axes of pictures and video) and attends to them along their paths (``attend(tree=)``), and
+``keep_rows`` then moves the rows of the accepted path together in all layers.  ``copy_pages`` copies pages in all layers, as forking a sequence does::
+
+    tree = caches[0].draft_tree(parents, seq_start, seq_pos0, max_new=64)
+    for cache in caches:
+        q = cache.append(k, v, seq_start, seq_pos0, block_table, max_new=64, q=q, freq=freq, positions=tree.positions)
+        out = cache.attend(q, seq_start, seq_pos0, block_table, max_new=64, max_len=8192, tree=tree)
+    keep_rows(caches, seq_pos0, block_table, accepted, counts)
 """
 from __future__ import annotations
 
 import ctypes as C
 import math
 import struct
-from typing import Dict, Optional, Tuple
+from array import array
+from typing import Dict, List, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _capi_lm
-from ._errors import SMOL_ERR_CAPACITY, SMOL_ERR_CUDA, SMOL_OK, SmolError
+from ._errors import SMOL_ERR_CAPACITY, SMOL_ERR_CUDA, SMOL_ERR_INVALID, SMOL_OK, SmolError
 
 BLOCK = 16          # positions that share a scale
+MOST_DRAFTED = 4096  # rows of a sequence in a tree
 _DTYPES = {torch.bfloat16: _capi_lm.SMOL_LM_BF16, torch.float32: _capi_lm.SMOL_LM_F32}
 # The arguments' structs of include/smoltts_b200_lm.h as native layouts: packing one takes a microsecond, filling a ctypes structure several.
 _BATCH = struct.Struct("@5i4P")
-_APPEND = struct.Struct("@i2P4Ni2P4N2iPf0P")
-_ATTEND = struct.Struct("@2i2P4N3f2i5PN0P")
-for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCache8Append), (_ATTEND, _capi_lm.SmolLmCache8Attend)):
+_APPEND = struct.Struct("@i2P4Ni2P4N2iPf2Pi0P")
+_ATTEND = struct.Struct("@2i2P4N3f2i5PN2Pi0P")
+_KEEP = struct.Struct("@3i4P")
+for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCache8Append), (_ATTEND, _capi_lm.SmolLmCache8Attend), (_KEEP, _capi_lm.SmolLmCache8Keep)):
     assert _s.size == C.sizeof(_m)
 
 
@@ -66,6 +79,14 @@ def _check_written(out: torch.Tensor, what: str, **read: torch.Tensor) -> None:
         a, b = _extent(x)
         if a < hi and lo < b:
             raise ValueError(f"{what} must not reach into {name}'s memory: it is read while {what} is written")
+
+
+class DraftTree(NamedTuple):
+    """Where drafted rows stand and what they see of one another: ``positions [tokens]``, and ``sees [tokens, words]`` (int32, bit ``i % 32`` of word
+    ``i // 32``: row ``i`` of the same sequence).  ``KVCache8.draft_tree`` makes one from parents; any other mask, and any positions from 0 to 2^31 - 129, will do."""
+
+    positions: torch.Tensor
+    sees: torch.Tensor
 
 
 class KVCache8:
@@ -160,13 +181,17 @@ class KVCache8:
     # ------------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, max_new: int,
                q: Optional[torch.Tensor] = None, freq: Optional[torch.Tensor] = None, rot_half: bool = True, rot_mult: float = 1.0,
-               q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+               q_out: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, axis: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
         """Writes the rows' keys ``k [tokens, kv_heads, dim]`` and values ``v [tokens, kv_heads, vdim]`` into their pages.
 
         With ``freq [pairs]`` (fp32) keys, and queries ``q [tokens, heads, dim]``, are rotated first: pair ``i`` by the angle position *
         ``freq[i]`` (computed in 64 bits), ``rot_half`` pairing coordinate ``i`` with ``i + pairs``, otherwise ``2i`` with ``2i + 1``; coordinates
         behind the pairs pass unchanged; ``rot_mult`` multiplies cosine and sine.  Returns the queries (in ``q_out``, or a new tensor), or None
         without ``q``.  ``max_new``: most rows a sequence brings (a host number).  Rows outside every sequence are left alone.
+
+        ``positions [tokens]`` or ``[axes, tokens]`` (int32) are the rows' rotary positions where these are not their places in the cache: of drafted rows, or of
+        pictures and video with an axis each for time, height and width.  ``axis [pairs]`` (int32) then says which of them turns a pair (without it, the
+        first); an axis that there is not is reported and counts as the first.
 
         A block's 16 positions share the smallest power of two with |value| <= 448 * scale; where an earlier call began the block the
         scale never shrinks, and the older codes follow it when it grows.  Magnitudes above 2^100 are clamped; a NaN stays a NaN.  Two
@@ -195,20 +220,35 @@ class KVCache8:
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
+        pos_ptr = axis_ptr = axes = 0
+        if positions is not None:
+            if freq is None:
+                raise ValueError("positions without freq")
+            axes = positions.shape[0] if positions.dim() == 2 else 1
+            if axes < 1:
+                raise ValueError("positions without an axis")
+            pos_ptr = self._ints(positions, (axes, tokens) if positions.dim() == 2 else (tokens,), "positions")
+            if axis is not None:
+                axis_ptr = self._ints(axis, (pairs,), "axis") if pairs else 0
+        elif axis is not None:
+            raise ValueError("axis without positions")
         self._call(self._append, batch, _pack(_APPEND, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, heads, q_ptr, out_ptr, q_row, q_head,
-                                              out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, _float(rot_mult, "rot_mult")))
+                                              out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, _float(rot_mult, "rot_mult"), pos_ptr, axis_ptr, axes))
         return q_out
 
     def attend(self, q: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, max_new: int, max_len: int,
                scale: Optional[float] = None, window: int = 0, first: int = 0, softcap: float = 0.0, sink: Optional[torch.Tensor] = None,
                slope: Optional[torch.Tensor] = None, penalty: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
-               kv_len: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+               kv_len: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, tree: Optional[DraftTree] = None) -> torch.Tensor:
         """Causal softmax attention of the rows ``q [tokens, heads, dim]`` over the cache (which holds the rows' own positions already).
 
         A row at position ``i`` sees the keys ``j <= i``; with ``window`` only ``i - j < window``, and the sequence's first ``first``
         positions whatever their distance; ``kv_len [sequences]`` hides keys from that position on.  Score: ``scale`` (default
         ``dim ** -0.5``) times q.k, bent by ``softcap * tanh(s / softcap)``, less ``penalty[0] * ln(1 + penalty[1] * (i - j))`` and ``slope * (i - j)``;
         ``sink``, a logit without a key, joins the denominator (all per query head, fp32).  A row that sees no key gives zeros.
+
+        With ``tree`` the rows are drafted ones: each sees all keys in front of its sequence's rows and, of the rows, those that its bits name (itself, if it is to,
+        among them).  ``i`` and ``j`` above are then positions, of rows those of the tree, and a distance below 0 counts as 0; ``kv_len`` goes on counting places.
 
         ``max_new``: most rows a sequence brings; ``max_len``: most positions a sequence holds, the rows included (host numbers;
         the grid is chosen by them -- a longer sequence is attended to as a whole all the same, rows beyond ``max_new`` are left alone).
@@ -226,12 +266,18 @@ class KVCache8:
             out_row, out_head = heads * self.vdim, self.vdim
         else:
             out_row, out_head = self._rows(out, tokens, heads, self.vdim, dtype, "out")
-            _check_written(out, "out", q=q)
+            _check_written(out, "out", q=q, **({} if tree is None else tree._asdict()))
         r1 = r2 = 0
         if penalty is not None:
             r1, r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
+        tree_pos = tree_sees = words = 0
+        if tree is not None:
+            words = tree.sees.shape[-1] if tree.sees.dim() == 2 else 0
+            if words < 1:
+                raise ValueError("tree.sees must be [tokens, words]")
+            tree_pos, tree_sees = self._ints(tree.positions, (tokens,), "tree.positions"), self._ints(tree.sees, (tokens, words), "tree.sees")
         a = _pack(_ATTEND, _DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else _float(scale, "scale"), _float(softcap, "softcap"), 1.0,
-                  window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0)
+                  window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0, tree_pos, tree_sees, words)
         key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first)
         need = self._need.get(key)
         if need is None:
@@ -245,6 +291,22 @@ class KVCache8:
         work = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
         self._call(self._attend, batch, a, work.data_ptr() if need else None, need)
         return out
+
+    def draft_tree(self, parents: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, max_new: int) -> DraftTree:
+        """The tree of a step's drafted rows, for all layers' ``append`` and ``attend``: ``parents [tokens]`` (int32) names every row's parent among the rows of its
+        sequence, -1 for one that follows what the sequence holds already.  A parent comes in front of its children; one that does not is reported (by this cache) and counts as -1.
+        ``max_new``: most rows a sequence brings, at most 4096; a sequence of more is left out and reported.  Rows outside every sequence are anything."""
+        if parents.dim() != 1 or parents.shape[0] < 1 or seq_pos0.dim() != 1 or seq_pos0.shape[0] < 1:
+            raise ValueError("parents must be [tokens] and seq_pos0 [sequences], with at least one each")
+        if not 1 <= max_new <= MOST_DRAFTED:
+            raise ValueError(f"max_new must be from 1 to {MOST_DRAFTED}")
+        tokens, n, words = parents.shape[0], seq_pos0.shape[0], (max_new + 31) // 32
+        at = [self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"), self._ints(parents, (tokens,), "parents")]
+        tree = DraftTree(parents.new_empty(tokens), parents.new_empty((tokens, words)))
+        with torch.cuda.device(self._index):
+            _capi_lm.check(_capi_lm.load().smol_lm_cache8_tree(tokens, n, max_new, *at, tree.positions.data_ptr(), tree.sees.data_ptr(), words, self._err.data_ptr(),
+                                                               torch._C._cuda_getCurrentRawStream(self._index)))
+        return tree
 
     # ------------------------------------------------------------------ looking in
     def values(self, pages: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -262,3 +324,63 @@ class KVCache8:
             raise SmolError(SMOL_ERR_CUDA, "device-side error word 3: a wait inside a kernel ran out, results of that call are missing")
         if word:
             raise SmolError(SMOL_ERR_CAPACITY, f"device-side error word {word}: " + ("a block table names a page outside the cache" if word == 1 else "a batch's arrays do not fit its sizes"))
+
+
+def _layers(caches: Union[KVCache8, Sequence[KVCache8]]) -> List[KVCache8]:
+    caches = [caches] if isinstance(caches, KVCache8) else list(caches)
+    if not caches:
+        raise ValueError("no cache")
+    if any(c.device != caches[0].device for c in caches):
+        raise ValueError("caches of several devices")
+    return caches
+
+
+def _call_layers(call, caches: List[KVCache8], *args) -> None:
+    """On the caches' device and its current stream.  What is refused on the host is the caller's."""
+    index = caches[0]._index
+    with torch.cuda.device(index):
+        rc = call(b"".join([c._c for c in caches]), len(caches), *args, torch._C._cuda_getCurrentRawStream(index))
+    if rc == SMOL_ERR_INVALID:
+        raise ValueError(_capi_lm.load().smol_lm_last_error().decode())
+    if rc != SMOL_OK:
+        _capi_lm.check(rc)
+
+
+def keep_rows(caches: Union[KVCache8, Sequence[KVCache8]], seq_pos0: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor) -> None:
+    """Keeps the rows of an accepted path, in all layers: row ``rows[s, i]`` behind position ``seq_pos0[s]`` becomes the row at ``seq_pos0[s] + i``, for ``i`` below ``counts[s]``
+    (int32 ``[sequences, most]`` and ``[sequences]``; rows in ascending order, what is behind ``counts[s]`` is not looked at).
+
+    The rows are written as ``append`` would write the values that the cache holds of them; the sequence's length is then ``seq_pos0[s] + counts[s]``, and what lies behind it
+    is no more to be read.  ``caches``: a cache, or the layers' (of one shape, none twice).  A sequence whose arrays do not fit is left as it is, and
+    ``check_device_errors`` of the caches tells.  No page may belong to two sequences that keep rows in it."""
+    layers = _layers(caches)
+    c = layers[0]
+    if rows.dim() != 2 or block_table.dim() != 2 or rows.shape[1] < 1 or block_table.shape[1] < 1 or rows.shape[0] < 1:
+        raise ValueError("rows must be [sequences, most] and block_table [sequences, pages], with at least one each")
+    n, most = rows.shape
+    a = _pack(_KEEP, n, block_table.shape[1], most, c._ints(seq_pos0, (n,), "seq_pos0"), c._ints(block_table, (n, block_table.shape[1]), "block_table"), c._ints(rows, (n, most), "rows"),
+              c._ints(counts, (n,), "counts"))
+    _call_layers(_packed_keep(), layers, a)
+
+
+def copy_pages(caches: Union[KVCache8, Sequence[KVCache8]], src: Sequence[int], dst: Sequence[int]) -> None:
+    """Copies pages ``src[i]`` to pages ``dst[i]``, in all layers.  The pages are host numbers, as a ``pool.PagePool`` hands them out; a page may be copied to several others, but none
+    may be written twice, nor read and written by one call.  A captured call copies the same pages whenever it is replayed."""
+    layers = _layers(caches)
+    if any(isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)):
+        raise ValueError("pages are host numbers")
+    try:
+        a, b = (array("i", x.tolist() if isinstance(x, torch.Tensor) else x) for x in (src, dst))
+    except OverflowError as e:
+        raise ValueError(f"a page outside the cache: {e}") from e
+    if len(a) != len(b):
+        raise ValueError(f"{len(a)} pages to {len(b)}")
+    if a:
+        _call_layers(_capi_lm.load().smol_lm_cache8_copy_pages, layers, a.buffer_info()[0], b.buffer_info()[0], len(a))
+
+
+def _packed_keep():
+    """``smol_lm_cache8_keep`` with its arguments as packed structs."""
+    call = _capi_lm.load()["smol_lm_cache8_keep"]
+    call.argtypes = [C.c_char_p, C.c_int32, C.c_char_p, C.c_void_p]
+    return call
