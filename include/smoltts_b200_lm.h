@@ -298,7 +298,7 @@ typedef struct SmolLm SmolLm;
 
 int smol_lm_abi_version(void);
 size_t smol_lm_struct_bytes(int which);          /* sizeof of SmolLmLayer (0), SmolLmConfig (1), SmolLmGlobals (2), SmolLmStep (3), SmolLmCache8 (4), SmolLmCache8Batch (5),
-                                                    SmolLmCache8Append (6), SmolLmCache8Attend (7), SmolLmCache8Keep (8): a binding checks its mirror */
+                                                    SmolLmCache8Append (6), SmolLmCache8Attend (7), SmolLmCache8Keep (8), SmolLmCache8Tree (9): a binding checks its mirror */
 const char* smol_lm_last_error(void);
 
 /* layers / run_layer are HOST arrays, copied.  run_layer[n] = index of the layer that run n executes. */
@@ -391,6 +391,17 @@ typedef struct SmolLmCache8Attend {
     int32_t tree_words;
 } SmolLmCache8Attend;
 
+/* A tree of rows, from every row's parent among the rows of its sequence (-1: the row follows what the sequence holds already; a parent comes in front of its
+ * children): positions[t] = seq_pos0 + the row's depth, and the bits sees[t][words] of the row itself and of those on its way up.  Rows outside every sequence are left alone; a
+ * sequence of more than max_new (at most 4096) rows is left out and reported, a parent that cannot be one counts as -1 and is reported (err: 2). */
+typedef struct SmolLmCache8Tree {
+    int32_t n_tokens, n_seqs, max_new, words;   /* words: at least max_new bits */
+    const int32_t *seq_start, *seq_pos0, *parents;      /* device: [n_seqs + 1], [n_seqs], [n_tokens] */
+    int32_t* positions;          /* device [n_tokens] */
+    uint32_t* sees;              /* device [n_tokens][words] */
+    int32_t* err;                /* device word */
+} SmolLmCache8Tree;
+
 /* Rows that stay: rows[s][0] < rows[s][1] < ... < rows[s][counts[s] - 1] of sequence s, counted from position seq_pos0[s]. */
 typedef struct SmolLmCache8Keep {
     int32_t n_seqs, max_pages, max_keep;
@@ -403,11 +414,7 @@ int smol_lm_cache8_append(const SmolLmCache8* cache, const SmolLmCache8Batch* ba
 int smol_lm_cache8_workspace_bytes(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, size_t* bytes);
 int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCache8Batch* batch, const SmolLmCache8Attend* a, void* workspace, size_t workspace_bytes, void* stream);
 
-/* A tree of rows, from every row's parent among the rows of its sequence (-1: the row follows what the sequence holds already; a parent comes in front of its
- * children): positions[t] = seq_pos0 + the row's depth, and the bits sees[t][words] of the row itself and of those on its way up.  Rows outside every sequence are left alone; a
- * sequence of more than max_new (at most 4096) rows is left out and reported, a parent that cannot be one counts as -1 and is reported (err: 2). */
-int smol_lm_cache8_tree(int32_t n_tokens, int32_t n_seqs, int32_t max_new, const int32_t* seq_start, const int32_t* seq_pos0, const int32_t* parents, int32_t* positions,
-                        uint32_t* sees, int32_t words, int32_t* err, void* stream);
+int smol_lm_cache8_tree(const SmolLmCache8Tree* a, void* stream);
 /* The rows that stay move together, in every one of `caches` (HOST array, all of one shape, none twice): row rows[s][i] becomes the row at position seq_pos0[s] + i, as if its
  * values, as the cache holds them, were appended there; what lies behind the last of them is as it was, or as it was with another scale.  A sequence whose arrays do not fit is left
  * as it is and reported in the caches' err (1: a page outside the cache, 2: rows not in order). */

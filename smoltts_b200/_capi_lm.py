@@ -86,6 +86,10 @@ class SmolLmCache8Attend(C.Structure):
         ("gate_row", C.c_size_t), ("tree_positions", C.c_void_p), ("tree_sees", C.c_void_p), ("tree_words", C.c_int32)]
 
 
+class SmolLmCache8Tree(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_tokens", "n_seqs", "max_new", "words")] + [(n, C.c_void_p) for n in ("seq_start", "seq_pos0", "parents", "positions", "sees", "err")]
+
+
 class SmolLmCache8Keep(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("n_seqs", "max_pages", "max_keep")] + [(n, C.c_void_p) for n in ("seq_pos0", "block_table", "rows", "counts")]
 
@@ -109,7 +113,7 @@ PROTOTYPES = {
                                                  C.POINTER(C.c_size_t)]),
     "smol_lm_cache8_attend": (C.c_int, [C.POINTER(SmolLmCache8), C.POINTER(SmolLmCache8Batch), C.POINTER(SmolLmCache8Attend), C.c_void_p,
                                         C.c_size_t, C.c_void_p]),
-    "smol_lm_cache8_tree": (C.c_int, [C.c_int32, C.c_int32, C.c_int32] + [C.c_void_p] * 5 + [C.c_int32, C.c_void_p, C.c_void_p]),
+    "smol_lm_cache8_tree": (C.c_int, [C.POINTER(SmolLmCache8Tree), C.c_void_p]),
     "smol_lm_cache8_keep": (C.c_int, [C.c_void_p, C.c_int32, C.POINTER(SmolLmCache8Keep), C.c_void_p]),
     "smol_lm_cache8_copy_pages": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p]),
     "smol_lm_launch_count": (C.c_int64, [C.c_void_p]),
@@ -136,7 +140,7 @@ def load() -> C.CDLL:
         fn.argtypes = args
     if lib.smol_lm_abi_version() != SMOL_LM_ABI_VERSION:
         raise RuntimeError(f"{path}: ABI version {lib.smol_lm_abi_version()} != {SMOL_LM_ABI_VERSION}")
-    for which, mirror in enumerate((SmolLmLayer, SmolLmConfig, SmolLmGlobals, SmolLmStep, SmolLmCache8, SmolLmCache8Batch, SmolLmCache8Append, SmolLmCache8Attend, SmolLmCache8Keep)):
+    for which, mirror in enumerate((SmolLmLayer, SmolLmConfig, SmolLmGlobals, SmolLmStep, SmolLmCache8, SmolLmCache8Batch, SmolLmCache8Append, SmolLmCache8Attend, SmolLmCache8Keep, SmolLmCache8Tree)):
         if lib.smol_lm_struct_bytes(which) != C.sizeof(mirror):
             raise RuntimeError(f"{path}: {mirror.__name__} is {lib.smol_lm_struct_bytes(which)} bytes in the library, {C.sizeof(mirror)} in the binding")
     _lib = lib

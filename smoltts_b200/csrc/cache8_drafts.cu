@@ -44,8 +44,8 @@ static void take_layers(Layers& l, const SmolLmCache8* caches, int n, const char
 }
 
 static cudaError_t keep(const KeepArgs& A, cudaStream_t st) {
-    const int ld = std::max(A.l.c.ldk, A.l.c.ldv), units = A.l.n * A.l.c.G * 2;
-    const dim3 grid((units + kKeepWarps - 1) / kKeepWarps, A.S);
+    const int ld = std::max(A.l.c.ldk, A.l.c.ldv);
+    const dim3 grid((A.l.c.G + kKeepWarps - 1) / kKeepWarps, A.S, A.l.n);
     return ld <= 64 ? launch(keep_kernel<2>, grid, kKeepWarps * 32, 0, st, A) : ld <= 128 ? launch(keep_kernel<4>, grid, kKeepWarps * 32, 0, st, A) : launch(keep_kernel<8>, grid, kKeepWarps * 32, 0, st, A);
 }
 
@@ -80,17 +80,16 @@ static int pairs_of(const int32_t* src, const int32_t* dst, int n, int n_pages, 
 using namespace smol::c8;
 using smol::lm::report;
 
-extern "C" int smol_lm_cache8_tree(int32_t n_tokens, int32_t n_seqs, int32_t max_new, const int32_t* seq_start, const int32_t* seq_pos0, const int32_t* parents, int32_t* positions,
-                                   uint32_t* sees, int32_t words, int32_t* err, void* stream) {
+extern "C" int smol_lm_cache8_tree(const SmolLmCache8Tree* a, void* stream) {
     const char* me = "smol_lm_cache8_tree";
-    if (!seq_start || !seq_pos0 || !parents || !positions || !sees || !err) return report(SMOL_ERR_INVALID, me, "null array");
-    if (n_tokens < 1 || n_seqs < 1 || max_new < 1) return report(SMOL_ERR_INVALID, me, "n_tokens, n_seqs and max_new must be positive");
-    if (max_new > kTreeRows) return report(SMOL_ERR_CAPACITY, me, "more than 4096 rows of a sequence");
-    if (words < (max_new + 31) / 32) return report(SMOL_ERR_INVALID, me, "fewer words than max_new bits");
+    if (!a || !a->seq_start || !a->seq_pos0 || !a->parents || !a->positions || !a->sees || !a->err) return report(SMOL_ERR_INVALID, me, "null argument");
+    if (a->n_tokens < 1 || a->n_seqs < 1 || a->max_new < 1) return report(SMOL_ERR_INVALID, me, "n_tokens, n_seqs and max_new must be positive");
+    if (a->max_new > kTreeRows) return report(SMOL_ERR_CAPACITY, me, "more than 4096 rows of a sequence");
+    if (a->words < (a->max_new + 31) / 32) return report(SMOL_ERR_INVALID, me, "fewer words than max_new bits");
     TreeArgs A{};
-    A.b.start = seq_start; A.b.pos0 = seq_pos0; A.b.S = n_seqs; A.b.T = n_tokens; A.b.max_new = max_new;
-    A.parents = parents; A.positions = positions; A.sees = sees; A.words = words; A.err = err;
-    const cudaError_t e = launch(tree_kernel, n_seqs, std::min(1024, (max_new + 31) / 32 * 32), 0, static_cast<cudaStream_t>(stream), A);
+    A.b.start = a->seq_start; A.b.pos0 = a->seq_pos0; A.b.S = a->n_seqs; A.b.T = a->n_tokens; A.b.max_new = a->max_new;
+    A.parents = a->parents; A.positions = a->positions; A.sees = a->sees; A.words = a->words; A.err = a->err;
+    const cudaError_t e = launch(tree_kernel, a->n_seqs, std::min(1024, (a->max_new + 31) / 32 * 32), 0, static_cast<cudaStream_t>(stream), A);
     return e == cudaSuccess ? SMOL_OK : report(SMOL_ERR_CUDA, me, cudaGetErrorString(e));
 }
 

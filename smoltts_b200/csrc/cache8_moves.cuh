@@ -85,14 +85,45 @@ struct Layers {
 
 // ---- rows ----
 // Rows rows[s][0] < rows[s][1] < ... < rows[s][counts[s] - 1] behind pos0[s] become the rows pos0[s], pos0[s] + 1, ...: written as an append of the values that they have would
-// write them.  A warp per (layer, keys or values, sequence, head) takes the blocks of 16 positions that rows go to one after the other: a block's rows are in registers before any of it
-// is written, and rows of later blocks come from behind it, so that nothing is overwritten that is still to be read.
-// What bounds it: latency, a chain of four loads (count, rows, page, codes and scales).
+// write them.  A warp per (layer, head, sequence) takes the blocks of 16 positions that rows go to one after the other, keys and values at once.  A block's rows are in registers before
+// any of it is written, and rows of later blocks come from behind it, so that nothing is overwritten that is still to be read.
+//
+// A code changes only where the scale does: rows whose block had the scale that they get are copied.  A block that holds older rows keeps its scale while no
+// row comes from a larger one (codes are at most 448, so that a row's values are at most 448 times its old scale); otherwise, and in a block of kept rows alone, the largest magnitude is found.
+// What bounds it: latency, a chain of four loads (count, rows, pages, codes and scales).
 struct KeepArgs {
     Layers l;
     const int32_t *pos0, *table, *rows, *counts;
     int S, max_pages, most;
 };
+// Sixteen codes times f.  In f16 where that is exact before the one rounding: codes are multiples of 2^-9 below 2^9, f a power of two from 2^-14 (products are multiples of 2^-23)
+// to 2^15 (what passes f16 passes 448 too).  (In float32 it is sixteen conversions more, of which an SM makes sixteen a cycle: 64 sequences' rows in 28 layers took 20 us.)
+__device__ __forceinline__ uint4 rescaled(uint4 codes, float f) {
+    uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+    const uint32_t bits = __float_as_uint(f);
+    if ((bits & 0x7fffffu) == 0u && bits >= (127u - 14u) << 23 && bits <= (127u + 15u) << 23) {
+        const __half2 f2 = __float2half2_rn(f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t part[2];
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const __half2_raw raw = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i] >> 16 * z & 0xffffu), __NV_E4M3);
+                part[z] = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(__hmul2(__half2(raw), f2)), __NV_SATFINITE, __NV_E4M3);
+            }
+            w[i] = part[0] | part[1] << 16;
+        }
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = from_e4m3x4(codes.x);
+            const uint32_t q = to_e4m3x4(v.x * f, v.y * f, v.z * f, v.w * f);
+            codes = make_uint4(codes.y, codes.z, codes.w, q);
+        }
+        return codes;
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 constexpr int kKeepWarps = 4;
 // PASSES of 16 / PASSES rows, 2 PASSES lanes a row of 16 codes each, as in append_kernel
 template <int PASSES>
@@ -102,24 +133,27 @@ __global__ void __launch_bounds__(kKeepWarps * 32) keep_kernel(const __grid_cons
     dep_go();
     const Cache& c = A.l.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, piece = lane % LANES, sub = lane / LANES;
-    const int unit = blockIdx.x * kKeepWarps + warp, s = blockIdx.y;      // unit: layer, head, keys or values
-    if (unit >= A.l.n * c.G * 2) return;
-    const Layer& L = A.l.of[unit / (c.G * 2)];
-    const int g = unit / 2 % c.G;
-    const bool value = unit & 1;
+    const int g = blockIdx.x * kKeepWarps + warp, s = blockIdx.y;
+    if (g >= c.G) return;
+    const Layer& L = A.l.of[blockIdx.z];
     const int32_t *rows = A.rows + (size_t)s * A.most, *table = A.table + (size_t)s * A.max_pages;
     const int pos0 = A.pos0[s], count = A.counts[s];
+    int r = lane < A.most ? rows[lane] : 0, before = lane > 0 && lane < A.most ? rows[lane - 1] : -1;      // (with the counts, not behind them)
     // ---- what the arrays say, before anything is made of it ----
-    auto page_of = [&](int p) {
-        const int pg = p / c.page;
-        return pg < A.max_pages ? table[pg] : -1;
-    };
     int wrong = pos0 < 0 || pos0 >= kPositions || count < 0 || count > A.most ? 2 : 0;
     if (wrong == 0)
         for (int i = lane; i < count; i += 32) {
-            const int r = rows[i], before = i > 0 ? rows[i - 1] : -1;
-            if (r <= before || r >= kPositions - pos0) wrong = 2;
-            else if ((unsigned)page_of(pos0 + i) >= (unsigned)c.n_pages || (unsigned)page_of(pos0 + r) >= (unsigned)c.n_pages) wrong = max(wrong, 1);
+            if (i >= 32) {
+                r = rows[i];
+                before = rows[i - 1];
+            }
+            if (r <= before || r >= kPositions - pos0) {
+                wrong = 2;
+            } else {
+                const int from = (pos0 + r) / c.page, to = (pos0 + i) / c.page;      // (to is not above from)
+                const int a = from < A.max_pages ? table[from] : -1, b = from < A.max_pages ? table[to] : -1;
+                if ((unsigned)a >= (unsigned)c.n_pages || (unsigned)b >= (unsigned)c.n_pages) wrong = max(wrong, 1);
+            }
         }
     wrong = __reduce_max_sync(0xffffffffu, wrong);
     if (wrong > 0) {
@@ -127,89 +161,95 @@ __global__ void __launch_bounds__(kKeepWarps * 32) keep_kernel(const __grid_cons
         return;
     }
     if (count == 0) return;
-    const int ld = value ? c.ldv : c.ldk;
-    uint8_t* const codes = value ? L.v : L.k;
-    float* const scales = value ? L.vs : L.ks;
-    const size_t page_bytes = value ? c.v_page : c.k_page, page_scales = value ? c.vs_page : c.ks_page;
-    const int blocks_of_page = c.page / kBlock;
+    const int blocks = g * (c.page / kBlock);
     for (int block = pos0 / kBlock; block <= (pos0 + count - 1) / kBlock; ++block) {
         const int p0 = block * kBlock, lo = max(pos0 - p0, 0), hi = min(pos0 + count - p0, kBlock);
         // lane r: where row r of the block comes from
-        size_t at = 0;
-        float scale = 0.0f;
-        if (lane >= lo && lane < hi) {
-            const int p = pos0 + rows[p0 + lane - pos0], pg = p / c.page, page = table[pg], in_page = p - pg * c.page;
-            at = (size_t)page * page_bytes + ((size_t)g * c.page + in_page) * ld;
-            scale = scales[(size_t)page * page_scales + g * blocks_of_page + in_page / kBlock];
+        int from_page = 0, from_row = 0;
+        const bool mine = lane >= lo && lane < hi;
+        bool moves = lo == 0;      // (rows that stay where they are, in a block whose scale has to stay: nothing to do)
+        if (mine) {
+            const int p = pos0 + rows[p0 + lane - pos0], pg = p / c.page;
+            from_page = table[pg];
+            from_row = p - pg * c.page;
+            moves |= p != p0 + lane;
         }
+        if (!__any_sync(0xffffffffu, moves)) continue;
         const int pg = p0 / c.page, page = table[pg], in_page = p0 - pg * c.page;
-        float* const to_scale = scales + (size_t)page * page_scales + g * blocks_of_page + in_page / kBlock;
-        uint8_t* const to = codes + (size_t)page * page_bytes + ((size_t)g * c.page + in_page) * ld;
-        uint4 x[PASSES];
-        float factor[PASSES];
-        float top = 0.0f;
-        bool nan = false;
+        uint4 x[2][PASSES];
+        float scale[2], had[2];      // lane r: of row r's block; of this block
 #pragma unroll
-        for (int y = 0; y < PASSES; ++y) {
-            const int r = y * ROWS + sub;
-            const size_t from = __shfl_sync(0xffffffffu, at, r);
-            factor[y] = fabsf(__shfl_sync(0xffffffffu, scale, r));
-            x[y] = make_uint4(0u, 0u, 0u, 0u);
-            if (r >= lo && r < hi && piece * 16 < ld) x[y] = *reinterpret_cast<const uint4*>(codes + from + piece * 16);
-        }
+        for (int z = 0; z < 2; ++z) {
+            const int ld = z ? c.ldv : c.ldk;
+            const uint8_t* row = (z ? L.v : L.k) + (size_t)from_page * (z ? c.v_page : c.k_page) + ((size_t)g * c.page + from_row) * ld;
 #pragma unroll
-        for (int y = 0; y < PASSES; ++y) {
-            // magnitudes order as codes do
-            const uint32_t w[4] = {x[y].x, x[y].y, x[y].z, x[y].w};
-            uint32_t most = 0;
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const uint32_t clean = without_nans(w[z]);
-                nan |= clean != w[z];
-                most = __vmaxu4(most, clean & 0x7f7f7f7fu);
+            for (int y = 0; y < PASSES; ++y) {
+                if (y * ROWS >= hi || (y + 1) * ROWS <= lo) continue;
+                const int r = y * ROWS + sub;
+                const uint8_t* at = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), r));
+                x[z][y] = make_uint4(0u, 0u, 0u, 0u);
+                if (r >= lo && r < hi && piece * 16 < ld) x[z][y] = *reinterpret_cast<const uint4*>(at + piece * 16);
             }
-            most = __vmaxu4(most, most >> 16);
-            most = max(most & 0xffu, most >> 8 & 0xffu);
-            top = fmaxf(top, from_e4m3x4(most).x * factor[y]);
+            const float* scales = (z ? L.vs : L.ks) + blocks;
+            const size_t stride = z ? c.vs_page : c.ks_page;
+            scale[z] = mine ? scales[(size_t)from_page * stride + from_row / kBlock] : 0.0f;
+            had[z] = scales[(size_t)page * stride + in_page / kBlock];
         }
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-        nan = __any_sync(0xffffffffu, nan);
-        // bits: m 2^e, 1 <= m < 2, and 448 = 1.75 2^8
-        int E = min(max((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), kLeastExp), kMostExp);
-        if (lo > 0) {
-            // older rows: the scale does not shrink under them, and their codes follow it when it grows
-            const float had = *to_scale;
-            const int Eold = min(max((int)((__float_as_uint(had) >> 23) & 0xffu) - 127, kLeastExp), kMostExp);
-            nan |= had < 0.0f;
-            if (E > Eold) {
+        __syncwarp();      // every lane has read the block
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const int ld = z ? c.ldv : c.ldk;
+            uint8_t* const to = (z ? L.v : L.k) + (size_t)page * (z ? c.v_page : c.k_page) + ((size_t)g * c.page + in_page) * ld;
+            const int Eold = lo > 0 ? min(max((int)((__float_as_uint(had[z]) >> 23) & 0xffu) - 127, kLeastExp), kMostExp) : kLeastExp;
+            int E = Eold;
+            bool nan = lo > 0 && had[z] < 0.0f;
+            if (lo == 0 || __any_sync(0xffffffffu, fabsf(scale[z]) > pow2(Eold) || scale[z] < 0.0f)) {
+                float top = 0.0f;
+                const bool marked = __any_sync(0xffffffffu, scale[z] < 0.0f);      // some row may hold a NaN
+#pragma unroll
+                for (int y = 0; y < PASSES; ++y) {
+                    if (y * ROWS >= hi || (y + 1) * ROWS <= lo) continue;
+                    // magnitudes order as codes do
+                    uint32_t w[4] = {x[z][y].x, x[z][y].y, x[z][y].z, x[z][y].w}, most = 0;
+                    if (marked) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t clean = without_nans(w[i]);
+                            nan |= clean != w[i];
+                            w[i] = clean;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) most = __vmaxu2(most, __vmaxu2(w[i] & 0x007f007fu, w[i] >> 8 & 0x007f007fu));
+                    most = max(most & 0xffffu, most >> 16);
+                    top = fmaxf(top, from_e4m3x4(most).x * fabsf(__shfl_sync(0xffffffffu, scale[z], y * ROWS + sub)));
+                }
+                const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                nan = __any_sync(0xffffffffu, nan);
+                // bits: m 2^e, 1 <= m < 2, and 448 = 1.75 2^8
+                E = max(Eold, min((int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), kMostExp));
+            }
+            if (E > Eold && lo > 0) {
+                // older rows' codes follow the scale that grows
                 const float down = pow2(max(Eold - E, -126));
                 for (int r = sub; r < lo; r += ROWS)
                     if (piece * 16 < ld) {
                         uint4* old = reinterpret_cast<uint4*>(to + (size_t)r * ld + piece * 16);
                         const uint4 w = *old;
-                        auto again = [&](uint32_t q) {
-                            const float4 v = from_e4m3x4(q);
-                            return to_e4m3x4(v.x * down, v.y * down, v.z * down, v.w * down);
-                        };
-                        *old = make_uint4(again(w.x), again(w.y), again(w.z), again(w.w));
+                        *old = rescaled(w, down);
                     }
             }
-            E = max(E, Eold);
-        }
-        __syncwarp();      // every lane has read the block, and its scale
-        const float up = pow2(-E);
+            const float f = fabsf(scale[z]) * pow2(-E);      // lane r: of row r
+            const bool same = __all_sync(0xffffffffu, !mine || f == 1.0f);
 #pragma unroll
-        for (int y = 0; y < PASSES; ++y) {
-            const int r = y * ROWS + sub;
-            if (r < lo || r >= hi || piece * 16 >= ld) continue;
-            const float f = factor[y] * up;
-            auto again = [&](uint32_t q) {
-                const float4 v = from_e4m3x4(q);
-                return to_e4m3x4(v.x * f, v.y * f, v.z * f, v.w * f);
-            };
-            *reinterpret_cast<uint4*>(to + (size_t)r * ld + piece * 16) = make_uint4(again(x[y].x), again(x[y].y), again(x[y].z), again(x[y].w));
+            for (int y = 0; y < PASSES; ++y) {
+                if (y * ROWS >= hi || (y + 1) * ROWS <= lo) continue;
+                const int r = y * ROWS + sub;
+                const float fr = same ? 1.0f : __shfl_sync(0xffffffffu, f, r);
+                if (r >= lo && r < hi && piece * 16 < ld) *reinterpret_cast<uint4*>(to + (size_t)r * ld + piece * 16) = fr == 1.0f ? x[z][y] : rescaled(x[z][y], fr);
+            }
+            if (lane == 0) (z ? L.vs : L.ks)[(size_t)page * (z ? c.vs_page : c.ks_page) + blocks + in_page / kBlock] = nan ? -pow2(E) : pow2(E);
         }
-        if (lane == 0) *to_scale = nan ? -pow2(E) : pow2(E);
         __syncwarp();
     }
 }

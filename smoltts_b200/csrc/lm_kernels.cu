@@ -2393,8 +2393,9 @@ static void push_frequencies(std::vector<float>& table, const SmolLmLayer& L, bo
 extern "C" int smol_lm_abi_version(void) { return SMOL_LM_ABI_VERSION; }
 extern "C" size_t smol_lm_struct_bytes(int which) {
     const size_t bytes[] = {sizeof(SmolLmLayer), sizeof(SmolLmConfig), sizeof(SmolLmGlobals), sizeof(SmolLmStep),
-                            sizeof(SmolLmCache8), sizeof(SmolLmCache8Batch), sizeof(SmolLmCache8Append), sizeof(SmolLmCache8Attend), sizeof(SmolLmCache8Keep)};
-    return which >= 0 && which < 9 ? bytes[which] : 0;
+                            sizeof(SmolLmCache8), sizeof(SmolLmCache8Batch), sizeof(SmolLmCache8Append), sizeof(SmolLmCache8Attend), sizeof(SmolLmCache8Keep),
+                            sizeof(SmolLmCache8Tree)};
+    return which >= 0 && which < 10 ? bytes[which] : 0;
 }
 extern "C" const char* smol_lm_last_error(void) { return g_err.c_str(); }
 

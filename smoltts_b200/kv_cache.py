@@ -40,7 +40,8 @@ _BATCH = struct.Struct("@5i4P")
 _APPEND = struct.Struct("@i2P4Ni2P4N2iPf2Pi0P")
 _ATTEND = struct.Struct("@2i2P4N3f2i5PN2Pi0P")
 _KEEP = struct.Struct("@3i4P")
-for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCache8Append), (_ATTEND, _capi_lm.SmolLmCache8Attend), (_KEEP, _capi_lm.SmolLmCache8Keep)):
+_TREE = struct.Struct("@4i6P")
+for _s, _m in ((_BATCH, _capi_lm.SmolLmCache8Batch), (_APPEND, _capi_lm.SmolLmCache8Append), (_ATTEND, _capi_lm.SmolLmCache8Attend), (_KEEP, _capi_lm.SmolLmCache8Keep), (_TREE, _capi_lm.SmolLmCache8Tree)):
     assert _s.size == C.sizeof(_m)
 
 
@@ -50,6 +51,35 @@ def _pack(layout: struct.Struct, *fields) -> bytes:
         return layout.pack(*fields)
     except struct.error as e:
         raise ValueError(f"an integer outside its range: {e}") from e
+
+
+# The library's entries, with arguments that are packed structs (functions of this module's own).
+_ENTRIES: Dict[str, C._CFuncPtr] = {}
+_ARGUMENTS = {
+    "append": [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p], "attend": [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p],
+    "workspace_bytes": [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p], "tree": [C.c_char_p, C.c_void_p], "keep": [C.c_char_p, C.c_int32, C.c_char_p, C.c_void_p],
+    "copy_pages": [C.c_char_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p],
+}
+
+
+def _entry(name: str):
+    call = _ENTRIES.get(name)
+    if call is None:
+        call = _capi_lm.load()["smol_lm_cache8_" + name]
+        call.argtypes = _ARGUMENTS[name]
+        _ENTRIES[name] = call
+    return call
+
+
+def _on_device(index: int, call, *args) -> None:
+    """On the device and its current stream."""
+    if index == torch._C._cuda_getDevice():      # (a few tenths of a microsecond; torch.cuda's own two functions take four)
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != SMOL_OK:
+        _capi_lm.check(rc)
 
 
 def _float(x: float, what: str) -> float:
@@ -115,12 +145,7 @@ class KVCache8:
         self._err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._c = bytes(_capi_lm.SmolLmCache8(k=k.data_ptr(), v=v.data_ptr(), k_scale=k_scale.data_ptr(), v_scale=v_scale.data_ptr(), n_pages=n, page_size=page,
                                               kv_heads=g, dim=self.dim, vdim=self.vdim, err=self._err.data_ptr()))
-        lib = _capi_lm.load()
-        # (functions of this module's own: their arguments are packed structs)
-        self._append, self._attend, self._workspace = lib["smol_lm_cache8_append"], lib["smol_lm_cache8_attend"], lib["smol_lm_cache8_workspace_bytes"]
-        self._append.argtypes = [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p]
-        self._attend.argtypes = [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p]
-        self._workspace.argtypes = [C.c_char_p, C.c_char_p, C.c_char_p, C.c_void_p]
+        self._append, self._attend, self._workspace = (_entry(x) for x in ("append", "attend", "workspace_bytes"))
         self._need: Dict[tuple, int] = {}      # bytes of workspace by what they depend on
 
     @classmethod
@@ -169,14 +194,7 @@ class KVCache8:
                      self._ints(block_table, (n, pages), "block_table"), 0 if kv_len is None else self._ints(kv_len, (n,), "kv_len"))
 
     def _call(self, call, *args) -> None:
-        """On the cache's device and its current stream."""
-        if self._index == torch._C._cuda_getDevice():      # (a few tenths of a microsecond; torch.cuda's own two functions take four)
-            rc = call(self._c, *args, torch._C._cuda_getCurrentRawStream(self._index))
-        else:
-            with torch.cuda.device(self._index):
-                rc = call(self._c, *args, torch._C._cuda_getCurrentRawStream(self._index))
-        if rc != SMOL_OK:
-            _capi_lm.check(rc)
+        _on_device(self._index, call, self._c, *args)
 
     # ------------------------------------------------------------------ operators
     def append(self, k: torch.Tensor, v: torch.Tensor, seq_start: torch.Tensor, seq_pos0: torch.Tensor, block_table: torch.Tensor, max_new: int,
@@ -301,11 +319,9 @@ class KVCache8:
         if not 1 <= max_new <= MOST_DRAFTED:
             raise ValueError(f"max_new must be from 1 to {MOST_DRAFTED}")
         tokens, n, words = parents.shape[0], seq_pos0.shape[0], (max_new + 31) // 32
-        at = [self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"), self._ints(parents, (tokens,), "parents")]
+        at = self._ints(seq_start, (n + 1,), "seq_start"), self._ints(seq_pos0, (n,), "seq_pos0"), self._ints(parents, (tokens,), "parents")
         tree = DraftTree(parents.new_empty(tokens), parents.new_empty((tokens, words)))
-        with torch.cuda.device(self._index):
-            _capi_lm.check(_capi_lm.load().smol_lm_cache8_tree(tokens, n, max_new, *at, tree.positions.data_ptr(), tree.sees.data_ptr(), words, self._err.data_ptr(),
-                                                               torch._C._cuda_getCurrentRawStream(self._index)))
+        _on_device(self._index, _entry("tree"), _pack(_TREE, tokens, n, max_new, words, *at, tree.positions.data_ptr(), tree.sees.data_ptr(), self._err.data_ptr()))
         return tree
 
     # ------------------------------------------------------------------ looking in
@@ -330,20 +346,19 @@ def _layers(caches: Union[KVCache8, Sequence[KVCache8]]) -> List[KVCache8]:
     caches = [caches] if isinstance(caches, KVCache8) else list(caches)
     if not caches:
         raise ValueError("no cache")
-    if any(c.device != caches[0].device for c in caches):
+    if len({c._index for c in caches}) > 1:
         raise ValueError("caches of several devices")
     return caches
 
 
 def _call_layers(call, caches: List[KVCache8], *args) -> None:
     """On the caches' device and its current stream.  What is refused on the host is the caller's."""
-    index = caches[0]._index
-    with torch.cuda.device(index):
-        rc = call(b"".join([c._c for c in caches]), len(caches), *args, torch._C._cuda_getCurrentRawStream(index))
-    if rc == SMOL_ERR_INVALID:
-        raise ValueError(_capi_lm.load().smol_lm_last_error().decode())
-    if rc != SMOL_OK:
-        _capi_lm.check(rc)
+    try:
+        _on_device(caches[0]._index, call, b"".join([c._c for c in caches]), len(caches), *args)
+    except SmolError as e:
+        if e.code == SMOL_ERR_INVALID:
+            raise ValueError(str(e)) from e
+        raise
 
 
 def keep_rows(caches: Union[KVCache8, Sequence[KVCache8]], seq_pos0: torch.Tensor, block_table: torch.Tensor, rows: torch.Tensor, counts: torch.Tensor) -> None:
@@ -360,7 +375,7 @@ def keep_rows(caches: Union[KVCache8, Sequence[KVCache8]], seq_pos0: torch.Tenso
     n, most = rows.shape
     a = _pack(_KEEP, n, block_table.shape[1], most, c._ints(seq_pos0, (n,), "seq_pos0"), c._ints(block_table, (n, block_table.shape[1]), "block_table"), c._ints(rows, (n, most), "rows"),
               c._ints(counts, (n,), "counts"))
-    _call_layers(_packed_keep(), layers, a)
+    _call_layers(_entry("keep"), layers, a)
 
 
 def copy_pages(caches: Union[KVCache8, Sequence[KVCache8]], src: Sequence[int], dst: Sequence[int]) -> None:
@@ -376,11 +391,4 @@ def copy_pages(caches: Union[KVCache8, Sequence[KVCache8]], src: Sequence[int], 
     if len(a) != len(b):
         raise ValueError(f"{len(a)} pages to {len(b)}")
     if a:
-        _call_layers(_capi_lm.load().smol_lm_cache8_copy_pages, layers, a.buffer_info()[0], b.buffer_info()[0], len(a))
-
-
-def _packed_keep():
-    """``smol_lm_cache8_keep`` with its arguments as packed structs."""
-    call = _capi_lm.load()["smol_lm_cache8_keep"]
-    call.argtypes = [C.c_char_p, C.c_int32, C.c_char_p, C.c_void_p]
-    return call
+        _call_layers(_entry("copy_pages"), layers, a.buffer_info()[0], b.buffer_info()[0], len(a))

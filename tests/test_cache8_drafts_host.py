@@ -12,7 +12,7 @@ P = 1 << 20
 def tree(**over):
     a = dict(n_tokens=5, n_seqs=2, max_new=3, seq_start=P, seq_pos0=P, parents=P, positions=P, sees=P, words=1, err=P)
     a.update(over)
-    return cl.load().smol_lm_cache8_tree(*a.values(), None)
+    return cl.load().smol_lm_cache8_tree(ctypes.byref(cl.SmolLmCache8Tree(**a)), None)
 
 
 @pytest.mark.parametrize("field,value,code", [("n_tokens", 0, -1), ("n_seqs", 0, -1), ("max_new", 0, -1), ("max_new", 4097, -5), ("max_new", 33, -1), ("words", 0, -1), ("seq_start", None, -1),
