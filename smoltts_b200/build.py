@@ -26,9 +26,9 @@ LM_LIB_PATH = os.path.join(LIB_DIR, "libsmoltts_b200_lm.so")
 # target -> (library, stamp, sources, headers)
 TARGETS = {
     "core": (LIB_PATH, STAMP, SOURCES, HEADERS),
-    "lm": (LM_LIB_PATH, os.path.join(LIB_DIR, "build_lm.stamp"), ["lm_kernels.cu", "cache8.cu", "cache8_drafts.cu"],
+    "lm": (LM_LIB_PATH, os.path.join(LIB_DIR, "build_lm.stamp"), ["lm_kernels.cu", "cache8.cu", "cache8_drafts.cu", "cache8_quads.cu"],
            ["common.cuh", "dev_model.h", "f32_tile.cuh", "sampler.cuh", "umma.cuh", "tmap_host.h", "lm_gemm_tc.cuh", "lm_flash_tc.cuh", "lm_quad_scan.cuh", "lm_chunk_scan.cuh", "lm_mechanisms.cuh", "lm_sigmoid_linear.cuh", "lm_delta_mlstm.cuh",
-            "cache8.cuh", "cache8_append.cuh", "cache8_rows.cuh", "cache8_few.cuh", "cache8_tiles.cuh", "cache8_tc.cuh", "cache8_launch.cuh", "cache8_moves.cuh", "lm_report.h",
+            "cache8.cuh", "cache8_append.cuh", "cache8_rows.cuh", "cache8_few.cuh", "cache8_tiles.cuh", "cache8_tc.cuh", "cache8_launch.cuh", "cache8_quads.cuh", "cache8_moves.cuh", "lm_report.h",
             os.path.join("..", "..", "include", "smoltts_b200.h"), os.path.join("..", "..", "include", "smoltts_b200_lm.h")]),
 }
 

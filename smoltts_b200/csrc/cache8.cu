@@ -47,10 +47,12 @@ static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     // as many shares as the SMs hold blocks at once, none of less than 256 keys (a token of 12 heads at 2048 positions, appended and
     // attended to: 10.9 us; with shares of 128, which are one step, 11.5; of 512 12.7).  More blocks than are held at once wait for whole others: one sequence at
     // 131072 34 us in 111 shares, 43 in 128.
-    const int held = f32 ? 2 : tiles ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
+    const int held = f32 ? 2 : tiles || quads_serve(A, f32) ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
     const long long slots = (long long)held * n_sms;
     auto at_once = [&](long long blocks) { return std::max(1ll, std::min({slots / blocks, (keys + 255) / 256, (long long)kMaxSplits})); };
-    const long long want = at_once(base);
+    long long want = at_once(base);
+    // (a little more than a cluster joins: without the other launch, and the shares' way through memory)
+    if (A.tree_pos && want > kMostCluster && want <= 2 * kMostCluster && joins_in_cluster(A, kMostCluster, f32)) want = kMostCluster;
     if (halves == 1) return (int)want;
     // Values of more than 128 columns take two blocks a tile, and so at most half as many shares at once: often fewer SMs at work, where two rounds of shorter shares may
     // take less time for all that they and their join cost.  In keys, with a block's own start at 512 and the join at 2048: 300 rows of 16 and 8 heads, 80 blocks, one share /
@@ -80,11 +82,12 @@ cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* laun
     if (two) A.rows_over = kFewMost;
     A.n_splits = splits_for(A, f32, n_sms);
     A.part = static_cast<float*>(workspace);
+    A.in_cluster = joins_in_cluster(A, A.n_splits, f32);
     if (cudaError_t e = A.tree_pos ? (f32 ? attend_tree_rows(A, st) : tiles_serve(A, f32) ? attend_tree_tiles(A, st) : attend_tree_few(A, st))
                                    : (f32 ? attend_rows<false>(A, st) : tiles_serve(A, f32) ? attend_tiles<false>(A, st) : attend_few<false>(A, st)))
         return e;
     *launches += 1;
-    if (A.n_splits > 1 && !joins_in_cluster(A, A.n_splits, f32)) {
+    if (A.n_splits > 1 && !A.in_cluster) {
         *launches += 1;
         if (cudaError_t e = f32 ? launch(attend_join_kernel<float>, A.b.T * A.H, kJoinWarps * 32, 0, st, A) : launch(attend_join_kernel<bf16>, A.b.T * A.H, kJoinWarps * 32, 0, st, A)) return e;
     }
@@ -93,6 +96,7 @@ cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* laun
     few.b.max_new = kFewMost / (A.H / A.c.G);
     few.n_splits = std::min(splits_for(few, f32, n_sms), kMostCluster);      // (joined without the workspace, which the tiles' shares may be in)
     few.part = nullptr;
+    few.in_cluster = few.n_splits > 1;
     *launches += 1;
     return A.tree_pos ? attend_tree_few(few, st) : attend_few<false>(few, st);
 }

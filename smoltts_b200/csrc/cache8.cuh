@@ -88,6 +88,7 @@ struct AttendArgs {
     const int32_t* tree_pos;         // rows of a tree: their positions [T] (nullptr: no tree, a row's position is its place in the cache) ...
     const uint32_t* tree_sees;       // ... and which of their sequence's rows they see [T][tree_words], a bit each
     int tree_words;
+    int in_cluster;                  // the shares are joined inside a cluster of blocks
 };
 
 constexpr int kMaxSplits = 128;
@@ -141,6 +142,7 @@ size_t attend_bytes_most(int dv);
 cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* launches, cudaStream_t st);
 // The kernels for rows of a tree (cache8_drafts.cu).
 cudaError_t attend_tree_few(const AttendArgs& A, cudaStream_t st);
+cudaError_t attend_tree_quads(const AttendArgs& A, cudaStream_t st);      // (cache8_quads.cu)
 cudaError_t attend_tree_tiles(const AttendArgs& A, cudaStream_t st);
 cudaError_t attend_tree_rows(const AttendArgs& A, cudaStream_t st);
 // What a caller that fills the structs itself leaves to be worked out: whether rows are whole, aligned pieces; the positions that a block table's row names.

@@ -18,7 +18,9 @@ namespace c8 {
 
 using lm::report;
 
-cudaError_t attend_tree_few(const AttendArgs& A, cudaStream_t st) { return attend_few<true>(A, st); }
+cudaError_t attend_tree_few(const AttendArgs& A, cudaStream_t st) {
+    return quads_serve(A, false) ? attend_tree_quads(A, st) : attend_few<true>(A, st);
+}
 cudaError_t attend_tree_tiles(const AttendArgs& A, cudaStream_t st) { return attend_tiles<true>(A, st); }
 cudaError_t attend_tree_rows(const AttendArgs& A, cudaStream_t st) { return attend_rows<true>(A, st); }
 

@@ -122,6 +122,57 @@ __device__ __forceinline__ float of_rank(const float* mine, int rank) {      // 
 }
 constexpr int kMostCluster = 8;      // shares of the keys that are joined inside a cluster of blocks; more go through memory and attend_join_kernel
 
+// The shares of a cluster of blocks are joined: block `split` of them has rows split, split + n_splits, ...; by THREADS threads of every block.  stat, joint: a row's maximum, denominator and e in
+// each block, and its unnormalised results; the other arrays are the block's own.  What the shares of a row count and what its results are multiplied by is worked out by a thread each.
+template <int THREADS>
+__device__ __forceinline__ void join_shares(const AttendArgs& A, int split, int rows, const float4* stat, const float* joint, int ld, const int* s_row, const int* s_head, float2* finish, size_t* to,
+                                            float (*counts)[kMostCluster]) {
+    const int me = threadIdx.x, count = rows > split ? (rows - split + A.n_splits - 1) / A.n_splits : 0;
+    if (me < count) {
+        const int r = split + me * A.n_splits, h = s_head[r];
+        float top[kMostCluster], f[kMostCluster], e[kMostCluster];
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) {
+            const float4 of = z < A.n_splits ? of_rank(&stat[r], z) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            top[z] = of.x;
+            f[z] = of.y;
+            e[z] = of.z;
+        }
+        float M = -INFINITY, E = -INFINITY, least = INFINITY, total = 0.0f;
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) {
+            M = fmaxf(M, top[z]);
+            E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z]);
+            least = fminf(least, top[z] == -INFINITY ? INFINITY : e[z]);
+        }
+        if (E - least > kNear) {      // (units far apart: not the largest, but that of the largest results)
+            E = -INFINITY;
+            for (int z = 0; z < kMostCluster; ++z) E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z] + (top[z] - M));
+        }
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) {
+            // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
+            total = fmaf(f[z], top[z] == -INFINITY ? (f[z] == 0.0f ? 0.0f : f[z]) : exp2_fast(top[z] - M), total);
+            counts[me][z] = top[z] == -INFINITY ? 0.0f : exp2_fast((e[z] - E) + (top[z] - M));
+        }
+        const Finish fin(A, h, M, total, E);
+        finish[me] = make_float2(fin.a, fin.b);
+        to[me] = (size_t)s_row[r] * A.o_row + (size_t)h * A.o_head;
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+#pragma unroll 2
+    for (int i = me; i < count * A.c.dv; i += THREADS) {
+        const int at = i / A.c.dv, col = i - at * A.c.dv, r = split + at * A.n_splits;
+        float v[kMostCluster], sum = 0.0f;
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) v[z] = z < A.n_splits ? of_rank(joint + r * ld + col, z) : 0.0f;
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) sum = fmaf(v[z], counts[at][z], sum);
+        const float2 f = finish[at];
+        static_cast<bf16*>(A.out)[to[at] + col] = __float2bfloat16_rn(finished(A, s_row[r], s_head[r], col, sum * f.x * f.y));
+    }
+}
+
 // D: head sizes padded (both); RA: query rows; BENT: soft cap or distance penalties; TREE: rows of a tree
 template <int D, int RA, bool BENT, bool TREE>
 __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
@@ -131,6 +182,9 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     __shared__ StepScales s_scales[NS];
     __shared__ float s_top[2][4][RA], s_rowmul[RA], s_sum[4][RA], s_r1[RA], s_r2[RA], s_slope[RA];
     __shared__ float4 s_stat[RA];      // of this block's share: maximum, denominator, e
+    __shared__ float2 s_finish[RA];    // what finished results are multiplied by, and where they go
+    __shared__ size_t s_to[RA];
+    __shared__ float s_counts[RA][kMostCluster];      // what the shares of the keys count
     __shared__ float s_far[2][4][RA], s_step_unit[2][RA], s_unit[2][RA];      // (value scales far apart)
     __shared__ int s_apart[2];      // some thread has met one: in even and odd steps, so that the next step's is written while this one's is read
     __shared__ int s_pos[RA], s_row[RA], s_head[RA], s_bad;      // positions; the step's rows; heads
@@ -167,8 +221,8 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     }
     const Seen seen = seen_steps(A, first_pos, behind, kv_len);
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
-    const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = min(split * share, seen.count);
-    const int steps = any ? min(lo + share, seen.count) - lo : 0;
+    const int share = (seen.count + A.n_splits - 1) / A.n_splits, lo = TREE ? (int)((long long)split * seen.count / A.n_splits) : min(split * share, seen.count);
+    const int steps = any ? (TREE ? (int)((long long)(split + 1) * seen.count / A.n_splits) : min(lo + share, seen.count)) - lo : 0;
     const bool clustered = A.n_splits > 1 && A.n_splits <= kMostCluster;
     float* joint = reinterpret_cast<float*>(KV);      // [row][D], once everything has been multiplied
     // a finished row's column, and a column of this block's share of the keys: maximum, denominator, unnormalised result in units of 2^(top + e)
@@ -385,11 +439,23 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             }
             const bool whole = j0 + kStep <= min(clear, seen.end) && (A.window == 0 || j0 > last_pos - A.window || j0 + kStep <= A.first);
             bool hidden = ks == 0.0f;      // from some row
-            if (!whole || hidden) {
+            if (TREE && !whole) {
+                // (all rows' bits on their way at once: one row after the other took 5600 cycles for 16)
+                const bool there = ks != 0.0f && j < seen.end;
+                const int row = j - pos0;      // of the sequence's rows (below 0: the context)
+                uint32_t named[RA];
+#pragma unroll
+                for (int r = 0; r < RA; ++r) named[r] = there && row >= 0 ? A.tree_sees[(size_t)s_row[r] * A.tree_words + (row >> 5)] : 0xffffffffu;
 #pragma unroll
                 for (int r = 0; r < RA; ++r) {
-                    bool on = ks != 0.0f && (TREE ? j < seen.end && (A.window == 0 || s_pos[r] - key < A.window || key < A.first) : sees(A, s_pos[r], j, seen.end));
-                    if (TREE && on && j >= pos0) on = A.tree_sees[(size_t)s_row[r] * A.tree_words + ((j - pos0) >> 5)] >> ((j - pos0) & 31) & 1u;
+                    const bool on = there && (named[r] >> (row & 31) & 1u) && (A.window == 0 || s_pos[r] - key < A.window || key < A.first);
+                    hidden |= !on;
+                    S[r] = on ? S[r] : -INFINITY;
+                }
+            } else if (!whole || hidden) {
+#pragma unroll
+                for (int r = 0; r < RA; ++r) {
+                    const bool on = ks != 0.0f && (TREE || sees(A, s_pos[r], j, seen.end));
                     hidden |= !on;
                     S[r] = on ? S[r] : -INFINITY;
                 }
@@ -476,11 +542,31 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
         }
         if (apart_step) sync4();
         join_product(steps - 1);
-        // ---- a column of the result per thread: written, put down as this share's, or left in shared memory for the cluster ----
+        // ---- a column of the result per thread: written, put down as this share's, or left in shared memory for the cluster.  What a row's results are multiplied by and where they go
+        // is worked out by a thread each (all rows by every thread: 11200 cycles for 16) ----
 #pragma unroll
         for (int r = 0; r < RA; ++r) {
             const float total = warp_sum(l[r]);
             if (lane == 0) s_sum[warp][r] = total;
+        }
+        sync4();
+        if (me < rows) {
+            float top = 0.0f;
+#pragma unroll
+            for (int r = 0; r < RA; ++r) top = me == r ? m[r] : top;
+            if (!apart_step) top -= unit;
+            const float total = (s_sum[0][me] + s_sum[1][me]) + (s_sum[2][me] + s_sum[3][me]), e = (apart_step ? s_unit[steps & 1][me] : unit) - 8.0f;
+            if (A.n_splits == 1) {
+                const Finish f(A, s_head[me], top, total, e);
+                s_finish[me] = make_float2(f.a, f.b);
+                s_to[me] = (size_t)s_row[me] * A.o_row + (size_t)s_head[me] * A.o_head;
+            } else if (clustered) {
+                s_stat[me] = make_float4(top, total, e, 0.0f);
+            } else {
+                const size_t at = ((size_t)s_row[me] * A.H + s_head[me]) * A.n_splits + split;
+                part_stats(A)[at] = make_float4(top, total, e, 0.0f);
+                s_to[me] = at * ((A.c.dv + 3) / 4 * 4);
+            }
         }
         sync4();
 #pragma unroll
@@ -488,10 +574,30 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
             const int col = x * 128 + me;
             if (col >= A.c.dv || *stop) continue;
             const uint32_t nans = s_bad ? nan_columns<RA, TREE>(A, W, col) : 0u;
+            if (nans != 0u) {
 #pragma unroll
-            for (int r = 0; r < RA; ++r) {
-                if (r >= rows) break;
-                put(r, col, apart_step ? m[r] : m[r] - unit, (s_sum[0][r] + s_sum[1][r]) + (s_sum[2][r] + s_sum[3][r]), (apart_step ? s_unit[steps & 1][r] : unit) - 8.0f, nans >> r & 1 ? __int_as_float(0x7fffffff) : o[x][r]);
+                for (int r = 0; r < RA; ++r) o[x][r] = nans >> r & 1 ? __int_as_float(0x7fffffff) : o[x][r];
+            }
+            if (clustered || (A.n_splits == 1 && A.gate)) {
+#pragma unroll
+                for (int r = 0; r < RA; ++r) joint[r * D + col] = o[x][r];
+            }
+            if (A.n_splits == 1 && A.gate) {
+#pragma unroll 1
+                for (int r = 0; r < rows; ++r) {
+                    const float2 f = s_finish[r];
+                    static_cast<bf16*>(A.out)[s_to[r] + col] = __float2bfloat16_rn(finished(A, s_row[r], s_head[r], col, joint[r * D + col] * f.x * f.y));
+                }
+            } else if (A.n_splits == 1) {
+#pragma unroll
+                for (int r = 0; r < RA; ++r) {
+                    const float2 f = s_finish[r];
+                    if (r < rows) static_cast<bf16*>(A.out)[s_to[r] + col] = __float2bfloat16_rn(o[x][r] * f.x * f.y * A.out_scale);
+                }
+            } else if (!clustered) {
+#pragma unroll
+                for (int r = 0; r < RA; ++r)
+                    if (r < rows) A.part[s_to[r] + col] = o[x][r];
             }
         }
     } else if (any) {
@@ -510,44 +616,7 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     __syncwarp();
     if (clustered) {
         cluster_sync();
-        if (any && warp < 4 && !*stop)
-            for (int r = split; r < rows; r += A.n_splits) {
-                float top[kMostCluster], f[kMostCluster], e[kMostCluster], v[D / 128][kMostCluster];
-#pragma unroll
-                for (int z = 0; z < kMostCluster; ++z) {
-                    const bool on = z < A.n_splits;
-                    const float4 stat = on ? of_rank(&s_stat[r], z) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
-                    top[z] = stat.x;
-                    f[z] = stat.y;
-                    e[z] = stat.z;
-#pragma unroll
-                    for (int x = 0; x < D / 128; ++x) v[x][z] = on && threadIdx.x + 128 * x < A.c.dv ? of_rank(joint + r * D + threadIdx.x + 128 * x, z) : 0.0f;
-                }
-                float M = -INFINITY, E = -INFINITY, least = INFINITY, total = 0.0f;
-#pragma unroll
-                for (int z = 0; z < kMostCluster; ++z) {
-                    M = fmaxf(M, top[z]);
-                    E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z]);
-                    least = fminf(least, top[z] == -INFINITY ? INFINITY : e[z]);
-                }
-                if (E - least > kNear) {      // (units far apart: not the largest, but that of the largest results)
-                    E = -INFINITY;
-                    for (int z = 0; z < kMostCluster; ++z) E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z] + (top[z] - M));
-                }
-#pragma unroll
-                for (int z = 0; z < kMostCluster; ++z) {
-                    // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
-                    total = fmaf(f[z], top[z] == -INFINITY ? (f[z] == 0.0f ? 0.0f : f[z]) : exp2_fast(top[z] - M), total);
-                    e[z] = top[z] == -INFINITY ? 0.0f : exp2_fast((e[z] - E) + (top[z] - M));
-                }
-#pragma unroll
-                for (int x = 0; x < D / 128; ++x) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int z = 0; z < kMostCluster; ++z) sum = fmaf(v[x][z], e[z], sum);
-                    if (threadIdx.x + 128 * x < A.c.dv) store(r, threadIdx.x + 128 * x, M, total, E, sum);
-                }
-            }
+        if (any && warp < 4 && !*stop) join_shares<128>(A, split, rows, s_stat, joint, D, s_row, s_head, s_finish, s_to, s_counts);
         cluster_sync();      // nobody leaves while others read
     }
     __syncwarp();

@@ -55,7 +55,14 @@ static cudaError_t more_smem(K kernel, int bytes, std::atomic<uint64_t>& asked) 
 // to fill the GPU the keys' shares are what counts: one at 2048 with 32 rows 16.6 / 16.6, with 64 18.1 / 19.6, with 96 33 / 21.
 constexpr int kFewMost = 16, kFewMostSmall = 64;
 constexpr long long kSmall = 1 << 16;      // sequences times heads times positions (16384: the last of these; 262144: the one at 32768)
+// Rows of a tree that the kernel for 32 rows takes (cache8_quads.cuh), and otherwise one of those for few or many.
+constexpr int kQuadLeast = 8, kQuadMost = 64, kQuadRows = 32;
+inline bool quads_serve(const AttendArgs& A, bool f32) {
+    const long long rows = A.b.max_new * (long long)(A.H / A.c.G);
+    return A.tree_pos && !f32 && std::max(A.c.d, A.c.dv) <= 128 && rows > kQuadLeast && rows <= kQuadMost;
+}
 inline bool tiles_serve(const AttendArgs& A, bool f32) {
+    if (quads_serve(A, f32)) return false;
     const long long rows = A.b.max_new * (long long)(A.H / A.c.G), most = (long long)A.b.S * A.c.G * A.b.max_len <= kSmall ? kFewMostSmall : kFewMost;
     return !f32 && rows > most;
 }
@@ -63,7 +70,7 @@ inline bool tiles_serve(const AttendArgs& A, bool f32) {
 // query rows of a block of threads
 static int row_tile(const AttendArgs& A, bool f32) {
     const long long rows = A.b.max_new * (long long)(A.H / A.c.G);
-    return f32 ? kRowTile : rows <= 4 ? 4 : rows <= 8 ? 8 : tiles_serve(A, f32) ? kTileRows : 16;
+    return f32 ? kRowTile : quads_serve(A, f32) ? kQuadRows : rows <= 4 ? 4 : rows <= 8 ? 8 : tiles_serve(A, f32) ? kTileRows : 16;
 }
 static int row_tiles(const AttendArgs& A, bool f32) { return (int)((A.b.max_new * (long long)(A.H / A.c.G) + row_tile(A, f32) - 1) / row_tile(A, f32)); }
 
@@ -79,7 +86,13 @@ static bool codes_map(CUtensorMap* map, const uint8_t* base, int ld, size_t page
 // positions that lie together and begin at a multiple of themselves: the largest power of two that divides the page, at most a step's
 static int box_of(const Cache& c) { return std::min(c.page & -c.page, kStep); }
 
-static bool joins_in_cluster(const AttendArgs& A, int splits, bool f32) { return !f32 && !tiles_serve(A, f32) && splits > 1 && splits <= kMostCluster; }
+// A block of 32 rows has an SM to itself, and a cluster's blocks have to lie in one part of the GPU: more than some 96 of them are not held at once (16 clusters of 8, 64 rows behind
+// 32768 positions: 78 us; in nine shares through memory 40).
+constexpr int kQuadClusters = 96;
+static bool joins_in_cluster(const AttendArgs& A, int splits, bool f32) {
+    if (quads_serve(A, f32) && (long long)A.b.S * A.c.G * row_tiles(A, f32) * splits > kQuadClusters) return false;
+    return !f32 && !tiles_serve(A, f32) && splits > 1 && splits <= kMostCluster;
+}
 
 template <int D, int RA, bool BENT, bool TREE>
 static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
@@ -95,7 +108,12 @@ static cudaError_t few_as(const AttendArgs& A, cudaStream_t st) {
 template <int D, int RA, bool TREE>
 static cudaError_t few_of(const AttendArgs& A, cudaStream_t st) { return plain_scores(A) ? few_as<D, RA, false, TREE>(A, st) : few_as<D, RA, true, TREE>(A, st); }
 template <int D, bool TREE>
-static cudaError_t few_rows(const AttendArgs& A, cudaStream_t st) { return row_tile(A, false) == 4 ? few_of<D, 4, TREE>(A, st) : row_tile(A, false) == 8 ? few_of<D, 8, TREE>(A, st) : few_of<D, 16, TREE>(A, st); }
+static cudaError_t few_rows(const AttendArgs& A, cudaStream_t st) {
+    if (row_tile(A, false) == 4) return few_of<D, 4, TREE>(A, st);
+    if (row_tile(A, false) == 8) return few_of<D, 8, TREE>(A, st);
+    if constexpr (TREE && D <= 128) return cudaErrorInvalidValue;      // (the kernel for 32 rows)
+    else return few_of<D, 16, TREE>(A, st);
+}
 template <bool TREE>
 static cudaError_t attend_few(const AttendArgs& A, cudaStream_t st) { return std::max(A.c.d, A.c.dv) <= 128 ? few_rows<128, TREE>(A, st) : few_rows<256, TREE>(A, st); }
 

@@ -119,6 +119,20 @@ __device__ __forceinline__ bool tree_sees(const AttendArgs& A, int t0, int pos0,
     const int key = tree_key(A, t0, pos0, j);
     return pos - key < A.window || key < A.first;
 }
+// which of the 32 keys from place jc on row tok sees.  (A call, so that the loops around it keep their registers.)
+static __device__ __noinline__ uint32_t tree_mask(const AttendArgs& A, int t0, int pos0, int tok, int pos, int jc, int end) {
+    const int i0 = jc - pos0, w = i0 >> 5;      // (of the sequence's rows; below 0: the context, all of it.  Rounded down)
+    const uint32_t* bits = A.tree_sees + (size_t)tok * A.tree_words;
+    const uint32_t low = w < 0 ? 0xffffffffu : w < A.tree_words ? bits[w] : 0u, high = w + 1 < 0 ? 0xffffffffu : w + 1 < A.tree_words ? bits[w + 1] : 0u;
+    uint32_t mask = __funnelshift_r(low, high, i0 & 31);
+    if (end < jc + 32) mask = end <= jc ? 0u : mask & (1u << (end - jc)) - 1u;
+    if (A.window > 0)
+        for (int e = 0; e < 32; ++e) {
+            const int key = jc + e < end ? tree_key(A, t0, pos0, jc + e) : 0;
+            if (pos - key >= A.window && key >= A.first) mask &= ~(1u << e);
+        }
+    return mask;
+}
 // Sequences of a tree lie behind a context of no fewer than zero positions.
 __device__ __forceinline__ bool tree_fits(const AttendArgs& A, int pos0, int n) {
     if (pos0 >= 0) return true;

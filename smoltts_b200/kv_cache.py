@@ -296,7 +296,7 @@ class KVCache8:
             tree_pos, tree_sees = self._ints(tree.positions, (tokens,), "tree.positions"), self._ints(tree.sees, (tokens, words), "tree.sees")
         a = _pack(_ATTEND, _DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else _float(scale, "scale"), _float(softcap, "softcap"), 1.0,
                   window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0, tree_pos, tree_sees, words)
-        key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first)
+        key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first, words)
         need = self._need.get(key)
         if need is None:
             size = C.c_size_t()
