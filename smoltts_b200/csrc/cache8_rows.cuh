@@ -119,12 +119,16 @@ __device__ __forceinline__ bool tree_sees(const AttendArgs& A, int t0, int pos0,
     const int key = tree_key(A, t0, pos0, j);
     return pos - key < A.window || key < A.first;
 }
-// which of the 32 keys from place jc on row tok sees.  (A call, so that the loops around it keep their registers.)
-static __device__ __noinline__ uint32_t tree_mask(const AttendArgs& A, int t0, int pos0, int tok, int pos, int jc, int end) {
-    const int i0 = jc - pos0, w = i0 >> 5;      // (of the sequence's rows; below 0: the context, all of it.  Rounded down)
+// which of the 32 keys from row i0 of the sequence's rows on (below 0: of the context, all of it) the bits of row tok name
+__device__ __forceinline__ uint32_t tree_named(const AttendArgs& A, int tok, int i0) {
+    const int w = i0 >> 5;      // (rounded down)
     const uint32_t* bits = A.tree_sees + (size_t)tok * A.tree_words;
     const uint32_t low = w < 0 ? 0xffffffffu : w < A.tree_words ? bits[w] : 0u, high = w + 1 < 0 ? 0xffffffffu : w + 1 < A.tree_words ? bits[w + 1] : 0u;
-    uint32_t mask = __funnelshift_r(low, high, i0 & 31);
+    return __funnelshift_r(low, high, i0 & 31);
+}
+// which of the 32 keys from place jc on row tok sees.  (A call, so that the loops around it keep their registers.)
+static __device__ __noinline__ uint32_t tree_mask(const AttendArgs& A, int t0, int pos0, int tok, int pos, int jc, int end) {
+    uint32_t mask = tree_named(A, tok, jc - pos0);
     if (end < jc + 32) mask = end <= jc ? 0u : mask & (1u << (end - jc)) - 1u;
     if (A.window > 0)
         for (int e = 0; e < 32; ++e) {
@@ -443,10 +447,11 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
     __syncthreads();
 
     float r1[2], r2[2], slope[2];
-    int pos[2];
+    int pos[2], tok[2];
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
         const int row = min(row0 + r + 8 * x, n * Gq - 1), h = g * Gq + row % Gq;
+        tok[x] = t0 + row / Gq;
         pos[x] = TREE ? tree_position(A, t0 + row / Gq) : pos0 + row / Gq;
         r1[x] = BENT && A.r1 ? A.r1[h] : 0.0f;
         r2[x] = BENT && A.r1 ? A.r2[h] : 0.0f;
@@ -507,6 +512,17 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
         const float km = fabsf(ks);
         const bool whole = j0 - 2 * c + kBlock <= min(clear, seen.end) && (A.window == 0 || j0 - 2 * c > last_pos - A.window || j0 - 2 * c + kBlock <= A.first);
         float p[2][4], top[2];
+        int key[4];                // positions of the keys
+        uint32_t named[2];         // the block's keys that the rows' bits name
+        if (TREE) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int j = j0 + (e & 1) + 8 * (e >> 1);
+                key[e] = !whole && j >= pos0 && j < seen.end ? tree_position(A, t0 + j - pos0) : j;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) named[x] = whole ? 0xffffffffu : tree_named(A, tok[x], j0 - 2 * c - pos0);
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const float mul = rowmul[x] * km;
@@ -514,8 +530,9 @@ __global__ void __launch_bounds__(kRowThreads) attend_rows_kernel(const AttendAr
             for (int e = 0; e < 4; ++e) {
                 const int j = j0 + (e & 1) + 8 * (e >> 1);
                 float v = sc[e >> 1][2 * x + (e & 1)] * mul;
-                if (BENT) v = bent_score(A, v, pos[x] - (TREE && j >= pos0 && j < seen.end ? tree_key(A, t0, pos0, j) : j), r1[x], r2[x], slope[x]);
-                p[x][e] = whole || (TREE ? tree_sees(A, t0, pos0, t0 + min(row0 + r + 8 * x, n * Gq - 1) / Gq, pos[x], j, seen.end) : sees(A, pos[x], j, seen.end)) ? v : -INFINITY;
+                if (BENT) v = bent_score(A, v, pos[x] - (TREE ? key[e] : j), r1[x], r2[x], slope[x]);
+                const bool on = whole || (TREE ? j < seen.end && (named[x] >> (j - j0 + 2 * c) & 1u) && (A.window == 0 || pos[x] - key[e] < A.window || key[e] < A.first) : sees(A, pos[x], j, seen.end));
+                p[x][e] = on ? v : -INFINITY;
             }
             top[x] = fmaxf(fmaxf(p[x][0], p[x][1]), fmaxf(p[x][2], p[x][3]));
             top[x] = fmaxf(top[x], __shfl_xor_sync(0xffffffffu, top[x], 1));
