@@ -497,12 +497,12 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
                     const float2 a = J.finish[r];
                     const float x[4] = {v.x * a.x * a.y, v.y * a.x * a.y, v.z * a.x * a.y, v.w * a.x * a.y};
                     bf16* to = static_cast<bf16*>(A.out) + J.to[r] + c;
-                    if (A.o_vec && c + 4 <= A.c.dv) {
+                    if (A.o_vec && !A.gate && c + 4 <= A.c.dv) {
                         *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(x[0] * A.out_scale, x[1] * A.out_scale), pack_bf16(x[2] * A.out_scale, x[3] * A.out_scale));
                     } else {
 #pragma unroll
                         for (int y = 0; y < 4; ++y)
-                            if (c + y < A.c.dv) to[y] = __float2bfloat16_rn(x[y] * A.out_scale);
+                            if (c + y < A.c.dv) to[y] = __float2bfloat16_rn(finished(A, s_row[r], s_head[r], c + y, x[y]));
                     }
                 }
             }

@@ -34,6 +34,7 @@ from ._errors import SMOL_ERR_CAPACITY, SMOL_ERR_CUDA, SMOL_ERR_INVALID, SMOL_OK
 
 BLOCK = 16          # positions that share a scale
 MOST_DRAFTED = 4096  # rows of a sequence in a tree
+_INT32 = torch.int32
 _DTYPES = {torch.bfloat16: _capi_lm.SMOL_LM_BF16, torch.float32: _capi_lm.SMOL_LM_F32}
 # The arguments' structs of include/smoltts_b200_lm.h as native layouts: packing one takes a microsecond, filling a ctypes structure several.
 _BATCH = struct.Struct("@5i4P")
@@ -173,7 +174,7 @@ class KVCache8:
         return row, head
 
     def _ints(self, x: torch.Tensor, shape: tuple, what: str) -> int:
-        if x.dtype != torch.int32 or x.shape != shape or x.device != self.device or not x.is_contiguous():
+        if x.dtype is not _INT32 or x.shape != shape or x.device != self.device or not x.is_contiguous():
             raise ValueError(f"{what} must be contiguous int32 {shape} on {self.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
         return x.data_ptr()
 
@@ -284,16 +285,17 @@ class KVCache8:
             out_row, out_head = heads * self.vdim, self.vdim
         else:
             out_row, out_head = self._rows(out, tokens, heads, self.vdim, dtype, "out")
-            _check_written(out, "out", q=q, **({} if tree is None else tree._asdict()))
+            _check_written(out, "out", q=q, **({} if tree is None else {"tree.positions": tree[0], "tree.sees": tree[1]}))
         r1 = r2 = 0
         if penalty is not None:
             r1, r2 = self._floats(penalty[0], heads, "penalty[0]"), self._floats(penalty[1], heads, "penalty[1]")
         tree_pos = tree_sees = words = 0
         if tree is not None:
-            words = tree.sees.shape[-1] if tree.sees.dim() == 2 else 0
+            positions, sees = tree
+            words = sees.shape[1] if sees.dim() == 2 else 0
             if words < 1:
                 raise ValueError("tree.sees must be [tokens, words]")
-            tree_pos, tree_sees = self._ints(tree.positions, (tokens,), "tree.positions"), self._ints(tree.sees, (tokens, words), "tree.sees")
+            tree_pos, tree_sees = self._ints(positions, (tokens,), "tree.positions"), self._ints(sees, (tokens, words), "tree.sees")
         a = _pack(_ATTEND, _DTYPES[dtype], heads, q.data_ptr(), out.data_ptr(), q_row, q_head, out_row, out_head, self.dim ** -0.5 if scale is None else _float(scale, "scale"), _float(softcap, "softcap"), 1.0,
                   window, first, self._floats(sink, heads, "sink"), self._floats(slope, heads, "slope"), r1, r2, 0, 0, tree_pos, tree_sees, words)
         key = (dtype, tokens, heads, block_table.shape, max_new, max_len, window, first, words)

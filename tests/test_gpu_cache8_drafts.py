@@ -232,7 +232,7 @@ def test_masks_and_scores_of_trees(dtype, name, counts, pos0):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("n", [3, 45])
+@pytest.mark.parametrize("n", [3, 17, 45])
 def test_any_mask_and_any_positions(dtype, n):
     """Bits at random (rows that see later ones, that do not see themselves, that see none), positions that agree, go back, lie far away or outside their range, with and
     without options; words for fewer rows than there are."""
@@ -260,7 +260,7 @@ def test_any_mask_and_any_positions(dtype, n):
     c.check_device_errors()
 
 
-@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("n", [1, 12, 40])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_hidden_keys_and_rows_of_nobody(n, dtype):
     """kv_len counts places; rows in front of, behind and between the sequences stay as they were; queries and results are slices."""
@@ -282,7 +282,7 @@ def test_hidden_keys_and_rows_of_nobody(n, dtype):
         check_tree(c, table, q, counts, pos0, tree, out[..., :d], at=2, kv_len=kv_len, **o)
 
 
-@pytest.mark.parametrize("n", [4, 90])
+@pytest.mark.parametrize("n", [4, 24, 90])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_nan_on_one_branch_is_not_seen_on_another(n, dtype):
     H, G, d, L = 4, 2, 64, 200
@@ -357,6 +357,36 @@ def test_trees_that_do_not_fit_are_refused():
         with pytest.raises(SmolError, match="word 2"):
             c.check_device_errors()
         c._err.zero_()
+
+
+@pytest.mark.parametrize("n,context", [(2, 100), (3, 5000), (9, 40), (9, 900), (20, 5000), (40, 100)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gates_and_factors_of_results(dtype, n, context):
+    """What the C entry takes beyond the class: results times out_scale and sigmoid(gate), whoever writes them (one block, a cluster, the kernel that joins shares)."""
+    import ctypes as C
+
+    from smoltts_b200 import _capi_lm as cl
+
+    H, G, d = 4, 2, 72
+    c, table = cache_of([context + n], 32, G, d, d)
+    fill(c, table, [context + n])
+    q, gate = randn(n, H, d, seed=3).to(dtype), randn(n, H * d + 5, seed=4)
+    tree = tree_of(c, [parents_of("fan", n)], [context])
+    want = c.attend(q, ints([0, n]), ints([context]), table, max_new=n, max_len=context + n, tree=tree).double() * 0.5 * torch.sigmoid(gate[:, :H * d].double()).view(n, H, d)
+    out = torch.full((n, H, d), 7.0, device="cuda", dtype=dtype)
+    start, pos0 = ints([0, n]), ints([context])
+    cache = cl.SmolLmCache8(k=c.k.data_ptr(), v=c.v.data_ptr(), k_scale=c.k_scale.data_ptr(), v_scale=c.v_scale.data_ptr(), n_pages=c.n_pages, page_size=32, kv_heads=G, dim=d, vdim=d, err=c._err.data_ptr())
+    batch = cl.SmolLmCache8Batch(n_tokens=n, n_seqs=1, max_pages=table.shape[1], max_new=n, max_len=context + n, seq_start=start.data_ptr(), seq_pos0=pos0.data_ptr(), block_table=table.data_ptr())
+    a = cl.SmolLmCache8Attend(dtype=0 if dtype == torch.bfloat16 else 1, heads=H, q=q.data_ptr(), out=out.data_ptr(), q_row=H * d, q_head=d, out_row=H * d, out_head=d, scale=d ** -0.5, out_scale=0.5,
+                              gate=gate.data_ptr(), gate_row=H * d + 5, tree_positions=tree.positions.data_ptr(), tree_sees=tree.sees.data_ptr(), tree_words=tree.sees.shape[1])
+    lib, need = cl.load(), C.c_size_t()
+    cl.check(lib.smol_lm_cache8_workspace_bytes(C.byref(cache), C.byref(batch), C.byref(a), C.byref(need)))
+    work = torch.empty(max(need.value, 16), dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    cl.check(lib.smol_lm_cache8_attend(C.byref(cache), C.byref(batch), C.byref(a), work.data_ptr(), need.value, stream))
+    # the result without a gate is rounded once, that with one after the product: half a step each, and four roundings of fp32 between
+    assert ((out.double() - want).abs() <= 2.01 * HALF_STEP[dtype] * want.abs() + 2.0 ** -21 * want.abs() + 1e-30).all()
+    c.check_device_errors()
 
 
 # ---------------------------------------------------------------------------------------------- rows that are kept
