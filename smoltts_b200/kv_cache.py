@@ -11,7 +11,8 @@ its softmax attention layers from such a cache with ``kv_bits=8``.
 
 Drafted tokens may form a tree: ``draft_tree`` lays it out once per step, every layer's cache appends the rows at the positions that their depths give
 them (``append(positions=)``, which also takes the several axes of pictures and video) and attends to them along their paths (``attend(tree=)``), and
-``keep_rows`` then moves the rows of the accepted path together in all layers.  ``copy_pages`` copies pages in all layers, as forking a sequence does::
+``keep_rows`` then moves the rows of the accepted path together in all layers.  ``copy_pages`` copies pages in all layers: a sequence that is forked shares its
+whole pages and copies the one that it goes on filling (``pool.PagePool.fork``)::
 
     tree = caches[0].draft_tree(parents, seq_start, seq_pos0, max_new=64)
     for cache in caches:

@@ -6,7 +6,7 @@ sequence is the first one reused, which keeps the working set of pages small and
 """
 from __future__ import annotations
 
-from typing import Iterable, List
+from typing import Dict, Iterable, List, Sequence, Tuple
 
 from ._errors import SMOL_ERR_CAPACITY, SmolError
 
@@ -40,11 +40,48 @@ class IndexPool:
 
 
 class PagePool(IndexPool):
-    """Pages of ``page_size`` cached positions each."""
+    """Pages of ``page_size`` cached positions each.  A page may belong to several sequences, forks of one another, and is free when the last of them has given it back."""
 
     def __init__(self, n_pages: int, page_size: int):
         super().__init__(n_pages, "KV page")
         self.page_size = int(page_size)
+        self._others: Dict[int, int] = {}      # owners of a page beside the first
+
+    def share(self, items: Iterable[int]) -> None:
+        """One owner more for every one of the pages, which are allocated."""
+        items = list(items)
+        self._check(items)
+        for i in items:
+            self._others[i] = self._others.get(i, 0) + 1
+
+    def _check(self, items: Iterable[int]) -> None:
+        for i in items:
+            if not 0 <= i < self.n or self._is_free[i]:
+                raise ValueError(f"{self.what} {i} is not an allocated index of this pool")
+
+    def free(self, items: Iterable[int]) -> None:
+        """One owner less; a page without owners is free."""
+        items, last = list(items), []
+        for i in items:
+            if self._others.get(i, 0) > 0:
+                self._others[i] -= 1
+                if self._others[i] == 0:
+                    del self._others[i]
+            else:
+                last.append(i)
+        super().free(last)
+
+    def fork(self, pages: Sequence[int], positions: int) -> Tuple[List[int], List[int], List[int]]:
+        """Pages of a sequence that goes on from the first ``positions`` of one that has ``pages``: whole ones are shared, the last one, which both will go on filling, is a new
+        one.  Returns the pages, and which are to be copied to which (``kv_cache.copy_pages``; at most one)."""
+        need = self.pages_for(positions)
+        if positions < 0 or need > len(pages):
+            raise ValueError(f"{len(pages)} pages of {self.page_size} do not hold {positions} positions")
+        whole = positions // self.page_size
+        self._check(pages[:need])      # (in front of the allocation, which may hand out one that was given back)
+        new = self.allocate(need - whole)
+        self.share(pages[:whole])
+        return [*pages[:whole], *new], list(pages[whole:need]), new
 
     def pages_for(self, positions: int) -> int:
         return (positions + self.page_size - 1) // self.page_size
