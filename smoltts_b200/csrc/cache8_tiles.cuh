@@ -98,7 +98,7 @@ constexpr float kFarAbove = 64.0f;      // in units of log2
 
 // DK: key size padded; BENT: soft cap or distance penalties; TREE: rows of a tree
 template <int DK, bool BENT, bool TREE>
-__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
+__global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __grid_constant__ AttendArgs A, const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, int box) {
     constexpr int NS = tile_stages(DK), SB = tile_stage_bytes(DK), KH = DK / 128;
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
