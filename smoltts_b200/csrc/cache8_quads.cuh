@@ -129,20 +129,25 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
     float4(*stats)[kQuadParts][kQuadRows] = reinterpret_cast<float4(*)[kQuadParts][kQuadRows]>(Qs + kQuadOperand);      // of a step: a row's maximum, what its weights are relative to on top of it, their sum
     QuadJoin& J = *reinterpret_cast<QuadJoin*>(Qs);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < NS; ++i) { umma::bar_init(&bars.full[i], 1); umma::bar_init(&bars.empty[i], 1); }
-        for (int i = 0; i < 2; ++i) {
-            umma::bar_init(&bars.s_full[i], 1);
-            umma::bar_init(&bars.p_full[i], kQuadSoft);
-            umma::bar_init(&bars.o_full[i], 2);
-        }
+    // ---- barriers, a thread each ----
+    if (threadIdx.x < NS) {
+        umma::bar_init(&bars.full[threadIdx.x], 1);
+        umma::bar_init(&bars.empty[threadIdx.x], 1);
+    } else if (threadIdx.x < NS + 2) {
+        umma::bar_init(&bars.s_full[threadIdx.x - NS], 1);
+        umma::bar_init(&bars.p_full[threadIdx.x - NS], kQuadSoft);
+        umma::bar_init(&bars.o_full[threadIdx.x - NS], 2);
+    } else if (threadIdx.x == NS + 2) {
         umma::bar_init(&bars.q_full, kQuadSoft);
         umma::bar_init(&bars.drained, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&kmap), "l"(&vmap) : "memory");
         bars.stop = 0;
+        bars.tmem = 0;      // (what it will be: all columns are taken)
         s_bad = 0;
+    } else if (threadIdx.x == NS + 3) {
+        asm volatile("prefetch.tensormap [%0];\n\tprefetch.tensormap [%1];" ::"l"(&kmap), "l"(&vmap) : "memory");
     }
+    if (threadIdx.x <= NS + 2) asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
     dep_wait();
     const int s = blockIdx.z, g = blockIdx.y, tile = blockIdx.x / A.n_splits, split = blockIdx.x % A.n_splits;
     const Sequence Q(A.b, s, A.c.err);
@@ -154,23 +159,24 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
         dep_go();
         return;
     }
-    if (warp == kQuadSoft + 1) tmem_take<512>(&bars.tmem);
     const TreeSpan span(A, t0 + row0 / Gq, (row0 + rows - 1) / Gq - row0 / Gq + 1, n_all, pos0);
     const int first_pos = span.first_pos, last_pos = span.last_pos, behind = span.behind;
     const Seen seen = seen_steps(A, first_pos, behind, kv_len);
     const Rows W{s, g, t0, row0, rows, pos0, Gq, kv_len, seen.end};
     const int lo = (int)((long long)split * seen.count / A.n_splits), steps = (int)((long long)(split + 1) * seen.count / A.n_splits) - lo;
     const bool clustered = A.in_cluster;
-    umma::fence_before_sync();
-    __syncthreads();
-    umma::fence_after_sync();
-    dep_go();      // behind the allocation: a kernel set up early that wants tensor memory too must not get it first
-    const uint32_t tmem = bars.tmem, tm_o = tmem + 2 * kStep;      // scores of even and odd steps, then products likewise
     volatile int* stop = &bars.stop;
     if (warp == kQuadSoft) {
         quad_copies(A, &kmap, &vmap, box, W, seen, lo, steps, first_pos, KV, s_scales, bars);
     } else if (warp == kQuadSoft + 1) {
+        // (nobody waits for the allocation but this warp: who reads tensor memory has been told of a product)
+        tmem_take<512>(&bars.tmem);
+        dep_go();      // behind the allocation: a kernel set up early that wants tensor memory too must not get it first
         if (steps > 0) {
+            umma::fence_before_sync();
+            __syncwarp();
+            umma::fence_after_sync();
+            const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem), tm_o = tmem + 2 * kStep;      // scores of even and odd steps, then products likewise
             // ---- products.  A step's scores go where the weights of the step before last were, which are multiplied in front of them (products are made in the order of
             // their issue).  (Weights in shared memory instead, and scores as soon as a group has read its last ones: 260 us where this takes 246, since two operands from there are all that it gives.) ----
             const uint32_t q0 = umma::s2u(Qs), id_s = desc_e4m3(128, kStep, false, false), id_o = desc_e4m3(128, 128, false, true);
@@ -258,6 +264,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
         float m = -INFINITY, unit = 0.0f, l = 0.0f, o[OC];      // l in units of 2^m, o of 2^(m + unit)
 #pragma unroll
         for (int c = 0; c < OC; ++c) o[c] = 0.0f;
+        uint32_t tmem = 0;      // (known from the first product on)
         // a step's product, whoever brought its weights
         auto join_product = [&](int j) {
             wait_bar(&bars.o_full[j & 1], (j >> 1) & 1, stop, A.c.err);
@@ -265,6 +272,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
             const float m_step = of.x, unit_step = of.y, l_step = of.z;
             __syncwarp();
             umma::fence_after_sync();
+            tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem);
             // what results and denominator are relative to is the first step's, and a later one's only where they would come near fp32's end (they are below 2^90)
             if (__any_sync(0xffffffffu, m_step > m + kFarAbove || (m_step - m) + unit_step > unit + kFarAbove)) {
                 const float mn = m_step > m + kFarAbove ? m_step : m, had = unit + (m - mn), has = unit_step + (m_step - mn), un = m == -INFINITY || has > had + kFarAbove ? has : had;
@@ -282,7 +290,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
             for (int x = 0; x < OC / 32; ++x) {
                 uint32_t v[4][8];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) umma::tmem_ld8_issue(tm_o + (j & 1) * 128 + group * OC + 32 * x + 8 * y + lanes, v[y]);
+                for (int y = 0; y < 4; ++y) umma::tmem_ld8_issue(tmem + 2 * kStep + (j & 1) * 128 + group * OC + 32 * x + 8 * y + lanes, v[y]);
                 umma::tmem_ld_wait();
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
@@ -320,6 +328,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
                 wait_bar(&bars.s_full[group], (i >> 1) & 1, stop, A.c.err);
                 __syncwarp();
                 umma::fence_after_sync();
+                tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem);
                 float S[kQuadCols];
                 {
                     uint32_t v[4][8];
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
     __syncwarp();
     umma::fence_before_sync();
     __syncthreads();
-    if (warp == kQuadSoft + 1) tmem_give<512>(tmem);
+    if (warp == kQuadSoft + 1) tmem_give<512>(*reinterpret_cast<volatile uint32_t*>(&bars.tmem));
 }
 
 }  // namespace c8

@@ -126,15 +126,25 @@ __device__ __forceinline__ uint32_t tree_named(const AttendArgs& A, int tok, int
     const uint32_t low = w < 0 ? 0xffffffffu : w < A.tree_words ? bits[w] : 0u, high = w + 1 < 0 ? 0xffffffffu : w + 1 < A.tree_words ? bits[w + 1] : 0u;
     return __funnelshift_r(low, high, i0 & 31);
 }
-// which of the 32 keys from place jc on row tok sees.  (A call, so that the loops around it keep their registers.)
+// which of the 32 keys from place jc on row tok sees; by a whole warp, whose lanes find a key's position each.  (A call, so that the loops around it keep their registers.)
 static __device__ __noinline__ uint32_t tree_mask(const AttendArgs& A, int t0, int pos0, int tok, int pos, int jc, int end) {
     uint32_t mask = tree_named(A, tok, jc - pos0);
     if (end < jc + 32) mask = end <= jc ? 0u : mask & (1u << (end - jc)) - 1u;
-    if (A.window > 0)
-        for (int e = 0; e < 32; ++e) {
-            const int key = jc + e < end ? tree_key(A, t0, pos0, jc + e) : 0;
-            if (pos - key >= A.window && key >= A.first) mask &= ~(1u << e);
+    if (A.window > 0) {
+        // of the context's places: those behind the window's beginning, and the first ones
+        const long long from = (long long)pos - A.window + 1 - jc, first = (long long)A.first - jc;
+        uint32_t near = (from <= 0 ? 0xffffffffu : from < 32 ? 0xffffffffu << from : 0u) | (first >= 32 ? 0xffffffffu : first > 0 ? (1u << first) - 1u : 0u);
+        if (jc + 32 > pos0) {      // of the rows' own: by their positions, which a lane each has found
+            const int at = jc + (threadIdx.x & 31), mine = at < end ? tree_key(A, t0, pos0, at) : 0;
+#pragma unroll 1
+            for (int e = max(pos0 - jc, 0); e < min(end - jc, 32); ++e) {      // (a loop: code that is fetched for a few steps takes longer than it runs, 5500 cycles unrolled)
+                const int key = __shfl_sync(0xffffffffu, mine, e);
+                const bool on = pos - key < A.window || key < A.first;
+                near = on ? near | 1u << e : near & ~(1u << e);
+            }
         }
+        mask &= near;
+    }
     return mask;
 }
 // Sequences of a tree lie behind a context of no fewer than zero positions.
