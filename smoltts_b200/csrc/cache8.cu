@@ -44,14 +44,16 @@ static int splits_for(const AttendArgs& A, bool f32, int n_sms) {
     const long long halves = tiles ? (A.c.dv + 127) / 128 : 1, base = (long long)A.b.S * A.c.G * row_tiles(A, f32) * halves;      // blocks of a share
     long long keys = A.b.max_len;
     if (A.window > 0) keys = std::min(keys, (long long)A.window + A.b.max_new + A.first + 2 * kBlock);
-    // as many shares as the SMs hold blocks at once, none of less than 256 keys (a token of 12 heads at 2048 positions, appended and
+    // As many shares as the SMs hold blocks at once, none of less than 256 keys (a token of 12 heads at 2048 positions, appended and
     // attended to: 10.9 us; with shares of 128, which are one step, 11.5; of 512 12.7).  More blocks than are held at once wait for whole others: one sequence at
     // 131072 34 us in 111 shares, 43 in 128.
     const int held = f32 ? 2 : tiles || quads_serve(A, f32) ? 1 : few_blocks(std::max(A.c.d, A.c.dv), row_tile(A, false));
-    const long long slots = (long long)held * n_sms;
-    auto at_once = [&](long long blocks) { return std::max(1ll, std::min({slots / blocks, (keys + 255) / 256, (long long)kMaxSplits})); };
+    // (float32 rows of a tree: 64, a block of 16 for each of a block of threads' warps.  3 sequences of 63 rows at 922 positions 25.6 us, with 256 29.4; one of 12 rows 13.2 and 19.3)
+    const long long slots = (long long)held * n_sms, least = f32 && A.tree_pos ? 64 : 256;
+    auto at_once = [&](long long blocks) { return std::max(1ll, std::min({slots / blocks, (keys + least - 1) / least, (long long)kMaxSplits})); };
     long long want = at_once(base);
-    // (a little more than a cluster joins: without the other launch, and the shares' way through memory)
+    // Rows of a tree, a little more than a cluster joins: eight, without the launch that joins shares in memory.  On the device that is within 0.9 us either way (4 to 32 rows of 8 heads of 128 at
+    // 2100 to 4000 positions; 48 rows of 4 heads of 64 at 2063 11.4 us, in nine 12.3), on the host 3 us less.
     if (A.tree_pos && want > kMostCluster && want <= 2 * kMostCluster && joins_in_cluster(A, kMostCluster, f32)) want = kMostCluster;
     if (halves == 1) return (int)want;
     // Values of more than 128 columns take two blocks a tile, and so at most half as many shares at once: often fewer SMs at work, where two rounds of shorter shares may
