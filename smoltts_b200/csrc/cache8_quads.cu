@@ -1,4 +1,4 @@
-// Attention of 9 to 64 rows of a tree over the 8-bit key/value cache: launches.  (A source of its own: the other kernels' registers are shared out otherwise where this one calls the same functions.)
+// Attention of 9 to 64 rows of a tree over the 8-bit key/value cache: launches.  (A source of its own, which is compiled beside the others.)
 #include "cache8_launch.cuh"
 #include "cache8_quads.cuh"
 

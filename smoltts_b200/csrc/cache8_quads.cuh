@@ -10,6 +10,11 @@
 // Queries and weights are two e4m3 parts of one unit as in the tiles, relative to what a row sees in 32 positions of a step rather than in 128.
 //
 // Roles: eight warps for the softmax, one that copies, one that issues the products.
+//
+// What bounds it: the chain of a group's two steps, 3550 cycles: products of 480 and 650 (two e4m3 parts, and a quarter of what is multiplied is wanted), their waits, a softmax of 1350 from
+// scores to weights, reading results 450.  DRAM gives a step's 32 KB in 1330 an SM.  Around the steps a block takes 8000 cycles to its first scores (the batch's arrays, queries, page, scales and
+// the first copy, one behind the other) and 3000 for its results.  64 sequences at up to 8192 positions, 32 and 8 heads of 128, 16 rows each 208 to 216 us (rows as columns, 16 of them, 247), 32 rows
+// 213 to 217 (tiles 407), 64 rows 383; 48 of 16 rows behind windows of 4000 and 4 122 us, with soft cap, slope and sink 155; one of 48 rows of 4 heads of 64 at 2063 positions 11.4 us.
 #pragma once
 
 #include "cache8_few.cuh"
@@ -45,7 +50,7 @@ struct QuadJoin {
 static_assert(sizeof(QuadJoin) <= kQuadOperand, "the join's place");
 
 // The copying warp: keys and values of every step into a ring of stages, 128-byte swizzle, in boxes of `box` positions that lie together.  All 32 lanes look blocks up, four steps at a time and
-// four ahead: an entry and then a scale that are waited for once a step cost 2000 cycles where memory is busy (300 us where this takes 246: 64 sequences at up to 8192 positions).
+// four ahead: an entry and then a scale that are waited for once a step cost 2000 cycles where memory is busy (64 sequences at up to 8192 positions 300 us, then 246).
 __device__ __forceinline__ void quad_copies(const AttendArgs& A, const CUtensorMap* kmap, const CUtensorMap* vmap, int box, const Rows& W, const Seen& seen, int lo, int steps, int first_pos,
                                             unsigned char* ring, StepScales* scales, QuadBars& bars) {
     constexpr int AHEAD = 32 / kStepBlocks, NS = kQuadStages;
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(kQuadThreads, 1) attend_quads_kernel(const __g
             umma::fence_after_sync();
             const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&bars.tmem), tm_o = tmem + 2 * kStep;      // scores of even and odd steps, then products likewise
             // ---- products.  A step's scores go where the weights of the step before last were, which are multiplied in front of them (products are made in the order of
-            // their issue).  (Weights in shared memory instead, and scores as soon as a group has read its last ones: 260 us where this takes 246, since two operands from there are all that it gives.) ----
+            // their issue).  (Weights in shared memory instead, and scores as soon as a group has read its last ones: 260 us where this then took 246, since two operands from there are all that it gives.) ----
             const uint32_t q0 = umma::s2u(Qs), id_s = desc_e4m3(128, kStep, false, false), id_o = desc_e4m3(128, 128, false, true);
             const int ksteps = (A.c.d + 31) / 32;
             auto scores = [&](int i) {

@@ -18,7 +18,7 @@
 // other is a power of two and rounds nothing.
 //
 // What bounds it: the instructions of its fragments (legacy mma.sync: f16 products of fp32's width would take three e4m3 parts on tcgen05).  A prompt of 300 tokens, 12
-// and 4 heads of 64, logarithmic penalty: 23 us, of 2000 195 us; a token each of 16 sequences at up to 8192 positions, 32 and 8 heads of 128, 153 us.
+// and 4 heads of 64, logarithmic penalty: 23 us, of 2000 195 us; trees of 21 rows of 3 sequences at 922 positions, 12 and 4 heads of 80 and 72, 26 us; a token each of 16 sequences at up to 8192 positions, 32 and 8 heads of 128, 153 us.
 #pragma once
 
 #include "cache8.cuh"

@@ -17,8 +17,8 @@
 //
 // What bounds it: the softmax warps, of which an SM holds one block's (registers, and all of tensor memory).  A step of 128 rows by 128 positions takes about
 // 3600 cycles, 2100 of them issuing (weights 1500 from end to end: an exponential, two roundings to codes, one back), the products 1100 beside
-// them; preparing a block's queries 9000 and its results 3400 more.  4096 tokens of 32 and 8 heads of 128: 302 us, 0.46 PFLOP/s of the definition's; 7900
-// behind a window of 1000, 16 and 4 heads: 227 us.  Two threads a row, two groups of softmax warps in turn with others joining, and joining a product
+// them; preparing a block's queries 9000 and its results 3400 more.  4096 tokens of 32 and 8 heads of 128: 280 us, 0.49 PFLOP/s of the definition's; 7900
+// behind a window of 1000, 16 and 4 heads: 206 us; trees of up to 64 rows behind up to 8192 positions, 32 sequences of 32 and 8 heads: 401 us.  Two threads a row, two groups of softmax warps in turn with others joining, and joining a product
 // two steps late were all slower (331 to 379 us where this took 326).
 #pragma once
 
