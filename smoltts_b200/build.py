@@ -38,6 +38,7 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-shared",
     "--expt-relaxed-constexpr",
     "-Xptxas", "-v",
+    "--threads", "4",      # sources beside one another
 ]
 
 

@@ -336,6 +336,55 @@ def test_rows_behind_max_new_are_left_alone_and_seen():
     assert ((out[:3].double() - want).abs() <= tolerance(q.dtype, want, spread, size)).all() and (out[3:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("most", [2, 9, 30, 40])
+def test_host_numbers_that_are_too_small(dtype, most):
+    """max_len sizes the grid and nothing else; rows beyond max_new are left as they were, and seen by the others where bits name them."""
+    H, G, d, n, L = 4, 2, 64, 45, 3000
+    c, table = cache_of([L, 100 + n], 64, G, d, d)
+    fill(c, table, [L, 100 + n])
+    q = randn(2 * n, H, d, seed=3).to(dtype)
+    pos0 = [L - n, 100]
+    tree = tree_of(c, [parents_of("fan", n), [-1] * n], pos0)
+    tree.sees[:, 1] |= 1 << 12      # everybody sees row 44
+    out = torch.full((2 * n, H, d), 7.0, device="cuda", dtype=dtype)
+    c.attend(q, ints([0, n, 2 * n]), ints(pos0), table, max_new=most, max_len=10, out=out, tree=tree)
+    for s, p in enumerate(pos0):
+        k, v = held(c, table, s, p + n)
+        rows = slice(s * n, s * n + most)
+        want, spread, size = tree_attention(q[rows], k, v, p, tree.positions[s * n:(s + 1) * n], tree.sees[rows], d ** -0.5)
+        assert ((out[rows].double() - want).abs() <= tolerance(dtype, want, spread, size)).all()
+        assert (out[s * n + most:(s + 1) * n] == 7).all()
+    c.check_device_errors()
+
+
+def test_pages_whose_bytes_pass_32_bits():
+    """The same step in a pool of a few pages and at the end of one of 4.6 GB of keys: equal to the bit."""
+    from smoltts_b200.kv_cache import KVCache8, copy_pages, keep_rows
+
+    G, H, d, page, n, far = 8, 16, 128, 64, 20, 70000
+    small, big = KVCache8.allocate(12, page, G, d), KVCache8.allocate(far, page, G, d)
+    assert big.k.numel() > 2 ** 32
+    freq = (10000.0 ** (-torch.arange(64, device="cuda") / 64)).float()
+    got = []
+    for c, base in ((small, 0), (big, far - 12)):
+        table = ints([[base + p for p in (5, 2, 9)], [base + p for p in (7, 0, 11)]])
+        k, v = randn(300, G, d, seed=1).to(torch.bfloat16), randn(300, G, d, seed=2).to(torch.bfloat16)
+        c.append(k, v, ints([0, 150, 300]), ints([0, 0]), table, max_new=150)
+        results = []
+        for dtype, m in ((torch.bfloat16, 2), (torch.bfloat16, n), (torch.bfloat16, 40), (torch.float32, 4)):
+            tree = c.draft_tree(ints(parents_of("fan", m) * 2), ints([0, m, 2 * m]), ints([140, 130]), max_new=m)
+            q = c.append(randn(2 * m, G, d, seed=3).to(dtype), randn(2 * m, G, d, seed=4).to(dtype), ints([0, m, 2 * m]), ints([140, 130]), table, max_new=m, q=randn(2 * m, H, d, seed=5).to(dtype), freq=freq,
+                         positions=tree.positions)
+            results.append(c.attend(q, ints([0, m, 2 * m]), ints([140, 130]), table, max_new=m, max_len=180, tree=tree))
+        keep_rows(c, ints([140, 130]), table, ints([[0, 3, 17], [1, 2, 30]]), ints([3, 3]))
+        copy_pages(c, [base + 9, base + 11], [base + 1, base + 3])
+        c.check_device_errors()
+        at = torch.arange(base, base + 12, device="cuda")
+        got.append([*results, *(x.view(torch.uint8)[at] for x in (c.k, c.v)), *(x[at] for x in (c.k_scale, c.v_scale))])
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and (big.k.view(torch.uint8)[:far - 12].amax() == 0)
+
+
 def test_trees_that_do_not_fit_are_refused():
     from smoltts_b200._errors import SmolError
     from smoltts_b200.kv_cache import DraftTree
