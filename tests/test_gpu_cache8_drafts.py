@@ -674,6 +674,41 @@ def test_draft_verify_keep_and_fork(dtype, n):
         c.check_device_errors()
 
 
+def test_calls_on_several_streams_at_once():
+    """Kernels for few, 32 and many rows, in clusters and with shares through memory, beside kept rows and copied pages: each as it is alone."""
+    from smoltts_b200.kv_cache import copy_pages, keep_rows
+
+    H, G, d = 8, 2, 128
+    calls = []
+    for i, (n, context, dtype) in enumerate([(1, 3000, torch.bfloat16), (5, 2100, torch.bfloat16), (16, 9000, torch.bfloat16), (70, 3000, torch.bfloat16), (9, 700, torch.float32)]):
+        c, table = cache_of([context + n, 300 + n], 64, G, d, d, seed=i)
+        fill(c, table, [context + n, 300 + n], seed=i)
+        q = randn(2 * n, H, d, seed=i + 50).to(dtype)
+        tree = tree_of(c, [parents_of("random", n, 1), parents_of("fan", n)], [context, 300])
+        args = (q, ints([0, n, 2 * n]), ints([context, 300]), table)
+        calls.append((c, lambda c=c, args=args, n=n, context=context, tree=tree: c.attend(*args, max_new=n, max_len=context + n, tree=tree)))
+    moved, table = cache_of([400], 64, G, d, d, seed=9)
+    fill(moved, table, [400], seed=9)
+    want = [call() for _, call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(len(calls) + 1)]
+    rows, counts, pos0, page = ints([[0, 20, 30]]), ints([3]), ints([350]), int(table[0, 0])
+    spare = next(p for p in range(moved.n_pages) if p not in table.flatten().tolist())
+    for _ in range(30):
+        got = []
+        for (_, call), stream in zip(calls, streams):
+            with torch.cuda.stream(stream):
+                got.append(call())
+        with torch.cuda.stream(streams[-1]):
+            keep_rows(moved, pos0, table, rows, counts)
+            copy_pages(moved, [page], [spare])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    assert torch.equal(moved.k.view(torch.uint8)[page], moved.k.view(torch.uint8)[spare])
+    for c, _ in calls:
+        c.check_device_errors()
+
+
 def test_a_captured_step_is_replayed_beside_another():
     """Tree, append, attention, rows and pages in two graphs on two streams, replayed in turn and at once with new inputs: as the calls themselves on the same contents."""
     from smoltts_b200.kv_cache import copy_pages, keep_rows
