@@ -148,10 +148,10 @@ __global__ void __launch_bounds__(kKeepWarps * 32) keep_kernel(const __grid_cons
                 r = rows[i];
                 before = rows[i - 1];
             }
-            if (r <= before || r >= kPositions - pos0) {
+            if (r < i || r <= before || r >= kPositions - pos0) {      // (rows that ascend from 0 on are not below their number: what a lane reads here, it has checked by itself)
                 wrong = 2;
             } else {
-                const int from = (pos0 + r) / c.page, to = (pos0 + i) / c.page;      // (to is not above from)
+                const int from = (pos0 + r) / c.page, to = (pos0 + i) / c.page;      // (0 <= to <= from)
                 const int a = from < A.max_pages ? table[from] : -1, b = from < A.max_pages ? table[to] : -1;
                 if ((unsigned)a >= (unsigned)c.n_pages || (unsigned)b >= (unsigned)c.n_pages) wrong = max(wrong, 1);
             }
