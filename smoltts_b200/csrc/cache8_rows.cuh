@@ -665,7 +665,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attend_join_kernel(const Atte
         else hi = mid;
     }
     const Sequence Q(A.b, lo, A.c.err);
-    if (t < Q.t0 || t - Q.t0 >= min(Q.n, A.b.max_new) || (long long)Q.n * (A.H / A.c.G) <= A.rows_over) return;
+    if (t < Q.t0 || t - Q.t0 >= min(Q.n, A.b.max_new) || (long long)Q.n * (A.H / A.c.G) <= A.rows_over || (A.tree_pos && !tree_fits(A, Q.pos0, 0))) return;      // (whoever has no shares)
     const int pieces = (A.c.dv + 3) / 4;
     const float4* stat = part_stats(A) + (size_t)unit * A.n_splits;      // maximum, denominator, e of the results
     const float4* part = reinterpret_cast<const float4*>(A.part) + (size_t)unit * A.n_splits * pieces;

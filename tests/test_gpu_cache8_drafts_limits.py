@@ -4,9 +4,10 @@ from __future__ import annotations
 import pytest
 import torch
 
-from cache8_util import ints
-from test_gpu_cache8 import cache_of
-from test_gpu_cache8_drafts import check_kept, contents, uneven
+from cache8_util import ints, starts
+from drafts_util import parents_of
+from test_gpu_cache8 import cache_of, fill, randn
+from test_gpu_cache8_drafts import check_kept, check_tree, contents, uneven
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,35 @@ def test_rows_in_no_order_are_reported_wherever_they_are(rows, pos0):
     check_kept(c, before, table, [pos0, 9], [[], good])
     with pytest.raises(SmolError, match="word 2"):
         c.check_device_errors()
+
+
+# ---------------------------------------------------------------------------------------------- attention along paths
+
+@pytest.mark.parametrize("dtype,rows", [(torch.bfloat16, [1, 2]), (torch.bfloat16, [6, 20]), (torch.bfloat16, [100, 40]), (torch.bfloat16, [90, 3]), (torch.float32, [1, 2]), (torch.float32, [30, 9])])
+@pytest.mark.parametrize("context", [40, 600, 9000])
+@pytest.mark.parametrize("first", [-1, -1000, -2 ** 31])
+def test_a_tree_in_front_of_the_first_position_is_left_out(dtype, rows, context, first):
+    """Few, 32 and many rows, both in one batch, and float32; keys in one share, in shares that a cluster joins, and in shares that go through memory.  The sequences beside it are served."""
+    from smoltts_b200._errors import SmolError
+
+    H, G, d = 4, 2, 64
+    counts, pos0 = [rows[0], rows[1], rows[0]], [context, 50, 17]
+    lens = [p + n for p, n in zip(pos0, counts)]
+    c, table = cache_of(lens, 64, G, d, d)
+    fill(c, table, lens)
+    q = randn(sum(counts), H, d, seed=3).to(dtype)
+    start = starts(counts)
+    tree = c.draft_tree(ints(sum([parents_of("fan", n) for n in counts], [])), ints(start), ints(pos0), max_new=max(counts))
+    c.check_device_errors()
+    given = ints([context, first, 17])
+    for _ in range(2):
+        junk = [torch.full((1 << 22,), 3.0, device="cuda") for _ in range(3)]      # what a workspace may find
+        del junk
+        out = torch.full((sum(counts), H, d), 7.0, device="cuda", dtype=dtype)
+        c.attend(q, ints(start), given, table, max_new=max(counts), max_len=context + max(counts), out=out, tree=tree)
+        assert (out[start[1]:start[2]] == 7).all()
+        out[start[1]:start[2]] = c.attend(q, ints(start), ints(pos0), table, max_new=max(counts), max_len=context + max(counts), tree=tree)[start[1]:start[2]]
+        check_tree(c, table, q, counts, pos0, tree, out)
+        with pytest.raises(SmolError, match="word 2"):
+            c.check_device_errors()
+        c._err.zero_()
