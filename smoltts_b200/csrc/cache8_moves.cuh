@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(kKeepWarps * 32) keep_kernel(const __grid_cons
                         *old = rescaled(w, down);
                     }
             }
-            const float f = fabsf(scale[z]) * pow2(-E);      // lane r: of row r
+            // lane r: of row r.  (From 2^18 on the row is zeros: the least code, 2^-9, would pass 448.  The quotient of two scales may be no fp32 number, and zeros times infinity NaN.)
+            const float f = fminf(fabsf(scale[z]) * pow2(-E), pow2(18));
             const bool same = __all_sync(0xffffffffu, !mine || f == 1.0f);
 #pragma unroll
             for (int y = 0; y < PASSES; ++y) {

@@ -7,7 +7,7 @@ import torch
 from cache8_util import ints, starts
 from drafts_util import parents_of
 from test_gpu_cache8 import cache_of, fill, randn
-from test_gpu_cache8_drafts import check_kept, check_tree, contents, uneven
+from test_gpu_cache8_drafts import arrays, check_kept, check_tree, contents, uneven
 
 pytestmark = pytest.mark.gpu
 
@@ -40,6 +40,32 @@ def test_rows_in_no_order_are_reported_wherever_they_are(rows, pos0):
     check_kept(c, before, table, [pos0, 9], [[], good])
     with pytest.raises(SmolError, match="word 2"):
         c.check_device_errors()
+
+
+@pytest.mark.parametrize("d,dv", [(64, 64), (128, 80), (256, 33)])
+@pytest.mark.parametrize("power", [16, 40, 99])
+def test_rows_of_zeros_from_blocks_of_any_scale(d, dv, power):
+    """Rows that are zeros, or far below what lies beside them, are kept from a block of a large scale: into a block of zeros, of small numbers, and behind older rows of either.  No code of
+    them may come out as anything but what its value is."""
+    from smoltts_b200.kv_cache import keep_rows
+
+    lens, pos0 = [64, 64, 64, 64], [16, 20, 16, 20]
+    rows = [[0, 3, 17], [1, 3, 17], [0, 3, 17], [1, 3, 17]]
+    c, table = cache_of(lens, 32, 2, d, dv)
+    T = sum(lens)
+    k, v = torch.zeros(T, 2, d, device="cuda"), torch.zeros(T, 2, dv, device="cuda")
+    for x in (k, v):
+        x = x.view(4, 64, *x.shape[1:])
+        x[2:, 16:32] = 2.0 ** -99      # (the smallest that a scale of its own holds is 2^-110 times the least code)
+        x[:, 34] = 2.0 ** power        # beside the last of the kept rows, and far above it
+        x[2:, 19] = 2.0 ** -80
+        x[1:, 36] = 2.0 ** (power - 12)
+    c.append(k, v, ints(starts(lens)), ints([0] * 4), table, max_new=64)
+    before = contents(c)
+    keep_rows(c, ints(pos0), table, *arrays(rows))
+    check_kept(c, before, table, pos0, rows)
+    for x in c.values(table.flatten().long()):
+        assert torch.isfinite(x).all()
 
 
 # ---------------------------------------------------------------------------------------------- attention along paths
