@@ -30,11 +30,27 @@ class IndexPool:
             self._is_free[i] = 0
         return got
 
-    def free(self, items: Iterable[int]) -> None:
-        items = list(items)
+    def _owners(self, i: int) -> int:
+        return 1
+
+    def _check(self, items: Iterable[int]) -> None:
         for i in items:
             if not 0 <= i < self.n or self._is_free[i]:
                 raise ValueError(f"{self.what} {i} is not an allocated index of this pool")
+
+    def _check_freed(self, items: List[int]) -> None:
+        """Before anything is changed: all of them are allocated, and none comes more often than it has owners."""
+        self._check(items)
+        times: Dict[int, int] = {}
+        for i in items:
+            times[i] = times.get(i, 0) + 1
+            if times[i] > self._owners(i):
+                raise ValueError(f"{self.what} {i} is given back more often than it has owners")
+
+    def free(self, items: Iterable[int]) -> None:
+        items = list(items)
+        self._check_freed(items)
+        for i in items:
             self._is_free[i] = 1
         self._free.extend(reversed(items))
 
@@ -54,14 +70,13 @@ class PagePool(IndexPool):
         for i in items:
             self._others[i] = self._others.get(i, 0) + 1
 
-    def _check(self, items: Iterable[int]) -> None:
-        for i in items:
-            if not 0 <= i < self.n or self._is_free[i]:
-                raise ValueError(f"{self.what} {i} is not an allocated index of this pool")
+    def _owners(self, i: int) -> int:
+        return 1 + self._others.get(i, 0)
 
     def free(self, items: Iterable[int]) -> None:
         """One owner less; a page without owners is free."""
         items, last = list(items), []
+        self._check_freed(items)
         for i in items:
             if self._others.get(i, 0) > 0:
                 self._others[i] -= 1
