@@ -236,7 +236,7 @@ class KVCache8:
                 out_row, out_head = heads * self.dim, self.dim
             else:
                 out_row, out_head = self._rows(q_out, tokens, heads, self.dim, dtype, "q_out")
-                _check_written(q_out, "q_out", q=q, k=k, v=v)
+                _check_written(q_out, "q_out", q=q, k=k, v=v, **{name: x for name, x in (("freq", freq), ("positions", positions), ("axis", axis)) if x is not None and x.numel()})
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")

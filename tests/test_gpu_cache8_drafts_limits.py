@@ -12,6 +12,36 @@ from test_gpu_cache8_drafts import arrays, check_kept, check_tree, contents, une
 pytestmark = pytest.mark.gpu
 
 
+# ---------------------------------------------------------------------------------------------- append
+
+@pytest.mark.parametrize("name", ["positions", "axis", "freq"])
+def test_queries_over_the_arrays_that_angles_are_made_of_are_refused(name):
+    """Every block of threads reads them while others write queries.  Beside them, within the same memory, there is room."""
+    c, table = cache_of([6], 16, 1, 16, 16, garbage=False)
+    T, H, pairs = 6, 2, 4
+    room = torch.zeros(T * H * 16 + 64, device="cuda")
+    sizes = {"positions": 3 * T, "axis": pairs, "freq": pairs}
+    x, q = randn(T, 1, 16), randn(T, H, 16, seed=1)
+    want = None
+    for at in (8, T * H * 16 - 3, T * H * 16 + 8):      # inside, over the end, behind
+        arrays = {"positions": torch.arange(3 * T, device="cuda").int(), "axis": ints([0, 1, 2, 0]), "freq": torch.ones(pairs, device="cuda")}
+        here = room[at:at + sizes[name]].view(arrays[name].dtype)
+        here.copy_(arrays[name].flatten())
+        arrays[name] = here
+        arrays["positions"] = arrays["positions"].view(3, T)
+        args = dict(q=q, q_out=room[:T * H * 16].view(T, H, 16), **arrays)
+        if at < T * H * 16:
+            with pytest.raises(ValueError, match=name):
+                c.append(x, x, ints([0, T]), ints([0]), table, max_new=T, **args)
+            assert (room[:8] == 0).all()
+        else:
+            got = c.append(x, x, ints([0, T]), ints([0]), table, max_new=T, **args)
+            want = c.append(x, x, ints([0, T]), ints([0]), table, max_new=T, **{**args, "q_out": None})
+            assert torch.equal(got, want)
+    none = torch.zeros(0, device="cuda")      # no pairs, nothing that is read
+    assert torch.equal(c.append(x, x, ints([0, T]), ints([0]), table, max_new=T, q=q, q_out=torch.empty_like(q), freq=none), q)
+
+
 # ---------------------------------------------------------------------------------------------- kept rows
 
 # (rows, pos0 of the sequence; 64 positions in four pages): entries behind the first wrong one that ascend among themselves, and destinations behind the table's last page
