@@ -100,8 +100,12 @@ def _extent(x: torch.Tensor) -> Tuple[int, int]:
     return at, at + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
 
 
-def _check_written(out: torch.Tensor, what: str, **read: torch.Tensor) -> None:
-    """A result must not overlap itself, nor what is read while it is written."""
+def _overlap(what: str, name: str) -> None:
+    raise ValueError(f"{what} must not reach into {name}'s memory: it is read while {what} is written")
+
+
+def _check_written(out: torch.Tensor, what: str, **read: torch.Tensor) -> Tuple[int, int]:
+    """A result must not overlap itself, nor what is read while it is written.  Returns its extent."""
     (tokens, heads, width), (row, head, _) = out.shape, out.stride()
     if not ((heads == 1 or head >= width) and (tokens == 1 or row >= (heads - 1) * head + width) or
             (tokens == 1 or row >= width) and (heads == 1 or head >= (tokens - 1) * row + width)):
@@ -110,7 +114,8 @@ def _check_written(out: torch.Tensor, what: str, **read: torch.Tensor) -> None:
     for name, x in read.items():
         a, b = _extent(x)
         if a < hi and lo < b:
-            raise ValueError(f"{what} must not reach into {name}'s memory: it is read while {what} is written")
+            _overlap(what, name)
+    return lo, hi
 
 
 class DraftTree(NamedTuple):
@@ -220,7 +225,7 @@ class KVCache8:
         k_row, k_head = self._rows(k, None, self.kv_heads, self.dim, None, "k")
         v_row, v_head = self._rows(v, tokens, self.kv_heads, self.vdim, dtype, "v")
         batch = self._batch(tokens, seq_start, seq_pos0, block_table, max_new, max_new)
-        pairs = freq_ptr = heads = q_ptr = q_row = q_head = out_ptr = out_row = out_head = 0
+        pairs = freq_ptr = heads = q_ptr = q_row = q_head = out_ptr = out_row = out_head = lo = hi = 0
         if freq is not None:
             if freq.dim() != 1 or 2 * freq.shape[0] > self.dim:
                 raise ValueError(f"freq must be [pairs] with at most {self.dim // 2} pairs")
@@ -236,7 +241,7 @@ class KVCache8:
                 out_row, out_head = heads * self.dim, self.dim
             else:
                 out_row, out_head = self._rows(q_out, tokens, heads, self.dim, dtype, "q_out")
-                _check_written(q_out, "q_out", q=q, k=k, v=v, **{name: x for name, x in (("freq", freq), ("positions", positions), ("axis", axis)) if x is not None and x.numel()})
+                lo, hi = _check_written(q_out, "q_out", q=q, k=k, v=v)
             q_ptr, out_ptr = q.data_ptr(), q_out.data_ptr()
         elif q_out is not None:
             raise ValueError("q_out without q")
@@ -252,6 +257,10 @@ class KVCache8:
                 axis_ptr = self._ints(axis, (pairs,), "axis") if pairs else 0
         elif axis is not None:
             raise ValueError("axis without positions")
+        if hi:
+            for name, at, count in (("freq", freq_ptr, pairs), ("positions", pos_ptr, axes * tokens), ("axis", axis_ptr, pairs)):      # (4 bytes each)
+                if lo < at + 4 * count and at < hi:
+                    _overlap("q_out", name)
         self._call(self._append, batch, _pack(_APPEND, _DTYPES[dtype], k.data_ptr(), v.data_ptr(), k_row, k_head, v_row, v_head, heads, q_ptr, out_ptr, q_row, q_head,
                                               out_row, out_head, 2 * pairs, 1 if rot_half else 0, freq_ptr, _float(rot_mult, "rot_mult"), pos_ptr, axis_ptr, axes))
         return q_out
