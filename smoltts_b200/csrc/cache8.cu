@@ -19,10 +19,12 @@ namespace c8 {
 
 using lm::report;
 
-template <class T, int PASSES>
-static cudaError_t append_of(const AppendArgs& A, dim3 grid, cudaStream_t st) {
-    return A.pairs % 8 == 0 ? launch(append_kernel<T, PASSES, false>, grid, kAppendThreads, 0, st, A) : launch(append_kernel<T, PASSES, true>, grid, kAppendThreads, 0, st, A);
+template <class T, int PASSES, bool ODD>
+static cudaError_t append_placed(const AppendArgs& A, dim3 grid, cudaStream_t st) {
+    return A.places ? launch(append_kernel<T, PASSES, ODD, true>, grid, kAppendThreads, 0, st, A) : launch(append_kernel<T, PASSES, ODD, false>, grid, kAppendThreads, 0, st, A);
 }
+template <class T, int PASSES>
+static cudaError_t append_of(const AppendArgs& A, dim3 grid, cudaStream_t st) { return A.pairs % 8 == 0 ? append_placed<T, PASSES, false>(A, grid, st) : append_placed<T, PASSES, true>(A, grid, st); }
 template <class T>
 static cudaError_t append_as(const AppendArgs& A, int n_sms, cudaStream_t st) {
     const int blocks = (A.b.max_new + 2 * kBlock - 2) / kBlock, units = 2 * A.c.G + A.H, warps = kAppendThreads / 32;

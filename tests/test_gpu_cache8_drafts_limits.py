@@ -42,6 +42,23 @@ def test_queries_over_the_arrays_that_angles_are_made_of_are_refused(name):
     assert torch.equal(c.append(x, x, ints([0, T]), ints([0]), table, max_new=T, q=q, q_out=torch.empty_like(q), freq=none), q)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,pairs,half", [(33, 5, True), (64, 20, False), (96, 12, True), (128, 60, True), (256, 100, False), (64, 24, True)])
+def test_positions_that_are_the_places_change_nothing_whatever_the_pairs(dtype, d, pairs, half):
+    lens, pos0, H, G = [5, 37, 1], [3, 21, 16], 6, 2
+    freq = (10000.0 ** (-torch.arange(pairs, device="cuda") / pairs)).float()
+    T = sum(lens)
+    k, v, q = randn(T, G, d, seed=1).to(dtype), randn(T, G, d, seed=2).to(dtype), randn(T, H, d, seed=3).to(dtype)
+    places = ints([p + i for p, n in zip(pos0, lens) for i in range(n)])
+    results = []
+    for more in (dict(), dict(positions=places), dict(positions=places.repeat(3, 1).contiguous(), axis=torch.randint(0, 3, (pairs,), device="cuda").int())):
+        c, table = cache_of([p + n for p, n in zip(pos0, lens)], 32, G, d, d, garbage=False)
+        out = c.append(k, v, ints(starts(lens)), ints(pos0), table, max_new=37, q=q, freq=freq, rot_half=half, **more)
+        results.append((out, c.k.view(torch.uint8), c.v.view(torch.uint8), c.k_scale, c.v_scale))
+    for r in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, results[0]))
+
+
 # ---------------------------------------------------------------------------------------------- kept rows
 
 # (rows, pos0 of the sequence; 64 positions in four pages): entries behind the first wrong one that ascend among themselves, and destinations behind the table's last page
