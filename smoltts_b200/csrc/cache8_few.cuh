@@ -122,6 +122,30 @@ __device__ __forceinline__ float of_rank(const float* mine, int rank) {      // 
 }
 constexpr int kMostCluster = 8;      // shares of the keys that are joined inside a cluster of blocks; more go through memory and attend_join_kernel
 
+// What the shares of a row, with their maxima, denominators and e, count when joined, and the maximum, denominator and e of all of them.
+struct SharesJoined {
+    float top, total, unit, counts[kMostCluster];
+    __device__ __forceinline__ SharesJoined(const float (&tops)[kMostCluster], const float (&f)[kMostCluster], const float (&e)[kMostCluster]) : top(-INFINITY), total(0.0f), unit(-INFINITY) {
+        float least = INFINITY;
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) {
+            top = fmaxf(top, tops[z]);
+            unit = fmaxf(unit, tops[z] == -INFINITY ? -INFINITY : e[z]);
+            least = fminf(least, tops[z] == -INFINITY ? INFINITY : e[z]);
+        }
+        if (unit - least > kNear) {      // (units far apart: not the largest, but that of the largest results)
+            unit = -INFINITY;
+            for (int z = 0; z < kMostCluster; ++z) unit = fmaxf(unit, tops[z] == -INFINITY ? -INFINITY : e[z] + (tops[z] - top));
+        }
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) {
+            // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
+            total = fmaf(f[z], tops[z] == -INFINITY ? (f[z] == 0.0f ? 0.0f : f[z]) : exp2_fast(tops[z] - top), total);
+            counts[z] = tops[z] == -INFINITY ? 0.0f : exp2_fast((e[z] - unit) + (tops[z] - top));
+        }
+    }
+};
+
 // The shares of a cluster of blocks are joined: block `split` of them has rows split, split + n_splits, ...; by THREADS threads of every block.  stat, joint: a row's maximum, denominator and e in
 // each block, and its unnormalised results; the other arrays are the block's own.  What the shares of a row count and what its results are multiplied by is worked out by a thread each.
 template <int THREADS>
@@ -138,24 +162,10 @@ __device__ __forceinline__ void join_shares(const AttendArgs& A, int split, int 
             f[z] = of.y;
             e[z] = of.z;
         }
-        float M = -INFINITY, E = -INFINITY, least = INFINITY, total = 0.0f;
+        const SharesJoined joined(top, f, e);
 #pragma unroll
-        for (int z = 0; z < kMostCluster; ++z) {
-            M = fmaxf(M, top[z]);
-            E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z]);
-            least = fminf(least, top[z] == -INFINITY ? INFINITY : e[z]);
-        }
-        if (E - least > kNear) {      // (units far apart: not the largest, but that of the largest results)
-            E = -INFINITY;
-            for (int z = 0; z < kMostCluster; ++z) E = fmaxf(E, top[z] == -INFINITY ? -INFINITY : e[z] + (top[z] - M));
-        }
-#pragma unroll
-        for (int z = 0; z < kMostCluster; ++z) {
-            // a share of no visible key weighs nothing, one of NaN scores makes its row NaN
-            total = fmaf(f[z], top[z] == -INFINITY ? (f[z] == 0.0f ? 0.0f : f[z]) : exp2_fast(top[z] - M), total);
-            counts[me][z] = top[z] == -INFINITY ? 0.0f : exp2_fast((e[z] - E) + (top[z] - M));
-        }
-        const Finish fin(A, h, M, total, E);
+        for (int z = 0; z < kMostCluster; ++z) counts[me][z] = joined.counts[z];
+        const Finish fin(A, h, joined.top, joined.total, joined.unit);
         finish[me] = make_float2(fin.a, fin.b);
         to[me] = (size_t)s_row[r] * A.o_row + (size_t)h * A.o_head;
     }
@@ -170,6 +180,35 @@ __device__ __forceinline__ void join_shares(const AttendArgs& A, int split, int 
         for (int z = 0; z < kMostCluster; ++z) sum = fmaf(v[z], counts[at][z], sum);
         const float2 f = finish[at];
         static_cast<bf16*>(A.out)[to[at] + col] = __float2bfloat16_rn(finished(A, s_row[r], s_head[r], col, sum * f.x * f.y));
+    }
+}
+
+// The same for up to four rows by four warps, whose threads each work out all of it for their own columns, the blocks' results on their way meanwhile.  (A thread a row that the others wait for
+// is better from eight rows on; a token of 16 and 8 heads of 64 behind a window of 1000, five shares, 9.6 us, so 10.0; of 256 11.5 and 12.1.)
+template <int D>
+__device__ __forceinline__ void join_few_shares(const AttendArgs& A, int split, int rows, const float4* stat, const float* joint, const int* s_row, const int* s_head) {
+    for (int r = split; r < rows; r += A.n_splits) {
+        float top[kMostCluster], f[kMostCluster], e[kMostCluster], v[D / 128][kMostCluster];
+#pragma unroll
+        for (int z = 0; z < kMostCluster; ++z) {
+            const bool on = z < A.n_splits;
+            const float4 of = on ? of_rank(&stat[r], z) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+            top[z] = of.x;
+            f[z] = of.y;
+            e[z] = of.z;
+#pragma unroll
+            for (int x = 0; x < D / 128; ++x) v[x][z] = on && threadIdx.x + 128 * x < A.c.dv ? of_rank(joint + r * D + threadIdx.x + 128 * x, z) : 0.0f;
+        }
+        const SharesJoined joined(top, f, e);
+        const Finish fin(A, s_head[r], joined.top, joined.total, joined.unit);
+#pragma unroll
+        for (int x = 0; x < D / 128; ++x) {
+            const int col = threadIdx.x + 128 * x;
+            float sum = 0.0f;
+#pragma unroll
+            for (int z = 0; z < kMostCluster; ++z) sum = fmaf(v[x][z], joined.counts[z], sum);
+            if (col < A.c.dv) static_cast<bf16*>(A.out)[(size_t)s_row[r] * A.o_row + (size_t)s_head[r] * A.o_head + col] = __float2bfloat16_rn(finished(A, s_row[r], s_head[r], col, sum * fin.a * fin.b));
+        }
     }
 }
 
@@ -616,7 +655,10 @@ __global__ void __launch_bounds__(kFewThreads, few_blocks(D, RA)) attend_few_ker
     __syncwarp();
     if (clustered) {
         cluster_sync();
-        if (any && warp < 4 && !*stop) join_shares<128>(A, split, rows, s_stat, joint, D, s_row, s_head, s_finish, s_to, s_counts);
+        if (any && warp < 4 && !*stop) {
+            if constexpr (RA <= 4) join_few_shares<D>(A, split, rows, s_stat, joint, s_row, s_head);
+            else join_shares<128>(A, split, rows, s_stat, joint, D, s_row, s_head, s_finish, s_to, s_counts);
+        }
         cluster_sync();      // nobody leaves while others read
     }
     __syncwarp();
