@@ -4,9 +4,9 @@ from __future__ import annotations
 import pytest
 import torch
 
-from cache8_util import ints, starts
+from cache8_util import exponent, ints, starts
 from drafts_util import parents_of
-from test_gpu_cache8 import cache_of, fill, randn
+from test_gpu_cache8 import cache_of, fill, held, randn
 from test_gpu_cache8_drafts import arrays, check_kept, check_tree, contents, uneven
 
 pytestmark = pytest.mark.gpu
@@ -113,6 +113,47 @@ def test_rows_of_zeros_from_blocks_of_any_scale(d, dv, power):
     check_kept(c, before, table, pos0, rows)
     for x in c.values(table.flatten().long()):
         assert torch.isfinite(x).all()
+
+
+def rounded(x, e):
+    """x as codes of scale 2^e hold it, in 64 bits."""
+    return (x.double() * 2.0 ** -e).float().to(torch.float8_e4m3fn).double() * 2.0 ** e
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("context", [16, 21])
+def test_a_rejected_row_leaves_its_scale_behind(dtype, context):
+    """One of six drafted rows is 2^12 larger than the others and rejected.  In a block that the context began, its rows and the kept ones hold what the raised scale leaves of them (2^-4 of
+    themselves, twice for the older ones, and 2^-10 of the scale); in a block of kept rows alone the scale is made anew, for codes that were rounded under the raised one."""
+    from smoltts_b200.kv_cache import keep_rows
+
+    G, d, accepted = 2, 64, [0, 1, 4]
+    c, table = cache_of([32], 32, G, d, d, garbage=False)
+    x = randn(context + 6, G, d, seed=1).clamp(-3, 3)
+    x[context + 3] *= 2.0 ** 12
+    x = x.to(dtype)
+    c.append(x[:context], x[:context], ints([0, context]), ints([0]), table, max_new=context)
+    first = held(c, table, 0, 16)
+    c.append(x[context:], x[context:], ints([0, 6]), ints([context]), table, max_new=6)
+    keep_rows(c, ints([context]), table, ints([accepted]), ints([3]))
+    for got, old in zip(held(c, table, 0, context + 3), first):
+        assert torch.equal(got[:16], old)      # (the block in front of the drafted rows')
+        for g in range(G):
+            older, new = x[16:context, g].double(), x[[context + r for r in accepted], g].double()
+            alone, raised = exponent(torch.cat([older, new]).abs().max().item()), exponent(x[16:, g].abs().max().item())
+            assert raised - alone in (11, 12, 13)
+            if context == 16:
+                want = rounded(new, raised)
+                want = rounded(want, exponent(want.abs().max().item()))
+            else:
+                want = torch.cat([rounded(rounded(older, exponent(older.abs().max().item())), raised), rounded(new, raised)])
+            assert torch.equal(got[16:, g].double(), want)
+            plain = torch.cat([older, new])
+            # two roundings: 2 * 2^-4 + 2^-8 of the value; the second one's half step at the least codes, and the first one's, which is 2^-11 of that
+            assert ((got[16:, g].double() - plain).abs() <= 0.1290 * plain.abs() + 1.001 * 2.0 ** (raised - 10)).all()
+            assert (want == 0).sum() > (rounded(plain, alone) == 0).sum()
+            assert c.k_scale[table[0, 0], g, 1].item() == 2.0 ** (exponent(want.abs().max().item()) if context == 16 else raised)
+    c.check_device_errors()
 
 
 # ---------------------------------------------------------------------------------------------- attention along paths
