@@ -10,7 +10,6 @@
 #define SMOL_OK 0
 #define SMOL_ERR_INVALID (-1)
 #define SMOL_ERR_CUDA (-3)
-#define SMOL_ERR_UNSUPPORTED (-4)
 #define SMOL_ERR_CAPACITY (-5)
 
 namespace smol {

@@ -338,10 +338,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attend_tiles_kernel(const __g
             }
             if (TREE && !whole) {
                 // which of the thread's keys the row's bits name (the context's all)
-                const int i0 = jc - pos0, w = i0 >> 5;      // (rounded down)
-                const uint32_t* bits = A.tree_sees + (size_t)(t0 + my_row / Gq) * A.tree_words;
-                const uint32_t low = w < 0 ? 0xffffffffu : w < A.tree_words ? bits[w] : 0u, high = w + 1 < 0 ? 0xffffffffu : w + 1 < A.tree_words ? bits[w + 1] : 0u;
-                const uint32_t named = __funnelshift_r(low, high, i0 & 31);
+                const uint32_t named = tree_named(A, t0 + my_row / Gq, jc - pos0);
                 const int last = seen.end - jc;
 #pragma unroll
                 for (int e = 0; e < kTileCols; ++e)
