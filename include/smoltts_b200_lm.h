@@ -416,7 +416,7 @@ int smol_lm_cache8_attend(const SmolLmCache8* cache, const SmolLmCache8Batch* ba
 
 int smol_lm_cache8_tree(const SmolLmCache8Tree* a, void* stream);
 /* The rows that stay move together, in every one of `caches` (HOST array, all of one shape, none twice): row rows[s][i] becomes the row at position seq_pos0[s] + i, as if its
- * values, as the cache holds them, were appended there; what lies behind the last of them is as it was, or as it was with another scale.  A sequence whose arrays do not fit is left
+ * values, as the cache holds them, were appended there (a block that older rows began keeps a scale that rows which do not stay have raised); what lies behind the last of them is as it was, or as it was with another scale.  A sequence whose arrays do not fit is left
  * as it is and reported in the caches' err (1: a page outside the cache, 2: rows not in order). */
 int smol_lm_cache8_keep(const SmolLmCache8* caches, int32_t n_caches, const SmolLmCache8Keep* a, void* stream);
 /* Pages src[i] into pages dst[i], codes and scales, in every one of `caches`.  src and dst are HOST arrays, copied by the call: no page may be written twice, nor read and written. */

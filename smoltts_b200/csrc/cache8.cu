@@ -99,6 +99,8 @@ cudaError_t attend(AttendArgs A, bool f32, int n_sms, void* workspace, int* laun
     few.rows_most = kFewMost;
     few.b.max_new = kFewMost / (A.H / A.c.G);
     few.n_splits = std::min(splits_for(few, f32, n_sms), kMostCluster);      // (joined without the workspace, which the tiles' shares may be in)
+    // Nor does it go by kQuadClusters, which is about clusters against shares through memory: fewer shares are what is left here, and slower.  Trees of 16 rows beside one of 85, 8 heads of 128,
+    // 8 shares / as many as make 96 blocks: one sequence at 32768 positions 60 / 70 us, two 76 / 95, seven at 8192 in two shares / one 76 / 96.
     few.part = nullptr;
     few.in_cluster = few.n_splits > 1;
     *launches += 1;

@@ -11,7 +11,7 @@
 //
 // What bounds it: the bytes of queries, keys and values.  10671 tokens of 32 query and 8 key/value heads of 128, slices of one projection: 55 us, 4.4 TB/s
 // (four coordinates a lane and the four they go with read again: 228); 10020 rows of pictures and text at
-// positions of three axes 62; a token of 12 and 4 heads of 64 3.2 us, which is launch and two dependent loads.
+// positions of three axes 62; a token of 12 and 4 heads of 64 3.0 us, which is launch and two dependent loads.
 #pragma once
 
 #include "cache8.cuh"

@@ -20,7 +20,7 @@
 // results that see one.
 //
 // What bounds it: the bytes of the cache.  64 sequences at up to 8192 positions, 32 and 8 heads of 128: 147 us, 5.5 TB/s; one of 12 and 4 heads at 131072
-// 34 us, 3.9 TB/s; 32 behind windows of 1024 19 us, and 2048 positions of 12 and 4 heads of 64 8 us, which are launch, page lookups and the join.  On the registers' way (mma.sync, e4m3 operands made f16 by the compiler's expansion) 32 positions took 965
+// 33 us, 4.1 TB/s; 32 behind windows of 1024 17 us, and 2048 positions of 12 and 4 heads of 64 8 us, which are launch, page lookups and the join.  On the registers' way (mma.sync, e4m3 operands made f16 by the compiler's expansion) 32 positions took 965
 // instructions of a warp and 64 sequences at up to 8192 positions 227 us.
 #pragma once
 
@@ -184,7 +184,7 @@ __device__ __forceinline__ void join_shares(const AttendArgs& A, int split, int 
 }
 
 // The same for up to four rows by four warps, whose threads each work out all of it for their own columns, the blocks' results on their way meanwhile.  (A thread a row that the others wait for
-// is better from eight rows on; a token of 16 and 8 heads of 64 behind a window of 1000, five shares, 9.6 us, so 10.0; of 256 11.5 and 12.1.)
+// is better from there on: 32 sequences of eight rows of 64 behind windows of 1000 23.1 us, this way 24.5; of two rows, one sequence, five shares, 10.0 and 9.7, of 256 12.1 and 11.4.)
 template <int D>
 __device__ __forceinline__ void join_few_shares(const AttendArgs& A, int split, int rows, const float4* stat, const float* joint, const int* s_row, const int* s_head) {
     for (int r = split; r < rows; r += A.n_splits) {

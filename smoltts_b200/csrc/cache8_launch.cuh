@@ -55,7 +55,8 @@ static cudaError_t more_smem(K kernel, int bytes, std::atomic<uint64_t>& asked) 
 // to fill the GPU the keys' shares are what counts: one at 2048 with 32 rows 16.6 / 16.6, with 64 18.1 / 19.6, with 96 33 / 21.
 constexpr int kFewMost = 16, kFewMostSmall = 64;
 constexpr long long kSmall = 1 << 16;      // sequences times heads times positions (16384: the last of these; 262144: the one at 32768)
-// Rows of a tree that the kernel for 32 rows takes (cache8_quads.cuh), and otherwise one of those for few or many.
+// Rows of a tree that the kernel for 32 rows takes (cache8_quads.cuh), and otherwise one of those for few or many.  64 sequences at up to 8192 positions, 8 heads of 128, few / 32 rows / tiles: 8 rows 168 / 208 /
+// 399 us, 16 rows 247 / 208 / 399, 32 rows 485 / 213 / 408, 64 rows - / 383 / 400.  (It has no form for rows without a tree.)
 constexpr int kQuadLeast = 8, kQuadMost = 64, kQuadRows = 32;
 inline bool quads_serve(const AttendArgs& A, bool f32) {
     const long long rows = A.b.max_new * (long long)(A.H / A.c.G);

@@ -7,7 +7,8 @@
 // The weights are the first operand of the second product with zeros beside a copy's own 32 positions, so that a copy's result is that of its positions; the copies are joined at the end as
 // shares of the keys are.  Two groups of four warps take even and odd steps' softmax, and half of the results' columns each of every step, whose running sums fit their registers so.
 //
-// Queries and weights are two e4m3 parts of one unit as in the tiles, relative to what a row sees in 32 positions of a step rather than in 128.
+// Queries and weights are two e4m3 parts of one unit as in the tiles, relative to what a row sees in 32 positions of a step rather than in 128: a weight to 2^-9 of itself or 2^-18 of the largest term,
+// since both parts are multiplied into one sum.  (The kernel for few rows has a sum for either, and 2^-22: a chain of 9 to 16 rows is answered that much more finely without a tree.)
 //
 // Roles: eight warps for the softmax, one that copies, one that issues the products.
 //

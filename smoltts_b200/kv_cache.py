@@ -219,7 +219,8 @@ class KVCache8:
         first); an axis that there is not is reported and counts as the first.
 
         A block's 16 positions share the smallest power of two with |value| <= 448 * scale; where an earlier call began the block the
-        scale never shrinks, and the older codes follow it when it grows.  Magnitudes above 2^100 are clamped; a NaN stays a NaN.  Two
+        scale never shrinks, and the older codes follow it when it grows: a row of drafted ones that is much larger than the rest takes bits from the up to 15 rows in
+        front of it for good, whether it is kept or not.  Magnitudes above 2^100 are clamped; a NaN stays a NaN.  Two
         sequences of a batch must not write the same page, nor one write a page twice.  The rows of a sequence have to follow what it already holds."""
         tokens, dtype = k.shape[0], k.dtype
         k_row, k_head = self._rows(k, None, self.kv_heads, self.dim, None, "k")
@@ -377,7 +378,8 @@ def keep_rows(caches: Union[KVCache8, Sequence[KVCache8]], seq_pos0: torch.Tenso
     """Keeps the rows of an accepted path, in all layers: row ``rows[s, i]`` behind position ``seq_pos0[s]`` becomes the row at ``seq_pos0[s] + i``, for ``i`` below ``counts[s]``
     (int32 ``[sequences, most]`` and ``[sequences]``; rows in ascending order, what is behind ``counts[s]`` is not looked at).
 
-    The rows are written as ``append`` would write the values that the cache holds of them; the sequence's length is then ``seq_pos0[s] + counts[s]``, and what lies behind it
+    The rows are written as ``append`` would write the values that the cache holds of them.  A block that holds older rows too keeps the scale that the drafted rows have given it,
+    rejected ones among them; one of kept rows alone gets a scale of its own, but what was rounded under the larger one stays so.  The sequence's length is then ``seq_pos0[s] + counts[s]``, and what lies behind it
     is no more to be read.  ``caches``: a cache, or the layers' (of one shape, none twice).  A sequence whose arrays do not fit is left as it is, and
     ``check_device_errors`` of the caches tells.  No page may belong to two sequences that keep rows in it."""
     layers = _layers(caches)
@@ -392,7 +394,7 @@ def keep_rows(caches: Union[KVCache8, Sequence[KVCache8]], seq_pos0: torch.Tenso
 
 def copy_pages(caches: Union[KVCache8, Sequence[KVCache8]], src: Sequence[int], dst: Sequence[int]) -> None:
     """Copies pages ``src[i]`` to pages ``dst[i]``, in all layers.  The pages are host numbers, as a ``pool.PagePool`` hands them out; a page may be copied to several others, but none
-    may be written twice, nor read and written by one call.  A captured call copies the same pages whenever it is replayed."""
+    may be written twice, nor read and written by one call.  A block's scale is copied with it, whatever rows behind the fork it was made for.  A captured call copies the same pages whenever it is replayed."""
     layers = _layers(caches)
     if any(isinstance(x, torch.Tensor) and x.is_cuda for x in (src, dst)):
         raise ValueError("pages are host numbers")
