@@ -184,7 +184,7 @@ __device__ __forceinline__ void join_shares(const AttendArgs& A, int split, int 
 }
 
 // The same for up to four rows by four warps, whose threads each work out all of it for their own columns, the blocks' results on their way meanwhile.  (A thread a row that the others wait for
-// is better from there on: 32 sequences of eight rows of 64 behind windows of 1000 23.1 us, this way 24.5; of two rows, one sequence, five shares, 10.0 and 9.7, of 256 12.1 and 11.4.)
+// is better from there on: 32 sequences of eight rows of 64 behind windows of 1000 23.1 us, this way (and a block's own results likewise) 24.5; of two rows, one sequence, five shares, 10.0 and 9.7, of 256 12.1 and 11.4.)
 template <int D>
 __device__ __forceinline__ void join_few_shares(const AttendArgs& A, int split, int rows, const float4* stat, const float* joint, const int* s_row, const int* s_head) {
     for (int r = split; r < rows; r += A.n_splits) {
